@@ -194,6 +194,26 @@ __device__ __forceinline__ float sum_lane_halves(float x) {
   return __builtin_bit_cast(float, (unsigned)p[0]) + __builtin_bit_cast(float, (unsigned)p[1]);
 }
 
+// Sum over groups of LPR neighbouring lanes, in every lane of the group: DPP
+// row rotations within 16 lanes, v_permlane16_swap and v_permlane32_swap beyond.
+template <int LPR>
+__device__ __forceinline__ float sum_lanes(float x) {
+  static_assert(LPR == 16 || LPR == 32 || LPR == 64, "16, 32 or 64 lanes per row");
+#define GP_DPP_F(v, ctrl) __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), ctrl, 0xF, 0xF, false))
+  x += GP_DPP_F(x, 0x128);  // row_ror:8
+  x += GP_DPP_F(x, 0x124);  // row_ror:4
+  x += GP_DPP_F(x, 0x4E);   // quad_perm [2,3,0,1]
+  x += GP_DPP_F(x, 0xB1);   // quad_perm [1,0,3,2]
+#undef GP_DPP_F
+  if constexpr (LPR >= 32) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = __builtin_bit_cast(float, (unsigned)a[0]) + __builtin_bit_cast(float, (unsigned)a[1]);
+  }
+  if constexpr (LPR == 64) x = sum_lane_halves(x);
+  return x;
+}
+
 // ---------------------------------------------------------------------------
 // Weight rows staged in LDS.  A weight matrix W (rows of 128 16-bit values)
 // is copied HBM->LDS in its own row-major shape, 256 bytes per row, four rows

@@ -279,4 +279,29 @@ hipError_t dlrm_bot_launch(int64_t M, int K0, const void* x, const void* const* 
                            const int* acts, void* out, void* ws, int num_cus, hipStream_t stream,
                            int dtype = GP_DTYPE_F16);
 
+// h = x + scale * act(gate) * Post(y), out = Pre(h) (gp_residual_norm_out);
+// pointers of any 2-byte alignment, D up to kNormMaxDim, gate_rows divides M.
+constexpr int64_t kNormMaxDim = 32768;
+struct ResidualNormArgs {
+  int64_t M, D;
+  const void* x;
+  const void* y;  // null: h = x
+  int post;       // GP_NORM_*
+  const void* post_gamma;
+  const void* post_beta;
+  float post_eps;
+  const void* gate;  // null: 1
+  int64_t gate_rows;
+  int gate_act;
+  float scale;
+  int pre;
+  const void* gamma;
+  const void* beta;
+  float eps;
+  void* h;    // null: not stored
+  void* out;  // null: not stored (pre none)
+  int dtype;
+};
+hipError_t residual_norm_launch(const ResidualNormArgs& a, int num_cus, hipStream_t stream);
+
 }  // namespace gp

@@ -352,24 +352,6 @@ hipError_t linear_launch(const LinearArgs& a, int num_cus, hipStream_t s) {
 // sums over a row's lanes are DPP row rotations and v_permlane16/32_swap, and
 // each wave issues the loads of U row groups before it reduces the first, so
 // that several memory latencies overlap (the kernel is HBM-bound).
-template <int LPR>
-__device__ __forceinline__ float sum_lanes(float x) {
-  static_assert(LPR == 16 || LPR == 32 || LPR == 64, "16, 32 or 64 lanes per row");
-#define GP_DPP_F(v, ctrl) __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), ctrl, 0xF, 0xF, false))
-  x += GP_DPP_F(x, 0x128);  // row_ror:8
-  x += GP_DPP_F(x, 0x124);  // row_ror:4
-  x += GP_DPP_F(x, 0x4E);   // quad_perm [2,3,0,1]
-  x += GP_DPP_F(x, 0xB1);   // quad_perm [1,0,3,2]
-#undef GP_DPP_F
-  if constexpr (LPR >= 32) {
-    const unsigned u = __builtin_bit_cast(unsigned, x);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    x = __builtin_bit_cast(float, (unsigned)a[0]) + __builtin_bit_cast(float, (unsigned)a[1]);
-  }
-  if constexpr (LPR == 64) x = sum_lane_halves(x);
-  return x;
-}
-
 template <int D>
 __global__ __launch_bounds__(kStageThreads) void layer_norm_rows_kernel(const half_t* x, const half_t* gamma,
                                                                         const half_t* beta, float eps, half_t* out,

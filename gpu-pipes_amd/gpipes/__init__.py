@@ -28,7 +28,7 @@ __all__ = [
     "gemm_out", "bert_ffn", "bert_ffn_out", "mlp_out", "dlrm_botmlp", "dlrm_botmlp_out", "dlrm_topmlp",
     "dlrm_topmlp_out", "nerf_full", "nerf_full_out", "nerf_full_out_noalloc", "bert_addln_ffn",
     "bert_addln_ffn_out", "nerf_a", "nerf_a_out", "pipe_handoff", "handoff_checksums", "phase_timers",
-    "probe_mfma", "fill_normal",
+    "probe_mfma", "fill_normal", "residual_norm_out", "residual_norm", "NORMS",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -42,7 +42,9 @@ IMPL_FUSED = 0
 IMPL_PIPELINED = 1
 IMPL_PIPELINED_SPLIT_LN = 2
 _IMPLS = {"fused": IMPL_FUSED, "pipelined": IMPL_PIPELINED, "pipelined_split_ln": IMPL_PIPELINED_SPLIT_LN}
-ACTS = {"none": 0, "relu": 1, "gelu_tanh": 2, "sigmoid": 3}
+# "silu" (GP_ACT_SILU) is the residual norm's gate's and the 4-bit products' only
+ACTS = {"none": 0, "relu": 1, "gelu_tanh": 2, "sigmoid": 3, "silu": 4}
+NORMS = {"none": 0, "layer": 1, "rms": 2}
 ROUTES = {"ident": 0, "broadcast": 1, "split": 2, "drain": 3, "handoff": 4, "reload": 5}
 
 
@@ -112,6 +114,9 @@ def _load():
     L.gp_nerf_a_dtype_out.argtypes = [i64, i64, vp, vp, vp, vp, i32, i32, vp]
     L.gp_nerf_a_dtype_out.restype = i32
     L.gp_nerf_full_out_noalloc.restype = i32
+    L.gp_residual_norm_out.argtypes = [i64, i64, vp, vp, i32, vp, vp, f32, vp, i64, i32, f32, i32, vp, vp, f32, vp, vp,
+                                       i32, vp]
+    L.gp_residual_norm_out.restype = i32
     for name in ("gp_mlp_out", "gp_dlrm_botmlp_out", "gp_dlrm_topmlp_out", "gp_nerf_full_out", "gp_gemm_out",
                  "gp_gemm_dtype_out", "gp_bert_ffn_out", "gp_bert_ffn_dtype_out", "gp_linear_out", "gp_linear_layer_norm_out", "gp_layer_norm_out", "gp_add_out",
                  "gp_concat_out", "gp_pipe_ident", "gp_pipeline_check"):
@@ -876,3 +881,71 @@ def nerf_full(x, d, *wb, rgb_act="none"):
     out_r = torch.empty((x.shape[0], wb[16].shape[1]), dtype=x.dtype, device=x.device)
     out_rgb = torch.empty((x.shape[0], wb[22].shape[1]), dtype=x.dtype, device=x.device)
     return nerf_full_out(x, d, *wb, out_r, out_rgb, rgb_act=rgb_act)
+
+
+# ---------------------------------------------------------------------------
+# A language model's feed-forward half
+# ---------------------------------------------------------------------------
+
+def residual_norm_out(x, y=None, gate=None, gate_act="none", scale=1.0, post="none", post_gamma=None, post_beta=None,
+                      post_eps=1e-5, norm="rms", gamma=None, beta=None, eps=1e-5, h=None, out=None):
+    """The norms around a transformer block with its gate, residual scale and sum (gp_residual_norm_out):
+
+        h = x + scale * gate_act(gate) * post_norm(y),    out = norm(h)
+
+    x, y [M, D]; post and norm are "none", "layer" or "rms", with gamma / beta [D] (None: 1 / 0);
+    gate None, [D], or [R, D] with R a divisor of M (each row for M / R consecutive rows).  y None:
+    h = x.  Every tensor float16, or every tensor bfloat16.  h and out are written where given;
+    out None with a norm: a new tensor; h None: not stored (norm "none": a new tensor).  They may
+    be x or y themselves.  Returns (h, out), with None in the place of what was not written."""
+    return _residual_norm(x, y, gate, gate_act, scale, post, post_gamma, post_beta, post_eps, norm, gamma, beta, eps, h,
+                          out)
+
+
+def _residual_norm(x, y, gate, gate_act, scale, post, post_gamma, post_beta, post_eps, norm, gamma, beta, eps, h, out):
+    dt = _dtype_of(x)
+    if not _ok(x, None, dt):
+        _check_input("x", x, dtype=dt)
+    shape = x.shape
+    if len(shape) != 2:
+        raise RuntimeError("x must be 2-D [M, D]")
+    M, D = shape
+    if y is not None and not _ok(y, shape, dt):
+        _check_input("y", y, shape, dt)
+    rows = 0
+    if gate is not None:
+        if not _ok(gate, None, dt):
+            _check_input("gate", gate, dtype=dt)
+        rows = gate.shape[0] if gate.dim() == 2 else 1
+        if gate.shape not in ((D,), (rows, D)):
+            raise RuntimeError(f"gate must be [{D}] or [R, {D}] (got {tuple(gate.shape)})")
+    for name, t in (("post_gamma", post_gamma), ("post_beta", post_beta), ("gamma", gamma), ("beta", beta)):
+        if t is not None and not _ok(t, (D,), dt):
+            _check_input(name, t, (D,), dt)
+    norm_id = NORMS.get(norm, norm)
+    if out is None:
+        if norm_id != 0:
+            out = torch.empty_like(x)
+        elif h is None:
+            h = torch.empty_like(x)
+    elif not _ok(out, shape, dt):
+        _check_input("out", out, shape, dt)
+    if h is not None and not _ok(h, shape, dt):
+        _check_input("h", h, shape, dt)
+    _same_device(x, y, gate, post_gamma, post_beta, gamma, beta, h, out)
+    with _on(x):
+        rc = lib.gp_residual_norm_out(M, D, x.data_ptr(), _ptr(y), NORMS.get(post, post), _ptr(post_gamma),
+                                      _ptr(post_beta), post_eps, _ptr(gate), rows, ACTS.get(gate_act, gate_act), scale,
+                                      norm_id, _ptr(gamma), _ptr(beta), eps, _ptr(h), _ptr(out), _DTYPES[dt],
+                                      _stream(x))
+    if rc:
+        _check(rc)
+    return h, out
+
+
+def residual_norm(x, y=None, gate=None, gate_act="none", scale=1.0, post="none", post_gamma=None, post_beta=None,
+                  post_eps=1e-5, norm="rms", gamma=None, beta=None, eps=1e-5):
+    """Allocating form of residual_norm_out: returns new (h, out) (norm "none": out is None)."""
+    _check_input("x", x, dtype=_dtype_of(x))
+    return _residual_norm(x, y, gate, gate_act, scale, post, post_gamma, post_beta, post_eps, norm, gamma, beta, eps,
+                          torch.empty_like(x), None)

@@ -57,6 +57,13 @@ extern "C" {
 #define GP_ACT_RELU 1
 #define GP_ACT_GELU_TANH 2
 #define GP_ACT_SIGMOID 3
+/* v / (1 + e^-v): gp_residual_norm_out's gate and the 4-bit products only. */
+#define GP_ACT_SILU 4
+
+/* Norms of gp_residual_norm_out over a row of D values, variance biased:  */
+#define GP_NORM_NONE 0  /* the row as it is                                 */
+#define GP_NORM_LAYER 1 /* (v - mean) / sqrt(var + eps) * gamma + beta      */
+#define GP_NORM_RMS 2   /* v / sqrt(mean(v^2) + eps) * gamma + beta         */
 
 /* Library version as 0xMMmmpp. */
 int gp_version(void);
@@ -530,6 +537,32 @@ int gp_set_wait_limit(int64_t polls);
  * returns GP_ERR_INVALID_ARG.  No counterpart in the reference.
  */
 int gp_phase_timers_read(void* dst, int64_t bytes);
+
+/*
+ * The norms around a transformer block with its gate, residual scale and sum,
+ * in one pass over the rows:
+ *   h[m]   = x[m] + scale * gate_act(gate[m / (M / gate_rows)]) * Post(y[m])
+ *   out[m] = Pre(h[m])
+ * Post (of the block whose output y is) and Pre (of the block that follows)
+ * are GP_NORM_*, each with its gamma / beta [D] (NULL: 1 / 0) and eps >= 0.
+ * x, y, h, out: [M, D], 1 <= D <= 32768; every tensor `dtype`.
+ * gate: [gate_rows, D], gate_rows a divisor of M: 1 (a value for each
+ * channel), one row a sequence, or M (one a token); NULL: 1, and gate_rows
+ * and gate_act are not looked at.  gate_act: any GP_ACT_*.
+ * y NULL: h = x; post must be GP_NORM_NONE and gate NULL.
+ * h NULL: h is not stored.  out: needed unless pre is GP_NORM_NONE, and not
+ * written then.  One of h and out has to be stored.
+ * All arithmetic is fp32; Pre takes h before it is rounded for memory.
+ * h and out may each be x, y or (gate_rows == M) gate itself, but not each
+ * other; other overlaps are not supported.  Any 2-byte alignment.  One launch,
+ * no workspace: can be captured into a graph.
+ * No counterpart in the reference (layer_norm_v2.cuh:129-147 and
+ * elemwise_add.cuh:42-54 are its separate norm and sum).
+ */
+int gp_residual_norm_out(int64_t M, int64_t D, const void* x, const void* y, int post, const void* post_gamma,
+                         const void* post_beta, float post_eps, const void* gate, int64_t gate_rows, int gate_act,
+                         float scale, int pre, const void* gamma, const void* beta, float eps, void* h, void* out,
+                         int dtype, void* stream);
 
 #ifdef __cplusplus
 }

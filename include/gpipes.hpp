@@ -160,6 +160,15 @@ inline void nerf_a_out(int64_t M, int64_t Kx, const void* x, const void* const* 
   check(gp_nerf_a_out(M, Kx, x, w, b, out, impl, stream));
 }
 
+// The norms around a block with its gate, residual scale and sum (gp_residual_norm_out).
+inline void residual_norm_out(int64_t M, int64_t D, const void* x, const void* y, int post, const void* post_gamma,
+                              const void* post_beta, float post_eps, const void* gate, int64_t gate_rows, int gate_act,
+                              float scale, int pre, const void* gamma, const void* beta, float eps, void* h, void* out,
+                              int dtype = GP_DTYPE_F16, void* stream = nullptr) {
+  check(gp_residual_norm_out(M, D, x, y, post, post_gamma, post_beta, post_eps, gate, gate_rows, gate_act, scale, pre,
+                             gamma, beta, eps, h, out, dtype, stream));
+}
+
 }  // namespace gpipes
 
 #endif  // GPIPES_HPP
