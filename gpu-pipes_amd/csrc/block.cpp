@@ -1,6 +1,7 @@
 // C ABI of the operators around a language model's feed-forward half: the norms
-// with the residual (gp_residual_norm_out).  Argument checks and dispatch; the
-// kernels are in residual_norm.hip.
+// with the residual (gp_residual_norm_out) and the products with 4-bit weights
+// (gp_q4_gemm_out, gp_q4_gated_out).  Argument checks and dispatch; the kernels
+// are in residual_norm.hip and q4.hip.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -37,6 +38,43 @@ int check_norm(int kind, const void* gamma, const void* beta, float eps, const c
     return fail(GP_ERR_INVALID_ARG, "the %s norm's eps must be >= 0 and finite", name);
   }
   return GP_OK;
+}
+
+constexpr int64_t kQ4MaxDim = int64_t(1) << 20;
+
+int check16(const void* p, const char* name, bool needed) {
+  if (!p) return needed ? fail(GP_ERR_INVALID_ARG, "%s is NULL", name) : GP_OK;
+  if (!aligned16(p)) return fail(GP_ERR_ALIGN, "%s must be 16-byte aligned", name);
+  return GP_OK;
+}
+
+int q4_run(const Q4Args& a, int64_t N, int64_t K, hipStream_t stream) {
+  clear_error();
+  int rc;
+  if ((rc = check_dtype(a.dtype)) || (rc = check_rows(a.M)) || (rc = check_act_ext(a.act))) return rc;
+  if (a.group != 32 && a.group != 64 && a.group != 128)
+    return fail(GP_ERR_SHAPE, "group must be 32, 64 or 128 (got %d)", a.group);
+  if (K < 8 || K % 8 || K > 65536) return fail(GP_ERR_SHAPE, "K must be a multiple of 8 in [8, 65536] (got %lld)", (long long)K);
+  if (N < 1 || N > kQ4MaxDim) return fail(GP_ERR_SHAPE, "N must be in [1, %lld] (got %lld)", (long long)kQ4MaxDim, (long long)N);
+  if (K * N / 2 >= (int64_t(1) << 31)) return fail(GP_ERR_SHAPE, "a weight must be smaller than 2 GiB");
+  if (a.M > (int64_t(1) << 21)) return fail(GP_ERR_SHAPE, "M must be at most 2097152 (got %lld)", (long long)a.M);
+  if (a.r && a.act != GP_ACT_NONE) return fail(GP_ERR_INVALID_ARG, "a residual is added without an activation only");
+  for (int i = 0; i < a.sides; ++i) {
+    const Q4Side& d = a.side[i];
+    if ((rc = check16(d.wq, "wq", true)) || (rc = check16(d.s, "scales", true)) ||
+        (rc = check16(d.z, "zeros", false)) || (rc = check16(d.b, "b", false)))
+      return rc;
+  }
+  if ((rc = check16(a.r, "r", false))) return rc;
+  if (a.M == 0) return GP_OK;
+  if ((rc = check16(a.x, "x", true)) || (rc = check16(a.out, "out", true))) return rc;
+  int dev = 0, ncu = 0;
+  if ((rc = current_device_info(&dev, &ncu))) return rc;
+  Q4Args b = a;
+  b.N = (int)N;
+  b.K = (int)K;
+  const hipError_t e = q4_launch(b, ncu, stream);
+  return e == hipSuccess ? GP_OK : fail_hip(e, "q4 launch");
 }
 
 }  // namespace
@@ -82,6 +120,20 @@ int gp_residual_norm_out(int64_t M, int64_t D, const void* x, const void* y, int
                            scale, pre,  gamma, beta, eps,  h,          out,       dtype};
   const hipError_t e = residual_norm_launch(a, ncu, (hipStream_t)stream);
   return e == hipSuccess ? GP_OK : fail_hip(e, "residual_norm launch");
+}
+
+int gp_q4_gemm_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq, const void* scales,
+                   const void* zeros, const void* b, const void* r, int act, void* out, int dtype, void* stream) {
+  const Q4Args a{M, 0, 0, group, 1, x, {{wq, scales, zeros, b}, {}}, r, act, out, dtype};
+  return q4_run(a, N, K, (hipStream_t)stream);
+}
+
+int gp_q4_gated_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq_g, const void* scales_g,
+                    const void* zeros_g, const void* b_g, const void* wq_u, const void* scales_u, const void* zeros_u,
+                    const void* b_u, int act, void* out, int dtype, void* stream) {
+  const Q4Args a{M,   0,  0, group, 2, x, {{wq_g, scales_g, zeros_g, b_g}, {wq_u, scales_u, zeros_u, b_u}}, nullptr,
+                 act, out, dtype};
+  return q4_run(a, N, K, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -304,4 +304,25 @@ struct ResidualNormArgs {
 };
 hipError_t residual_norm_launch(const ResidualNormArgs& a, int num_cus, hipStream_t stream);
 
+// Products with 4-bit weights (gp_q4_gemm_out: one side; gp_q4_gated_out: two,
+// the gate's first).  K a multiple of 8, group 32, 64 or 128, K N / 2 below
+// 2^31, every pointer 16-byte aligned.
+struct Q4Side {
+  const void* wq;  // [K / 8, N] words of eight k
+  const void* s;   // [ceil(K / group), N]
+  const void* z;   // the same shape, or null: 8
+  const void* b;   // [N] or null
+};
+struct Q4Args {
+  int64_t M;
+  int N, K, group, sides;
+  const void* x;  // [M, K]
+  Q4Side side[2];
+  const void* r;  // [M, N] or null
+  int act;
+  void* out;  // [M, N]
+  int dtype;
+};
+hipError_t q4_launch(const Q4Args& a, int num_cus, hipStream_t stream);
+
 }  // namespace gp

@@ -28,7 +28,8 @@ __all__ = [
     "gemm_out", "bert_ffn", "bert_ffn_out", "mlp_out", "dlrm_botmlp", "dlrm_botmlp_out", "dlrm_topmlp",
     "dlrm_topmlp_out", "nerf_full", "nerf_full_out", "nerf_full_out_noalloc", "bert_addln_ffn",
     "bert_addln_ffn_out", "nerf_a", "nerf_a_out", "pipe_handoff", "handoff_checksums", "phase_timers",
-    "probe_mfma", "fill_normal", "residual_norm_out", "residual_norm", "NORMS",
+    "probe_mfma", "fill_normal", "residual_norm_out", "residual_norm", "NORMS", "q4_gemm_out",
+    "q4_gated_out",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -117,6 +118,10 @@ def _load():
     L.gp_residual_norm_out.argtypes = [i64, i64, vp, vp, i32, vp, vp, f32, vp, i64, i32, f32, i32, vp, vp, f32, vp, vp,
                                        i32, vp]
     L.gp_residual_norm_out.restype = i32
+    L.gp_q4_gemm_out.argtypes = [i64, i64, i64, i32] + [vp] * 6 + [i32, vp, i32, vp]
+    L.gp_q4_gemm_out.restype = i32
+    L.gp_q4_gated_out.argtypes = [i64, i64, i64, i32] + [vp] * 9 + [i32, vp, i32, vp]
+    L.gp_q4_gated_out.restype = i32
     for name in ("gp_mlp_out", "gp_dlrm_botmlp_out", "gp_dlrm_topmlp_out", "gp_nerf_full_out", "gp_gemm_out",
                  "gp_gemm_dtype_out", "gp_bert_ffn_out", "gp_bert_ffn_dtype_out", "gp_linear_out", "gp_linear_layer_norm_out", "gp_layer_norm_out", "gp_add_out",
                  "gp_concat_out", "gp_pipe_ident", "gp_pipeline_check"):
@@ -949,3 +954,80 @@ def residual_norm(x, y=None, gate=None, gate_act="none", scale=1.0, post="none",
     _check_input("x", x, dtype=_dtype_of(x))
     return _residual_norm(x, y, gate, gate_act, scale, post, post_gamma, post_beta, post_eps, norm, gamma, beta, eps,
                           torch.empty_like(x), None)
+
+
+def _check_q4(wq, scales, zeros, K, N, group, dt, side=""):
+    """A 4-bit weight [K, N]: words [K / 8, N], scales and zeros [ceil(K / group), N]."""
+    if not _ok(wq, (K // 8, N), torch.int32):
+        _check_input("wq" + side, wq, (K // 8, N), torch.int32)
+    shape = (-(-K // group), N)
+    if not _ok(scales, shape, dt):
+        _check_input("scales" + side, scales, shape, dt)
+    if zeros is not None and not _ok(zeros, shape, dt):
+        _check_input("zeros" + side, zeros, shape, dt)
+
+
+def _q4_shape(x, wq, group, dt):
+    if not _ok(x, None, dt):
+        _check_input("x", x, dtype=dt)
+    if x.dim() != 2:
+        raise RuntimeError("x must be 2-D [M, K]")
+    if not isinstance(wq, torch.Tensor) or wq.dim() != 2:
+        raise RuntimeError("the packed weight must be a 2-D tensor [K / 8, N]")
+    if group not in (32, 64, 128):
+        raise RuntimeError(f"group must be 32, 64 or 128 (got {group})")
+    M, K = x.shape
+    if K % 8:
+        raise RuntimeError(f"K must be a multiple of 8 (got {K})")
+    return M, K, wq.shape[1]
+
+
+def q4_gemm_out(x, wq, scales, zeros=None, b=None, r=None, act="none", group=128, out=None):
+    """out[M,N] = act(x @ W + b), or x @ W + b + r, with W[k, n] = scales[k // group, n] *
+    (q[k, n] - zeros[k // group, n]) in 4 bits (gp_q4_gemm_out): wq int32 [K / 8, N], word [i, n]
+    holding q[8 i .. 8 i + 7, n], the lowest k in the lowest bits (gpipes.q4.pack); zeros None: 8.
+    group 32, 64 or 128; K a multiple of 8, any N; M from one token to whole prompts.  Every other
+    tensor float16, or every other tensor bfloat16.  act: a name of ACTS."""
+    dt = _dtype_of(x)
+    M, K, N = _q4_shape(x, wq, group, dt)
+    _check_q4(wq, scales, zeros, K, N, group, dt)
+    if b is not None and not _ok(b, (N,), dt):
+        _check_input("b", b, (N,), dt)
+    if r is not None and not _ok(r, (M, N), dt):
+        _check_input("r", r, (M, N), dt)
+    if out is None:
+        out = torch.empty((M, N), dtype=dt, device=x.device)
+    elif not _ok(out, (M, N), dt):
+        _check_input("out", out, (M, N), dt)
+    _same_device(x, wq, scales, zeros, b, r, out)
+    with _on(x):
+        rc = lib.gp_q4_gemm_out(M, N, K, group, x.data_ptr(), wq.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(b),
+                                _ptr(r), ACTS.get(act, act), out.data_ptr(), _DTYPES[dt], _stream(x))
+    if rc:
+        _check(rc)
+    return out
+
+
+def q4_gated_out(x, wq_g, scales_g, zeros_g, wq_u, scales_u, zeros_u, bg=None, bu=None, act="silu", group=128,
+                 out=None):
+    """out[M,N] = act(x @ Wg + bg) * (x @ Wu + bu), the first half of a gated feed-forward block, both
+    weights as q4_gemm_out's and of one shape (gp_q4_gated_out)."""
+    dt = _dtype_of(x)
+    M, K, N = _q4_shape(x, wq_g, group, dt)
+    _check_q4(wq_g, scales_g, zeros_g, K, N, group, dt, "_g")
+    _check_q4(wq_u, scales_u, zeros_u, K, N, group, dt, "_u")
+    for name, t in (("bg", bg), ("bu", bu)):
+        if t is not None and not _ok(t, (N,), dt):
+            _check_input(name, t, (N,), dt)
+    if out is None:
+        out = torch.empty((M, N), dtype=dt, device=x.device)
+    elif not _ok(out, (M, N), dt):
+        _check_input("out", out, (M, N), dt)
+    _same_device(x, wq_g, scales_g, zeros_g, wq_u, scales_u, zeros_u, bg, bu, out)
+    with _on(x):
+        rc = lib.gp_q4_gated_out(M, N, K, group, x.data_ptr(), wq_g.data_ptr(), scales_g.data_ptr(), _ptr(zeros_g),
+                                 _ptr(bg), wq_u.data_ptr(), scales_u.data_ptr(), _ptr(zeros_u), _ptr(bu),
+                                 ACTS.get(act, act), out.data_ptr(), _DTYPES[dt], _stream(x))
+    if rc:
+        _check(rc)
+    return out

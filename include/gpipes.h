@@ -564,6 +564,36 @@ int gp_residual_norm_out(int64_t M, int64_t D, const void* x, const void* y, int
                          float scale, int pre, const void* gamma, const void* beta, float eps, void* h, void* out,
                          int dtype, void* stream);
 
+/*
+ * Products with 4-bit weights, one token to whole prompts:
+ *   out[M,N] = act(x[M,K] W + b), or x W + b + r (act GP_ACT_NONE),
+ *   W[k][n] = scales[k / group][n] * (q[k][n] - zeros[k / group][n]).
+ * wq: [K / 8, N] 32-bit words, word [i][n] the 4-bit q[8 i .. 8 i + 7][n], the
+ * lowest k in the lowest bits.  scales, zeros: [ceil(K / group), N] of the
+ * element type, zeros NULL: 8; group 32, 64 or 128.  K a multiple of 8 up to
+ * 65536 (the last group may be short), N any up to 2^20, a weight below 2 GiB,
+ * M up to 2097152.  b [N], r [M,N] or NULL; act any GP_ACT_*.  Every tensor
+ * but wq `dtype`, every pointer 16-byte aligned.
+ * Weights are not rounded: products are exact, sums fp32, out rounded once.
+ * x has to be finite and, in bf16, 32 times a group's sum of |x| below fp32's
+ * largest number: a row of x that is not gives NaN in that row of out alone.
+ * One launch, no workspace: can be captured into a graph; out must not
+ * overlap x (it may be r).
+ * No counterpart in the reference (16-bit weights only).
+ */
+int gp_q4_gemm_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq, const void* scales,
+                   const void* zeros, const void* b, const void* r, int act, void* out, int dtype, void* stream);
+
+/*
+ * The first half of a gated feed-forward block:
+ *   out[M,N] = act(x Wg + b_g) * (x Wu + b_u),
+ * both weights as in gp_q4_gemm_out, of one shape and group.  The two products
+ * stay in fp32 until out.
+ */
+int gp_q4_gated_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq_g, const void* scales_g,
+                    const void* zeros_g, const void* b_g, const void* wq_u, const void* scales_u, const void* zeros_u,
+                    const void* b_u, int act, void* out, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

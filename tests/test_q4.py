@@ -1,0 +1,410 @@
+"""Products with 4-bit weights: q4_gemm_out and q4_gated_out, and gpipes.q4, which makes such weights.
+
+The refusals and gpipes.q4 need no GPU.  Results are compared with the formulas in 64 bits, to a
+bound from the arithmetic (product(), below), and as a whole: the error's norm may hardly be
+larger than that of the exact result rounded to the element type.
+"""
+import ctypes
+
+import pytest
+import torch
+
+import gpipes
+from gpipes import q4
+
+F16, BF16 = torch.float16, torch.bfloat16
+U = 2.0 ** -24
+
+
+# ---------------------------------------------------------------------------
+# Without a GPU
+# ---------------------------------------------------------------------------
+
+def _call(M=4, N=256, K=512, group=128, x=16, wq=16, s=16, z=0, b=0, r=0, act=0, out=32, dtype=0, two=False, u=16):
+    vp = ctypes.c_void_p
+    P = lambda v: vp(v) if v else None  # noqa: E731
+    if two:
+        return gpipes.lib.gp_q4_gated_out(M, N, K, group, P(x), P(wq), P(s), P(z), P(b), P(u), P(s), P(z), P(b), act,
+                                          P(out), dtype, None)
+    return gpipes.lib.gp_q4_gemm_out(M, N, K, group, P(x), P(wq), P(s), P(z), P(b), P(r), act, P(out), dtype, None)
+
+
+@pytest.mark.parametrize("two", [False, True])
+@pytest.mark.parametrize("kw,code", [
+    (dict(M=-1), -1), (dict(M=(1 << 21) + 1), -2), (dict(N=0), -2), (dict(N=(1 << 20) + 1), -2), (dict(K=0), -2),
+    (dict(K=12), -2), (dict(K=65544), -2), (dict(K=65536, N=65536), -2), (dict(group=16), -2), (dict(group=256), -2),
+    (dict(group=0), -2), (dict(dtype=2), -1), (dict(act=5), -1), (dict(act=-1), -1), (dict(x=0), -1), (dict(wq=0), -1),
+    (dict(s=0), -1), (dict(out=0), -1), (dict(x=24), -3), (dict(wq=20), -3), (dict(s=18), -3), (dict(z=8), -3),
+    (dict(b=2), -3), (dict(out=40), -3),
+])
+def test_argument_errors(kw, code, two):
+    assert _call(**kw, two=two) == code
+    assert gpipes.lib.gp_last_error().decode() != ""
+
+
+def test_argument_errors_of_one_form():
+    assert _call(r=16, act=1) == -1
+    assert _call(r=8) == -3
+    assert _call(u=0, two=True) == -1
+    assert _call(u=24, two=True) == -3
+
+
+def test_empty_batch_is_a_noop():
+    assert _call(M=0, x=0, out=0) == 0
+    assert _call(M=0, x=0, out=0, two=True) == 0
+    assert gpipes.lib.gp_last_error().decode() == ""
+
+
+def test_python_refuses():
+    x, wq, s = torch.zeros(1, 64, dtype=F16), torch.zeros(8, 32, dtype=torch.int32), torch.zeros(1, 32, dtype=F16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        gpipes.q4_gemm_out(x, wq, s)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        gpipes.q4_gated_out(x, wq, s, None, wq, s, None)
+
+
+def test_pack_and_unpack():
+    g = torch.Generator().manual_seed(0)
+    q = torch.randint(0, 16, (40, 13), generator=g)
+    wq = q4.pack(q)
+    assert wq.dtype == torch.int32 and wq.shape == (5, 13)
+    assert torch.equal(q4.unpack(wq).long(), q)
+    assert (int(wq[2, 3]) & 15, (int(wq[2, 3]) >> 28) & 15) == (int(q[16, 3]), int(q[23, 3]))
+    for bad in (q[:7], q - 1, q + 1):
+        with pytest.raises(RuntimeError):
+            q4.pack(bad)
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_quantize(group, zeros, dt):
+    """Off by half a step, and by what rounding the step to dt moves the ends by: seven or fifteen steps of a step that
+    is off by half of dt's eps; and a whole zero moves an end by up to half a step."""
+    g = torch.Generator().manual_seed(1)
+    w = (torch.randn(200, 17, generator=g) * 0.05 + 0.02).to(dt)
+    w[:, 3], w[:, 4], w[:, 5] = 0, 0.75, -0.5
+    wq, s, z = q4.quantize(w, group, zeros)
+    assert s.shape == (-(-200 // group), 17) and (z is None) == (not zeros)
+    step = s.double().repeat_interleave(group, 0)[:200]
+    got = q4.dequantize(wq, s, z, group).double()
+    assert ((got - w.double()).abs() <= step * (1.0 if zeros else 0.5) + step * 16 * torch.finfo(dt).eps).all()
+    assert (got[:, 3] == 0).all()
+
+
+def test_quantize_refuses():
+    w = torch.ones(16, 4, dtype=F16)
+    for bad, kw in ((w[:9], {}), (w.float(), {}), (w, dict(group=16)), (w * float("inf"), {})):
+        with pytest.raises(RuntimeError):
+            q4.quantize(bad, **kw)
+
+
+# ---------------------------------------------------------------------------
+# The formulas in 64 bits
+# ---------------------------------------------------------------------------
+
+def act64(v, act):
+    return {"none": v, "relu": v.clamp(min=0), "sigmoid": torch.sigmoid(v), "silu": v * torch.sigmoid(v),
+            "gelu_tanh": v * torch.sigmoid(2 * (2 / torch.pi) ** 0.5 * (v + 0.044715 * v ** 3))}[act]
+
+
+def weight(K, N, group, zeros, dt, gen):
+    q = torch.randint(0, 16, (K, N), generator=gen)
+    groups = -(-K // group)
+    s = ((0.3 + torch.rand(groups, N, generator=gen)) / (4.6 * K ** 0.5)).to(dt)
+    z = (torch.randint(0, 31, (groups, N), generator=gen) / 2).to(dt) if zeros else None
+    return q, s, z
+
+
+def product(x, q, s, z, group):
+    """x W, and a bound on the kernel's distance from it.  Products of x with 16 + q are exact; a group's sum of at
+    most 128 of them, and that of x, take sixteen roundings each at most (eight products a step), the running
+    sum one a group and one a wave, under 100 for what the tests use."""
+    x, q, s = x.double(), q.double(), s.double()
+    K = q.shape[0]
+    zz = z.double() if z is not None else torch.full_like(s, 8)
+    sr, zr = (t.repeat_interleave(group, 0)[:K] for t in (s, zz))
+    out = x @ (sr * (q - zr))
+    near = x.abs() @ (sr * (32 + q + zr))
+    run = torch.zeros_like(out)
+    for k in range(0, K, group):
+        run += (x[:, k:k + group] @ (sr * (q - zr))[k:k + group]).abs()
+    return out, 16 * U * near + 100 * U * run
+
+
+def moved(v, dv, act):
+    """act(v), and the bound on from where v is off by dv: no activation here is steeper than 1.13."""
+    a = act64(v, act)
+    return a, 1.13 * dv + 2.0 ** -20 * a.abs() + 2.0 ** -22 * v.abs() * (act not in ("none", "relu"))
+
+
+def check(got, want, bound, dt):
+    got = got.double().cpu()
+    half = torch.finfo(dt).eps / 2
+    tol = bound + (want.abs() + bound) * half + (2.0 ** -25 if dt == F16 else 0)
+    assert torch.isfinite(got).all()
+    over = (got - want).abs() / tol.clamp(min=1e-300)
+    assert over.max() <= 1, (over.max().item(), divmod(int(over.argmax()), got.shape[1]))
+    if got.numel() >= 256:  # errors that are half a step at most, spread evenly: those of fp32 add little to them
+        best = (want.to(dt).double() - want).norm()
+        assert (got - want).norm() <= 1.1 * best, ((got - want).norm() / want.norm(), best / want.norm())
+
+
+def dev(t, d):
+    return None if t is None else t.to(d)
+
+
+def run_gemm(M, K, N, group, zeros, dt, d, bias=False, residual=False, act="none", seed=0, x=None):
+    gen = torch.Generator().manual_seed(seed)
+    n = lambda *sh: torch.randn(*sh, generator=gen).to(dt)  # noqa: E731
+    x = n(M, K) if x is None else x
+    q, s, z = weight(K, N, group, zeros, dt, gen)
+    b, r = n(N) if bias else None, n(M, N) if residual else None
+    v, dv = product(x, q, s, z, group)
+    if bias:
+        v, dv = v + b.double(), dv + 2 * U * (v.abs() + b.double().abs())
+    v, dv = moved(v, dv, act)
+    if residual:
+        v, dv = v + r.double(), dv + 2 * U * (v.abs() + r.double().abs())
+    # what lies behind the last row stays as it was
+    buf = torch.full((M * N + 512,), 7.0, dtype=dt, device=d)
+    out = buf[:M * N].view(M, N)
+    got = gpipes.q4_gemm_out(dev(x, d), dev(q4.pack(q), d), dev(s, d), dev(z, d), dev(b, d), dev(r, d), act, group, out)
+    check(got, v, dv, dt)
+    assert (buf[M * N:] == 7).all()
+    return got
+
+
+def run_gated(M, K, N, group, zeros, dt, d, bias=False, act="silu", seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    n = lambda *sh: torch.randn(*sh, generator=gen).to(dt)  # noqa: E731
+    x = n(M, K)
+    sides, args, bs = [], [], []
+    for _ in range(2):
+        q, s, z = weight(K, N, group, zeros, dt, gen)
+        b = n(N) if bias else None
+        v, dv = product(x, q, s, z, group)
+        if bias:
+            v, dv = v + b.double(), dv + 2 * U * (v.abs() + b.double().abs())
+        sides.append((v, dv))
+        args += [dev(q4.pack(q), d), dev(s, d), dev(z, d)]
+        bs.append(dev(b, d))
+    g, dg = moved(*sides[0], act)
+    u, du = sides[1]
+    want, bound = g * u, dg * (u.abs() + du) + g.abs() * du + 2 * U * (g * u).abs()
+    buf = torch.full((M * N + 512,), 7.0, dtype=dt, device=d)
+    got = gpipes.q4_gated_out(dev(x, d), *args, bg=bs[0], bu=bs[1], act=act, group=group, out=buf[:M * N].view(M, N))
+    check(got, want, bound, dt)
+    assert (buf[M * N:] == 7).all()
+    return got
+
+
+ROWS = [1, 2, 3, 4, 5, 15, 16, 17, 31, 33, 48, 64, 65, 130, 255, 300]
+SHAPES = [(8, 1), (24, 3), (32, 16), (64, 61), (96, 64), (128, 128), (136, 65), (1000, 257), (2048, 512), (520, 1021)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", ROWS)
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_sizes(cuda, M, group):
+    for i, (K, N) in enumerate(SHAPES):
+        dt = (F16, BF16)[(i + M) % 2]
+        print(M, K, N, group, dt, flush=True)
+        run_gemm(M, K, N, group, i % 3 == 0, dt, cuda, bias=i % 2 == 0, residual=i % 4 == 1,
+                 act="none" if i % 4 == 1 else ("none", "relu", "gelu_tanh", "sigmoid", "silu")[i % 5], seed=i + M)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 4, 5, 20, 64, 200, 520])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_gated_sizes(cuda, M, dt):
+    for i, (K, N) in enumerate(SHAPES):
+        group = (32, 64, 128)[i % 3]
+        print(M, K, N, group, dt, flush=True)
+        run_gated(M, K, N, group, i % 2 == 0, dt, cuda, bias=i % 3 == 1,
+                  act=("silu", "gelu_tanh", "none", "relu", "sigmoid")[i % 5], seed=i + M)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,group,zeros", [
+    (1, 512, 8192, 64, True), (3, 256, 8209, 32, True), (2, 264, 16384, 128, False), (16, 128, 16411, 128, True),
+    (40, 384, 9001, 64, False), (1, 16384, 96, 128, True), (7, 16376, 40, 32, False), (70, 4096, 130, 64, True),
+    (1, 65536, 16, 128, False), (129, 8200, 260, 32, True), (1024, 256, 2048, 128, False), (2100, 136, 300, 64, True)])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_wide_and_deep(cuda, M, K, N, group, zeros, dt):
+    run_gemm(M, K, N, group, zeros, dt, cuda, bias=True, seed=N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(1, 1024, 16390), (4, 2048, 4100), (30, 512, 8192), (513, 1024, 1088)])
+def test_gated_wide(cuda, M, K, N):
+    run_gated(M, K, N, 128, True, BF16, cuda, bias=True, seed=N)
+    run_gated(M, K, N, 64, False, F16, cuda, act="gelu_tanh", seed=N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 3, 17, 64, 150, 300])
+def test_large_and_small_values_of_x(cuda, M):
+    """Rows far apart in size, zeros among them, and fp16's largest and smallest values."""
+    gen = torch.Generator().manual_seed(M)
+    for dt in (F16, BF16):
+        x = torch.randn(M, 640, generator=gen)
+        x *= 10.0 ** torch.randint(-3, 4, (M, 1), generator=gen)
+        x[M // 2, ::2] = 0
+        x = x.to(dt)
+        if M > 1:
+            x[0] = 0
+        run_gemm(M, 640, 144, 64, True, dt, cuda, seed=M, x=x / 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [2, 5, 40, 100, 300])
+def test_infinities_and_nans_stay_in_their_rows(cuda, M):
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(M, 512, generator=gen).to(BF16)
+    q, s, z = weight(512, 200, 64, True, BF16, gen)
+    args = [dev(t, cuda) for t in (q4.pack(q), s, z)]
+    clean = gpipes.q4_gemm_out(x.to(cuda), *args, group=64)
+    bad = x.clone()
+    bad[M // 2, 100], bad[M - 1, 511] = float("inf"), float("nan")
+    got = gpipes.q4_gemm_out(bad.to(cuda), *args, group=64)
+    rows = {M // 2, M - 1}
+    for m in range(M):
+        assert torch.isnan(got[m]).all() if m in rows else torch.equal(got[m], clean[m])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 16, 50, 200, 600])
+def test_rows_do_not_depend_on_their_neighbours(cuda, M):
+    """Two calls give the same bits, residual in place too."""
+    gen = torch.Generator().manual_seed(5)
+    x = torch.randn(M, 1024, generator=gen).to(F16).to(cuda)
+    q, s, z = weight(1024, 328, 128, True, F16, gen)
+    r = torch.randn(M, 328, generator=gen).to(F16).to(cuda)
+    args = [dev(t, cuda) for t in (q4.pack(q), s, z)]
+    a = gpipes.q4_gemm_out(x, *args, r=r)
+    b = r.clone()
+    gpipes.q4_gemm_out(x, *args, r=b, out=b)
+    assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_python_refusals(cuda):
+    gen = torch.Generator().manual_seed(6)
+    q, s, z = weight(256, 64, 64, True, F16, gen)
+    wq, s, z = q4.pack(q).to(cuda), s.to(cuda), z.to(cuda)
+    x = torch.zeros(3, 256, dtype=F16, device=cuda)
+    ok = dict(group=64)
+    for args, kw, what in (
+            ((x, wq, s, z), dict(group=128), "scales"), ((x, wq, s, z), dict(group=48), "group"),
+            ((x[:, :128].contiguous(), wq, s, z), ok, "wq"), ((x, wq.long(), s, z), ok, "int32"),
+            ((x, wq.t(), s, z), ok, "contiguous|shape"), ((x, wq, s.to(BF16), z), ok, "float16"),
+            ((x, wq, s, z[:2]), ok, "zeros"), ((x.t(), wq, s, z), ok, "contiguous"), ((x, wq, s, z, x), ok, "b must"),
+            ((x, wq, s, z, None, x), ok, "r must"), ((x[0], wq, s, z), ok, "2-D"), ((x.float(), wq, s, z), ok, "float16"),
+            ((x, wq, s, z), dict(group=64, out=x), "out"), ((x[:, :252].contiguous(), wq, s, z), ok, "multiple of 8"),
+            ((x, wq, s, z), dict(group=64, act=9), "activation")):
+        with pytest.raises(RuntimeError, match=what):
+            gpipes.q4_gemm_out(*args, **kw)
+    with pytest.raises(RuntimeError, match="_u"):
+        gpipes.q4_gated_out(x, wq, s, z, wq[:, :32].contiguous(), s, z, group=64)
+    assert gpipes.q4_gemm_out(x[:0], wq, s, z, group=64).shape == (0, 64)
+
+
+# ---------------------------------------------------------------------------
+# The operators together: the feed-forward half of a block, as a program runs it
+# ---------------------------------------------------------------------------
+
+def block64(x, y, p):
+    """x, y -> (h1, z1) after norm + residual, gated product, product, norm + residual, rounded where the kernels store."""
+    def rms(v, g):
+        return v / torch.sqrt((v * v).mean(1, keepdim=True) + 1e-5) * g
+    rnd = lambda t: t.to(p["dt"]).double()  # noqa: E731
+    d = lambda t: t.double()  # noqa: E731
+    h = d(x) + rms(d(y), d(p["g0"]))
+    z = rnd(rms(h, d(p["g1"])))
+    h = rnd(h)
+    w = [q4.dequantize(*p[k], group=64).double() for k in ("wg", "wu", "wd")]
+    a = z @ w[0]
+    a = rnd(a * torch.sigmoid(a) * (z @ w[1]))
+    f = rnd(a @ w[2])
+    h2 = h + 0.5 * rms(f, d(p["g2"]))
+    return rnd(h2), rnd(rms(h2, d(p["g3"])))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 12, 77, 260])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_block(cuda, M, dt):
+    """Eager, and captured into a graph that is replayed with other work between: the same bits each time, and close
+    to the block in 64 bits.  Three roundings to dt between input and output, each relative to its row (2^-8 and less
+    in bf16) and passed on by products whose outputs are sums of many such terms: as a whole off by a few half steps."""
+    H, FF = 512, 1088
+    gen = torch.Generator().manual_seed(M)
+    n = lambda *sh, m=0.0, k=1.0: (torch.randn(*sh, generator=gen) * k + m).to(dt)  # noqa: E731
+    p = {"dt": dt, **{k: n(H, m=1, k=0.1) for k in ("g0", "g1", "g2", "g3")}}
+    for k, a, b in (("wg", H, FF), ("wu", H, FF), ("wd", FF, H)):
+        p[k] = q4.quantize(n(a, b, k=a ** -0.5), 64, zeros=k == "wu")
+    c = {k: tuple(dev(t, cuda) for t in v) if isinstance(v, tuple) else v.to(cuda) for k, v in p.items() if k != "dt"}
+    x, y = n(M, H), n(M, H)
+    xc, yc = x.to(cuda), y.to(cuda)
+    bufs = {k: torch.empty(M, w, dtype=dt, device=cuda) for k, w in (("h", H), ("z", H), ("a", FF), ("f", H), ("h2", H), ("o", H))}
+
+    def step():
+        gpipes.residual_norm_out(xc, yc, post="rms", post_gamma=c["g0"], gamma=c["g1"], h=bufs["h"], out=bufs["z"])
+        gpipes.q4_gated_out(bufs["z"], *c["wg"], *c["wu"], group=64, out=bufs["a"])
+        gpipes.q4_gemm_out(bufs["a"], *c["wd"], group=64, out=bufs["f"])
+        gpipes.residual_norm_out(bufs["h"], bufs["f"], post="rms", post_gamma=c["g2"], scale=0.5, gamma=c["g3"],
+                                 h=bufs["h2"], out=bufs["o"])
+
+    def close():
+        want = block64(xc.cpu(), yc.cpu(), p)
+        for got, w in zip((bufs["h2"], bufs["o"]), want):
+            assert (got.double().cpu() - w).norm() / w.norm() <= 3 * torch.finfo(dt).eps / 2
+
+    step()
+    torch.cuda.synchronize()
+    close()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(3):
+        xc.copy_(n(M, H)), yc.copy_(n(M, H))
+        step()
+        eager = [bufs[k].clone() for k in ("h2", "o")]
+        for t in bufs.values():
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(bufs["h2"], eager[0]) and torch.equal(bufs["o"], eager[1])
+        close()
+
+
+@pytest.mark.gpu
+def test_two_streams_and_two_graphs(cuda):
+    """Calls on two streams at once, and two graphs replayed together: nothing is shared between them."""
+    gen = torch.Generator().manual_seed(8)
+    sets = []
+    for M in (1, 33):
+        q, s, z = weight(2048, 1024, 128, True, F16, gen)
+        x = torch.randn(M, 2048, generator=gen).to(F16).to(cuda)
+        args = [dev(t, cuda) for t in (q4.pack(q), s, z)]
+        out = torch.empty(M, 1024, dtype=F16, device=cuda)
+        want = gpipes.q4_gemm_out(x, *args)
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            for _ in range(20):
+                gpipes.q4_gemm_out(x, *args, out=out)
+        sets.append((x, args, out, want, g, torch.cuda.Stream(cuda)))
+    for _ in range(3):
+        for x, args, out, want, g, st in sets:
+            out.zero_()
+        torch.cuda.synchronize()
+        for x, args, out, want, g, st in sets:
+            with torch.cuda.stream(st):
+                g.replay()
+                gpipes.q4_gemm_out(x, *args, out=out)
+        torch.cuda.synchronize()
+        for x, args, out, want, g, st in sets:
+            assert torch.equal(out, want)
