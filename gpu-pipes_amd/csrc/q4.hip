@@ -16,6 +16,7 @@
 // in fp32, and times s into the running sum.  The weights are never rounded:
 // what is lost is a few bits of fp32 where the two sums cancel.
 #include <hip/hip_runtime.h>
+#include <type_traits>
 
 #include "../../include/gpipes.h"
 #include "gp_kernels.hpp"
@@ -24,8 +25,6 @@
 namespace gp {
 namespace {
 
-typedef unsigned short us4 __attribute__((ext_vector_type(4), aligned(2)));
-
 template <class T>
 struct Q4;
 template <>
@@ -33,6 +32,10 @@ struct Q4<F16> : F16 {
   static constexpr int kShift = 6;  // q to the top of fp16's ten mantissa bits
   static constexpr unsigned kMask = 0x03C003C0u, kBase = 0x4C004C00u;
   __device__ static f4 mma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+  // s + both halves of u
+  __device__ static float add2(unsigned u, float s) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, u), h2{(half_t)1.f, (half_t)1.f}, s, false);
+  }
 };
 template <>
 struct Q4<BF16> : BF16 {
@@ -41,19 +44,32 @@ struct Q4<BF16> : BF16 {
   __device__ static f4 mma16(h8 a, h8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
   }
+  __device__ static float add2(unsigned u, float s) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, u), bf2{(__bf16)1.f, (__bf16)1.f}, s, false);
+  }
 };
 
-// The operand 16 + q of a word, k order 0 4 1 5 2 6 3 7.
+// The mask and the base of an operand, in registers whose values the compiler
+// does not know: v_and_or_b32 takes no literals, and it would use two
+// instructions with them.
 template <class T>
-__device__ __forceinline__ h8 q4_operand(unsigned w) {
-  constexpr int s = Q4<T>::kShift;
-  u32x4 o;
-  o[0] = ((w << s) & Q4<T>::kMask) | Q4<T>::kBase;
-  o[1] = ((s >= 4 ? w << (s - 4) : w >> (4 - s)) & Q4<T>::kMask) | Q4<T>::kBase;
-  o[2] = ((w >> (8 - s)) & Q4<T>::kMask) | Q4<T>::kBase;
-  o[3] = ((w >> (12 - s)) & Q4<T>::kMask) | Q4<T>::kBase;
-  return __builtin_bit_cast(h8, o);
-}
+struct Q4Bits {
+  unsigned mask = Q4<T>::kMask, base = Q4<T>::kBase;
+  __device__ __forceinline__ Q4Bits() {
+    asm("" : "+s"(mask));
+    asm("" : "+v"(base));
+  }
+  // The operand 16 + q of a word, k order 0 4 1 5 2 6 3 7.
+  __device__ __forceinline__ h8 operand(unsigned w) const {
+    constexpr int s = Q4<T>::kShift;
+    u32x4 o;
+    o[0] = ((w << s) & mask) | base;
+    o[1] = ((s >= 4 ? w << (s - 4) : w >> (4 - s)) & mask) | base;
+    o[2] = ((w >> (8 - s)) & mask) | base;
+    o[3] = ((w >> (12 - s)) & mask) | base;
+    return __builtin_bit_cast(h8, o);
+  }
+};
 
 // Eight values of x in that order.
 __device__ __forceinline__ h8 x_operand(u32x4 v) {
@@ -76,34 +92,102 @@ __device__ __forceinline__ void q4_store(const Q4Args& p, int64_t m, int n, floa
   ((half_t*)p.out)[m * p.N + n] = T::cvt1(v);
 }
 
-constexpr int kChunk = 128;  // k that a wave loads at a time: four MFMA steps, one to four groups
+// Eight neighbouring outputs of row m from column n (cnt of them inside the row).
+template <class T>
+__device__ __forceinline__ void q4_store8(const Q4Args& p, int64_t m, int n, int cnt, float (&v)[8],
+                                          const float (&u)[8]) {
+  float t[8];
+  if (p.side[0].b) {
+    load8<T>((const half_t*)p.side[0].b + n, cnt, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += t[e];
+  }
+  if (p.act != GP_ACT_NONE) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = apply_act_ext(v[e], p.act);
+  }
+  if (p.sides == 2) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = 0.f;
+    if (p.side[1].b) load8<T>((const half_t*)p.side[1].b + n, cnt, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= u[e] + t[e];
+  }
+  if (p.r) {
+    load8<T>((const half_t*)p.r + m * p.N + n, cnt, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += t[e];
+  }
+  store8<T>((half_t*)p.out + m * p.N + n, cnt, v);
+}
+
+// Workgroup b of n, renumbered so that neighbours in the result run on one XCD
+// (b % 8): they read neighbouring columns, and 16 of them are half of a
+// 128-byte line, which two XCDs would each fetch whole.
+__device__ __forceinline__ int xcd_order(int b, int n) {
+  const int x = b & 7, i = b >> 3, q = n >> 3, rem = n & 7;
+  return x * q + (x < rem ? x : rem) + i;
+}
+
+// v has its value here: the compiler does not put off what it comes from (two
+// groups' sums at once would not fit the registers).
+__device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
+
+constexpr int kChunk = 128;  // k that a wave takes at a time, the largest group
+constexpr int kHalf = 64;    // k of a wave's one load: two MFMA steps
+
+// The scales (or zeros) of CW neighbouring columns as they lie in memory.  A
+// load that would pass the matrix's end begins CW values before it instead:
+// only columns of its last row can then be misplaced, and shifted() puts them
+// right.  No branch lies between the load and its first use.
+template <int CW>
+struct Cols {
+  typedef unsigned short vec __attribute__((ext_vector_type(CW), aligned(2)));
+  typedef typename std::conditional<CW == 4, unsigned long long, unsigned>::type bits;
+  bits v;
+  __device__ __forceinline__ void load(const unsigned short* m, int64_t at, int64_t last) {
+    const unsigned short* p = m + (at < last ? at : last);
+    if constexpr (CW == 1) v = *p;
+    if constexpr (CW == 2) v = __builtin_bit_cast(unsigned, *(const vec*)p);
+    if constexpr (CW == 4) v = __builtin_bit_cast(unsigned long long, *(const vec*)p);
+  }
+  __device__ __forceinline__ Cols shifted(int64_t at, int64_t last) const {
+    Cols r = *this;
+    if constexpr (CW > 1) r.v >>= at > last ? 16 * ((int)(at - last) & (CW - 1)) : 0;
+    return r;
+  }
+  template <class T>
+  __device__ __forceinline__ float val(int t) const {
+    return T::val(__builtin_bit_cast(half_t, (unsigned short)(v >> (16 * t))));
+  }
+};
 
 // ---------------------------------------------------------------------------
 // Few rows: every wave of a workgroup multiplies its share of k with the
 // workgroup's 16 CW columns, and the shares are joined through LDS in the
 // order of the waves.  With two weights, half of the waves take each.
 // ---------------------------------------------------------------------------
-template <int CW, int MT, int SPC>
-struct Chunk {
-  unsigned w[4][CW];
-  u32x4 x[4][MT];
-  unsigned short s[SPC][CW], z[SPC][CW];
+template <int CW, int MT, int SG>
+struct Half {
+  unsigned w[2][CW];
+  u32x4 x[2][MT];
+  Cols<CW> s[SG], z[SG];
 };
 
-template <class T, int CW, int MT, int G, bool FOUR>
+template <class T, int CW, int MT, int G, bool FOUR, int NB>
 __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void q4_rows_kernel(Q4Args p) {
-  constexpr int SPC = kChunk / G;        // groups a chunk
-  constexpr int SPG = G / 32;            // MFMA steps a group
-  constexpr int E = FOUR ? 1 : 4;        // accumulator elements that hold rows (FOUR: at most four rows)
+  constexpr int SG = G < kHalf ? kHalf / G : 1;  // groups a half (G 128: one every other half)
+  constexpr int E = FOUR ? 1 : 4;                // accumulator elements that hold rows (FOUR: at most four rows)
   constexpr int COLS = 16 * CW;
   constexpr int TOK = FOUR ? 4 : 16;
+  static_assert(NB % 2 == 0, "a buffer holds first halves or second halves");
   __shared__ float part[(MT == 1 ? 16 : 8) * TOK * COLS];
   const int lane = threadIdx.x & 63, j = lane & 15, lg = lane >> 4;
   const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per = waves / p.sides;  // waves a weight
   const int side = wave / per, wk = wave - side * per;
   const int N = p.N, K = p.K;
-  const int n0 = blockIdx.x * COLS;
+  const int n0 = xcd_order(blockIdx.x, gridDim.x) * COLS;
   const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
   const int rows = p.M - m0 < 16 * MT ? (int)(p.M - m0) : 16 * MT;
   const int groups = (K + G - 1) / G;
@@ -112,91 +196,118 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void q4_rows_kernel(Q4Args p)
   const auto wr = make_rsrc(sd.wq, (int)((int64_t)K * N / 2));
   const auto xr = make_rsrc((const half_t*)p.x + m0 * K, rows * K * 2);
   const unsigned short* sp = (const unsigned short*)sd.s;
-  const unsigned short* zp = (const unsigned short*)sd.z;
+  const unsigned short* zp = (const unsigned short*)(sd.z ? sd.z : sd.s);
   const int col = n0 + CW * j;
   const bool inside = n0 + COLS <= N;
+  const int64_t last = (int64_t)groups * N - CW;
   // Row i of the x operand: row i, or with at most four rows row i / 4, which
   // lands in element 0 of the accumulators of the lanes of group i / 4.
   const int xrow = FOUR ? j >> 2 : j;
 
-  auto load = [&](int c, Chunk<CW, MT, SPC>& q) {
+  // half t of this wave: chunks wk, wk + per, ..., two halves each
+  auto load = [&](int t, Half<CW, MT, SG>& q, bool second) {
+    const int k0 = (wk + (t >> 1) * per) * kChunk + (second ? kHalf : 0);
 #pragma unroll
-    for (int st = 0; st < 4; ++st) {
-      const int k8 = c * (kChunk / 8) + st * 4 + lg;
-      const int off = (int)(((unsigned)k8 * (unsigned)N + (unsigned)col) * 4u);  // past the weight's end: zeros
+    for (int st = 0; st < 2; ++st) {
+      const int k = k0 + st * 32 + lg * 8;
+      // past the weight's end and past the rows' end (and the last row) nothing is read: zeros, and a zero of x is
+      // what no word can make count
+      const unsigned off = k < K ? ((unsigned)(k >> 3) * (unsigned)N + (unsigned)col) * 4u : 0xFFFFFFE0u;
       if constexpr (CW == 4) {
-        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(wr, off, 0, 0);
-        for (int t = 0; t < 4; ++t) q.w[st][t] = v[t];
+        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(wr, (int)off, 0, 0);
+        for (int c = 0; c < 4; ++c) q.w[st][c] = v[c];
       } else if constexpr (CW == 2) {
-        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(wr, off, 0, 0);
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(wr, (int)off, 0, 0);
         q.w[st][0] = v[0], q.w[st][1] = v[1];
       } else {
-        q.w[st][0] = __builtin_amdgcn_raw_buffer_load_b32(wr, off, 0, 0);
+        q.w[st][0] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)off, 0, 0);
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        // past the row's end (and past the last row) nothing is read: zeros, which no word can make count
-        const int xo = ((mt * 16 + xrow) * K + k8 * 8) * 2;
-        q.x[st][mt] = __builtin_amdgcn_raw_buffer_load_b128(xr, k8 * 8 < K ? xo : 0x7FFFFFF0, 0, 0);
+        const int xo = ((mt * 16 + xrow) * K + k) * 2;
+        q.x[st][mt] = __builtin_amdgcn_raw_buffer_load_b128(xr, k < K ? xo : 0x7FFFFFE0, 0, 0);
       }
     }
+    if (G < kChunk || second) {
 #pragma unroll
-    for (int g = 0; g < SPC; ++g) {
-      const int gi = c * SPC + g < groups ? c * SPC + g : groups - 1;
-      const int64_t at = (int64_t)gi * N;
-#pragma unroll
-      for (int t = 0; t < CW; ++t) {
-        const int cc = inside || col + t < N ? col + t : N - 1;
-        q.s[g][t] = sp[at + cc];
-        q.z[g][t] = zp ? zp[at + cc] : 0;
+      for (int g = 0; g < SG; ++g) {
+        int gi = k0 / G + g;
+        gi = gi < groups ? gi : groups - 1;
+        const int64_t at = (int64_t)gi * N + col;
+        q.s[g].load(sp, at, last);
+        q.z[g].load(zp, at, last);
       }
     }
   };
 
+  const Q4Bits<T> bits;
   float tot[CW][MT][E] = {};
+  f4 acc[CW][MT], sum[MT];
   const h8 ones = __builtin_bit_cast(h8, u32x4{T::kOne * 0x10001u, T::kOne * 0x10001u, T::kOne * 0x10001u,
                                                T::kOne * 0x10001u});
-  auto mul = [&](const Chunk<CW, MT, SPC>& q) {
+  auto mul = [&](int h, const Half<CW, MT, SG>& q, bool second) {
 #pragma unroll
-    for (int g = 0; g < SPC; ++g) {
-      f4 acc[CW][MT] = {}, sum[MT] = {};
-#pragma unroll
-      for (int st = g * SPG; st < (g + 1) * SPG; ++st) {
-        h8 b[CW];
-#pragma unroll
-        for (int t = 0; t < CW; ++t) b[t] = q4_operand<T>(q.w[st][t]);
+    for (int st = 0; st < 2; ++st) {
+      const int k = (second ? kHalf : 0) + st * 32;
+      if (k % G == 0) {  // a group begins
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          const h8 a = x_operand(q.x[st][mt]);
-          sum[mt] = Q4<T>::mma16(a, ones, sum[mt]);
+          sum[mt] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int t = 0; t < CW; ++t) acc[t][mt] = Q4<T>::mma16(a, b[t], acc[t][mt]);
+          for (int t = 0; t < CW; ++t) acc[t][mt] = f4{0.f, 0.f, 0.f, 0.f};
         }
       }
+      h8 b[CW];
 #pragma unroll
-      for (int t = 0; t < CW; ++t) {
-        const float s = T::val(__builtin_bit_cast(half_t, q.s[g][t]));
-        const float z = zp ? 16.f + T::val(__builtin_bit_cast(half_t, q.z[g][t])) : 24.f;
+      for (int t = 0; t < CW; ++t) b[t] = bits.operand(q.w[st][t]);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt) {
+        const h8 a = x_operand(q.x[st][mt]);
+        sum[mt] = Q4<T>::mma16(a, ones, sum[mt]);
 #pragma unroll
-          for (int e = 0; e < E; ++e)
-            tot[t][mt][e] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[mt][e], acc[t][mt][e]), tot[t][mt][e]);
+        for (int t = 0; t < CW; ++t) acc[t][mt] = Q4<T>::mma16(a, b[t], acc[t][mt]);
       }
+      if ((k + 32) % G == 0) {  // and ends
+        const int g = G < kHalf ? st : 0;
+        Cols<CW> qs = q.s[g], qz = q.z[g];
+        if (!inside) {
+          int gi = (wk + (h >> 1) * per) * (kChunk / G) + k / G;
+          gi = gi < groups ? gi : groups - 1;
+          const int64_t at = (int64_t)gi * N + col;
+          qs = qs.shifted(at, last), qz = qz.shifted(at, last);
+        }
+#pragma unroll
+        for (int t = 0; t < CW; ++t) {
+          const float s = qs.template val<T>(t);
+          const float z = sd.z ? 16.f + qz.template val<T>(t) : 24.f;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              tot[t][mt][e] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[mt][e], acc[t][mt][e]), tot[t][mt][e]);
+              pin(tot[t][mt][e]);
+            }
+        }
+      }
+      // steps are not mixed: the compiler would spread their operands over more registers than there are
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  // wave wk of the weight's `per` takes chunks wk, wk + per, ..., the next one's loads under this one's products
-  Chunk<CW, MT, SPC> qa, qb;
-  int c = wk;
-  if (c < chunks) load(c, qa);
-  while (c < chunks) {
-    if (c + per < chunks) load(c + per, qb);
-    mul(qa);
-    if ((c += per) >= chunks) break;
-    if (c + per < chunks) load(c + per, qa);
-    mul(qb);
-    c += per;
+  // NB halves in flight.  Loads are issued without a condition, so that the
+  // compiler counts them: those past the wave's last chunk read nothing.
+  const int halves = wk < chunks ? 2 * ((chunks - 1 - wk) / per + 1) : 0;
+  Half<CW, MT, SG> q[NB];
+  if (halves) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) load(i, q[i], i & 1);
+    for (int t = 0; t < halves; t += NB) {
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        mul(t + i, q[i], i & 1);
+        load(t + NB + i, q[i], i & 1);
+      }
+    }
   }
 
 #pragma unroll
@@ -219,13 +330,479 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void q4_rows_kernel(Q4Args p)
   }
 }
 
-template <class T, int CW, int MT, bool FOUR>
+// ---------------------------------------------------------------------------
+// A token, or up to four.  Words come faster than 16-bit operands can be made
+// of them (eight operations a word), so here the operands are 8 bits: a byte
+// 0 .. 15 read as e4m3 is q 2^-9, denormal or not, and a word is two dwords of
+// such bytes, w and w >> 4 masked -- k in the order 0 2 4 6, 1 3 5 7.  x, in
+// chunks of 128 k, is written with four signed digits to the base 32, each a
+// whole number up to 16 that e4m3 holds: x = 2^e (d0 + d1 / 32 + d2 / 32^2 +
+// d3 / 32^3), 2^e such that the chunk's largest value has d0 in [8, 16].  That
+// is x to 2^-19 of the chunk's largest, the last bits of an fp32 sum.
+//
+// Whole numbers, because the 8-bit MFMAs add their products with fewer bits
+// than fp32: of products far apart in size they lose what is 2^-14 of the
+// largest (measured).  Those of a digit with q are whole and at most 240, so
+// nothing is lost, and the four digits' sums are added in fp32.
+//
+// Digit p of token m is row 4 m + p of the MFMA (16 x 16 x 128, whose scale
+// operand brings 2^e / 32^p), so a token's and column's digits are one lane's
+// accumulators.  A group shorter than 128 has an MFMA of its own, where the
+// other blocks of the weight go under 2^-127.
+//
+// Such a call is over in the time of a few memory latencies, and code that no
+// wave has run yet is fetched from memory too.  So all that the workgroup will
+// read is asked for first: x, the scales and kRing chunks of every wave's
+// words, the latter by copies into LDS that hold no registers; and the code
+// is short (rolled loops, no copy of it for a size of group).
+// ---------------------------------------------------------------------------
+constexpr int kTokenCols = 16;
+constexpr int kDigits = 4;
+constexpr int kRing = 2;  // chunks of 1 KiB that a wave has in flight
+
+// LDS, in this order: x's digits, rows of K bytes 16 bytes apart in banks; the
+// powers, a byte a chunk; every wave's ring; every wave's scales and zeros, 32
+// bytes a group, in copies of 256.
+struct TokenLds {
+  int xstride, powers, ring, scales, wave_scales, bytes;
+};
+inline TokenLds token_lds(int M, int K, int group, int waves, int kw, bool z) {
+  TokenLds l;
+  const int chunks = (K + kChunk - 1) / kChunk, cpw = (chunks + kw - 1) / kw;
+  l.xstride = (chunks * kChunk + 255) / 256 * 256 + 16;
+  l.powers = M * kDigits * l.xstride;
+  l.ring = (l.powers + M * chunks + 1023) / 1024 * 1024;
+  l.scales = l.ring + waves * kRing * 1024;
+  l.wave_scales = (cpw * (kChunk / group) + 7) / 8 * 256;
+  l.bytes = l.scales + waves * l.wave_scales * (z ? 2 : 1);
+  return l;
+}
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// Eight values of x, a sixteenth of a chunk (the others are in the lanes of
+// this row of sixteen): their digits to LDS rows 0 .. 3, the chunk's power.
+template <class T>
+__device__ __forceinline__ void put_digits(u32x4 v, GP_LDS char* at, int xstride, GP_LDS char* power, bool first) {
+  float x[8];
+  float top = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    x[2 * e] = T::val(__builtin_bit_cast(half_t, (unsigned short)(v[e] & 0xFFFF)));
+    x[2 * e + 1] = T::val(__builtin_bit_cast(half_t, (unsigned short)(v[e] >> 16)));
+    // the maximum drops a NaN, which stays one in its own digits
+    top = fmaxf(top, fmaxf(fabsf(x[2 * e]), fabsf(x[2 * e + 1])));
+  }
+#define GP_DPP_F(v, ctrl) __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), ctrl, 0xF, 0xF, false))
+  top = fmaxf(top, GP_DPP_F(top, 0x128));  // row_ror:8
+  top = fmaxf(top, GP_DPP_F(top, 0x124));  // row_ror:4
+  top = fmaxf(top, GP_DPP_F(top, 0x4E));
+  top = fmaxf(top, GP_DPP_F(top, 0xB1));
+#undef GP_DPP_F
+  // e, biased; not so small that the last digit's power would pass zero
+  int e = (__builtin_bit_cast(int, top) >> 23) - 3;
+  e = e < 20 ? 20 : e;
+  const float up = __builtin_bit_cast(float, (254 - e) << 23);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= up;
+#pragma unroll
+  for (int p = 0; p < kDigits; ++p) {
+    float d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      d[i] = __builtin_rintf(x[i]);
+      x[i] = (x[i] - d[i]) * 32.f;  // exact: at most 16
+    }
+    u32x2 o;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // even k, odd k
+      const int w = __builtin_amdgcn_cvt_pk_fp8_f32(d[h], d[2 + h], 0, false);
+      o[h] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(d[4 + h], d[6 + h], w, true);
+    }
+    *(GP_LDS u32x2*)(at + p * xstride) = o;
+  }
+  if (first) *power = (char)e;
+}
+
+// CT: tiles of 16 columns a workgroup; KW: waves along k.  Wave
+// (side CT + ct) KW + kw takes chunks [kw cpw, (kw + 1) cpw) of column tile ct
+// of weight `side`.
+template <class T>
+__global__ __launch_bounds__(1024) void q4_token_kernel(Q4Args p, int ctshift, int kwshift, int gshift, TokenLds l) {
+  __shared__ float part[16 * kTokenCols * 4];
+  GP_LDS char* lds = dyn_lds();
+  const int CT = 1 << ctshift, KW = 1 << kwshift;
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, lg = lane >> 4;
+  const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kw = wave & (KW - 1), tile = wave >> kwshift, ct = tile & (CT - 1), side = tile >> ctshift;
+  const int N = p.N, K = p.K, M = (int)p.M;
+  const int n0 = xcd_order(blockIdx.x, gridDim.x) * (kTokenCols * CT);
+  const int chunks = (K + kChunk - 1) / kChunk, cpw = (chunks + KW - 1) >> kwshift;
+  const int c0 = kw * cpw, nc = chunks - c0 < cpw ? chunks - c0 : cpw;  // may be 0 or less: nothing
+  const Q4Side sd = side ? p.side[1] : p.side[0];
+  const int tcol = n0 + ct * kTokenCols;  // the tile's first column
+
+  // Reads past the end of x's row, of the weight or of the scales bring zeros:
+  // a zero of x is what no word can make count.
+  // Scales: eight groups of 16 columns a copy, two columns a lane (N is even here).
+  GP_LDS char* sl = lds + l.scales + wave * l.wave_scales;
+  GP_LDS char* zl = sd.z ? sl + waves * l.wave_scales : sl;
+  const int g0 = (c0 * kChunk) >> gshift, gbytes = ((K + (1 << gshift) - 1) >> gshift) * N * 2;
+  const auto sr = make_rsrc(sd.s, gbytes), zr = make_rsrc(sd.z, gbytes);
+#pragma unroll 1
+  for (int i = 0; i < l.wave_scales / 256; ++i) {
+    const int off = ((g0 + i * 8 + (lane >> 3)) * N + tcol + 2 * (lane & 7)) * 2;
+    dma4_buf(sr, off, sl + i * 256);
+    if (sd.z) dma4_buf(zr, off, zl + i * 256);
+  }
+  // x: a thread has eight k, and the conversion waits for them
+  const int kend = chunks * kChunk;
+  u32x4 xv = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(p.x, K * 2), tid * 16, 0, 0);
+  // A chunk's copy: 16 word rows of 16 columns, 16 bytes a lane.  A lane of the
+  // MFMA's group lg holds k 16 lg .. + 15 of the chunk and of its second half,
+  // so its words are rows 2 lg, 2 lg + 1, 8 + 2 lg, 9 + 2 lg; word i of group lg
+  // lies at place 4 i + lg, where a wave's read of word i is 256 bytes in a row.
+  const auto wr = make_rsrc(sd.wq, (int)((int64_t)K * N / 2));
+  GP_LDS char* ring = lds + l.ring + wave * (kRing * 1024);
+  const int wrow = 2 * ((lane >> 2) & 3) + ((lane >> 4) & 1) + 8 * (lane >> 5);
+  unsigned woff = ((unsigned)(c0 * (kChunk / 8) + wrow) * (unsigned)N + (unsigned)(tcol + 4 * (lane & 3))) * 4u;
+  const unsigned wstep = (unsigned)N * (kChunk / 8 * 4);
+#pragma unroll
+  for (int i = 0; i < kRing; ++i, woff += wstep) dma16_buf(wr, (int)(i < nc ? woff : 0xFFFFFFE0u), ring + i * 1024);
+  wait_vmcnt<kRing>();  // this wave's scales, and its first part of x
+  auto put = [&](int m, int k) {
+    if (k < kend)  // rows of sixteen threads, a chunk each
+      put_digits<T>(xv, lds + m * kDigits * l.xstride + k, l.xstride, lds + l.powers + m * chunks + k / kChunk,
+                    !(tid & 15));
+  };
+  put(0, tid * 8);
+#pragma unroll 1
+  for (int m = 0, k0 = blockDim.x * 8; m < M; ++m, k0 = 0) {
+    const auto xr = make_rsrc((const half_t*)p.x + m * K, K * 2);
+#pragma unroll 1
+    for (; k0 < kend; k0 += blockDim.x * 8) {
+      xv = __builtin_amdgcn_raw_buffer_load_b128(xr, (k0 + tid * 8) * 2, 0, 0);
+      put(m, k0 + tid * 8);
+    }
+  }
+  lds_barrier();
+
+  // Row j of the A operand: token j / 4's digit j % 4 (past the last token another one's, whose sums go unread).
+  const int m = j >> 2 < M ? j >> 2 : M - 1;
+  GP_LDS const char* xl = lds + (m * kDigits + (j & 3)) * l.xstride + c0 * kChunk + lg * 16;
+  GP_LDS const char* pl = lds + l.powers + m * chunks + c0;
+  const i32x8 one = {0x01010101, 0x01010101, 0x01010101, 0x01010101, 0x01010101, 0x01010101, 0x01010101, 0x01010101};
+  const int ng = kChunk >> gshift, gb = (lg * 32) >> gshift;  // groups a chunk; the one of block lg, whose power this lane gives
+  float tot = 0.f;
+  int at = 0;
+#pragma unroll 1
+  for (int t = 0; t < nc; ++t) {
+    wait_vmcnt<kRing - 1>();
+    GP_LDS char* slot = ring + at * 1024;
+    at = at + 1 == kRing ? 0 : at + 1;
+    unsigned w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = *(GP_LDS const unsigned*)(slot + i * 256 + lg * 64 + j * 4);
+    const u32x4 a0 = *(GP_LDS const u32x4*)(xl + t * kChunk), a1 = *(GP_LDS const u32x4*)(xl + t * kChunk + 64);
+    const int pw = (int)*(GP_LDS const unsigned char*)(pl + t) - 5 * (j & 3);
+    // what was read is in registers before the slot takes the chunk kRing further on
+    compiler_fence();
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    dma16_buf(wr, (int)(t + kRing < nc ? woff : 0xFFFFFFE0u), slot);
+    woff += wstep;
+    i32x8 a, b;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = (int)a0[i], a[4 + i] = (int)a1[i];
+      b[2 * i] = (int)(w[i] & 0x0F0F0F0Fu), b[2 * i + 1] = (int)((w[i] >> 4) & 0x0F0F0F0Fu);
+    }
+#pragma unroll 1
+    for (int g = 0; g < ng; ++g) {
+      const f4 zero = {0.f, 0.f, 0.f, 0.f};
+      const int wp = gb == g ? 127 + 9 : 0;
+      const f4 d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, zero, 0, 0, 0, pw, 0, wp);
+      const f4 sum = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, one, zero, 0, 0, 0, pw, 0, wp);
+      const int sat = (t * ng + g) * 32 + j * 2;
+      const float s = T::val(*(GP_LDS const half_t*)(sl + sat));
+      const float zv = T::val(*(GP_LDS const half_t*)(zl + sat)), z = sd.z ? zv : 8.f;
+      const float v = (d[0] + d[1]) + (d[2] + d[3]), x = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tot = __builtin_fmaf(s, __builtin_fmaf(-z, x, v), tot);
+    }
+  }
+
+  // the waves of a column tile in their order
+  part[(wave * 4 + lg) * kTokenCols + j] = tot;
+  __syncthreads();
+  const int n = tid & (kTokenCols - 1), row = (tid / kTokenCols) & 3, tl = tid / (kTokenCols * 4);
+  if (tl < CT && row < M && n0 + tl * kTokenCols + n < N) {
+    float v = 0.f, u = 0.f;
+    const float* pv = part + (tl * KW * 4 + row) * kTokenCols + n;
+    for (int w = 0; w < KW; ++w) v += pv[w * 4 * kTokenCols];
+    if (p.sides == 2)
+      for (int w = 0; w < KW; ++w) u += pv[(CT * KW + w) * 4 * kTokenCols];
+    q4_store<T>(p, row, n0 + tl * kTokenCols + n, v, u);
+  }
+}
+
+template <class T>
+hipError_t token_launch(const Q4Args& a, int waves, int ct, int kw, const TokenLds& l, hipStream_t s) {
+  const auto kern = &q4_token_kernel<T>;
+  if (l.bytes > 60 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, l.bytes);
+    if (e != hipSuccess) return e;
+  }
+  const int cols = kTokenCols * ct;
+  const int gshift = a.group == 32 ? 5 : a.group == 64 ? 6 : 7;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((a.N + cols - 1) / cols)), dim3(waves * kWave), l.bytes, s, a,
+                     __builtin_ctz(ct), __builtin_ctz(kw), gshift, l);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Prompts: a workgroup of four waves computes 64 rows of 64 CW columns, a wave
+// 64 rows of 16 CW.  x goes through LDS, in the operands' order, with its
+// groups' sums; a wave takes its words from memory itself and makes operands
+// of each once for its four row tiles.  With two weights two waves take each,
+// the same 32 CW columns of both.
+// ---------------------------------------------------------------------------
+constexpr int kTileRows = 64;
+
+// Sum of eight 16-bit values.
+template <class T>
+__device__ __forceinline__ float sum8(h8 v) {
+  const u32x4 u = __builtin_bit_cast(u32x4, v);
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s = Q4<T>::add2(u[e], s);
+  return s;
+}
+
+// v + (v of the lane that the DPP control names), within sixteen lanes.
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+
+template <class T, int CW, int G, bool Z>
+__global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, int ntiles) {
+  constexpr int MT = kTileRows / 16;
+  constexpr int GPC = kChunk / G;  // groups a chunk
+  constexpr int SPG = G / 32;      // MFMA steps a group
+  constexpr int XB = kTileRows * kChunk * 2;
+  __shared__ __attribute__((aligned(1024))) struct {
+    char x[2][XB];
+    float s[2][GPC][kTileRows];
+  } lds;
+  auto& xs = lds.x;
+  auto& ss = lds.s;
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int N = p.N, K = p.K;
+  // Neighbours of one XCD take eight row tiles of a column tile, then of the
+  // next: 64 of them read eight tiles of x and eight of the weight.
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  const int gm0 = id / (8 * ntiles) * 8, rest = id % (8 * ntiles);
+  const int gm = mtiles - gm0 < 8 ? mtiles - gm0 : 8;
+  const int side = p.sides == 2 ? wave >> 1 : 0;
+  const int64_t m0 = (int64_t)(gm0 + rest % gm) * kTileRows;
+  const int wcols = 64 * CW / p.sides;
+  const int n0 = rest / gm * wcols, wn0 = n0 + (p.sides == 2 ? wave & 1 : wave) * (16 * CW);
+  const int col = wn0 + CW * j;
+  const int rows = p.M - m0 < kTileRows ? (int)(p.M - m0) : kTileRows;
+  const int groups = (K + G - 1) / G, chunks = (K + kChunk - 1) / kChunk;
+  const Q4Side sd = side ? p.side[1] : p.side[0];
+  const auto wr = make_rsrc(sd.wq, (int)((int64_t)K * N / 2));
+  const auto xr = make_rsrc((const half_t*)p.x + m0 * K, rows * K * 2);
+  const unsigned short* sp = (const unsigned short*)sd.s;
+  const unsigned short* zp = (const unsigned short*)(sd.z ? sd.z : sd.s);
+  const bool inside = wn0 + 16 * CW <= N;
+  const int64_t last = (int64_t)groups * N - CW;
+
+  // this thread's part of a chunk of x: eight k of rows tid / 16 + 16 q
+  const int xk = (tid & 15) * 8, xrow = tid >> 4;
+  u32x4 xv[MT];
+  unsigned wv[4][CW];
+  Cols<CW> sv[GPC], zv[GPC];
+  auto load_x = [&](int c) {
+    const int k = c * kChunk + xk;
+#pragma unroll
+    for (int q = 0; q < MT; ++q)
+      xv[q] = __builtin_amdgcn_raw_buffer_load_b128(xr, k < K ? ((xrow + 16 * q) * K + k) * 2 : 0x7FFFFFE0, 0, 0);
+  };
+  auto load_w = [&](int c) {
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      const unsigned off = ((unsigned)(c * (kChunk / 8) + st * 4 + lg) * (unsigned)N + (unsigned)col) * 4u;
+      if constexpr (CW == 4) {
+        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(wr, (int)off, 0, 0);
+        for (int t = 0; t < 4; ++t) wv[st][t] = v[t];
+      } else if constexpr (CW == 2) {
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(wr, (int)off, 0, 0);
+        wv[st][0] = v[0], wv[st][1] = v[1];
+      } else {
+        wv[st][0] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)off, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < GPC; ++g) {
+      const int gi = c * GPC + g < groups ? c * GPC + g : groups - 1;
+      sv[g].load(sp, (int64_t)gi * N + col, last);
+      if constexpr (Z) zv[g].load(zp, (int64_t)gi * N + col, last);
+    }
+  };
+  // 16-byte piece c of a row lies at c ^ row % 16: sixteen rows' reads of one piece fall into different banks
+  auto put_x = [&](int buf) {
+#pragma unroll
+    for (int q = 0; q < MT; ++q) {
+      const int row = xrow + 16 * q;
+      const h8 v = x_operand(xv[q]);
+      *(h8*)(xs[buf] + row * (kChunk * 2) + (((tid & 15) ^ (row & 15)) << 4)) = v;
+      float s = sum8<T>(v);
+      s = add_dpp<0xB1>(s);                       // quad_perm [1,0,3,2]
+      s = add_dpp<0x4E>(s);                       // quad_perm [2,3,0,1]
+      if constexpr (G >= 64) s = add_dpp<0x141>(s);   // row_half_mirror
+      if constexpr (G >= 128) s = add_dpp<0x140>(s);  // row_mirror
+      if ((tid & (G / 8 - 1)) == 0) ss[buf][(tid & 15) / (G / 8)][row] = Z ? -s : -24.f * s;
+    }
+  };
+
+  const Q4Bits<T> bits;
+  float tot[CW][MT][4] = {};
+  load_x(0);
+  load_w(0);
+  put_x(0);
+  __syncthreads();
+#pragma unroll 2
+  for (int c = 0; c < chunks; ++c) {
+    const int buf = c & 1;
+    unsigned w[4][CW];
+    Cols<CW> qs[GPC], qz[GPC];
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+#pragma unroll
+      for (int t = 0; t < CW; ++t) w[st][t] = wv[st][t];
+#pragma unroll
+    for (int g = 0; g < GPC; ++g) qs[g] = sv[g], qz[g] = zv[g];
+    if (!inside) {
+#pragma unroll
+      for (int g = 0; g < GPC; ++g) {
+        const int gi = c * GPC + g < groups ? c * GPC + g : groups - 1;
+        qs[g] = qs[g].shifted((int64_t)gi * N + col, last);
+        if constexpr (Z) qz[g] = qz[g].shifted((int64_t)gi * N + col, last);
+      }
+    }
+    if (c + 1 < chunks) {
+      load_x(c + 1);
+      load_w(c + 1);
+    }
+#pragma unroll
+    for (int g = 0; g < GPC; ++g) {
+      f4 acc[CW][MT];
+#pragma unroll
+      for (int st = g * SPG; st < (g + 1) * SPG; ++st) {
+        h8 b[CW];
+#pragma unroll
+        for (int t = 0; t < CW; ++t) b[t] = bits.operand(w[st][t]);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const h8 a = *(const h8*)(xs[buf] + (mt * 16 + j) * (kChunk * 2) + (((st * 4 + lg) ^ j) << 4));
+          if (st == g * SPG) {
+            // a group's sum begins at -(16 + z) times that of x
+            const f4 m = *(const f4*)&ss[buf][g][mt * 16 + 4 * lg];
+#pragma unroll
+            for (int t = 0; t < CW; ++t) {
+              const float z = sd.z ? 16.f + qz[g].template val<T>(t) : 24.f;
+              acc[t][mt] = Q4<T>::mma16(a, b[t], Z ? f4{z * m[0], z * m[1], z * m[2], z * m[3]} : m);
+            }
+          } else {
+#pragma unroll
+            for (int t = 0; t < CW; ++t) acc[t][mt] = Q4<T>::mma16(a, b[t], acc[t][mt]);
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < CW; ++t) {
+        const float s = qs[g].template val<T>(t);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            tot[t][mt][e] = __builtin_fmaf(s, acc[t][mt][e], tot[t][mt][e]);
+            if constexpr (GPC > 1) pin(tot[t][mt][e]);
+          }
+      }
+      if constexpr (GPC > 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    if (c + 1 < chunks) put_x(buf ^ 1);
+    __syncthreads();
+  }
+
+  // Out through LDS, half of the rows at a time: eight columns a thread, whole
+  // lines a wave, and the epilogue's code once.  Of two weights the columns lie
+  // side by side.
+  constexpr int TC = 64 * CW, LD = TC + 4;
+  static_assert((kTileRows / 2) * LD * 4 <= (int)sizeof(lds), "half a tile fits x's buffers");
+  float* tile = (float*)&lds;
+#pragma unroll 1
+  for (int half = 0; half < 2; ++half) {
+    auto put = [&](int mt) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float* at = tile + ((mt & 1) * 16 + 4 * lg + e) * LD + wave * (16 * CW) + CW * j;
+#pragma unroll
+        for (int t = 0; t < CW; ++t) at[t] = tot[t][mt][e];
+      }
+    };
+    if (half) {
+      put(2);
+      put(3);
+    } else {
+      put(0);
+      put(1);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < (kTileRows / 2) * (wcols / 8); i += 256) {
+      const int row = i / (wcols / 8), n = i % (wcols / 8) * 8;
+      if (half * (kTileRows / 2) + row >= rows || n0 + n >= N) continue;
+      float v[8], u[8];
+      const float* at = tile + row * LD + n;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = at[e], u[e] = p.sides == 2 ? at[wcols + e] : 0.f;
+      q4_store8<T>(p, m0 + half * (kTileRows / 2) + row, n0 + n, N - n0 - n, v, u);
+    }
+    __syncthreads();
+  }
+}
+
+template <class T, int CW>
+hipError_t tile_launch(const Q4Args& a, hipStream_t s) {
+  const int64_t mtiles = (a.M + kTileRows - 1) / kTileRows, cols = 64 * CW / a.sides, ntiles = (a.N + cols - 1) / cols;
+  if (mtiles * ntiles > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)(mtiles * ntiles)), block(256);
+  const bool z = a.side[0].z || a.side[1].z;
+#define GP_CASE(g)                                                                                                  \
+  case g:                                                                                                           \
+    if (z)                                                                                                          \
+      hipLaunchKernelGGL((q4_tile_kernel<T, CW, g, true>), grid, block, 0, s, a, (int)mtiles, (int)ntiles);         \
+    else                                                                                                            \
+      hipLaunchKernelGGL((q4_tile_kernel<T, CW, g, false>), grid, block, 0, s, a, (int)mtiles, (int)ntiles);        \
+    break;
+  switch (a.group) {
+    GP_CASE(32) GP_CASE(64) GP_CASE(128)
+    default: return hipErrorInvalidValue;
+  }
+#undef GP_CASE
+  return hipGetLastError();
+}
+
+template <class T, int CW, int MT, bool FOUR, int NB>
 hipError_t rows_launch(const Q4Args& a, int waves, dim3 grid, hipStream_t s) {
   const dim3 block(waves * kWave);
   switch (a.group) {
-    case 32: hipLaunchKernelGGL((q4_rows_kernel<T, CW, MT, 32, FOUR>), grid, block, 0, s, a); break;
-    case 64: hipLaunchKernelGGL((q4_rows_kernel<T, CW, MT, 64, FOUR>), grid, block, 0, s, a); break;
-    case 128: hipLaunchKernelGGL((q4_rows_kernel<T, CW, MT, 128, FOUR>), grid, block, 0, s, a); break;
+    case 32: hipLaunchKernelGGL((q4_rows_kernel<T, CW, MT, 32, FOUR, NB>), grid, block, 0, s, a); break;
+    case 64: hipLaunchKernelGGL((q4_rows_kernel<T, CW, MT, 64, FOUR, NB>), grid, block, 0, s, a); break;
+    case 128: hipLaunchKernelGGL((q4_rows_kernel<T, CW, MT, 128, FOUR, NB>), grid, block, 0, s, a); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
@@ -234,17 +811,38 @@ hipError_t rows_launch(const Q4Args& a, int waves, dim3 grid, hipStream_t s) {
 template <class T>
 hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
   const int chunks = (a.K + kChunk - 1) / kChunk;
-  const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+  if (a.M <= 4 && a.N % 2 == 0) {
+    int ct = a.N >= 64 * num_cus ? 4 : a.N >= 32 * num_cus ? 2 : 1;
+    int kw = 16 / (ct * a.sides);
+    while (kw > 1 && kw / 2 >= chunks) kw /= 2;
+    const int waves = kw * ct * a.sides;
+    const bool z = a.side[0].z || a.side[1].z;
+    const TokenLds l = token_lds((int)a.M, a.K, a.group, waves, kw, z);
+    if (l.bytes <= 155 * 1024) return token_launch<T>(a, waves, ct, kw, l, s);
+  }
+  if (a.M > 64) {
+    // The widest tiles that leave every CU the two workgroups that fit it: a
+    // wave's operands and its reads of x serve more columns.  509 x 1024 x
+    // 2 x 4096: 128 columns 21.7 us, 64 25.1, 256 24.0.
+    const int64_t mtiles = (a.M + kTileRows - 1) / kTileRows;
+    int cw = 4;
+    while (cw > 1 && mtiles * ((a.N + 64 * cw / a.sides - 1) / (64 * cw / a.sides)) < 2 * num_cus) cw /= 2;
+    if ((int64_t)((a.K + a.group - 1) / a.group) * a.N < 4) cw = 1;
+    return cw == 4 ? tile_launch<T, 4>(a, s) : cw == 2 ? tile_launch<T, 2>(a, s) : tile_launch<T, 1>(a, s);
+  }
+  const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : a.M <= 48 ? 3 : 4;
   int waves = mt == 1 ? 16 : 8;
   while (waves > 2 * a.sides && waves / 2 >= chunks * a.sides) waves /= 2;
-  const int cw = a.N >= 64 * num_cus ? 4 : a.N >= 32 * num_cus ? 2 : 1;
+  int cw = a.N >= 64 * num_cus ? 4 : a.N >= 32 * num_cus ? 2 : 1;
+  if ((int64_t)((a.K + a.group - 1) / a.group) * a.N < 4) cw = 1;
   const dim3 grid((unsigned)((a.N + 16 * cw - 1) / (16 * cw)), (unsigned)((a.M + 16 * mt - 1) / (16 * mt)));
-#define GP_CASE(c, m, four) \
-  if (cw == c && mt == m && (a.M <= 4) == four) return rows_launch<T, c, m, four>(a, waves, grid, s);
-  GP_CASE(1, 1, true) GP_CASE(2, 1, true) GP_CASE(4, 1, true)
-  GP_CASE(1, 1, false) GP_CASE(2, 1, false) GP_CASE(4, 1, false)
-  GP_CASE(1, 2, false) GP_CASE(2, 2, false) GP_CASE(4, 2, false)
-  GP_CASE(1, 4, false) GP_CASE(2, 4, false) GP_CASE(4, 4, false)
+#define GP_CASE(c, m, four, nb) \
+  if (cw == c && mt == m && (a.M <= 4) == four) return rows_launch<T, c, m, four, nb>(a, waves, grid, s);
+  GP_CASE(1, 1, true, 4) GP_CASE(2, 1, true, 4) GP_CASE(4, 1, true, 2)
+  GP_CASE(1, 1, false, 4) GP_CASE(2, 1, false, 2) GP_CASE(4, 1, false, 2)
+  GP_CASE(1, 2, false, 2) GP_CASE(2, 2, false, 2) GP_CASE(4, 2, false, 2)
+  GP_CASE(1, 3, false, 2) GP_CASE(2, 3, false, 2) GP_CASE(4, 3, false, 2)
+  GP_CASE(1, 4, false, 2) GP_CASE(2, 4, false, 2) GP_CASE(4, 4, false, 2)
 #undef GP_CASE
   return hipErrorInvalidValue;
 }

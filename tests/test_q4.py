@@ -119,17 +119,22 @@ def weight(K, N, group, zeros, dt, gen):
 def product(x, q, s, z, group):
     """x W, and a bound on the kernel's distance from it.  Products of x with 16 + q are exact; a group's sum of at
     most 128 of them, and that of x, take sixteen roundings each at most (eight products a step), the running
-    sum one a group and one a wave, under 100 for what the tests use."""
+    sum one a group and one a wave, under 100 for what the tests use.  Up to four rows may be taken in whole numbers
+    instead, each value to 2^-19 of the largest of its 128: 2^-19 of that largest times |W| a product."""
     x, q, s = x.double(), q.double(), s.double()
     K = q.shape[0]
     zz = z.double() if z is not None else torch.full_like(s, 8)
     sr, zr = (t.repeat_interleave(group, 0)[:K] for t in (s, zz))
     out = x @ (sr * (q - zr))
-    near = x.abs() @ (sr * (32 + q + zr))
+    near = 16 * U * (x.abs() @ (sr * (32 + q + zr)))
+    if x.shape[0] <= 4:
+        for k in range(0, K, 128):
+            top = x[:, k:k + 128].abs().amax(1, keepdim=True)
+            near += 2.0 ** -19 * top * (sr * (q - zr)).abs()[k:k + 128].sum(0)
     run = torch.zeros_like(out)
     for k in range(0, K, group):
         run += (x[:, k:k + group] @ (sr * (q - zr))[k:k + group]).abs()
-    return out, 16 * U * near + 100 * U * run
+    return out, near + 100 * U * run
 
 
 def moved(v, dv, act):
@@ -229,7 +234,7 @@ def test_gated_sizes(cuda, M, dt):
 @pytest.mark.parametrize("M,K,N,group,zeros", [
     (1, 512, 8192, 64, True), (3, 256, 8209, 32, True), (2, 264, 16384, 128, False), (16, 128, 16411, 128, True),
     (40, 384, 9001, 64, False), (1, 16384, 96, 128, True), (7, 16376, 40, 32, False), (70, 4096, 130, 64, True),
-    (1, 65536, 16, 128, False), (129, 8200, 260, 32, True), (1024, 256, 2048, 128, False), (2100, 136, 300, 64, True)])
+    (1, 65536, 16, 128, False), (4, 16384, 50, 64, True), (4, 15000, 33, 32, False), (3, 65536, 20, 128, True), (129, 8200, 260, 32, True), (1024, 256, 2048, 128, False), (2100, 136, 300, 64, True)])
 @pytest.mark.parametrize("dt", [F16, BF16])
 def test_wide_and_deep(cuda, M, K, N, group, zeros, dt):
     run_gemm(M, K, N, group, zeros, dt, cuda, bias=True, seed=N)
@@ -240,6 +245,20 @@ def test_wide_and_deep(cuda, M, K, N, group, zeros, dt):
 def test_gated_wide(cuda, M, K, N):
     run_gated(M, K, N, 128, True, BF16, cuda, bias=True, seed=N)
     run_gated(M, K, N, 64, False, F16, cuda, act="gelu_tanh", seed=N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 2, 9, 40, 130])
+def test_gated_with_zeros_on_one_side(cuda, M):
+    gen = torch.Generator().manual_seed(M)
+    x = torch.randn(M, 512, generator=gen).to(F16)
+    (qg, sg, zg), (qu, su, _) = (weight(512, 192, 64, True, F16, gen) for _ in range(2))
+    for a, b in ((zg, None), (None, zg)):
+        g, dg = moved(*product(x, qg, sg, a, 64), "silu")
+        u, du = product(x, qu, su, b, 64)
+        got = gpipes.q4_gated_out(x.to(cuda), q4.pack(qg).to(cuda), sg.to(cuda), dev(a, cuda), q4.pack(qu).to(cuda),
+                                  su.to(cuda), dev(b, cuda), group=64)
+        check(got, g * u, dg * (u.abs() + du) + g.abs() * du + 2 * U * (g * u).abs(), F16)
 
 
 @pytest.mark.gpu
@@ -255,6 +274,17 @@ def test_large_and_small_values_of_x(cuda, M):
         if M > 1:
             x[0] = 0
         run_gemm(M, 640, 144, 64, True, dt, cuda, seed=M, x=x / 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 4, 16, 64, 200])
+def test_outlying_channels(cuda, M):
+    """A few channels a thousand times as large as the others, as activations have them."""
+    gen = torch.Generator().manual_seed(M)
+    x = torch.randn(M, 1024, generator=gen)
+    x[:, [3, 500, 1000]] *= 1000
+    for dt in (F16, BF16):
+        run_gemm(M, 1024, 256, 128, True, dt, cuda, seed=M, x=x.to(dt))
 
 
 @pytest.mark.gpu
