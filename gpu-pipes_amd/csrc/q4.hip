@@ -102,10 +102,7 @@ __device__ __forceinline__ void q4_store8(const Q4Args& p, int64_t m, int n, int
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += t[e];
   }
-  if (p.act != GP_ACT_NONE) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = apply_act_ext(v[e], p.act);
-  }
+  apply_act8(v, p.act);
   if (p.sides == 2) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = 0.f;

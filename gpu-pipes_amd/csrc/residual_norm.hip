@@ -38,43 +38,48 @@ typedef Part Parts[2][2][kMaxWaves];
 // registers give the wave's own mean and squared distances; the waves' parts
 // are joined through LDS by the rule for joining two sets,
 // M2 = sum(m2) + sum(n (mean_w - mean)^2), one barrier for a norm.  Sums and
-// statistics are in 32 bits throughout.
-template <int C>
-__device__ __forceinline__ void row_stats(const float (&v)[C][8], const int (&nv)[C], int kind, int64_t D, int W, int w,
+// statistics are in 32 bits throughout.  TAIL: a piece of eight may be cut short.
+template <int C, bool TAIL>
+__device__ __forceinline__ void row_stats(const float (&v)[C][8], const int (&nv)[C], int kind, int D, int W, int w,
                                           float eps, Part* parts, float& mean, float& rstd) {
   Part p{0.f, 0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < C; ++j) {
-    const int64_t left = D - (int64_t)(j * W + w) * kPiece;
-    p.n += (float)(left < 0 ? 0 : left > kPiece ? kPiece : left);
-  }
   if (kind == GP_NORM_LAYER) {
+    int n = 0;
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < C; ++j)
+    for (int j = 0; j < C; ++j) {
+      const int left = D - (j * W + w) * kPiece;
+      n += left < 0 ? 0 : left > kPiece ? kPiece : left;
 #pragma unroll
       for (int e = 0; e < 8; ++e) s += v[j][e];  // values past the row's end are zeros
-    p.mean = p.n > 0.f ? sum_lanes<64>(s) / p.n : 0.f;
+    }
+    p.n = (float)n;
+    p.mean = n > 0 ? sum_lanes<64>(s) / p.n : 0.f;
   }
   float q = 0.f;
 #pragma unroll
-  for (int j = 0; j < C; ++j)
+  for (int j = 0; j < C; ++j) {
+    if (nv[j] <= 0) continue;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float d = e < nv[j] ? v[j][e] - p.mean : 0.f;
+      const float d = !TAIL || e < nv[j] ? v[j][e] - p.mean : 0.f;
       q = __builtin_fmaf(d, d, q);
     }
+  }
   p.m2 = sum_lanes<64>(q);
   if (W > 1) {
     const int lane = threadIdx.x & 63, wb = threadIdx.x >> 6;
     if (lane == 0) parts[wb] = p;
-    __syncthreads();
+    lds_barrier();
     const int i = lane & 15;
     p = Part{0.f, 0.f, 0.f};
     if (i < W) p = parts[wb - w + i];
-    const float m = sum_lanes<16>(p.n * p.mean) / (float)D;
-    p.m2 = sum_lanes<16>(__builtin_fmaf(p.n * (p.mean - m), p.mean - m, p.m2));
-    p.mean = m;
+    if (kind == GP_NORM_LAYER) {
+      const float m = sum_lanes<16>(p.n * p.mean) / (float)D;
+      p.m2 = __builtin_fmaf(p.n * (p.mean - m), p.mean - m, p.m2);
+      p.mean = m;
+    }
+    p.m2 = sum_lanes<16>(p.m2);
   }
   mean = p.mean;
   // a precise division and root: once a row, and rsq's last bit would scale every value
@@ -84,75 +89,115 @@ __device__ __forceinline__ void row_stats(const float (&v)[C][8], const int (&nv
 struct Args {
   ResidualNormArgs a;
   int W;          // waves a row
+  int64_t rows;   // consecutive rows a team of W waves takes
   int64_t per;    // rows that share a gate row
 };
 
-// (v - mean) rstd gamma + beta over this thread's values.
+// A vector over the channels as this thread's lanes need it, in its 16 bits.
+template <int C, bool BACK>
+__device__ __forceinline__ void load_channels(u32x4 (&u)[C], const half_t* p, const int (&at)[C], const int (&nv)[C],
+                                              unsigned none) {
+#pragma unroll
+  for (int j = 0; j < C; ++j) u[j] = p ? load_raw8<BACK>(p + at[j], nv[j]) : u32x4{none, none, none, none};
+}
+
+// (v - mean) rstd gamma + beta over this thread's values (those past the row's end: anything).
 template <class T, int C>
-__device__ __forceinline__ void affine(float (&v)[C][8], const int (&nv)[C], const int (&at)[C], float mean, float rstd,
-                                       const void* gamma, const void* beta) {
+__device__ __forceinline__ void affine(float (&v)[C][8], float mean, float rstd, const u32x4 (&gamma)[C],
+                                       const u32x4 (&beta)[C], bool add) {
 #pragma unroll
   for (int j = 0; j < C; ++j) {
-    float g[8], b[8];
-    if (gamma) load8<T>((const half_t*)gamma + at[j], nv[j], g);
-    if (beta) load8<T>((const half_t*)beta + at[j], nv[j], b);
+    float g[8];
+    widen8<T>(gamma[j], g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float u = (v[j][e] - mean) * rstd;
-      u = __builtin_fmaf(u, gamma ? g[e] : 1.f, beta ? b[e] : 0.f);
-      v[j][e] = e < nv[j] ? u : 0.f;
-    }
+    for (int e = 0; e < 8; ++e) v[j][e] = (v[j][e] - mean) * rstd * g[e];
+  }
+  if (!add) return;
+#pragma unroll
+  for (int j = 0; j < C; ++j) {
+    float b[8];
+    widen8<T>(beta[j], b);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[j][e] += b[e];
   }
 }
 
-template <class T, int C, int BLOCK>
+// TAIL: D is no multiple of eight; BACK: and above eight, so that a cut piece
+// has its row's values before it.
+//
+// A team takes consecutive rows: what belongs to the channels is loaded once,
+// before the first row (so that one row's call waits for memory once), and a
+// gate row's activation is computed once for the rows that share it.
+template <class T, int C, int BLOCK, bool TAIL, bool BACK>
 __global__ __launch_bounds__(BLOCK) void residual_norm_kernel(Args p) {
   __shared__ Parts parts;
   const ResidualNormArgs& a = p.a;
-  const int lane = threadIdx.x & 63, wb = threadIdx.x >> 6;
-  const int W = p.W, w = wb % W, team = wb / W, teams = BLOCK / kWave / W;
+  const int lane = threadIdx.x & 63, wb = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int W = p.W, w = wb & (W - 1), team = wb / W, teams = BLOCK / kWave / W, D = (int)a.D;
+  const half_t *ax = (const half_t*)a.x, *ay = (const half_t*)a.y, *ag = (const half_t*)a.gate;
   int at[C], nv[C];
 #pragma unroll
   for (int j = 0; j < C; ++j) {
     at[j] = (j * W + w) * kPiece + lane * 8;
-    const int64_t left = a.D - at[j];
-    nv[j] = left < 0 ? 0 : left > 8 ? 8 : (int)left;
+    const int left = D - at[j];
+    nv[j] = left < 0 ? 0 : left > 8 ? 8 : left;
   }
-  int par = 0;
+  const int64_t first = ((int64_t)blockIdx.x * teams + team) * p.rows;
+  const unsigned one = T::kOne * 0x10001u;
+  u32x4 qg[C], qb[C], rg[C], rb[C];
+  load_channels<C, BACK>(qg, (const half_t*)a.post_gamma, at, nv, one);
+  load_channels<C, BACK>(qb, (const half_t*)a.post_beta, at, nv, 0);
+  load_channels<C, BACK>(rg, (const half_t*)a.gamma, at, nv, one);
+  load_channels<C, BACK>(rb, (const half_t*)a.beta, at, nv, 0);
+  // the gate row in hand, and the first row that it no longer serves
+  float g[C][8];
+  int64_t grow = ag ? first / p.per : 0, gend = 0;
   // the whole workgroup walks the rows together: every wave takes every barrier
-  for (int64_t r0 = (int64_t)blockIdx.x * teams; r0 < a.M; r0 += (int64_t)gridDim.x * teams, par ^= 1) {
-    const int64_t row = r0 + team;
-    const bool live = row < a.M;
-    const int64_t base = (live ? row : a.M - 1) * a.D;
+  for (int64_t i = 0; i < p.rows; ++i) {
+    const bool live = first + i < a.M;
+    const int64_t row = live ? first + i : a.M - 1, base = row * D;
     float v[C][8];
-    if (a.y) {
-      float x[C][8];
+    if (ay) {
+      u32x4 x[C], y[C];
 #pragma unroll
-      for (int j = 0; j < C; ++j) load8<T>((const half_t*)a.y + base + at[j], nv[j], v[j]);
+      for (int j = 0; j < C; ++j) y[j] = load_raw8<BACK>(ay + base + at[j], nv[j]);
 #pragma unroll
-      for (int j = 0; j < C; ++j) load8<T>((const half_t*)a.x + base + at[j], nv[j], x[j]);
-      if (a.post != GP_NORM_NONE) {
-        float mean, rstd;
-        row_stats<C>(v, nv, a.post, a.D, W, w, a.post_eps, parts[par][0], mean, rstd);
-        affine<T, C>(v, nv, at, mean, rstd, a.post_gamma, a.post_beta);
-      }
-      if (a.gate) {
-        const int64_t gb = (live ? row : a.M - 1) / p.per * a.D;
+      for (int j = 0; j < C; ++j) x[j] = load_raw8<BACK>(ax + base + at[j], nv[j]);
+      if (ag && live && row >= gend) {
+        if (i) ++grow;
+        gend = (grow + 1) * p.per;
 #pragma unroll
         for (int j = 0; j < C; ++j) {
-          float g[8];
-          load8<T>((const half_t*)a.gate + gb + at[j], nv[j], g);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[j][e] *= apply_act_ext(g[e], a.gate_act);
+          load8<T, BACK>(ag + grow * D + at[j], nv[j], g[j]);
+          apply_act8(g[j], a.gate_act);
         }
       }
 #pragma unroll
-      for (int j = 0; j < C; ++j)
+      for (int j = 0; j < C; ++j) widen8<T>(y[j], v[j]);
+      if (a.post != GP_NORM_NONE) {
+        float mean, rstd;
+        row_stats<C, TAIL>(v, nv, a.post, D, W, w, a.post_eps, parts[i & 1][0], mean, rstd);
+        affine<T, C>(v, mean, rstd, qg, qb, a.post_beta != nullptr);
+      }
+      if (ag) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] = e < nv[j] ? __builtin_fmaf(a.scale, v[j][e], x[j][e]) : 0.f;
+        for (int j = 0; j < C; ++j)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j][e] *= g[j][e];
+      }
+#pragma unroll
+      for (int j = 0; j < C; ++j) {
+        float f[8];
+        widen8<T>(x[j], f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float h = __builtin_fmaf(a.scale, v[j][e], f[e]);
+          v[j][e] = (TAIL ? e < nv[j] : nv[j] > 0) ? h : 0.f;
+        }
+      }
     } else {
 #pragma unroll
-      for (int j = 0; j < C; ++j) load8<T>((const half_t*)a.x + base + at[j], nv[j], v[j]);
+      for (int j = 0; j < C; ++j) load8<T, BACK>(ax + base + at[j], nv[j], v[j]);
     }
     if (a.h && live) {
 #pragma unroll
@@ -162,8 +207,8 @@ __global__ __launch_bounds__(BLOCK) void residual_norm_kernel(Args p) {
     // has then one rounding, its own
     if (a.pre != GP_NORM_NONE) {
       float mean, rstd;
-      row_stats<C>(v, nv, a.pre, a.D, W, w, a.eps, parts[par][1], mean, rstd);
-      affine<T, C>(v, nv, at, mean, rstd, a.gamma, a.beta);
+      row_stats<C, TAIL>(v, nv, a.pre, D, W, w, a.eps, parts[i & 1][1], mean, rstd);
+      affine<T, C>(v, mean, rstd, rg, rb, a.beta != nullptr);
       if (live) {
 #pragma unroll
         for (int j = 0; j < C; ++j) store8<T>((half_t*)a.out + base + at[j], nv[j], v[j]);
@@ -172,34 +217,52 @@ __global__ __launch_bounds__(BLOCK) void residual_norm_kernel(Args p) {
   }
 }
 
-template <class T>
+template <class T, bool TAIL, bool BACK>
 hipError_t launch(const Args& p, int C, int block, unsigned grid, hipStream_t s) {
-#define GP_CASE(c, b)                                                                                \
-  if (C <= c && block == b) {                                                                        \
-    hipLaunchKernelGGL((residual_norm_kernel<T, c, b>), dim3(grid), dim3(b), 0, s, p);               \
-    return hipGetLastError();                                                                        \
+#define GP_CASE(c, b)                                                                                  \
+  if (C <= c && block == b) {                                                                          \
+    hipLaunchKernelGGL((residual_norm_kernel<T, c, b, TAIL, BACK>), dim3(grid), dim3(b), 0, s, p);     \
+    return hipGetLastError();                                                                          \
   }
-  GP_CASE(1, 256) GP_CASE(2, 256) GP_CASE(4, 256)
-  GP_CASE(1, 512) GP_CASE(2, 512) GP_CASE(4, 512)
-  GP_CASE(1, 1024) GP_CASE(2, 1024) GP_CASE(4, 1024)
+  // rows above 16,384 values only have more than two pieces a wave
+  GP_CASE(1, 256) GP_CASE(2, 256) GP_CASE(1, 512) GP_CASE(2, 512) GP_CASE(1, 1024) GP_CASE(2, 1024) GP_CASE(4, 1024)
 #undef GP_CASE
   return hipErrorInvalidValue;
+}
+
+template <class T>
+hipError_t by_tail(const Args& p, int C, int block, unsigned grid, hipStream_t s) {
+  if (p.a.D % 8 == 0) return launch<T, false, false>(p, C, block, grid, s);
+  if (p.a.D > 8) return launch<T, true, true>(p, C, block, grid, s);
+  hipLaunchKernelGGL((residual_norm_kernel<T, 1, 256, true, false>), dim3(grid), dim3(256), 0, s, p);
+  return hipGetLastError();
 }
 
 }  // namespace
 
 hipError_t residual_norm_launch(const ResidualNormArgs& a, int num_cus, hipStream_t s) {
   const int pieces = (int)((a.D + kPiece - 1) / kPiece);
+  // Waves a row: two pieces each where rows are many (16,384 x 4,096: four waves
+  // 103 us, eight 111, two 133; 16,288 x 1,021: one 47, two 47), one piece where
+  // rows leave CUs without work (one row of 4,096: eight waves 3.6 us, four 4.3;
+  // 128 rows of 8,192: sixteen 6.0, eight 6.8).
   int W = 1;
-  while (W < kMaxWaves && pieces > 4 * W) W *= 2;
+  while (W < kMaxWaves && pieces > 2 * W) W *= 2;
+  if (a.M * W < 8 * num_cus)
+    while (W < kMaxWaves && pieces > W) W *= 2;
   const int C = (pieces + W - 1) / W;
   const int block = W <= 4 ? 256 : W * kWave;
   const int64_t teams = block / kWave / W;
-  const int64_t groups = (a.M + teams - 1) / teams;
-  const int64_t most = (int64_t)num_cus * (2048 / block);
-  const Args p{a, W, a.gate ? a.M / a.gate_rows : 1};
-  const unsigned grid = (unsigned)(groups < most ? groups : most);
-  return a.dtype == GP_DTYPE_BF16 ? launch<BF16>(p, C, block, grid, s) : launch<F16>(p, C, block, grid, s);
+  // Up to four rows a team, so that what belongs to the channels is loaded once
+  // for them, but not so many that workgroups get fewer than four a CU
+  // (16,384 x 4,096: four rows 103 us, two 112, sixteen 125).
+  const int64_t groups = (a.M + teams - 1) / teams, most = (groups + 4 * num_cus - 1) / (4 * num_cus);
+  const int64_t rows = most < 4 ? most : 4;
+  const int64_t grid = (a.M + teams * rows - 1) / (teams * rows);
+  if (grid > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
+  const Args p{a, W, rows, a.gate ? a.M / a.gate_rows : 1};
+  return a.dtype == GP_DTYPE_BF16 ? by_tail<BF16>(p, C, block, (unsigned)grid, s)
+                                  : by_tail<F16>(p, C, block, (unsigned)grid, s);
 }
 
 }  // namespace gp

@@ -907,44 +907,78 @@ def residual_norm_out(x, y=None, gate=None, gate_act="none", scale=1.0, post="no
                           out)
 
 
-def _residual_norm(x, y, gate, gate_act, scale, post, post_gamma, post_beta, post_eps, norm, gamma, beta, eps, h, out):
+# These calls run for a few microseconds on one token, no longer than their host
+# side: a tensor is checked in one expression (a device index of -1 is a CPU
+# tensor's, so one comparison says both that a tensor is on a GPU and on x's),
+# and the slow path is taken only to say what is wrong.
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _fits(t, shape, dtype, dev):
+    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == dev
+            and t.is_contiguous())
+
+
+def _refuse(name, t, shape, dtype):
+    """Raises for a tensor that _fits() refused."""
+    _check_input(name, t, shape, dtype)
+    raise RuntimeError("all tensors must be on the same device")
+
+
+def _run_on(dev, fn, args):
+    """fn(*args, current stream of device dev) with that device current."""
+    if _raw_stream is not None and _current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        _check(rc)
+
+
+def _rows_of(x):
+    """(element type, rows, columns, device index) of a call's x."""
     dt = _dtype_of(x)
     if not _ok(x, None, dt):
         _check_input("x", x, dtype=dt)
     shape = x.shape
     if len(shape) != 2:
-        raise RuntimeError("x must be 2-D [M, D]")
-    M, D = shape
-    if y is not None and not _ok(y, shape, dt):
-        _check_input("y", y, shape, dt)
+        raise RuntimeError("x must be 2-D")
+    return dt, shape[0], shape[1], x.get_device()
+
+
+def _residual_norm(x, y, gate, gate_act, scale, post, post_gamma, post_beta, post_eps, norm, gamma, beta, eps, h, out):
+    dt, M, D, dev = _rows_of(x)
+    shape, vec = x.shape, (D,)
+    if y is not None and not _fits(y, shape, dt, dev):
+        _refuse("y", y, shape, dt)
     rows = 0
     if gate is not None:
-        if not _ok(gate, None, dt):
-            _check_input("gate", gate, dtype=dt)
-        rows = gate.shape[0] if gate.dim() == 2 else 1
-        if gate.shape not in ((D,), (rows, D)):
-            raise RuntimeError(f"gate must be [{D}] or [R, {D}] (got {tuple(gate.shape)})")
-    for name, t in (("post_gamma", post_gamma), ("post_beta", post_beta), ("gamma", gamma), ("beta", beta)):
-        if t is not None and not _ok(t, (D,), dt):
-            _check_input(name, t, (D,), dt)
+        rows = gate.shape[0] if isinstance(gate, torch.Tensor) and gate.dim() == 2 else 1
+        if not _fits(gate, (rows, D), dt, dev) and not _fits(gate, vec, dt, dev):
+            _refuse("gate", gate, (rows, D), dt)
+    if post_gamma is not None and not _fits(post_gamma, vec, dt, dev):
+        _refuse("post_gamma", post_gamma, vec, dt)
+    if post_beta is not None and not _fits(post_beta, vec, dt, dev):
+        _refuse("post_beta", post_beta, vec, dt)
+    if gamma is not None and not _fits(gamma, vec, dt, dev):
+        _refuse("gamma", gamma, vec, dt)
+    if beta is not None and not _fits(beta, vec, dt, dev):
+        _refuse("beta", beta, vec, dt)
     norm_id = NORMS.get(norm, norm)
     if out is None:
         if norm_id != 0:
             out = torch.empty_like(x)
         elif h is None:
             h = torch.empty_like(x)
-    elif not _ok(out, shape, dt):
-        _check_input("out", out, shape, dt)
-    if h is not None and not _ok(h, shape, dt):
-        _check_input("h", h, shape, dt)
-    _same_device(x, y, gate, post_gamma, post_beta, gamma, beta, h, out)
-    with _on(x):
-        rc = lib.gp_residual_norm_out(M, D, x.data_ptr(), _ptr(y), NORMS.get(post, post), _ptr(post_gamma),
-                                      _ptr(post_beta), post_eps, _ptr(gate), rows, ACTS.get(gate_act, gate_act), scale,
-                                      norm_id, _ptr(gamma), _ptr(beta), eps, _ptr(h), _ptr(out), _DTYPES[dt],
-                                      _stream(x))
-    if rc:
-        _check(rc)
+    elif not _fits(out, shape, dt, dev):
+        _refuse("out", out, shape, dt)
+    if h is not None and not _fits(h, shape, dt, dev):
+        _refuse("h", h, shape, dt)
+    _run_on(dev, lib.gp_residual_norm_out,
+            (M, D, x.data_ptr(), _ptr(y), NORMS.get(post, post), _ptr(post_gamma), _ptr(post_beta), post_eps,
+             _ptr(gate), rows, ACTS.get(gate_act, gate_act), scale, norm_id, _ptr(gamma), _ptr(beta), eps, _ptr(h),
+             _ptr(out), _DTYPES[dt]))
     return h, out
 
 
@@ -956,30 +990,27 @@ def residual_norm(x, y=None, gate=None, gate_act="none", scale=1.0, post="none",
                           torch.empty_like(x), None)
 
 
-def _check_q4(wq, scales, zeros, K, N, group, dt, side=""):
+def _check_q4(wq, scales, zeros, K, N, group, dt, dev, side=""):
     """A 4-bit weight [K, N]: words [K / 8, N], scales and zeros [ceil(K / group), N]."""
-    if not _ok(wq, (K // 8, N), torch.int32):
-        _check_input("wq" + side, wq, (K // 8, N), torch.int32)
+    shape = (K // 8, N)
+    if not _fits(wq, shape, torch.int32, dev):
+        _refuse("wq" + side, wq, shape, torch.int32)
     shape = (-(-K // group), N)
-    if not _ok(scales, shape, dt):
-        _check_input("scales" + side, scales, shape, dt)
-    if zeros is not None and not _ok(zeros, shape, dt):
-        _check_input("zeros" + side, zeros, shape, dt)
+    if not _fits(scales, shape, dt, dev):
+        _refuse("scales" + side, scales, shape, dt)
+    if zeros is not None and not _fits(zeros, shape, dt, dev):
+        _refuse("zeros" + side, zeros, shape, dt)
 
 
-def _q4_shape(x, wq, group, dt):
-    if not _ok(x, None, dt):
-        _check_input("x", x, dtype=dt)
-    if x.dim() != 2:
-        raise RuntimeError("x must be 2-D [M, K]")
+def _q4_shape(x, wq, group):
+    dt, M, K, dev = _rows_of(x)
     if not isinstance(wq, torch.Tensor) or wq.dim() != 2:
         raise RuntimeError("the packed weight must be a 2-D tensor [K / 8, N]")
     if group not in (32, 64, 128):
         raise RuntimeError(f"group must be 32, 64 or 128 (got {group})")
-    M, K = x.shape
     if K % 8:
         raise RuntimeError(f"K must be a multiple of 8 (got {K})")
-    return M, K, wq.shape[1]
+    return dt, M, K, wq.shape[1], dev
 
 
 def q4_gemm_out(x, wq, scales, zeros=None, b=None, r=None, act="none", group=128, out=None):
@@ -988,23 +1019,19 @@ def q4_gemm_out(x, wq, scales, zeros=None, b=None, r=None, act="none", group=128
     holding q[8 i .. 8 i + 7, n], the lowest k in the lowest bits (gpipes.q4.pack); zeros None: 8.
     group 32, 64 or 128; K a multiple of 8, any N; M from one token to whole prompts.  Every other
     tensor float16, or every other tensor bfloat16.  act: a name of ACTS."""
-    dt = _dtype_of(x)
-    M, K, N = _q4_shape(x, wq, group, dt)
-    _check_q4(wq, scales, zeros, K, N, group, dt)
-    if b is not None and not _ok(b, (N,), dt):
-        _check_input("b", b, (N,), dt)
-    if r is not None and not _ok(r, (M, N), dt):
-        _check_input("r", r, (M, N), dt)
+    dt, M, K, N, dev = _q4_shape(x, wq, group)
+    _check_q4(wq, scales, zeros, K, N, group, dt, dev)
+    if b is not None and not _fits(b, (N,), dt, dev):
+        _refuse("b", b, (N,), dt)
+    if r is not None and not _fits(r, (M, N), dt, dev):
+        _refuse("r", r, (M, N), dt)
     if out is None:
         out = torch.empty((M, N), dtype=dt, device=x.device)
-    elif not _ok(out, (M, N), dt):
-        _check_input("out", out, (M, N), dt)
-    _same_device(x, wq, scales, zeros, b, r, out)
-    with _on(x):
-        rc = lib.gp_q4_gemm_out(M, N, K, group, x.data_ptr(), wq.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(b),
-                                _ptr(r), ACTS.get(act, act), out.data_ptr(), _DTYPES[dt], _stream(x))
-    if rc:
-        _check(rc)
+    elif not _fits(out, (M, N), dt, dev):
+        _refuse("out", out, (M, N), dt)
+    _run_on(dev, lib.gp_q4_gemm_out,
+            (M, N, K, group, x.data_ptr(), wq.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(b), _ptr(r),
+             ACTS.get(act, act), out.data_ptr(), _DTYPES[dt]))
     return out
 
 
@@ -1012,22 +1039,19 @@ def q4_gated_out(x, wq_g, scales_g, zeros_g, wq_u, scales_u, zeros_u, bg=None, b
                  out=None):
     """out[M,N] = act(x @ Wg + bg) * (x @ Wu + bu), the first half of a gated feed-forward block, both
     weights as q4_gemm_out's and of one shape (gp_q4_gated_out)."""
-    dt = _dtype_of(x)
-    M, K, N = _q4_shape(x, wq_g, group, dt)
-    _check_q4(wq_g, scales_g, zeros_g, K, N, group, dt, "_g")
-    _check_q4(wq_u, scales_u, zeros_u, K, N, group, dt, "_u")
-    for name, t in (("bg", bg), ("bu", bu)):
-        if t is not None and not _ok(t, (N,), dt):
-            _check_input(name, t, (N,), dt)
+    dt, M, K, N, dev = _q4_shape(x, wq_g, group)
+    _check_q4(wq_g, scales_g, zeros_g, K, N, group, dt, dev, "_g")
+    _check_q4(wq_u, scales_u, zeros_u, K, N, group, dt, dev, "_u")
+    if bg is not None and not _fits(bg, (N,), dt, dev):
+        _refuse("bg", bg, (N,), dt)
+    if bu is not None and not _fits(bu, (N,), dt, dev):
+        _refuse("bu", bu, (N,), dt)
     if out is None:
         out = torch.empty((M, N), dtype=dt, device=x.device)
-    elif not _ok(out, (M, N), dt):
-        _check_input("out", out, (M, N), dt)
-    _same_device(x, wq_g, scales_g, zeros_g, wq_u, scales_u, zeros_u, bg, bu, out)
-    with _on(x):
-        rc = lib.gp_q4_gated_out(M, N, K, group, x.data_ptr(), wq_g.data_ptr(), scales_g.data_ptr(), _ptr(zeros_g),
-                                 _ptr(bg), wq_u.data_ptr(), scales_u.data_ptr(), _ptr(zeros_u), _ptr(bu),
-                                 ACTS.get(act, act), out.data_ptr(), _DTYPES[dt], _stream(x))
-    if rc:
-        _check(rc)
+    elif not _fits(out, (M, N), dt, dev):
+        _refuse("out", out, (M, N), dt)
+    _run_on(dev, lib.gp_q4_gated_out,
+            (M, N, K, group, x.data_ptr(), wq_g.data_ptr(), scales_g.data_ptr(), _ptr(zeros_g), _ptr(bg),
+             wq_u.data_ptr(), scales_u.data_ptr(), _ptr(zeros_u), _ptr(bu), ACTS.get(act, act), out.data_ptr(),
+             _DTYPES[dt]))
     return out
