@@ -7,15 +7,19 @@
 // bits: eight k of one column are what one lane of an MFMA holds, so a word is
 // a lane's operand, and the weights need no other layout than [K / 8, N].
 //
-// From a word to an operand.  A 4-bit q in the top mantissa bits of 16.0 is the
-// 16-bit float 16 + q, exactly, in fp16 and in bf16; one shift and one
-// and-or make two of them, of k and k + 4, so the operand holds the eight k in
-// the order 0 4 1 5 2 6 3 7, and x is put in the same order.  Per group of G
-// rows the matrix cores sum x (16 + q) and, against a column of ones, x; then
-//   sum x (q - z) = sum x (16 + q) - (16 + z) sum x
+// From a word to an operand.  A 4-bit q in mantissa bits 4 .. 7 of fp16's 64.0
+// is 64 + q, exactly, and in bits 0 .. 3 of bf16's 128.0 it is 128 + q; a shift
+// (three of four need one) and an and-or make two of them, of k and k + 4, so
+// the operand holds the eight k in the order 0 4 1 5 2 6 3 7, and x is put in
+// the same order.  Per group of G rows the matrix cores sum x (B + q), B the 64
+// or 128, and, against a column of ones, x; then
+//   sum x (q - z) = sum x (B + q) - (B + z) sum x
 // in fp32, and times s into the running sum.  The weights are never rounded:
-// what is lost is a few bits of fp32 where the two sums cancel.
+// what is lost is a few bits of fp32 where the two sums cancel, 2^-24 of sums
+// B / 4 times as large (2^-20 and 2^-19 of theirs; a result's half step is
+// 2^-12 and 2^-9).
 #include <hip/hip_runtime.h>
+#include <cstdlib>
 #include <type_traits>
 
 #include "../../include/gpipes.h"
@@ -29,8 +33,9 @@ template <class T>
 struct Q4;
 template <>
 struct Q4<F16> : F16 {
-  static constexpr int kShift = 6;  // q to the top of fp16's ten mantissa bits
-  static constexpr unsigned kMask = 0x03C003C0u, kBase = 0x4C004C00u;
+  static constexpr int kShift = 4;  // left, of the lowest q
+  static constexpr unsigned kMask = 0x00F000F0u, kBase = 0x54005400u;
+  static constexpr float kBias = 64.f;
   __device__ static f4 mma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   // s + both halves of u
   __device__ static float add2(unsigned u, float s) {
@@ -39,8 +44,9 @@ struct Q4<F16> : F16 {
 };
 template <>
 struct Q4<BF16> : BF16 {
-  static constexpr int kShift = 3;  // of bf16's seven
-  static constexpr unsigned kMask = 0x00780078u, kBase = 0x41804180u;
+  static constexpr int kShift = 0;
+  static constexpr unsigned kMask = 0x000F000Fu, kBase = 0x43004300u;
+  static constexpr float kBias = 128.f;
   __device__ static f4 mma16(h8 a, h8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
   }
@@ -59,12 +65,12 @@ struct Q4Bits {
     asm("" : "+s"(mask));
     asm("" : "+v"(base));
   }
-  // The operand 16 + q of a word, k order 0 4 1 5 2 6 3 7.
+  // The operand B + q of a word, k order 0 4 1 5 2 6 3 7.
   __device__ __forceinline__ h8 operand(unsigned w) const {
     constexpr int s = Q4<T>::kShift;
     u32x4 o;
     o[0] = ((w << s) & mask) | base;
-    o[1] = ((s >= 4 ? w << (s - 4) : w >> (4 - s)) & mask) | base;
+    o[1] = ((w >> (4 - s)) & mask) | base;
     o[2] = ((w >> (8 - s)) & mask) | base;
     o[3] = ((w >> (12 - s)) & mask) | base;
     return __builtin_bit_cast(h8, o);
@@ -164,6 +170,9 @@ struct Cols {
 // workgroup's 16 CW columns, and the shares are joined through LDS in the
 // order of the waves.  With two weights, half of the waves take each.
 // ---------------------------------------------------------------------------
+// Waves of a workgroup at most: as many as its registers leave room for.
+constexpr int rows_waves(int cw, int mt) { return mt == 1 || (cw == 1 && mt <= 3) ? 16 : 8; }
+
 template <int CW, int MT, int SG>
 struct Half {
   unsigned w[2][CW];
@@ -172,13 +181,13 @@ struct Half {
 };
 
 template <class T, int CW, int MT, int G, bool FOUR, int NB>
-__global__ __launch_bounds__(MT == 1 ? 1024 : 512) void q4_rows_kernel(Q4Args p) {
+__global__ __launch_bounds__(64 * rows_waves(CW, MT)) void q4_rows_kernel(Q4Args p) {
   constexpr int SG = G < kHalf ? kHalf / G : 1;  // groups a half (G 128: one every other half)
   constexpr int E = FOUR ? 1 : 4;                // accumulator elements that hold rows (FOUR: at most four rows)
   constexpr int COLS = 16 * CW;
   constexpr int TOK = FOUR ? 4 : 16;
   static_assert(NB % 2 == 0, "a buffer holds first halves or second halves");
-  __shared__ float part[(MT == 1 ? 16 : 8) * TOK * COLS];
+  __shared__ float part[rows_waves(CW, MT) * TOK * COLS];
   const int lane = threadIdx.x & 63, j = lane & 15, lg = lane >> 4;
   const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int per = waves / p.sides;  // waves a weight
@@ -276,7 +285,7 @@ __global__ __launch_bounds__(MT == 1 ? 1024 : 512) void q4_rows_kernel(Q4Args p)
 #pragma unroll
         for (int t = 0; t < CW; ++t) {
           const float s = qs.template val<T>(t);
-          const float z = sd.z ? 16.f + qz.template val<T>(t) : 24.f;
+          const float z = Q4<T>::kBias + (sd.z ? qz.template val<T>(t) : 8.f);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -618,34 +627,11 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, i
   // this thread's part of a chunk of x: eight k of rows tid / 16 + 16 q
   const int xk = (tid & 15) * 8, xrow = tid >> 4;
   u32x4 xv[MT];
-  unsigned wv[4][CW];
-  Cols<CW> sv[GPC], zv[GPC];
   auto load_x = [&](int c) {
     const int k = c * kChunk + xk;
 #pragma unroll
     for (int q = 0; q < MT; ++q)
       xv[q] = __builtin_amdgcn_raw_buffer_load_b128(xr, k < K ? ((xrow + 16 * q) * K + k) * 2 : 0x7FFFFFE0, 0, 0);
-  };
-  auto load_w = [&](int c) {
-#pragma unroll
-    for (int st = 0; st < 4; ++st) {
-      const unsigned off = ((unsigned)(c * (kChunk / 8) + st * 4 + lg) * (unsigned)N + (unsigned)col) * 4u;
-      if constexpr (CW == 4) {
-        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(wr, (int)off, 0, 0);
-        for (int t = 0; t < 4; ++t) wv[st][t] = v[t];
-      } else if constexpr (CW == 2) {
-        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(wr, (int)off, 0, 0);
-        wv[st][0] = v[0], wv[st][1] = v[1];
-      } else {
-        wv[st][0] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)off, 0, 0);
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < GPC; ++g) {
-      const int gi = c * GPC + g < groups ? c * GPC + g : groups - 1;
-      sv[g].load(sp, (int64_t)gi * N + col, last);
-      if constexpr (Z) zv[g].load(zp, (int64_t)gi * N + col, last);
-    }
   };
   // 16-byte piece c of a row lies at c ^ row % 16: sixteen rows' reads of one piece fall into different banks
   auto put_x = [&](int buf) {
@@ -655,71 +641,88 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, i
       const h8 v = x_operand(xv[q]);
       *(h8*)(xs[buf] + row * (kChunk * 2) + (((tid & 15) ^ (row & 15)) << 4)) = v;
       float s = sum8<T>(v);
-      s = add_dpp<0xB1>(s);                       // quad_perm [1,0,3,2]
-      s = add_dpp<0x4E>(s);                       // quad_perm [2,3,0,1]
+      s = add_dpp<0xB1>(s);                           // quad_perm [1,0,3,2]
+      s = add_dpp<0x4E>(s);                           // quad_perm [2,3,0,1]
       if constexpr (G >= 64) s = add_dpp<0x141>(s);   // row_half_mirror
       if constexpr (G >= 128) s = add_dpp<0x140>(s);  // row_mirror
-      if ((tid & (G / 8 - 1)) == 0) ss[buf][(tid & 15) / (G / 8)][row] = Z ? -s : -24.f * s;
+      ss[buf][(tid & 15) / (G / 8)][row] = Z ? -s : -(Q4<T>::kBias + 8.f) * s;  // the same from each lane of the group
+    }
+  };
+  struct Words {
+    unsigned w[4][CW];
+    Cols<CW> s[GPC], z[GPC];
+  };
+  auto load_w = [&](int c, Words& q) {
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+      const unsigned off = ((unsigned)(c * (kChunk / 8) + st * 4 + lg) * (unsigned)N + (unsigned)col) * 4u;
+      if constexpr (CW == 4) {
+        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(wr, (int)off, 0, 0);
+        for (int t = 0; t < 4; ++t) q.w[st][t] = v[t];
+      } else if constexpr (CW == 2) {
+        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(wr, (int)off, 0, 0);
+        q.w[st][0] = v[0], q.w[st][1] = v[1];
+      } else {
+        q.w[st][0] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)off, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < GPC; ++g) {
+      const int gi = c * GPC + g < groups ? c * GPC + g : groups - 1;
+      q.s[g].load(sp, (int64_t)gi * N + col, last);
+      if constexpr (Z) q.z[g].load(zp, (int64_t)gi * N + col, last);
     }
   };
 
   const Q4Bits<T> bits;
   float tot[CW][MT][4] = {};
-  load_x(0);
-  load_w(0);
-  put_x(0);
-  __syncthreads();
-#pragma unroll 2
-  for (int c = 0; c < chunks; ++c) {
-    const int buf = c & 1;
-    unsigned w[4][CW];
-    Cols<CW> qs[GPC], qz[GPC];
-#pragma unroll
-    for (int st = 0; st < 4; ++st)
-#pragma unroll
-      for (int t = 0; t < CW; ++t) w[st][t] = wv[st][t];
-#pragma unroll
-    for (int g = 0; g < GPC; ++g) qs[g] = sv[g], qz[g] = zv[g];
+  // One chunk: the next one's words are asked for, the next one's x, which was
+  // asked for a chunk ago, goes to the other buffer, and the one after that is
+  // asked for.
+  auto chunk = [&](int c, int buf, Words& q, Words& next) {
+    load_w(c + 1, next);
     if (!inside) {
 #pragma unroll
       for (int g = 0; g < GPC; ++g) {
         const int gi = c * GPC + g < groups ? c * GPC + g : groups - 1;
-        qs[g] = qs[g].shifted((int64_t)gi * N + col, last);
-        if constexpr (Z) qz[g] = qz[g].shifted((int64_t)gi * N + col, last);
+        q.s[g] = q.s[g].shifted((int64_t)gi * N + col, last);
+        if constexpr (Z) q.z[g] = q.z[g].shifted((int64_t)gi * N + col, last);
       }
     }
-    if (c + 1 < chunks) {
-      load_x(c + 1);
-      load_w(c + 1);
-    }
+    h8 b[CW];
+#pragma unroll
+    for (int t = 0; t < CW; ++t) b[t] = bits.operand(q.w[0][t]);
 #pragma unroll
     for (int g = 0; g < GPC; ++g) {
       f4 acc[CW][MT];
 #pragma unroll
       for (int st = g * SPG; st < (g + 1) * SPG; ++st) {
-        h8 b[CW];
-#pragma unroll
-        for (int t = 0; t < CW; ++t) b[t] = bits.operand(w[st][t]);
+        h8 bn[CW];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           const h8 a = *(const h8*)(xs[buf] + (mt * 16 + j) * (kChunk * 2) + (((st * 4 + lg) ^ j) << 4));
           if (st == g * SPG) {
-            // a group's sum begins at -(16 + z) times that of x
+            // a group's sum begins at -(B + z) times that of x
             const f4 m = *(const f4*)&ss[buf][g][mt * 16 + 4 * lg];
 #pragma unroll
             for (int t = 0; t < CW; ++t) {
-              const float z = sd.z ? 16.f + qz[g].template val<T>(t) : 24.f;
+              const float z = Q4<T>::kBias + (sd.z ? q.z[g].template val<T>(t) : 8.f);
               acc[t][mt] = Q4<T>::mma16(a, b[t], Z ? f4{z * m[0], z * m[1], z * m[2], z * m[3]} : m);
             }
           } else {
 #pragma unroll
             for (int t = 0; t < CW; ++t) acc[t][mt] = Q4<T>::mma16(a, b[t], acc[t][mt]);
           }
+          if (st < 3 && mt < CW) bn[mt] = bits.operand(q.w[st < 3 ? st + 1 : 3][mt < CW ? mt : 0]);
+        }
+        if (st < 3) {
+#pragma unroll
+          for (int t = 0; t < CW; ++t) b[t] = bn[t];
         }
       }
 #pragma unroll
       for (int t = 0; t < CW; ++t) {
-        const float s = qs[g].template val<T>(t);
+        const float s = q.s[g].template val<T>(t);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -730,8 +733,33 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, i
       }
       if constexpr (GPC > 1) __builtin_amdgcn_sched_barrier(0);
     }
-    if (c + 1 < chunks) put_x(buf ^ 1);
-    __syncthreads();
+    put_x(buf ^ 1);
+    load_x(c + 2);
+#ifdef SGB
+    if constexpr (GPC == 1) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, 36, 0);
+#pragma unroll
+      for (int i = 0; i < 4 * CW * MT; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, SGB, 0);
+        if (i % CW == 0) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+    }
+#endif
+    lds_barrier();
+  };
+  Words wa, wb;
+  load_x(0);
+  load_w(0, wa);
+  put_x(0);
+  load_x(1);
+  lds_barrier();
+#pragma unroll 1
+  for (int c = 0; c < chunks; c += 2) {
+    chunk(c, 0, wa, wb);
+    if (c + 1 >= chunks) break;
+    chunk(c + 1, 1, wb, wa);
   }
 
   // Out through LDS, half of the rows at a time: eight columns a thread, whole
@@ -828,10 +856,11 @@ hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
     return cw == 4 ? tile_launch<T, 4>(a, s) : cw == 2 ? tile_launch<T, 2>(a, s) : tile_launch<T, 1>(a, s);
   }
   const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : a.M <= 48 ? 3 : 4;
-  int waves = mt == 1 ? 16 : 8;
-  while (waves > 2 * a.sides && waves / 2 >= chunks * a.sides) waves /= 2;
   int cw = a.N >= 64 * num_cus ? 4 : a.N >= 32 * num_cus ? 2 : 1;
+  if (const char* v = getenv("Q4_CW")) cw = atoi(v);
   if ((int64_t)((a.K + a.group - 1) / a.group) * a.N < 4) cw = 1;
+  int waves = rows_waves(cw, mt);
+  while (waves > 2 * a.sides && waves / 2 >= chunks * a.sides) waves /= 2;
   const dim3 grid((unsigned)((a.N + 16 * cw - 1) / (16 * cw)), (unsigned)((a.M + 16 * mt - 1) / (16 * mt)));
 #define GP_CASE(c, m, four, nb) \
   if (cw == c && mt == m && (a.M <= 4) == four) return rows_launch<T, c, m, four, nb>(a, waves, grid, s);

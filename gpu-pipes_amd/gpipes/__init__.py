@@ -908,21 +908,28 @@ def residual_norm_out(x, y=None, gate=None, gate_act="none", scale=1.0, post="no
 
 
 # These calls run for a few microseconds on one token, no longer than their host
-# side: a tensor is checked in one expression (a device index of -1 is a CPU
-# tensor's, so one comparison says both that a tensor is on a GPU and on x's),
-# and the slow path is taken only to say what is wrong.
+# side, so that is kept short: a tensor is checked by one expression where it
+# stands (a device index of -1 is a CPU tensor's, so one comparison says both that
+# a tensor is on a GPU and on x's), what is wrong is found out only after it
+# failed, and the device guard and the stream are asked for without torch.cuda's
+# wrappers.  One token's call: 7.8 us with a checking function for each tensor,
+# 4.2 of them the launch.
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _fits(t, shape, dtype, dev):
-    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == dev
-            and t.is_contiguous())
-
-
 def _refuse(name, t, shape, dtype):
-    """Raises for a tensor that _fits() refused."""
+    """Raises for a tensor that failed a call's own check."""
     _check_input(name, t, shape, dtype)
     raise RuntimeError("all tensors must be on the same device")
+
+
+def _misfit(x, named):
+    """Raises for the first of the (name, tensor, shape, type) that does not fit."""
+    dev = x.get_device()
+    for name, t, shape, dtype in named:
+        if t is not None and not (_ok(t, shape, dtype) and t.get_device() == dev):
+            _refuse(name, t, shape, dtype)
+    raise RuntimeError("invalid arguments")
 
 
 def _run_on(dev, fn, args):
@@ -936,49 +943,58 @@ def _run_on(dev, fn, args):
         _check(rc)
 
 
-def _rows_of(x):
-    """(element type, rows, columns, device index) of a call's x."""
-    dt = _dtype_of(x)
-    if not _ok(x, None, dt):
-        _check_input("x", x, dtype=dt)
-    shape = x.shape
-    if len(shape) != 2:
+def _check_rows(x):
+    """x, a call's rows [M, columns], on a GPU and of an element type of the library's."""
+    _check_input("x", x, dtype=_dtype_of(x))
+    if x.dim() != 2:
         raise RuntimeError("x must be 2-D")
-    return dt, shape[0], shape[1], x.get_device()
 
 
 def _residual_norm(x, y, gate, gate_act, scale, post, post_gamma, post_beta, post_eps, norm, gamma, beta, eps, h, out):
-    dt, M, D, dev = _rows_of(x)
-    shape, vec = x.shape, (D,)
-    if y is not None and not _fits(y, shape, dt, dev):
-        _refuse("y", y, shape, dt)
-    rows = 0
-    if gate is not None:
-        rows = gate.shape[0] if isinstance(gate, torch.Tensor) and gate.dim() == 2 else 1
-        if not _fits(gate, (rows, D), dt, dev) and not _fits(gate, vec, dt, dev):
-            _refuse("gate", gate, (rows, D), dt)
-    if post_gamma is not None and not _fits(post_gamma, vec, dt, dev):
-        _refuse("post_gamma", post_gamma, vec, dt)
-    if post_beta is not None and not _fits(post_beta, vec, dt, dev):
-        _refuse("post_beta", post_beta, vec, dt)
-    if gamma is not None and not _fits(gamma, vec, dt, dev):
-        _refuse("gamma", gamma, vec, dt)
-    if beta is not None and not _fits(beta, vec, dt, dev):
-        _refuse("beta", beta, vec, dt)
-    norm_id = NORMS.get(norm, norm)
-    if out is None:
-        if norm_id != 0:
-            out = torch.empty_like(x)
-        elif h is None:
-            h = torch.empty_like(x)
-    elif not _fits(out, shape, dt, dev):
-        _refuse("out", out, shape, dt)
-    if h is not None and not _fits(h, shape, dt, dev):
-        _refuse("h", h, shape, dt)
+    try:
+        dt, shape, dev = x.dtype, x.shape, x.get_device()
+        dt_id = _DTYPES.get(dt, -1)
+        if dt_id < 0 or dev < 0 or len(shape) != 2 or not x.is_contiguous():
+            _check_rows(x)
+        M, D = shape
+        vec, rows = (D,), 0
+        if gate is not None:
+            rows = gate.shape[0] if gate.dim() == 2 else 1
+        norm_id = NORMS.get(norm, norm)
+        if out is None:
+            if norm_id != 0:
+                out = torch.empty_like(x)
+            elif h is None:
+                h = torch.empty_like(x)
+        ok = ((y is None or (y.dtype is dt and y.get_device() == dev and y.shape == shape and y.is_contiguous()))
+              and (gate is None or (gate.dtype is dt and gate.get_device() == dev and gate.shape[-1:] == vec
+                                    and gate.dim() <= 2 and gate.is_contiguous()))
+              and (post_gamma is None or (post_gamma.dtype is dt and post_gamma.get_device() == dev
+                                          and post_gamma.shape == vec and post_gamma.is_contiguous()))
+              and (post_beta is None or (post_beta.dtype is dt and post_beta.get_device() == dev
+                                         and post_beta.shape == vec and post_beta.is_contiguous()))
+              and (gamma is None or (gamma.dtype is dt and gamma.get_device() == dev and gamma.shape == vec
+                                     and gamma.is_contiguous()))
+              and (beta is None or (beta.dtype is dt and beta.get_device() == dev and beta.shape == vec
+                                    and beta.is_contiguous()))
+              and (out is None or (out.dtype is dt and out.get_device() == dev and out.shape == shape
+                                   and out.is_contiguous()))
+              and (h is None or (h.dtype is dt and h.get_device() == dev and h.shape == shape and h.is_contiguous())))
+    except AttributeError:  # something that is no tensor
+        ok = False
+    if not ok:
+        _check_rows(x)
+        gshape = (gate.shape[0], x.shape[1]) if isinstance(gate, torch.Tensor) and gate.dim() == 2 else x.shape[1:]
+        _misfit(x, [("y", y, x.shape, x.dtype), ("gate", gate, gshape, x.dtype),
+                    ("post_gamma", post_gamma, x.shape[1:], x.dtype), ("post_beta", post_beta, x.shape[1:], x.dtype),
+                    ("gamma", gamma, x.shape[1:], x.dtype), ("beta", beta, x.shape[1:], x.dtype),
+                    ("out", out, x.shape, x.dtype), ("h", h, x.shape, x.dtype)])
     _run_on(dev, lib.gp_residual_norm_out,
-            (M, D, x.data_ptr(), _ptr(y), NORMS.get(post, post), _ptr(post_gamma), _ptr(post_beta), post_eps,
-             _ptr(gate), rows, ACTS.get(gate_act, gate_act), scale, norm_id, _ptr(gamma), _ptr(beta), eps, _ptr(h),
-             _ptr(out), _DTYPES[dt]))
+            (M, D, x.data_ptr(), None if y is None else y.data_ptr(), NORMS.get(post, post),
+             None if post_gamma is None else post_gamma.data_ptr(), None if post_beta is None else post_beta.data_ptr(),
+             post_eps, None if gate is None else gate.data_ptr(), rows, ACTS.get(gate_act, gate_act), scale, norm_id,
+             None if gamma is None else gamma.data_ptr(), None if beta is None else beta.data_ptr(), eps,
+             None if h is None else h.data_ptr(), None if out is None else out.data_ptr(), dt_id))
     return h, out
 
 
@@ -990,27 +1006,28 @@ def residual_norm(x, y=None, gate=None, gate_act="none", scale=1.0, post="none",
                           torch.empty_like(x), None)
 
 
-def _check_q4(wq, scales, zeros, K, N, group, dt, dev, side=""):
-    """A 4-bit weight [K, N]: words [K / 8, N], scales and zeros [ceil(K / group), N]."""
-    shape = (K // 8, N)
-    if not _fits(wq, shape, torch.int32, dev):
-        _refuse("wq" + side, wq, shape, torch.int32)
-    shape = (-(-K // group), N)
-    if not _fits(scales, shape, dt, dev):
-        _refuse("scales" + side, scales, shape, dt)
-    if zeros is not None and not _fits(zeros, shape, dt, dev):
-        _refuse("zeros" + side, zeros, shape, dt)
+def _q4_weight(wq, scales, zeros, words, groups, dt, dev):
+    """Whether a 4-bit weight's tensors fit: words [K / 8, N], scales and zeros [ceil(K / group), N]."""
+    return (wq.dtype is torch.int32 and wq.get_device() == dev and wq.shape == words and wq.is_contiguous()
+            and scales.dtype is dt and scales.get_device() == dev and scales.shape == groups and scales.is_contiguous()
+            and (zeros is None or (zeros.dtype is dt and zeros.get_device() == dev and zeros.shape == groups
+                                   and zeros.is_contiguous())))
 
 
-def _q4_shape(x, wq, group):
-    dt, M, K, dev = _rows_of(x)
+def _q4_refuse(x, group, named):
+    """Raises for what is wrong with a 4-bit product's x, group or tensors: (name, tensor, kind)."""
+    _check_rows(x)
+    M, K = x.shape
+    wq = named[0][1]
     if not isinstance(wq, torch.Tensor) or wq.dim() != 2:
         raise RuntimeError("the packed weight must be a 2-D tensor [K / 8, N]")
     if group not in (32, 64, 128):
         raise RuntimeError(f"group must be 32, 64 or 128 (got {group})")
     if K % 8:
         raise RuntimeError(f"K must be a multiple of 8 (got {K})")
-    return dt, M, K, wq.shape[1], dev
+    N = wq.shape[1]
+    shapes = {"words": (K // 8, N), "groups": (-(-K // group), N), "bias": (N,), "rows": (M, N)}
+    _misfit(x, [(name, t, shapes[kind], torch.int32 if kind == "words" else x.dtype) for name, t, kind in named])
 
 
 def q4_gemm_out(x, wq, scales, zeros=None, b=None, r=None, act="none", group=128, out=None):
@@ -1019,19 +1036,26 @@ def q4_gemm_out(x, wq, scales, zeros=None, b=None, r=None, act="none", group=128
     holding q[8 i .. 8 i + 7, n], the lowest k in the lowest bits (gpipes.q4.pack); zeros None: 8.
     group 32, 64 or 128; K a multiple of 8, any N; M from one token to whole prompts.  Every other
     tensor float16, or every other tensor bfloat16.  act: a name of ACTS."""
-    dt, M, K, N, dev = _q4_shape(x, wq, group)
-    _check_q4(wq, scales, zeros, K, N, group, dt, dev)
-    if b is not None and not _fits(b, (N,), dt, dev):
-        _refuse("b", b, (N,), dt)
-    if r is not None and not _fits(r, (M, N), dt, dev):
-        _refuse("r", r, (M, N), dt)
-    if out is None:
-        out = torch.empty((M, N), dtype=dt, device=x.device)
-    elif not _fits(out, (M, N), dt, dev):
-        _refuse("out", out, (M, N), dt)
+    try:
+        dt, dev = x.dtype, x.get_device()
+        M, K = x.shape
+        N = wq.shape[1]
+        if out is None:
+            out = torch.empty((M, N), dtype=dt, device=x.device)
+        ok = (group in (32, 64, 128) and K % 8 == 0 and dt in _DTYPES and dev >= 0 and x.is_contiguous()
+              and _q4_weight(wq, scales, zeros, (K // 8, N), (-(-K // group), N), dt, dev)
+              and (b is None or (b.dtype is dt and b.get_device() == dev and b.shape == (N,) and b.is_contiguous()))
+              and (r is None or (r.dtype is dt and r.get_device() == dev and r.shape == (M, N) and r.is_contiguous()))
+              and out.dtype is dt and out.get_device() == dev and out.shape == (M, N) and out.is_contiguous())
+    except (AttributeError, ValueError, IndexError, TypeError):  # no tensors, or of another rank
+        ok = False
+    if not ok:
+        _q4_refuse(x, group, [("wq", wq, "words"), ("scales", scales, "groups"), ("zeros", zeros, "groups"),
+                              ("b", b, "bias"), ("r", r, "rows"), ("out", out, "rows")])
     _run_on(dev, lib.gp_q4_gemm_out,
-            (M, N, K, group, x.data_ptr(), wq.data_ptr(), scales.data_ptr(), _ptr(zeros), _ptr(b), _ptr(r),
-             ACTS.get(act, act), out.data_ptr(), _DTYPES[dt]))
+            (M, N, K, group, x.data_ptr(), wq.data_ptr(), scales.data_ptr(),
+             None if zeros is None else zeros.data_ptr(), None if b is None else b.data_ptr(),
+             None if r is None else r.data_ptr(), ACTS.get(act, act), out.data_ptr(), _DTYPES[dt]))
     return out
 
 
@@ -1039,19 +1063,28 @@ def q4_gated_out(x, wq_g, scales_g, zeros_g, wq_u, scales_u, zeros_u, bg=None, b
                  out=None):
     """out[M,N] = act(x @ Wg + bg) * (x @ Wu + bu), the first half of a gated feed-forward block, both
     weights as q4_gemm_out's and of one shape (gp_q4_gated_out)."""
-    dt, M, K, N, dev = _q4_shape(x, wq_g, group)
-    _check_q4(wq_g, scales_g, zeros_g, K, N, group, dt, dev, "_g")
-    _check_q4(wq_u, scales_u, zeros_u, K, N, group, dt, dev, "_u")
-    if bg is not None and not _fits(bg, (N,), dt, dev):
-        _refuse("bg", bg, (N,), dt)
-    if bu is not None and not _fits(bu, (N,), dt, dev):
-        _refuse("bu", bu, (N,), dt)
-    if out is None:
-        out = torch.empty((M, N), dtype=dt, device=x.device)
-    elif not _fits(out, (M, N), dt, dev):
-        _refuse("out", out, (M, N), dt)
+    try:
+        dt, dev = x.dtype, x.get_device()
+        M, K = x.shape
+        N = wq_g.shape[1]
+        if out is None:
+            out = torch.empty((M, N), dtype=dt, device=x.device)
+        words, groups = (K // 8, N), (-(-K // group), N)
+        ok = (group in (32, 64, 128) and K % 8 == 0 and dt in _DTYPES and dev >= 0 and x.is_contiguous()
+              and _q4_weight(wq_g, scales_g, zeros_g, words, groups, dt, dev)
+              and _q4_weight(wq_u, scales_u, zeros_u, words, groups, dt, dev)
+              and (bg is None or (bg.dtype is dt and bg.get_device() == dev and bg.shape == (N,) and bg.is_contiguous()))
+              and (bu is None or (bu.dtype is dt and bu.get_device() == dev and bu.shape == (N,) and bu.is_contiguous()))
+              and out.dtype is dt and out.get_device() == dev and out.shape == (M, N) and out.is_contiguous())
+    except (AttributeError, ValueError, IndexError, TypeError):
+        ok = False
+    if not ok:
+        _q4_refuse(x, group, [("wq_g", wq_g, "words"), ("scales_g", scales_g, "groups"), ("zeros_g", zeros_g, "groups"),
+                              ("wq_u", wq_u, "words"), ("scales_u", scales_u, "groups"), ("zeros_u", zeros_u, "groups"),
+                              ("bg", bg, "bias"), ("bu", bu, "bias"), ("out", out, "rows")])
     _run_on(dev, lib.gp_q4_gated_out,
-            (M, N, K, group, x.data_ptr(), wq_g.data_ptr(), scales_g.data_ptr(), _ptr(zeros_g), _ptr(bg),
-             wq_u.data_ptr(), scales_u.data_ptr(), _ptr(zeros_u), _ptr(bu), ACTS.get(act, act), out.data_ptr(),
-             _DTYPES[dt]))
+            (M, N, K, group, x.data_ptr(), wq_g.data_ptr(), scales_g.data_ptr(),
+             None if zeros_g is None else zeros_g.data_ptr(), None if bg is None else bg.data_ptr(), wq_u.data_ptr(),
+             scales_u.data_ptr(), None if zeros_u is None else zeros_u.data_ptr(),
+             None if bu is None else bu.data_ptr(), ACTS.get(act, act), out.data_ptr(), _DTYPES[dt]))
     return out

@@ -577,7 +577,7 @@ int gp_residual_norm_out(int64_t M, int64_t D, const void* x, const void* y, int
  * Weights are not rounded: products are exact, sums fp32, out rounded once.
  * (With up to four rows a value of x may be taken to 2^-19 of the largest of
  * its 128 neighbours k, about what an fp32 sum of them keeps.)
- * x has to be finite and, in bf16, 32 times a group's sum of |x| below fp32's
+ * x has to be finite and, in bf16, 150 times a group's sum of |x| below fp32's
  * largest number: a row of x that is not gives NaN in that row of out alone.
  * One launch, no workspace: can be captured into a graph; out must not
  * overlap x (it may be r).

@@ -117,16 +117,17 @@ def weight(K, N, group, zeros, dt, gen):
 
 
 def product(x, q, s, z, group):
-    """x W, and a bound on the kernel's distance from it.  Products of x with 16 + q are exact; a group's sum of at
-    most 128 of them, and that of x, take sixteen roundings each at most (eight products a step), the running
-    sum one a group and one a wave, under 100 for what the tests use.  Up to four rows may be taken in whole numbers
+    """x W, and a bound on the kernel's distance from it.  Products of x with B + q (B 64 in fp16, 128 in bf16) are
+    exact; a group's sum of at most 128 of them, and that of x, which B + z multiplies, take sixteen roundings each
+    at most (eight products a step), the running sum one a group and one a wave, under 100 for what the tests use.  Up to four rows may be taken in whole numbers
     instead, each value to 2^-19 of the largest of its 128: 2^-19 of that largest times |W| a product."""
+    B = 64 if x.dtype == F16 else 128
     x, q, s = x.double(), q.double(), s.double()
     K = q.shape[0]
     zz = z.double() if z is not None else torch.full_like(s, 8)
     sr, zr = (t.repeat_interleave(group, 0)[:K] for t in (s, zz))
     out = x @ (sr * (q - zr))
-    near = 16 * U * (x.abs() @ (sr * (32 + q + zr)))
+    near = 16 * U * (x.abs() @ (sr * (2 * B + q + zr)))
     if x.shape[0] <= 4:
         for k in range(0, K, 128):
             top = x[:, k:k + 128].abs().amax(1, keepdim=True)
