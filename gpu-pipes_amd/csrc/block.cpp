@@ -48,16 +48,24 @@ int check16(const void* p, const char* name, bool needed) {
   return GP_OK;
 }
 
-int q4_run(const Q4Args& a, int64_t N, int64_t K, hipStream_t stream) {
-  clear_error();
-  int rc;
-  if ((rc = check_dtype(a.dtype)) || (rc = check_rows(a.M)) || (rc = check_act_ext(a.act))) return rc;
-  if (a.group != 32 && a.group != 64 && a.group != 128)
-    return fail(GP_ERR_SHAPE, "group must be 32, 64 or 128 (got %d)", a.group);
+int q4_check_shape(int64_t M, int64_t N, int64_t K, int group) {
+  const int rc = check_rows(M);
+  if (rc) return rc;
+  if (group != 32 && group != 64 && group != 128)
+    return fail(GP_ERR_SHAPE, "group must be 32, 64 or 128 (got %d)", group);
   if (K < 8 || K % 8 || K > 65536) return fail(GP_ERR_SHAPE, "K must be a multiple of 8 in [8, 65536] (got %lld)", (long long)K);
   if (N < 1 || N > kQ4MaxDim) return fail(GP_ERR_SHAPE, "N must be in [1, %lld] (got %lld)", (long long)kQ4MaxDim, (long long)N);
   if (K * N / 2 >= (int64_t(1) << 31)) return fail(GP_ERR_SHAPE, "a weight must be smaller than 2 GiB");
-  if (a.M > (int64_t(1) << 21)) return fail(GP_ERR_SHAPE, "M must be at most 2097152 (got %lld)", (long long)a.M);
+  if (M > (int64_t(1) << 21)) return fail(GP_ERR_SHAPE, "M must be at most 2097152 (got %lld)", (long long)M);
+  return GP_OK;
+}
+
+int q4_run(const Q4Args& a, int64_t N, int64_t K, hipStream_t stream) {
+  clear_error();
+  int rc;
+  if ((rc = check_dtype(a.dtype)) || (rc = check_act_ext(a.act)) || (rc = q4_check_shape(a.M, N, K, a.group))) return rc;
+  if (a.ws_bytes < 0) return fail(GP_ERR_INVALID_ARG, "workspace_bytes must be >= 0");
+  if (a.ws_bytes && (rc = check16(a.ws, "workspace", true))) return rc;
   if (a.r && a.act != GP_ACT_NONE) return fail(GP_ERR_INVALID_ARG, "a residual is added without an activation only");
   for (int i = 0; i < a.sides; ++i) {
     const Q4Side& d = a.side[i];
@@ -122,17 +130,30 @@ int gp_residual_norm_out(int64_t M, int64_t D, const void* x, const void* y, int
   return e == hipSuccess ? GP_OK : fail_hip(e, "residual_norm launch");
 }
 
+int64_t gp_q4_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int weights) {
+  clear_error();
+  int rc = q4_check_shape(M, N, K, group);
+  if (rc) return rc;
+  if (weights != 1 && weights != 2) return fail(GP_ERR_INVALID_ARG, "weights must be 1 or 2 (got %d)", weights);
+  if (M == 0) return 0;
+  int dev = 0, ncu = 0;
+  if ((rc = current_device_info(&dev, &ncu))) return rc;
+  return q4_workspace(M, (int)N, (int)K, group, weights, ncu);
+}
+
 int gp_q4_gemm_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq, const void* scales,
-                   const void* zeros, const void* b, const void* r, int act, void* out, int dtype, void* stream) {
-  const Q4Args a{M, 0, 0, group, 1, x, {{wq, scales, zeros, b}, {}}, r, act, out, dtype};
+                   const void* zeros, const void* b, const void* r, int act, void* out, void* workspace,
+                   int64_t workspace_bytes, int dtype, void* stream) {
+  const Q4Args a{M, 0, 0, group, 1, x, {{wq, scales, zeros, b}, {}}, r, act, out, dtype, workspace, workspace_bytes};
   return q4_run(a, N, K, (hipStream_t)stream);
 }
 
 int gp_q4_gated_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq_g, const void* scales_g,
                     const void* zeros_g, const void* b_g, const void* wq_u, const void* scales_u, const void* zeros_u,
-                    const void* b_u, int act, void* out, int dtype, void* stream) {
-  const Q4Args a{M,   0,  0, group, 2, x, {{wq_g, scales_g, zeros_g, b_g}, {wq_u, scales_u, zeros_u, b_u}}, nullptr,
-                 act, out, dtype};
+                    const void* b_u, int act, void* out, void* workspace, int64_t workspace_bytes, int dtype,
+                    void* stream) {
+  const Q4Args a{M,   0,  0,       group, 2, x, {{wq_g, scales_g, zeros_g, b_g}, {wq_u, scales_u, zeros_u, b_u}},
+                 nullptr, act, out, dtype, workspace, workspace_bytes};
   return q4_run(a, N, K, (hipStream_t)stream);
 }
 

@@ -322,7 +322,10 @@ struct Q4Args {
   int act;
   void* out;  // [M, N]
   int dtype;
+  void* ws;  // 16-byte aligned, or null: what q4_workspace asks for is then done without, more slowly
+  int64_t ws_bytes;
 };
+int64_t q4_workspace(int64_t M, int N, int K, int group, int sides, int num_cus);
 hipError_t q4_launch(const Q4Args& a, int num_cus, hipStream_t stream);
 
 }  // namespace gp

@@ -19,7 +19,6 @@
 // B / 4 times as large (2^-20 and 2^-19 of theirs; a result's half step is
 // 2^-12 and 2^-9).
 #include <hip/hip_runtime.h>
-#include <cstdlib>
 #include <type_traits>
 
 #include "../../include/gpipes.h"
@@ -167,42 +166,40 @@ struct Cols {
 
 // ---------------------------------------------------------------------------
 // Few rows: every wave of a workgroup multiplies its share of k with the
-// workgroup's 16 CW columns, and the shares are joined through LDS in the
-// order of the waves.  With two weights, half of the waves take each.
+// workgroup's 16 CW columns of S weights, and the shares are joined through
+// LDS in the order of the waves.  A workgroup reads all of x, from L2, which
+// costs more than its words where rows are many; the two weights of a gated
+// product share those reads.
 // ---------------------------------------------------------------------------
 // Waves of a workgroup at most: as many as its registers leave room for.
-constexpr int rows_waves(int cw, int mt) { return mt == 1 || (cw == 1 && mt <= 3) ? 16 : 8; }
+constexpr int rows_waves(int tiles, int mt) { return mt == 1 ? 16 : 8; }
 
-template <int CW, int MT, int SG>
+template <int CW, int S, int MT, int SG>
 struct Half {
-  unsigned w[2][CW];
+  unsigned w[2][S * CW];
   u32x4 x[2][MT];
-  Cols<CW> s[SG], z[SG];
+  Cols<CW> s[S][SG], z[S][SG];
 };
 
-template <class T, int CW, int MT, int G, bool FOUR, int NB>
-__global__ __launch_bounds__(64 * rows_waves(CW, MT)) void q4_rows_kernel(Q4Args p) {
+template <class T, int CW, int S, int MT, int G, bool FOUR, int NB>
+__global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4Args p) {
   constexpr int SG = G < kHalf ? kHalf / G : 1;  // groups a half (G 128: one every other half)
   constexpr int E = FOUR ? 1 : 4;                // accumulator elements that hold rows (FOUR: at most four rows)
-  constexpr int COLS = 16 * CW;
+  constexpr int COLS = 16 * CW, NT = S * CW;
   constexpr int TOK = FOUR ? 4 : 16;
   static_assert(NB % 2 == 0, "a buffer holds first halves or second halves");
-  __shared__ float part[rows_waves(CW, MT) * TOK * COLS];
+  __shared__ float part[rows_waves(NT, MT) * TOK * COLS * S];
   const int lane = threadIdx.x & 63, j = lane & 15, lg = lane >> 4;
   const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int per = waves / p.sides;  // waves a weight
-  const int side = wave / per, wk = wave - side * per;
   const int N = p.N, K = p.K;
   const int n0 = xcd_order(blockIdx.x, gridDim.x) * COLS;
   const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
   const int rows = p.M - m0 < 16 * MT ? (int)(p.M - m0) : 16 * MT;
   const int groups = (K + G - 1) / G;
   const int chunks = (K + kChunk - 1) / kChunk;
-  const Q4Side sd = side ? p.side[1] : p.side[0];
-  const auto wr = make_rsrc(sd.wq, (int)((int64_t)K * N / 2));
+  const auto wr0 = make_rsrc(p.side[0].wq, (int)((int64_t)K * N / 2));
+  const auto wr1 = make_rsrc(p.side[S - 1].wq, (int)((int64_t)K * N / 2));
   const auto xr = make_rsrc((const half_t*)p.x + m0 * K, rows * K * 2);
-  const unsigned short* sp = (const unsigned short*)sd.s;
-  const unsigned short* zp = (const unsigned short*)(sd.z ? sd.z : sd.s);
   const int col = n0 + CW * j;
   const bool inside = n0 + COLS <= N;
   const int64_t last = (int64_t)groups * N - CW;
@@ -210,23 +207,28 @@ __global__ __launch_bounds__(64 * rows_waves(CW, MT)) void q4_rows_kernel(Q4Args
   // lands in element 0 of the accumulators of the lanes of group i / 4.
   const int xrow = FOUR ? j >> 2 : j;
 
-  // half t of this wave: chunks wk, wk + per, ..., two halves each
-  auto load = [&](int t, Half<CW, MT, SG>& q, bool second) {
-    const int k0 = (wk + (t >> 1) * per) * kChunk + (second ? kHalf : 0);
+  // half t of this wave: chunks wave, wave + waves, ..., two halves each
+  auto load = [&](int t, Half<CW, S, MT, SG>& q, bool second) {
+    const int k0 = (wave + (t >> 1) * waves) * kChunk + (second ? kHalf : 0);
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const int k = k0 + st * 32 + lg * 8;
       // past the weight's end and past the rows' end (and the last row) nothing is read: zeros, and a zero of x is
       // what no word can make count
       const unsigned off = k < K ? ((unsigned)(k >> 3) * (unsigned)N + (unsigned)col) * 4u : 0xFFFFFFE0u;
-      if constexpr (CW == 4) {
-        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(wr, (int)off, 0, 0);
-        for (int c = 0; c < 4; ++c) q.w[st][c] = v[c];
-      } else if constexpr (CW == 2) {
-        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(wr, (int)off, 0, 0);
-        q.w[st][0] = v[0], q.w[st][1] = v[1];
-      } else {
-        q.w[st][0] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)off, 0, 0);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const auto wr = s ? wr1 : wr0;
+        unsigned* w = q.w[st] + s * CW;
+        if constexpr (CW == 4) {
+          const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(wr, (int)off, 0, 0);
+          w[0] = v[0], w[1] = v[1], w[2] = v[2], w[3] = v[3];
+        } else if constexpr (CW == 2) {
+          const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(wr, (int)off, 0, 0);
+          w[0] = v[0], w[1] = v[1];
+        } else {
+          w[0] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)off, 0, 0);
+        }
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -240,18 +242,22 @@ __global__ __launch_bounds__(64 * rows_waves(CW, MT)) void q4_rows_kernel(Q4Args
         int gi = k0 / G + g;
         gi = gi < groups ? gi : groups - 1;
         const int64_t at = (int64_t)gi * N + col;
-        q.s[g].load(sp, at, last);
-        q.z[g].load(zp, at, last);
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const Q4Side& sd = p.side[s];
+          q.s[s][g].load((const unsigned short*)sd.s, at, last);
+          q.z[s][g].load((const unsigned short*)(sd.z ? sd.z : sd.s), at, last);
+        }
       }
     }
   };
 
   const Q4Bits<T> bits;
-  float tot[CW][MT][E] = {};
-  f4 acc[CW][MT], sum[MT];
+  float tot[NT][MT][E] = {};
+  f4 acc[NT][MT], sum[MT];
   const h8 ones = __builtin_bit_cast(h8, u32x4{T::kOne * 0x10001u, T::kOne * 0x10001u, T::kOne * 0x10001u,
                                                T::kOne * 0x10001u});
-  auto mul = [&](int h, const Half<CW, MT, SG>& q, bool second) {
+  auto mul = [&](int h, const Half<CW, S, MT, SG>& q, bool second) {
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const int k = (second ? kHalf : 0) + st * 32;
@@ -260,39 +266,43 @@ __global__ __launch_bounds__(64 * rows_waves(CW, MT)) void q4_rows_kernel(Q4Args
         for (int mt = 0; mt < MT; ++mt) {
           sum[mt] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int t = 0; t < CW; ++t) acc[t][mt] = f4{0.f, 0.f, 0.f, 0.f};
+          for (int t = 0; t < NT; ++t) acc[t][mt] = f4{0.f, 0.f, 0.f, 0.f};
         }
       }
-      h8 b[CW];
+      h8 b[NT];
 #pragma unroll
-      for (int t = 0; t < CW; ++t) b[t] = bits.operand(q.w[st][t]);
+      for (int t = 0; t < NT; ++t) b[t] = bits.operand(q.w[st][t]);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         const h8 a = x_operand(q.x[st][mt]);
         sum[mt] = Q4<T>::mma16(a, ones, sum[mt]);
 #pragma unroll
-        for (int t = 0; t < CW; ++t) acc[t][mt] = Q4<T>::mma16(a, b[t], acc[t][mt]);
+        for (int t = 0; t < NT; ++t) acc[t][mt] = Q4<T>::mma16(a, b[t], acc[t][mt]);
       }
       if ((k + 32) % G == 0) {  // and ends
         const int g = G < kHalf ? st : 0;
-        Cols<CW> qs = q.s[g], qz = q.z[g];
-        if (!inside) {
-          int gi = (wk + (h >> 1) * per) * (kChunk / G) + k / G;
-          gi = gi < groups ? gi : groups - 1;
-          const int64_t at = (int64_t)gi * N + col;
-          qs = qs.shifted(at, last), qz = qz.shifted(at, last);
-        }
 #pragma unroll
-        for (int t = 0; t < CW; ++t) {
-          const float s = qs.template val<T>(t);
-          const float z = Q4<T>::kBias + (sd.z ? qz.template val<T>(t) : 8.f);
+        for (int sd = 0; sd < S; ++sd) {
+          Cols<CW> qs = q.s[sd][g], qz = q.z[sd][g];
+          if (!inside) {
+            int gi = (wave + (h >> 1) * waves) * (kChunk / G) + k / G;
+            gi = gi < groups ? gi : groups - 1;
+            const int64_t at = (int64_t)gi * N + col;
+            qs = qs.shifted(at, last), qz = qz.shifted(at, last);
+          }
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int t = 0; t < CW; ++t) {
+            const float s = qs.template val<T>(t);
+            const float z = Q4<T>::kBias + (p.side[sd].z ? qz.template val<T>(t) : 8.f);
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              tot[t][mt][e] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[mt][e], acc[t][mt][e]), tot[t][mt][e]);
-              pin(tot[t][mt][e]);
-            }
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int e = 0; e < E; ++e) {
+                float& v = tot[sd * CW + t][mt][e];
+                v = __builtin_fmaf(s, __builtin_fmaf(-z, sum[mt][e], acc[sd * CW + t][mt][e]), v);
+                pin(v);
+              }
+          }
         }
       }
       // steps are not mixed: the compiler would spread their operands over more registers than there are
@@ -302,8 +312,8 @@ __global__ __launch_bounds__(64 * rows_waves(CW, MT)) void q4_rows_kernel(Q4Args
 
   // NB halves in flight.  Loads are issued without a condition, so that the
   // compiler counts them: those past the wave's last chunk read nothing.
-  const int halves = wk < chunks ? 2 * ((chunks - 1 - wk) / per + 1) : 0;
-  Half<CW, MT, SG> q[NB];
+  const int halves = wave < chunks ? 2 * ((chunks - 1 - wave) / waves + 1) : 0;
+  Half<CW, S, MT, SG> q[NB];
   if (halves) {
 #pragma unroll
     for (int i = 0; i < NB; ++i) load(i, q[i], i & 1);
@@ -322,16 +332,18 @@ __global__ __launch_bounds__(64 * rows_waves(CW, MT)) void q4_rows_kernel(Q4Args
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
-      for (int t = 0; t < CW; ++t)
-        part[(wave * TOK + (FOUR ? lg : 4 * lg + e)) * COLS + CW * j + t] = tot[t][mt][e];
+      for (int t = 0; t < NT; ++t)
+        part[((wave * TOK + (FOUR ? lg : 4 * lg + e)) * S + t / CW) * COLS + CW * j + t % CW] = tot[t][mt][e];
     __syncthreads();
     for (int i = threadIdx.x; i < TOK * COLS; i += blockDim.x) {
-      const int row = mt * 16 + i / COLS, n = n0 + i % COLS;
-      if (row >= rows || n >= N) continue;
+      const int tok = i / COLS, row = mt * 16 + tok, n = i % COLS;
+      if (row >= rows || n0 + n >= N) continue;
       float v = 0.f, u = 0.f;
-      for (int w = 0; w < per; ++w) v += part[w * TOK * COLS + i];
-      for (int w = per; w < waves; ++w) u += part[w * TOK * COLS + i];
-      q4_store<T>(p, m0 + row, n, v, u);
+      for (int w = 0; w < waves; ++w) {
+        v += part[(w * TOK + tok) * S * COLS + n];
+        if (S == 2) u += part[((w * TOK + tok) * S + 1) * COLS + n];
+      }
+      q4_store<T>(p, m0 + row, n0 + n, v, u);
     }
   }
 }
@@ -565,11 +577,13 @@ hipError_t token_launch(const Q4Args& a, int waves, int ct, int kw, const TokenL
 }
 
 // ---------------------------------------------------------------------------
-// Prompts: a workgroup of four waves computes 64 rows of 64 CW columns, a wave
-// 64 rows of 16 CW.  x goes through LDS, in the operands' order, with its
+// Many rows: a workgroup of four waves computes 64 rows of 64 CW columns, a
+// wave 16 CW of them.  x goes through LDS, in the operands' order, with its
 // groups' sums; a wave takes its words from memory itself and makes operands
 // of each once for its four row tiles.  With two weights two waves take each,
-// the same 32 CW columns of both.
+// the same 32 CW columns of both.  Where tiles are few, several workgroups share
+// one, each with a part of k, leave their sums in a workspace in fp32, and a
+// second kernel adds them in order.
 // ---------------------------------------------------------------------------
 constexpr int kTileRows = 64;
 
@@ -590,14 +604,13 @@ __device__ __forceinline__ float add_dpp(float v) {
 }
 
 template <class T, int CW, int G, bool Z>
-__global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, int ntiles) {
-  constexpr int MT = kTileRows / 16;
+__global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, int ntiles, float* ws) {
+  constexpr int MT = 4, ROWS = kTileRows;
   constexpr int GPC = kChunk / G;  // groups a chunk
   constexpr int SPG = G / 32;      // MFMA steps a group
-  constexpr int XB = kTileRows * kChunk * 2;
   __shared__ __attribute__((aligned(1024))) struct {
-    char x[2][XB];
-    float s[2][GPC][kTileRows];
+    char x[2][ROWS * kChunk * 2];
+    float s[2][GPC][ROWS];
   } lds;
   auto& xs = lds.x;
   auto& ss = lds.s;
@@ -610,11 +623,11 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, i
   const int gm0 = id / (8 * ntiles) * 8, rest = id % (8 * ntiles);
   const int gm = mtiles - gm0 < 8 ? mtiles - gm0 : 8;
   const int side = p.sides == 2 ? wave >> 1 : 0;
-  const int64_t m0 = (int64_t)(gm0 + rest % gm) * kTileRows;
+  const int64_t m0 = (int64_t)(gm0 + rest % gm) * ROWS;
   const int wcols = 64 * CW / p.sides;
   const int n0 = rest / gm * wcols, wn0 = n0 + (p.sides == 2 ? wave & 1 : wave) * (16 * CW);
   const int col = wn0 + CW * j;
-  const int rows = p.M - m0 < kTileRows ? (int)(p.M - m0) : kTileRows;
+  const int rows = p.M - m0 < ROWS ? (int)(p.M - m0) : ROWS;
   const int groups = (K + G - 1) / G, chunks = (K + kChunk - 1) / kChunk;
   const Q4Side sd = side ? p.side[1] : p.side[0];
   const auto wr = make_rsrc(sd.wq, (int)((int64_t)K * N / 2));
@@ -648,189 +661,279 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, i
       ss[buf][(tid & 15) / (G / 8)][row] = Z ? -s : -(Q4<T>::kBias + 8.f) * s;  // the same from each lane of the group
     }
   };
-  struct Words {
-    unsigned w[4][CW];
-    Cols<CW> s[GPC], z[GPC];
+  unsigned w[4][CW];
+  Cols<CW> qs[GPC], qz[GPC];
+  auto load_w = [&](int c, int st) {
+    const unsigned off = ((unsigned)(c * (kChunk / 8) + st * 4 + lg) * (unsigned)N + (unsigned)col) * 4u;
+    if constexpr (CW == 4) {
+      const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(wr, (int)off, 0, 0);
+      w[st][0] = v[0], w[st][1] = v[1], w[st][2] = v[2], w[st][3] = v[3];
+    } else if constexpr (CW == 2) {
+      const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(wr, (int)off, 0, 0);
+      w[st][0] = v[0], w[st][1] = v[1];
+    } else {
+      w[st][0] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)off, 0, 0);
+    }
   };
-  auto load_w = [&](int c, Words& q) {
-#pragma unroll
-    for (int st = 0; st < 4; ++st) {
-      const unsigned off = ((unsigned)(c * (kChunk / 8) + st * 4 + lg) * (unsigned)N + (unsigned)col) * 4u;
-      if constexpr (CW == 4) {
-        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(wr, (int)off, 0, 0);
-        for (int t = 0; t < 4; ++t) q.w[st][t] = v[t];
-      } else if constexpr (CW == 2) {
-        const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(wr, (int)off, 0, 0);
-        q.w[st][0] = v[0], q.w[st][1] = v[1];
-      } else {
-        q.w[st][0] = __builtin_amdgcn_raw_buffer_load_b32(wr, (int)off, 0, 0);
-      }
-    }
-#pragma unroll
-    for (int g = 0; g < GPC; ++g) {
-      const int gi = c * GPC + g < groups ? c * GPC + g : groups - 1;
-      q.s[g].load(sp, (int64_t)gi * N + col, last);
-      if constexpr (Z) q.z[g].load(zp, (int64_t)gi * N + col, last);
-    }
+  auto group_at = [&](int c, int g) {
+    const int gi = c * GPC + g < groups ? c * GPC + g : groups - 1;
+    return (int64_t)gi * N + col;
+  };
+  auto load_s = [&](int c, int g) {
+    qs[g].load(sp, group_at(c, g), last);
+    if constexpr (Z) qz[g].load(zp, group_at(c, g), last);
   };
 
   const Q4Bits<T> bits;
   float tot[CW][MT][4] = {};
-  // One chunk: the next one's words are asked for, the next one's x, which was
-  // asked for a chunk ago, goes to the other buffer, and the one after that is
-  // asked for.
-  auto chunk = [&](int c, int buf, Words& q, Words& next) {
-    load_w(c + 1, next);
+  // One chunk.  Registers hold one chunk's words and scales, and each is asked
+  // for again, a chunk ahead, when it has been used; the next chunk's x, which
+  // was asked for a chunk ago, goes to the other buffer.
+  auto chunk = [&](int c, int buf) {
     if (!inside) {
 #pragma unroll
       for (int g = 0; g < GPC; ++g) {
-        const int gi = c * GPC + g < groups ? c * GPC + g : groups - 1;
-        q.s[g] = q.s[g].shifted((int64_t)gi * N + col, last);
-        if constexpr (Z) q.z[g] = q.z[g].shifted((int64_t)gi * N + col, last);
+        qs[g] = qs[g].shifted(group_at(c, g), last);
+        if constexpr (Z) qz[g] = qz[g].shifted(group_at(c, g), last);
       }
     }
     h8 b[CW];
 #pragma unroll
-    for (int t = 0; t < CW; ++t) b[t] = bits.operand(q.w[0][t]);
+    for (int t = 0; t < CW; ++t) b[t] = bits.operand(w[0][t]);
+    load_w(c + 1, 0);
+    f4 acc[CW][MT];
 #pragma unroll
-    for (int g = 0; g < GPC; ++g) {
-      f4 acc[CW][MT];
+    for (int st = 0; st < 4; ++st) {
+      const int g = st / SPG;
+      h8 bn[CW];
 #pragma unroll
-      for (int st = g * SPG; st < (g + 1) * SPG; ++st) {
-        h8 bn[CW];
+      for (int mt = 0; mt < MT; ++mt) {
+        const h8 x = *(const h8*)(xs[buf] + (mt * 16 + j) * (kChunk * 2) + (((st * 4 + lg) ^ j) << 4));
+        if (st % SPG == 0) {
+          // a group's sum begins at -(B + z) times that of x
+          const f4 m = *(const f4*)&ss[buf][g][mt * 16 + 4 * lg];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const h8 a = *(const h8*)(xs[buf] + (mt * 16 + j) * (kChunk * 2) + (((st * 4 + lg) ^ j) << 4));
-          if (st == g * SPG) {
-            // a group's sum begins at -(B + z) times that of x
-            const f4 m = *(const f4*)&ss[buf][g][mt * 16 + 4 * lg];
-#pragma unroll
-            for (int t = 0; t < CW; ++t) {
-              const float z = Q4<T>::kBias + (sd.z ? q.z[g].template val<T>(t) : 8.f);
-              acc[t][mt] = Q4<T>::mma16(a, b[t], Z ? f4{z * m[0], z * m[1], z * m[2], z * m[3]} : m);
-            }
-          } else {
-#pragma unroll
-            for (int t = 0; t < CW; ++t) acc[t][mt] = Q4<T>::mma16(a, b[t], acc[t][mt]);
+          for (int t = 0; t < CW; ++t) {
+            const float z = Q4<T>::kBias + (sd.z ? qz[g].template val<T>(t) : 8.f);
+            acc[t][mt] = Q4<T>::mma16(x, b[t], Z ? f4{z * m[0], z * m[1], z * m[2], z * m[3]} : m);
           }
-          if (st < 3 && mt < CW) bn[mt] = bits.operand(q.w[st < 3 ? st + 1 : 3][mt < CW ? mt : 0]);
+        } else {
+#pragma unroll
+          for (int t = 0; t < CW; ++t) acc[t][mt] = Q4<T>::mma16(x, b[t], acc[t][mt]);
         }
         if (st < 3) {
 #pragma unroll
-          for (int t = 0; t < CW; ++t) b[t] = bn[t];
+          for (int t = mt * CW / MT; t < (mt + 1) * CW / MT; ++t) bn[t] = bits.operand(w[st < 3 ? st + 1 : 3][t]);
+        }
+        if ((st + 1) % SPG == 0) {
+#pragma unroll
+          for (int t = 0; t < CW; ++t) {
+            const float s = qs[g].template val<T>(t);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              tot[t][mt][e] = __builtin_fmaf(s, acc[t][mt][e], tot[t][mt][e]);
+              pin(tot[t][mt][e]);
+            }
+          }
         }
       }
+      if (st < 3) {
+        load_w(c + 1, st + 1);
 #pragma unroll
-      for (int t = 0; t < CW; ++t) {
-        const float s = q.s[g].template val<T>(t);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            tot[t][mt][e] = __builtin_fmaf(s, acc[t][mt][e], tot[t][mt][e]);
-            if constexpr (GPC > 1) pin(tot[t][mt][e]);
-          }
+        for (int t = 0; t < CW; ++t) b[t] = bn[t];
       }
-      if constexpr (GPC > 1) __builtin_amdgcn_sched_barrier(0);
+      if ((st + 1) % SPG == 0) load_s(c + 1, g);
     }
     put_x(buf ^ 1);
     load_x(c + 2);
-#ifdef SGB
-    if constexpr (GPC == 1) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      __builtin_amdgcn_sched_group_barrier(0x002, 36, 0);
-#pragma unroll
-      for (int i = 0; i < 4 * CW * MT; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x002, SGB, 0);
-        if (i % CW == 0) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-    }
-#endif
     lds_barrier();
   };
-  Words wa, wb;
-  load_x(0);
-  load_w(0, wa);
+  // this workgroup's part of k: all of it, or gridDim.y-th
+  const int per = (chunks + gridDim.y - 1) / gridDim.y, c0 = blockIdx.y * per, c1 = c0 + per < chunks ? c0 + per : chunks;
+  load_x(c0);
+#pragma unroll
+  for (int st = 0; st < 4; ++st) load_w(c0, st);
+#pragma unroll
+  for (int g = 0; g < GPC; ++g) load_s(c0, g);
   put_x(0);
-  load_x(1);
+  load_x(c0 + 1);
   lds_barrier();
 #pragma unroll 1
-  for (int c = 0; c < chunks; c += 2) {
-    chunk(c, 0, wa, wb);
-    if (c + 1 >= chunks) break;
-    chunk(c + 1, 1, wb, wa);
+  for (int c = c0; c < c1; c += 2) {
+    chunk(c, 0);
+    if (c + 1 >= c1) break;
+    chunk(c + 1, 1);
+  }
+
+  if (gridDim.y > 1) {
+    typedef float vec __attribute__((ext_vector_type(CW), aligned(4)));
+    float* part = ws + ((int64_t)blockIdx.y * p.sides + side) * p.M * N;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = mt * 16 + 4 * lg + e;
+        float* at = part + (m0 + row) * N + col;
+        if (row < rows && col + CW <= N) {
+          vec v;
+          if constexpr (CW == 1) v = tot[0][mt][e];
+          else
+#pragma unroll
+            for (int t = 0; t < CW; ++t) v[t] = tot[t][mt][e];
+          *(vec*)at = v;
+        } else if (row < rows) {
+#pragma unroll
+          for (int t = 0; t < CW - 1; ++t)
+            if (col + t < N) at[t] = tot[t][mt][e];
+        }
+      }
+    return;
   }
 
   // Out through LDS, half of the rows at a time: eight columns a thread, whole
   // lines a wave, and the epilogue's code once.  Of two weights the columns lie
   // side by side.
-  constexpr int TC = 64 * CW, LD = TC + 4;
-  static_assert((kTileRows / 2) * LD * 4 <= (int)sizeof(lds), "half a tile fits x's buffers");
+  constexpr int LD = 64 * CW + 4;
+  static_assert((ROWS / 2) * LD * 4 <= (int)sizeof(lds), "half a tile fits x's buffers");
   float* tile = (float*)&lds;
 #pragma unroll 1
   for (int half = 0; half < 2; ++half) {
     auto put = [&](int mt) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float* at = tile + ((mt & 1) * 16 + 4 * lg + e) * LD + wave * (16 * CW) + CW * j;
+        float* at = tile + ((mt % (MT / 2)) * 16 + 4 * lg + e) * LD + wave * (16 * CW) + CW * j;
 #pragma unroll
         for (int t = 0; t < CW; ++t) at[t] = tot[t][mt][e];
       }
     };
-    if (half) {
-      put(2);
-      put(3);
-    } else {
-      put(0);
-      put(1);
+#pragma unroll
+    for (int mt = 0; mt < MT / 2; ++mt) {
+      if (half) {
+        put(MT / 2 + mt);
+      } else {
+        put(mt);
+      }
     }
     __syncthreads();
 #pragma unroll 1
-    for (int i = tid; i < (kTileRows / 2) * (wcols / 8); i += 256) {
+    for (int i = tid; i < (ROWS / 2) * (wcols / 8); i += 256) {
       const int row = i / (wcols / 8), n = i % (wcols / 8) * 8;
-      if (half * (kTileRows / 2) + row >= rows || n0 + n >= N) continue;
+      if (half * (ROWS / 2) + row >= rows || n0 + n >= N) continue;
       float v[8], u[8];
       const float* at = tile + row * LD + n;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = at[e], u[e] = p.sides == 2 ? at[wcols + e] : 0.f;
-      q4_store8<T>(p, m0 + half * (kTileRows / 2) + row, n0 + n, N - n0 - n, v, u);
+      q4_store8<T>(p, m0 + half * (ROWS / 2) + row, n0 + n, N - n0 - n, v, u);
     }
     __syncthreads();
   }
 }
 
+// The parts of k added in order, and the epilogue: eight columns of a row a thread.
+template <class T>
+__global__ __launch_bounds__(256) void q4_join_kernel(Q4Args p, const float* ws, int parts) {
+  typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+  const int pieces = (p.N + 7) / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.M * pieces) return;
+  const int64_t m = i / pieces;
+  const int n = (int)(i - m * pieces) * 8, cnt = p.N - n;
+  float v[2][8] = {};
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      if (s >= p.sides) continue;
+      const float* at = ws + (((int64_t)k * p.sides + s) * p.M + m) * p.N + n;
+      if (cnt >= 8) {
+        const f4u a = *(const f4u*)at, b = *(const f4u*)(at + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[s][e] += a[e], v[s][4 + e] += b[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (e < cnt) v[s][e] += at[e];
+      }
+    }
+  q4_store8<T>(p, m, n, cnt, v[0], v[1]);
+}
+
+// How a product on tiles is cut: columns of a tile (64 CW) and parts of k.
+struct TilePlan {
+  int cw, parts;
+};
+// The least of an estimate in us.  A chunk takes a workgroup `alone` by itself
+// on its CU and `shared` in company (4096 k are 32 chunks: 64 rows of 4,096
+// columns 50, 37 and 30 us with CW 4, 2 and 1; 1,024 rows, which are one, two and
+// four workgroups a CU, 52, 53 and 63); the second kernel takes 3 us and the
+// workspace's way to memory and back.  128 rows of 4,096 columns from 4,096 k:
+// 64 columns a tile and three parts 20 us, 256 columns in one part 50.
+TilePlan tile_plan(int64_t M, int N, int K, int sides, int num_cus) {
+  const int64_t mtiles = (M + kTileRows - 1) / kTileRows;
+  const int chunks = (K + kChunk - 1) / kChunk;
+  TilePlan best{4, 1};
+  float least = 0.f;
+  for (int cw = 4; cw >= 1; cw /= 2) {
+    const int64_t cols = 64 * cw / sides, tiles = mtiles * ((N + cols - 1) / cols);
+    const float alone = cw == 4 ? 1.5f : cw == 2 ? 1.1f : 0.85f, shared = cw == 4 ? 1.25f : cw == 2 ? 0.8f : 0.47f;
+    for (int parts = 1; parts <= 16 && parts <= chunks; ++parts) {
+      const float per_cu = (float)((tiles * parts + num_cus - 1) / num_cus);
+      const float turn = shared * per_cu > alone ? shared * per_cu : alone;
+      float t = (float)((chunks + parts - 1) / parts) * turn;
+      if (parts > 1) t += 3.f + (float)parts * (float)M * (float)N * (float)sides * 8.f / 4e6f;
+      if (least == 0.f || t < least) best = TilePlan{cw, parts}, least = t;
+    }
+  }
+  return best;
+}
+
 template <class T, int CW>
-hipError_t tile_launch(const Q4Args& a, hipStream_t s) {
-  const int64_t mtiles = (a.M + kTileRows - 1) / kTileRows, cols = 64 * CW / a.sides, ntiles = (a.N + cols - 1) / cols;
+hipError_t tile_launch(const Q4Args& a, int parts, hipStream_t s) {
+  const int64_t mtiles = (a.M + kTileRows - 1) / kTileRows, cols = 64 * CW / a.sides;
+  const int64_t ntiles = (a.N + cols - 1) / cols;
   if (mtiles * ntiles > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)(mtiles * ntiles)), block(256);
+  const dim3 grid((unsigned)(mtiles * ntiles), (unsigned)parts), block(256);
   const bool z = a.side[0].z || a.side[1].z;
-#define GP_CASE(g)                                                                                                  \
-  case g:                                                                                                           \
-    if (z)                                                                                                          \
-      hipLaunchKernelGGL((q4_tile_kernel<T, CW, g, true>), grid, block, 0, s, a, (int)mtiles, (int)ntiles);         \
-    else                                                                                                            \
-      hipLaunchKernelGGL((q4_tile_kernel<T, CW, g, false>), grid, block, 0, s, a, (int)mtiles, (int)ntiles);        \
+  float* ws = (float*)a.ws;
+#define GP_CASE(g)                                                                                                \
+  case g:                                                                                                         \
+    if (z)                                                                                                        \
+      hipLaunchKernelGGL((q4_tile_kernel<T, CW, g, true>), grid, block, 0, s, a, (int)mtiles, (int)ntiles, ws);   \
+    else                                                                                                          \
+      hipLaunchKernelGGL((q4_tile_kernel<T, CW, g, false>), grid, block, 0, s, a, (int)mtiles, (int)ntiles, ws);  \
     break;
   switch (a.group) {
     GP_CASE(32) GP_CASE(64) GP_CASE(128)
     default: return hipErrorInvalidValue;
   }
 #undef GP_CASE
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || parts == 1) return e;
+  const int64_t pieces = a.M * ((a.N + 7) / 8);
+  hipLaunchKernelGGL((q4_join_kernel<T>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, a,
+                     (const float*)a.ws, parts);
   return hipGetLastError();
 }
 
-template <class T, int CW, int MT, bool FOUR, int NB>
+template <class T, int CW, int S, int MT, bool FOUR, int NB>
 hipError_t rows_launch(const Q4Args& a, int waves, dim3 grid, hipStream_t s) {
   const dim3 block(waves * kWave);
   switch (a.group) {
-    case 32: hipLaunchKernelGGL((q4_rows_kernel<T, CW, MT, 32, FOUR, NB>), grid, block, 0, s, a); break;
-    case 64: hipLaunchKernelGGL((q4_rows_kernel<T, CW, MT, 64, FOUR, NB>), grid, block, 0, s, a); break;
-    case 128: hipLaunchKernelGGL((q4_rows_kernel<T, CW, MT, 128, FOUR, NB>), grid, block, 0, s, a); break;
+    case 32: hipLaunchKernelGGL((q4_rows_kernel<T, CW, S, MT, 32, FOUR, NB>), grid, block, 0, s, a); break;
+    case 64: hipLaunchKernelGGL((q4_rows_kernel<T, CW, S, MT, 64, FOUR, NB>), grid, block, 0, s, a); break;
+    case 128: hipLaunchKernelGGL((q4_rows_kernel<T, CW, S, MT, 128, FOUR, NB>), grid, block, 0, s, a); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
+}
+
+// Products that run on tiles: those of more than 64 rows, and of more than 48
+// where the few-row kernel would read x for too many columns (64 rows, k 4096:
+// 4,096 columns 20 us against 18 on tiles, 16,384 28 against 23, 2 x 16,384 55
+// against 34; k 1024, 2 x 4,096 9.3 against 10).
+bool on_tiles(int64_t M, int N, int K, int group, int sides) {
+  if ((int64_t)((K + group - 1) / group) * N < 4) return false;  // a tile's loads of scales are four wide
+  return M > 64 || (M > 48 && (int64_t)N * sides > 8192);
 }
 
 template <class T>
@@ -845,25 +948,29 @@ hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
     const TokenLds l = token_lds((int)a.M, a.K, a.group, waves, kw, z);
     if (l.bytes <= 155 * 1024) return token_launch<T>(a, waves, ct, kw, l, s);
   }
-  if (a.M > 64) {
-    // The widest tiles that leave every CU the two workgroups that fit it: a
-    // wave's operands and its reads of x serve more columns.  509 x 1024 x
-    // 2 x 4096: 128 columns 21.7 us, 64 25.1, 256 24.0.
-    const int64_t mtiles = (a.M + kTileRows - 1) / kTileRows;
-    int cw = 4;
-    while (cw > 1 && mtiles * ((a.N + 64 * cw / a.sides - 1) / (64 * cw / a.sides)) < 2 * num_cus) cw /= 2;
-    if ((int64_t)((a.K + a.group - 1) / a.group) * a.N < 4) cw = 1;
-    return cw == 4 ? tile_launch<T, 4>(a, s) : cw == 2 ? tile_launch<T, 2>(a, s) : tile_launch<T, 1>(a, s);
+  if (on_tiles(a.M, a.N, a.K, a.group, a.sides)) {
+    TilePlan plan = tile_plan(a.M, a.N, a.K, a.sides, num_cus);
+    if (a.ws_bytes < (plan.parts > 1 ? (int64_t)plan.parts * a.sides * a.M * a.N * 4 : 0)) plan.parts = 1;
+    return plan.cw == 4   ? tile_launch<T, 4>(a, plan.parts, s)
+           : plan.cw == 2 ? tile_launch<T, 2>(a, plan.parts, s)
+                          : tile_launch<T, 1>(a, plan.parts, s);
   }
   const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : a.M <= 48 ? 3 : 4;
-  int cw = a.N >= 64 * num_cus ? 4 : a.N >= 32 * num_cus ? 2 : 1;
-  if (const char* v = getenv("Q4_CW")) cw = atoi(v);
-  if ((int64_t)((a.K + a.group - 1) / a.group) * a.N < 4) cw = 1;
-  int waves = rows_waves(cw, mt);
-  while (waves > 2 * a.sides && waves / 2 >= chunks * a.sides) waves /= 2;
+  // Tiles of 16 columns a wave, both weights' together: as many as leave every
+  // CU a workgroup, so that x is read for more columns at once.
+  const int64_t n = (int64_t)a.N * a.sides;
+  int nt = n >= 64 * num_cus ? 4 : n >= 32 * num_cus ? 2 : 1;
+  if ((int64_t)((a.K + a.group - 1) / a.group) * a.N < 4) nt = 1;
+  const int cw = nt > a.sides ? nt / a.sides : 1;
+  int waves = rows_waves(cw * a.sides, mt);
+  while (waves > 2 && waves / 2 >= chunks) waves /= 2;
   const dim3 grid((unsigned)((a.N + 16 * cw - 1) / (16 * cw)), (unsigned)((a.M + 16 * mt - 1) / (16 * mt)));
-#define GP_CASE(c, m, four, nb) \
-  if (cw == c && mt == m && (a.M <= 4) == four) return rows_launch<T, c, m, four, nb>(a, waves, grid, s);
+#define GP_CASE(c, m, four, nb)                                                                                \
+  if (cw == c && a.sides == 1 && mt == m && (a.M <= 4) == four)                                               \
+    return rows_launch<T, c, 1, m, four, nb>(a, waves, grid, s);                                              \
+  if constexpr (c <= 2)                                                                                       \
+    if (cw == c && a.sides == 2 && mt == m && (a.M <= 4) == four)                                             \
+      return rows_launch<T, c, 2, m, four, 2>(a, waves, grid, s);
   GP_CASE(1, 1, true, 4) GP_CASE(2, 1, true, 4) GP_CASE(4, 1, true, 2)
   GP_CASE(1, 1, false, 4) GP_CASE(2, 1, false, 2) GP_CASE(4, 1, false, 2)
   GP_CASE(1, 2, false, 2) GP_CASE(2, 2, false, 2) GP_CASE(4, 2, false, 2)
@@ -874,6 +981,12 @@ hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
 }
 
 }  // namespace
+
+int64_t q4_workspace(int64_t M, int N, int K, int group, int sides, int num_cus) {
+  if (!on_tiles(M, N, K, group, sides)) return 0;
+  const TilePlan plan = tile_plan(M, N, K, sides, num_cus);
+  return plan.parts == 1 ? 0 : (int64_t)plan.parts * sides * M * N * 4;
+}
 
 hipError_t q4_launch(const Q4Args& a, int num_cus, hipStream_t s) {
   return a.dtype == GP_DTYPE_BF16 ? launch<BF16>(a, num_cus, s) : launch<F16>(a, num_cus, s);

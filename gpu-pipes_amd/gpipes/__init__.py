@@ -118,9 +118,11 @@ def _load():
     L.gp_residual_norm_out.argtypes = [i64, i64, vp, vp, i32, vp, vp, f32, vp, i64, i32, f32, i32, vp, vp, f32, vp, vp,
                                        i32, vp]
     L.gp_residual_norm_out.restype = i32
-    L.gp_q4_gemm_out.argtypes = [i64, i64, i64, i32] + [vp] * 6 + [i32, vp, i32, vp]
+    L.gp_q4_gemm_out.argtypes = [i64, i64, i64, i32] + [vp] * 6 + [i32, vp, vp, i64, i32, vp]
     L.gp_q4_gemm_out.restype = i32
-    L.gp_q4_gated_out.argtypes = [i64, i64, i64, i32] + [vp] * 9 + [i32, vp, i32, vp]
+    L.gp_q4_gated_out.argtypes = [i64, i64, i64, i32] + [vp] * 9 + [i32, vp, vp, i64, i32, vp]
+    L.gp_q4_workspace_bytes.argtypes = [i64, i64, i64, i32, i32]
+    L.gp_q4_workspace_bytes.restype = i64
     L.gp_q4_gated_out.restype = i32
     for name in ("gp_mlp_out", "gp_dlrm_botmlp_out", "gp_dlrm_topmlp_out", "gp_nerf_full_out", "gp_gemm_out",
                  "gp_gemm_dtype_out", "gp_bert_ffn_out", "gp_bert_ffn_dtype_out", "gp_linear_out", "gp_linear_layer_norm_out", "gp_layer_norm_out", "gp_add_out",
@@ -1014,6 +1016,19 @@ def _q4_weight(wq, scales, zeros, words, groups, dt, dev):
                                    and zeros.is_contiguous())))
 
 
+def _q4_workspace(M, N, K, group, weights, x):
+    """(tensor, address, bytes) of a 4-bit product's workspace: the call's own, from torch's allocator, which hands it
+    on in the stream's order and keeps it for a graph that is being captured."""
+    with _on(x):
+        n = lib.gp_q4_workspace_bytes(M, N, K, group, weights)
+    if n < 0:
+        _check(n)
+    if n == 0:
+        return None, None, 0
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    return ws, ws.data_ptr(), n
+
+
 def _q4_refuse(x, group, named):
     """Raises for what is wrong with a 4-bit product's x, group or tensors: (name, tensor, kind)."""
     _check_rows(x)
@@ -1052,10 +1067,11 @@ def q4_gemm_out(x, wq, scales, zeros=None, b=None, r=None, act="none", group=128
     if not ok:
         _q4_refuse(x, group, [("wq", wq, "words"), ("scales", scales, "groups"), ("zeros", zeros, "groups"),
                               ("b", b, "bias"), ("r", r, "rows"), ("out", out, "rows")])
+    ws, at, n = (None, None, 0) if M <= 48 else _q4_workspace(M, N, K, group, 1, x)
     _run_on(dev, lib.gp_q4_gemm_out,
             (M, N, K, group, x.data_ptr(), wq.data_ptr(), scales.data_ptr(),
              None if zeros is None else zeros.data_ptr(), None if b is None else b.data_ptr(),
-             None if r is None else r.data_ptr(), ACTS.get(act, act), out.data_ptr(), _DTYPES[dt]))
+             None if r is None else r.data_ptr(), ACTS.get(act, act), out.data_ptr(), at, n, _DTYPES[dt]))
     return out
 
 
@@ -1082,9 +1098,10 @@ def q4_gated_out(x, wq_g, scales_g, zeros_g, wq_u, scales_u, zeros_u, bg=None, b
         _q4_refuse(x, group, [("wq_g", wq_g, "words"), ("scales_g", scales_g, "groups"), ("zeros_g", zeros_g, "groups"),
                               ("wq_u", wq_u, "words"), ("scales_u", scales_u, "groups"), ("zeros_u", zeros_u, "groups"),
                               ("bg", bg, "bias"), ("bu", bu, "bias"), ("out", out, "rows")])
+    ws, at, n = (None, None, 0) if M <= 48 else _q4_workspace(M, N, K, group, 2, x)
     _run_on(dev, lib.gp_q4_gated_out,
             (M, N, K, group, x.data_ptr(), wq_g.data_ptr(), scales_g.data_ptr(),
              None if zeros_g is None else zeros_g.data_ptr(), None if bg is None else bg.data_ptr(), wq_u.data_ptr(),
              scales_u.data_ptr(), None if zeros_u is None else zeros_u.data_ptr(),
-             None if bu is None else bu.data_ptr(), ACTS.get(act, act), out.data_ptr(), _DTYPES[dt]))
+             None if bu is None else bu.data_ptr(), ACTS.get(act, act), out.data_ptr(), at, n, _DTYPES[dt]))
     return out

@@ -565,6 +565,13 @@ int gp_residual_norm_out(int64_t M, int64_t D, const void* x, const void* y, int
                          int dtype, void* stream);
 
 /*
+ * Bytes of workspace with which gp_q4_gemm_out (weights 1) or gp_q4_gated_out
+ * (weights 2) is fastest at these sizes on the current device; 0 up to 48 rows
+ * and for large products; negative: GP_ERR_*.
+ */
+int64_t gp_q4_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int weights);
+
+/*
  * Products with 4-bit weights, one token to whole prompts:
  *   out[M,N] = act(x[M,K] W + b), or x W + b + r (act GP_ACT_NONE),
  *   W[k][n] = scales[k / group][n] * (q[k][n] - zeros[k / group][n]).
@@ -579,12 +586,18 @@ int gp_residual_norm_out(int64_t M, int64_t D, const void* x, const void* y, int
  * its 128 neighbours k, about what an fp32 sum of them keeps.)
  * x has to be finite and, in bf16, 150 times a group's sum of |x| below fp32's
  * largest number: a row of x that is not gives NaN in that row of out alone.
- * One launch, no workspace: can be captured into a graph; out must not
- * overlap x (it may be r).
+ * workspace: scratch of the call's own, workspace_bytes long (16-byte aligned,
+ * contents of no matter), as gp_q4_workspace_bytes gives it: with more than 48
+ * rows and few columns parts of K are multiplied apart and added in a second
+ * launch, always in one order.  With less (0 and NULL) the product is computed
+ * in one launch, more slowly, and may differ in a sum's last bits.  Calls that
+ * may run at the same time, in graphs too, need workspaces of their own.
+ * Can be captured into a graph; out must not overlap x (it may be r).
  * No counterpart in the reference (16-bit weights only).
  */
 int gp_q4_gemm_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq, const void* scales,
-                   const void* zeros, const void* b, const void* r, int act, void* out, int dtype, void* stream);
+                   const void* zeros, const void* b, const void* r, int act, void* out, void* workspace,
+                   int64_t workspace_bytes, int dtype, void* stream);
 
 /*
  * The first half of a gated feed-forward block:
@@ -594,7 +607,8 @@ int gp_q4_gemm_out(int64_t M, int64_t N, int64_t K, int group, const void* x, co
  */
 int gp_q4_gated_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq_g, const void* scales_g,
                     const void* zeros_g, const void* b_g, const void* wq_u, const void* scales_u, const void* zeros_u,
-                    const void* b_u, int act, void* out, int dtype, void* stream);
+                    const void* b_u, int act, void* out, void* workspace, int64_t workspace_bytes, int dtype,
+                    void* stream);
 
 #ifdef __cplusplus
 }

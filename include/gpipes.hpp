@@ -169,18 +169,21 @@ inline void residual_norm_out(int64_t M, int64_t D, const void* x, const void* y
                              gamma, beta, eps, h, out, dtype, stream));
 }
 
-// Products with 4-bit weights (gp_q4_gemm_out, gp_q4_gated_out).
+// Products with 4-bit weights (gp_q4_gemm_out, gp_q4_gated_out); workspace as
+// gp_q4_workspace_bytes says, or none.
 inline void q4_gemm_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq, const void* scales,
                         const void* zeros, const void* b, const void* r, int act, void* out,
-                        int dtype = GP_DTYPE_F16, void* stream = nullptr) {
-  check(gp_q4_gemm_out(M, N, K, group, x, wq, scales, zeros, b, r, act, out, dtype, stream));
+                        int dtype = GP_DTYPE_F16, void* stream = nullptr, void* workspace = nullptr,
+                        int64_t workspace_bytes = 0) {
+  check(gp_q4_gemm_out(M, N, K, group, x, wq, scales, zeros, b, r, act, out, workspace, workspace_bytes, dtype, stream));
 }
 inline void q4_gated_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq_g,
                          const void* scales_g, const void* zeros_g, const void* b_g, const void* wq_u,
                          const void* scales_u, const void* zeros_u, const void* b_u, int act, void* out,
-                         int dtype = GP_DTYPE_F16, void* stream = nullptr) {
-  check(gp_q4_gated_out(M, N, K, group, x, wq_g, scales_g, zeros_g, b_g, wq_u, scales_u, zeros_u, b_u, act, out, dtype,
-                        stream));
+                         int dtype = GP_DTYPE_F16, void* stream = nullptr, void* workspace = nullptr,
+                         int64_t workspace_bytes = 0) {
+  check(gp_q4_gated_out(M, N, K, group, x, wq_g, scales_g, zeros_g, b_g, wq_u, scales_u, zeros_u, b_u, act, out,
+                        workspace, workspace_bytes, dtype, stream));
 }
 
 }  // namespace gpipes

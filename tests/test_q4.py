@@ -20,13 +20,15 @@ U = 2.0 ** -24
 # Without a GPU
 # ---------------------------------------------------------------------------
 
-def _call(M=4, N=256, K=512, group=128, x=16, wq=16, s=16, z=0, b=0, r=0, act=0, out=32, dtype=0, two=False, u=16):
+def _call(M=4, N=256, K=512, group=128, x=16, wq=16, s=16, z=0, b=0, r=0, act=0, out=32, dtype=0, two=False, u=16,
+          ws=0, wsb=0):
     vp = ctypes.c_void_p
     P = lambda v: vp(v) if v else None  # noqa: E731
     if two:
         return gpipes.lib.gp_q4_gated_out(M, N, K, group, P(x), P(wq), P(s), P(z), P(b), P(u), P(s), P(z), P(b), act,
-                                          P(out), dtype, None)
-    return gpipes.lib.gp_q4_gemm_out(M, N, K, group, P(x), P(wq), P(s), P(z), P(b), P(r), act, P(out), dtype, None)
+                                          P(out), P(ws), wsb, dtype, None)
+    return gpipes.lib.gp_q4_gemm_out(M, N, K, group, P(x), P(wq), P(s), P(z), P(b), P(r), act, P(out), P(ws), wsb, dtype,
+                                     None)
 
 
 @pytest.mark.parametrize("two", [False, True])
@@ -35,7 +37,7 @@ def _call(M=4, N=256, K=512, group=128, x=16, wq=16, s=16, z=0, b=0, r=0, act=0,
     (dict(K=12), -2), (dict(K=65544), -2), (dict(K=65536, N=65536), -2), (dict(group=16), -2), (dict(group=256), -2),
     (dict(group=0), -2), (dict(dtype=2), -1), (dict(act=5), -1), (dict(act=-1), -1), (dict(x=0), -1), (dict(wq=0), -1),
     (dict(s=0), -1), (dict(out=0), -1), (dict(x=24), -3), (dict(wq=20), -3), (dict(s=18), -3), (dict(z=8), -3),
-    (dict(b=2), -3), (dict(out=40), -3),
+    (dict(b=2), -3), (dict(out=40), -3), (dict(wsb=-1), -1), (dict(wsb=64), -1), (dict(ws=24, wsb=64), -3),
 ])
 def test_argument_errors(kw, code, two):
     assert _call(**kw, two=two) == code
@@ -53,6 +55,13 @@ def test_empty_batch_is_a_noop():
     assert _call(M=0, x=0, out=0) == 0
     assert _call(M=0, x=0, out=0, two=True) == 0
     assert gpipes.lib.gp_last_error().decode() == ""
+
+
+@pytest.mark.parametrize("args,code", [((-1, 64, 64, 32, 1), -1), ((64, 0, 64, 32, 1), -2), ((64, 64, 60, 32, 1), -2),
+                                       ((64, 64, 64, 33, 1), -2), ((64, 64, 64, 32, 3), -1), ((64, 64, 64, 32, 0), -1),
+                                       ((0, 64, 64, 32, 1), 0)])
+def test_workspace_arguments(args, code):
+    assert gpipes.lib.gp_q4_workspace_bytes(*args) == code
 
 
 def test_python_refuses():
@@ -317,6 +326,44 @@ def test_rows_do_not_depend_on_their_neighbours(cuda, M):
     b = r.clone()
     gpipes.q4_gemm_out(x, *args, r=b, out=b)
     assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,two", [(65, 4096, 520, False), (100, 4096, 4098, False), (64, 8200, 4104, True),
+                                       (128, 8192, 256, True), (200, 5000, 250, False)])
+def test_parts_of_k(cuda, M, K, N, two):
+    """With the workspace that is asked for, without one, and with one that is too small: within the bounds each time,
+    nothing behind the workspace's end written, the last two the same bits."""
+    L, vp = gpipes.lib, ctypes.c_void_p
+    weights = 2 if two else 1
+    need = L.gp_q4_workspace_bytes(M, N, K, 64, weights)
+    assert need > 0
+    gen = torch.Generator().manual_seed(M)
+    x = torch.randn(M, K, generator=gen).to(BF16)
+    sides = [weight(K, N, 64, True, BF16, gen) for _ in range(weights)]
+    v, dv = product(x, *sides[0], 64)
+    if two:
+        u, du = product(x, *sides[1], 64)
+        g, dg = moved(v, dv, "silu")
+        v, dv = g * u, dg * (u.abs() + du) + g.abs() * du + 2 * U * (g * u).abs()
+    xd, ts = x.to(cuda), [[dev(t, cuda) for t in (q4.pack(q), s, z)] for q, s, z in sides]
+    ws = torch.full((need // 4 + 1024,), 7.0, device=cuda)
+    outs = []
+    for n in (need, need - 16, 0):
+        out = torch.empty(M, N, dtype=BF16, device=cuda)
+        args = [vp(t.data_ptr()) for side in ts for t in side]
+        stream = vp(torch.cuda.current_stream().cuda_stream)
+        if two:
+            rc = L.gp_q4_gated_out(M, N, K, 64, vp(xd.data_ptr()), *args[:3], None, *args[3:], None, 4,
+                                   vp(out.data_ptr()), vp(ws.data_ptr()), n, 1, stream)
+        else:
+            rc = L.gp_q4_gemm_out(M, N, K, 64, vp(xd.data_ptr()), *args, None, None, 0, vp(out.data_ptr()),
+                                  vp(ws.data_ptr()), n, 1, stream)
+        assert rc == 0, L.gp_last_error().decode()
+        check(out, v, dv, BF16)
+        outs.append(out)
+    assert (ws[need // 4:] == 7).all()
+    assert torch.equal(outs[1], outs[2])
 
 
 @pytest.mark.gpu
