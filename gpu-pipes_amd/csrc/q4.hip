@@ -172,7 +172,7 @@ struct Cols {
 // product share those reads.
 // ---------------------------------------------------------------------------
 // Waves of a workgroup at most: as many as its registers leave room for.
-constexpr int rows_waves(int tiles, int mt) { return mt == 1 ? 16 : 8; }
+constexpr int rows_waves(int mt) { return mt == 1 ? 16 : 8; }
 
 template <int CW, int S, int MT, int SG>
 struct Half {
@@ -182,13 +182,13 @@ struct Half {
 };
 
 template <class T, int CW, int S, int MT, int G, bool FOUR, int NB>
-__global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4Args p) {
+__global__ __launch_bounds__(64 * rows_waves(MT)) void q4_rows_kernel(Q4Args p) {
   constexpr int SG = G < kHalf ? kHalf / G : 1;  // groups a half (G 128: one every other half)
   constexpr int E = FOUR ? 1 : 4;                // accumulator elements that hold rows (FOUR: at most four rows)
   constexpr int COLS = 16 * CW, NT = S * CW;
   constexpr int TOK = FOUR ? 4 : 16;
   static_assert(NB % 2 == 0, "a buffer holds first halves or second halves");
-  __shared__ float part[rows_waves(NT, MT) * TOK * COLS * S];
+  __shared__ float part[rows_waves(MT) * TOK * COLS * S];
   const int lane = threadIdx.x & 63, j = lane & 15, lg = lane >> 4;
   const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int N = p.N, K = p.K;
@@ -377,6 +377,7 @@ __global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4
 constexpr int kTokenCols = 16;
 constexpr int kDigits = 4;
 constexpr int kRing = 2;  // chunks of 1 KiB that a wave has in flight
+constexpr int kTokenLds = 155 * 1024;  // of dynamic LDS at most: a CU's 160 KiB less 4 for the waves' sums
 
 // LDS, in this order: x's digits, rows of K bytes 16 bytes apart in banks; the
 // powers, a byte a chunk; every wave's ring; every wave's scales and zeros, 32
@@ -566,7 +567,7 @@ template <class T>
 hipError_t token_launch(const Q4Args& a, int waves, int ct, int kw, const TokenLds& l, hipStream_t s) {
   const auto kern = &q4_token_kernel<T>;
   if (l.bytes > 60 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, l.bytes);
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kTokenLds);
     if (e != hipSuccess) return e;
   }
   const int cols = kTokenCols * ct;
@@ -946,7 +947,7 @@ hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
     const int waves = kw * ct * a.sides;
     const bool z = a.side[0].z || a.side[1].z;
     const TokenLds l = token_lds((int)a.M, a.K, a.group, waves, kw, z);
-    if (l.bytes <= 155 * 1024) return token_launch<T>(a, waves, ct, kw, l, s);
+    if (l.bytes <= kTokenLds) return token_launch<T>(a, waves, ct, kw, l, s);
   }
   if (on_tiles(a.M, a.N, a.K, a.group, a.sides)) {
     TilePlan plan = tile_plan(a.M, a.N, a.K, a.sides, num_cus);
@@ -962,7 +963,7 @@ hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
   int nt = n >= 64 * num_cus ? 4 : n >= 32 * num_cus ? 2 : 1;
   if ((int64_t)((a.K + a.group - 1) / a.group) * a.N < 4) nt = 1;
   const int cw = nt > a.sides ? nt / a.sides : 1;
-  int waves = rows_waves(cw * a.sides, mt);
+  int waves = rows_waves(mt);
   while (waves > 2 && waves / 2 >= chunks) waves /= 2;
   const dim3 grid((unsigned)((a.N + 16 * cw - 1) / (16 * cw)), (unsigned)((a.M + 16 * mt - 1) / (16 * mt)));
 #define GP_CASE(c, m, four, nb)                                                                                \

@@ -486,3 +486,29 @@ def test_two_streams_and_two_graphs(cuda):
         torch.cuda.synchronize()
         for x, args, out, want, g, st in sets:
             assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(1, 16384, 1040), (4, 8192, 520), (100, 4096, 1032), (64, 8192, 8200)])
+def test_graph_of_a_deep_product(cuda, M, K, N):
+    """Calls whose LDS is above the default limit, and calls with parts of k in a workspace: a graph replayed with other
+    calls before and behind it gives the eager call's bits each time."""
+    gen = torch.Generator().manual_seed(K + M)
+    q, s, z = weight(K, N, 128, True, BF16, gen)
+    args = [dev(t, cuda) for t in (q4.pack(q), s, z)]
+    x, x2 = (torch.randn(M, K, generator=gen).to(BF16).to(cuda) for _ in range(2))
+    out = torch.empty(M, N, dtype=BF16, device=cuda)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        gpipes.q4_gemm_out(x, *args, out=out)
+    for i in range(3):
+        x.copy_(torch.randn(M, K, generator=gen).to(BF16))
+        want = gpipes.q4_gemm_out(x, *args)
+        out.zero_()
+        gpipes.q4_gemm_out(x2, *args)
+        torch.cuda.synchronize()
+        graph.replay()
+        gpipes.q4_gemm_out(x2, *args)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
