@@ -169,9 +169,15 @@ struct Cols {
 // workgroup's 16 CW columns of S weights, and the shares are joined through
 // LDS in the order of the waves.  A workgroup reads all of x, from L2, which
 // costs more than its words where rows are many; the two weights of a gated
-// product share those reads.
+// product share those reads.  Bound by a CU's loads (16 rows, 8,192 columns
+// from 8,192 k: 13.6 us, 2.7 TB/s; a CU's 128 KiB of words would take 5 us at
+// the 26 bytes a ns that it gets from the last cache, its 256 KiB of x 3.7 us
+// at the 70 from L2, and the rest is the first loads' latency and the join);
+// with 48 rows (2 x 8,192 columns from 2,048 k: 14.0 us) by those of x alone.
 // ---------------------------------------------------------------------------
-// Waves of a workgroup at most: as many as its registers leave room for.
+// Waves of a workgroup at most.  Above 16 rows sixteen fit the registers too
+// where a wave's tiles are few, and are slower (4,096 columns from 4,096 k, 48
+// rows: eight waves 15.5 us, sixteen 16.5; 20 rows 9.0 and 9.8).
 constexpr int rows_waves(int mt) { return mt == 1 ? 16 : 8; }
 
 template <int CW, int S, int MT, int SG>
@@ -372,7 +378,12 @@ __global__ __launch_bounds__(64 * rows_waves(MT)) void q4_rows_kernel(Q4Args p) 
 // wave has run yet is fetched from memory too.  So all that the workgroup will
 // read is asked for first: x, the scales and kRing chunks of every wave's
 // words, the latter by copies into LDS that hold no registers; and the code
-// is short (rolled loops, no copy of it for a size of group).
+// is short (rolled loops, no copy of it for a size of group).  One row, 2 x
+// 16,384 columns from 4,096 k: 12.7 us, 5.5 TB/s; 4,096 columns from 16,384 k:
+// 10.2 us, 3.4 TB/s, of which 5 are the words and 2 to 3 the digits of x, that
+// every workgroup makes for itself; 1,024 from 1,024: 3.6 us, the latencies of
+// a launch, two loads and the join.  Rings of four to eight chunks were slower
+// (more LDS to hand out, later first words).
 // ---------------------------------------------------------------------------
 constexpr int kTokenCols = 16;
 constexpr int kDigits = 4;
@@ -585,6 +596,15 @@ hipError_t token_launch(const Q4Args& a, int waves, int ct, int kw, const TokenL
 // the same 32 CW columns of both.  Where tiles are few, several workgroups share
 // one, each with a part of k, leave their sums in a workspace in fp32, and a
 // second kernel adds them in order.
+//
+// Bound by instruction issue: two waves a SIMD run about 430 instructions a
+// chunk for 64 MFMAs (64 and-ors and 48 shifts that make operands, 64 fused
+// multiply-adds of the groups' ends), the matrix cores busy 38% of the time and
+// the vector units 57%.  4,096 rows, 4,096 columns from 4,096 k: 147 us, 0.93
+// PFLOP/s (this card's library product of 16-bit operands of that size: 127).
+// Tried and no faster: operands one to four steps ahead, words copied to LDS
+// two chunks ahead, MFMAs and operand instructions interleaved by the scheduler's
+// groups (163), wave priorities, offsets in scalar registers.
 // ---------------------------------------------------------------------------
 constexpr int kTileRows = 64;
 

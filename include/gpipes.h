@@ -583,7 +583,8 @@ int64_t gp_q4_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int we
  * but wq `dtype`, every pointer 16-byte aligned.
  * Weights are not rounded: products are exact, sums fp32, out rounded once.
  * (With up to four rows a value of x may be taken to 2^-19 of the largest of
- * its 128 neighbours k, about what an fp32 sum of them keeps.)
+ * its 128 neighbours k, about what an fp32 sum of them keeps.  In bf16 values
+ * of x below 2^-122 may count as zero.)
  * x has to be finite and, in bf16, 150 times a group's sum of |x| below fp32's
  * largest number: a row of x that is not gives NaN in that row of out alone.
  * workspace: scratch of the call's own, workspace_bytes long (16-byte aligned,
