@@ -40,6 +40,11 @@ int check_norm(int kind, const void* gamma, const void* beta, float eps, const c
   return GP_OK;
 }
 
+// Whether `n` values of 16 bits at a and `m` at b have memory in common (NULL has none).
+bool meet(const void* a, int64_t n, const void* b, int64_t m) {
+  return a && b && (uintptr_t)a < (uintptr_t)b + 2 * (uintptr_t)m && (uintptr_t)b < (uintptr_t)a + 2 * (uintptr_t)n;
+}
+
 constexpr int64_t kQ4MaxDim = int64_t(1) << 20;
 
 int check16(const void* p, const char* name, bool needed) {
@@ -76,6 +81,12 @@ int q4_run(const Q4Args& a, int64_t N, int64_t K, hipStream_t stream) {
   if ((rc = check16(a.r, "r", false))) return rc;
   if (a.M == 0) return GP_OK;
   if ((rc = check16(a.x, "x", true)) || (rc = check16(a.out, "out", true))) return rc;
+  if (meet(a.out, a.M * N, a.x, a.M * K)) return fail(GP_ERR_INVALID_ARG, "out must not overlap x");
+  if (a.r != a.out && meet(a.out, a.M * N, a.r, a.M * N))
+    return fail(GP_ERR_INVALID_ARG, "out may be r, but not overlap it otherwise");
+  if (meet(a.ws, a.ws_bytes / 2, a.x, a.M * K) || meet(a.ws, a.ws_bytes / 2, a.out, a.M * N) ||
+      meet(a.ws, a.ws_bytes / 2, a.r, a.M * N))
+    return fail(GP_ERR_INVALID_ARG, "the workspace must not overlap x, r or out");
   int dev = 0, ncu = 0;
   if ((rc = current_device_info(&dev, &ncu))) return rc;
   Q4Args b = a;
@@ -122,6 +133,16 @@ int gp_residual_norm_out(int64_t M, int64_t D, const void* x, const void* y, int
   const void* all[] = {x, y, post_gamma, post_beta, gate, gamma, beta, h, out};
   for (const void* p : all)
     if ((uintptr_t)p % 2) return fail(GP_ERR_ALIGN, "every tensor must be 2-byte aligned");
+  if (meet(h, M * D, out, M * D)) return fail(GP_ERR_INVALID_ARG, "h and out must not overlap");
+  for (const void* o : {(const void*)h, (const void*)out}) {
+    for (const void* p : {x, y})
+      if (o != p && meet(o, M * D, p, M * D))
+        return fail(GP_ERR_INVALID_ARG, "h and out may be x or y, but not overlap them otherwise");
+    if ((o != gate || gate_rows != M) && meet(o, M * D, gate, gate_rows * D))
+      return fail(GP_ERR_INVALID_ARG, "h and out may be a gate of M rows, but not overlap it otherwise");
+    for (const void* p : {post_gamma, post_beta, gamma, beta})
+      if (meet(o, M * D, p, D)) return fail(GP_ERR_INVALID_ARG, "h and out must not overlap a gamma or beta");
+  }
   int dev = 0, ncu = 0;
   if ((rc = current_device_info(&dev, &ncu))) return rc;
   const ResidualNormArgs a{M,     D,    x,   y,     post, post_gamma, post_beta, post_eps, gate, gate_rows, gate_act,

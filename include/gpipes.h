@@ -554,7 +554,7 @@ int gp_phase_timers_read(void* dst, int64_t bytes);
  * written then.  One of h and out has to be stored.
  * All arithmetic is fp32; Pre takes h before it is rounded for memory.
  * h and out may each be x, y or (gate_rows == M) gate itself, but not each
- * other; other overlaps are not supported.  Any 2-byte alignment.  One launch,
+ * other; other overlaps are refused.  Any 2-byte alignment.  One launch,
  * no workspace: can be captured into a graph.
  * No counterpart in the reference (layer_norm_v2.cuh:129-147 and
  * elemwise_add.cuh:42-54 are its separate norm and sum).
@@ -593,7 +593,8 @@ int64_t gp_q4_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int we
  * launch, always in one order.  With less (0 and NULL) the product is computed
  * in one launch, more slowly, and may differ in a sum's last bits.  Calls that
  * may run at the same time, in graphs too, need workspaces of their own.
- * Can be captured into a graph; out must not overlap x (it may be r).
+ * Can be captured into a graph.  out may be r; that it overlaps x, or r
+ * otherwise, or that the workspace overlaps one of them, is refused.
  * No counterpart in the reference (16-bit weights only).
  */
 int gp_q4_gemm_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq, const void* scales,

@@ -51,6 +51,22 @@ def test_argument_errors_of_one_form():
     assert _call(u=24, two=True) == -3
 
 
+@pytest.mark.parametrize("two", [False, True])
+@pytest.mark.parametrize("kw", [
+    dict(out=1 << 20), dict(out=(1 << 20) + 4080), dict(out=(1 << 20) - 2032), dict(ws=(1 << 20) - 64, wsb=80),
+    dict(ws=(1 << 21) + 2032, wsb=64),
+])
+def test_overlaps_are_refused(kw, two):
+    a = dict(x=1 << 20, out=1 << 21)  # x 4 x 512, out 4 x 256: 4,096 and 2,048 bytes
+    assert _call(**{**a, **kw}, two=two) == -1
+    assert "overlap" in gpipes.lib.gp_last_error().decode()
+
+
+def test_a_residual_that_overlaps_is_refused():
+    assert _call(x=1 << 20, out=1 << 21, r=(1 << 21) + 16) == -1
+    assert _call(x=1 << 20, out=1 << 21, r=1 << 22, ws=(1 << 22) + 2032, wsb=16) == -1
+
+
 def test_empty_batch_is_a_noop():
     assert _call(M=0, x=0, out=0) == 0
     assert _call(M=0, x=0, out=0, two=True) == 0
@@ -512,3 +528,30 @@ def test_graph_of_a_deep_product(cuda, M, K, N):
         gpipes.q4_gemm_out(x2, *args)
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,N,two", [(64, 1088, False), (1088, 64, False), (32, 1032, True)])
+def test_more_values_than_32_bits_count(cuda, K, N, two):
+    """2^31 values of x or out and more, at the largest M: rows on both sides of that offset, and the last."""
+    M, group = 1 << 21, 32
+    gen = torch.Generator().manual_seed(K)
+    w = [weight(K, N, group, True, F16, gen) for _ in range(2)]
+    args = [[dev(t, cuda) for t in (q4.pack(q), s, z)] for q, s, z in w]
+    x = torch.randn(1 << 20, generator=gen).to(F16).to(cuda).repeat(M * K >> 20).view(M, K)
+    if two:
+        out = gpipes.q4_gated_out(x, *args[0], *args[1], group=group)
+    else:
+        r = torch.randn(1 << 20, generator=gen).to(F16).to(cuda).repeat(M * N >> 20).view(M, N)
+        out = gpipes.q4_gemm_out(x, *args[0], r=r, group=group)
+    mid = (1 << 31) // max(K, N)
+    for i in (0, mid - 80, mid, M - 80):
+        rows = slice(i, i + 80)
+        sides = [product(x[rows].cpu(), *t, group) for t in w]
+        if two:
+            (g, dg), (u, du) = moved(*sides[0], "silu"), sides[1]
+            want, bound = g * u, dg * (u.abs() + du) + g.abs() * du + 2 * U * (g * u).abs()
+        else:
+            v, d = sides[0][0], r[rows].double().cpu()
+            want, bound = v + d, sides[0][1] + 2 * U * (v.abs() + d.abs())
+        check(out[rows], want, bound, F16)

@@ -42,6 +42,18 @@ def test_argument_errors(kw, code):
     assert gpipes.lib.gp_last_error().decode() != ""
 
 
+@pytest.mark.parametrize("kw", [
+    dict(h=(1 << 20) + 2), dict(out=(1 << 20) - 4094), dict(h=(1 << 21) + 4094), dict(out=(1 << 21) + 256),
+    dict(h=1 << 24, out=(1 << 24) + 4094), dict(gate=1 << 24, rows=1, h=1 << 24), dict(gate=1 << 24, rows=8, out=1 << 24),
+    dict(gate=(1 << 24) + 4094, rows=1, out=1 << 24), dict(gate=1 << 24, rows=16, h=(1 << 24) + 256),
+    dict(pg=(1 << 22) + 4094), dict(g=(1 << 23) - 254), dict(pb=1 << 23), dict(b=(1 << 22) + 256),
+])
+def test_overlaps_are_refused(kw):
+    a = dict(x=1 << 20, y=1 << 21, h=1 << 22, out=1 << 23, pg=0, g=0)  # 16 rows of 128: 4,096 bytes
+    assert _call(**{**a, **kw}) == -1
+    assert "overlap" in gpipes.lib.gp_last_error().decode()
+
+
 def test_empty_batch_is_a_noop():
     assert _call(M=0, x=0, y=0, h=0, out=0) == 0
     assert _call(M=0, gate=16, rows=0) == 0
@@ -306,3 +318,17 @@ def test_python_refusals(cuda):
     e = x[:0]
     h, out = gpipes.residual_norm(e, e, gate=e)
     assert h.shape == out.shape == (0, 64)
+
+
+@pytest.mark.gpu
+def test_more_values_than_32_bits_count(cuda):
+    """2^31 values and more: rows on both sides of that offset, and the last."""
+    M, D = (1 << 31) // 4093 + 700, 4093
+    a = make(256, D, BF16, cuda, post="rms", norm="layer", scale=0.5, seed=4)
+    x, y = (a[k].repeat(M // 256 + 1, 1)[:M] for k in ("x", "y"))
+    h, out = gpipes.residual_norm_out(**{**a, "x": x, "y": y}, h=torch.empty_like(x))
+    for i in (0, (1 << 31) // D - 8, (1 << 31) // D, M - 8):
+        rows = slice(i, i + 8)
+        (h64, dh), (o64, do) = ref({**a, "x": x[rows], "y": y[rows]})
+        check(h[rows], h64, dh, BF16)
+        check(out[rows], o64, do, BF16)
