@@ -170,10 +170,9 @@ struct Cols {
 // LDS in the order of the waves.  A workgroup reads all of x, from L2, which
 // costs more than its words where rows are many; the two weights of a gated
 // product share those reads.  Bound by a CU's loads (16 rows, 8,192 columns
-// from 8,192 k: 13.6 us, 2.7 TB/s; a CU's 128 KiB of words would take 5 us at
+// from 8,192 k: 10.8 us, 3.3 TB/s; a CU's 128 KiB of words would take 5 us at
 // the 26 bytes a ns that it gets from the last cache, its 256 KiB of x 3.7 us
-// at the 70 from L2, and the rest is the first loads' latency and the join);
-// with 48 rows (2 x 8,192 columns from 2,048 k: 14.0 us) by those of x alone.
+// at the 70 from L2, and the rest is the first loads' latency and the join).
 // ---------------------------------------------------------------------------
 // Waves of a workgroup at most.  Above 16 rows sixteen fit the registers too
 // where a wave's tiles are few, and are slower (4,096 columns from 4,096 k, 48
@@ -194,7 +193,8 @@ __global__ __launch_bounds__(64 * rows_waves(MT)) void q4_rows_kernel(Q4Args p) 
   constexpr int COLS = 16 * CW, NT = S * CW;
   constexpr int TOK = FOUR ? 4 : 16;
   static_assert(NB % 2 == 0, "a buffer holds first halves or second halves");
-  __shared__ float part[rows_waves(MT) * TOK * COLS * S];
+  constexpr int PART = rows_waves(MT) * TOK * COLS * S * 4, XS = FOUR ? 0 : rows_waves(MT) * MT * 2048;
+  __shared__ __attribute__((aligned(1024))) char lds[PART > XS ? PART : XS];
   const int lane = threadIdx.x & 63, j = lane & 15, lg = lane >> 4;
   const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int N = p.N, K = p.K;
@@ -211,7 +211,15 @@ __global__ __launch_bounds__(64 * rows_waves(MT)) void q4_rows_kernel(Q4Args p) 
   const int64_t last = (int64_t)groups * N - CW;
   // Row i of the x operand: row i, or with at most four rows row i / 4, which
   // lands in element 0 of the accumulators of the lanes of group i / 4.
-  const int xrow = FOUR ? j >> 2 : j;
+  //
+  // An operand takes 64 bytes of each of 16 rows, half a line, and a line whose
+  // halves two instructions ask for is fetched twice from L2.  So eight lanes
+  // load a row's 128 bytes of a half, and the rows turn into operands through a
+  // piece of LDS that is the wave's own (16 rows, 8,192 columns from 8,192 k:
+  // 13.4 us by halves of lines, 10.8 so; 64 rows, 4,096 from 4,096: 20 and 13).
+  // 16-byte piece c of a row lies there at c ^ row % 8.
+  char* const xs = lds + (FOUR ? 0 : wave * (MT * 2048));
+  const int xrow = FOUR ? j >> 2 : lane >> 3;
 
   // half t of this wave: chunks wave, wave + waves, ..., two halves each
   auto load = [&](int t, Half<CW, S, MT, SG>& q, bool second) {
@@ -238,8 +246,9 @@ __global__ __launch_bounds__(64 * rows_waves(MT)) void q4_rows_kernel(Q4Args p) 
       }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const int xo = ((mt * 16 + xrow) * K + k) * 2;
-        q.x[st][mt] = __builtin_amdgcn_raw_buffer_load_b128(xr, k < K ? xo : 0x7FFFFFE0, 0, 0);
+        const int xk = FOUR ? k : k0 + (lane & 7) * 8;
+        const int xo = ((FOUR ? xrow : mt * 16 + st * 8 + xrow) * K + xk) * 2;
+        q.x[st][mt] = __builtin_amdgcn_raw_buffer_load_b128(xr, xk < K ? xo : 0x7FFFFFE0, 0, 0);
       }
     }
     if (G < kChunk || second) {
@@ -264,6 +273,13 @@ __global__ __launch_bounds__(64 * rows_waves(MT)) void q4_rows_kernel(Q4Args p) 
   const h8 ones = __builtin_bit_cast(h8, u32x4{T::kOne * 0x10001u, T::kOne * 0x10001u, T::kOne * 0x10001u,
                                                T::kOne * 0x10001u});
   auto mul = [&](int h, const Half<CW, S, MT, SG>& q, bool second) {
+    if constexpr (!FOUR) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+          *(h8*)(xs + mt * 2048 + (st * 8 + xrow) * 128 + (((lane & 7) ^ xrow) << 4)) = x_operand(q.x[st][mt]);
+    }
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
       const int k = (second ? kHalf : 0) + st * 32;
@@ -280,7 +296,12 @@ __global__ __launch_bounds__(64 * rows_waves(MT)) void q4_rows_kernel(Q4Args p) 
       for (int t = 0; t < NT; ++t) b[t] = bits.operand(q.w[st][t]);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        const h8 a = x_operand(q.x[st][mt]);
+        h8 a;
+        if constexpr (FOUR) {
+          a = x_operand(q.x[st][mt]);
+        } else {
+          a = *(const h8*)(xs + mt * 2048 + j * 128 + (((st * 4 + lg) ^ (j & 7)) << 4));
+        }
         sum[mt] = Q4<T>::mma16(a, ones, sum[mt]);
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t][mt] = Q4<T>::mma16(a, b[t], acc[t][mt]);
@@ -332,9 +353,10 @@ __global__ __launch_bounds__(64 * rows_waves(MT)) void q4_rows_kernel(Q4Args p) 
     }
   }
 
+  float* const part = (float*)lds;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    if (mt) __syncthreads();
+    if (mt || !FOUR) __syncthreads();  // every wave is done with what lies there
 #pragma unroll
     for (int e = 0; e < E; ++e)
 #pragma unroll
