@@ -174,10 +174,10 @@ struct Cols {
 // the 26 bytes a ns that it gets from the last cache, its 256 KiB of x 3.7 us
 // at the 70 from L2, and the rest is the first loads' latency and the join).
 // ---------------------------------------------------------------------------
-// Waves of a workgroup at most.  Above 16 rows sixteen fit the registers too
-// where a wave's tiles are few, and are slower (4,096 columns from 4,096 k, 48
-// rows: eight waves 15.5 us, sixteen 16.5; 20 rows 9.0 and 9.8).
-constexpr int rows_waves(int mt) { return mt == 1 ? 16 : 8; }
+// Waves of a workgroup at most: sixteen where a wave's tiles leave registers for
+// them and k is worth it (20 rows, 4,096 columns from 16,384 k: 18.9 us, with
+// eight 21.1; from 4,096 k 7.4 and 7.5; 48 rows of 4,093 k 14.4 and 14.1).
+constexpr int rows_waves(int tiles, int mt) { return mt == 1 || tiles * mt <= 2 ? 16 : 8; }
 
 template <int CW, int S, int MT, int SG>
 struct Half {
@@ -187,13 +187,13 @@ struct Half {
 };
 
 template <class T, int CW, int S, int MT, int G, bool FOUR, int NB>
-__global__ __launch_bounds__(64 * rows_waves(MT)) void q4_rows_kernel(Q4Args p) {
+__global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4Args p) {
   constexpr int SG = G < kHalf ? kHalf / G : 1;  // groups a half (G 128: one every other half)
   constexpr int E = FOUR ? 1 : 4;                // accumulator elements that hold rows (FOUR: at most four rows)
   constexpr int COLS = 16 * CW, NT = S * CW;
   constexpr int TOK = FOUR ? 4 : 16;
   static_assert(NB % 2 == 0, "a buffer holds first halves or second halves");
-  constexpr int PART = rows_waves(MT) * TOK * COLS * S * 4, XS = FOUR ? 0 : rows_waves(MT) * MT * 2048;
+  constexpr int PART = rows_waves(NT, MT) * TOK * COLS * S * 4, XS = FOUR ? 0 : rows_waves(NT, MT) * MT * 2048;
   __shared__ __attribute__((aligned(1024))) char lds[PART > XS ? PART : XS];
   const int lane = threadIdx.x & 63, j = lane & 15, lg = lane >> 4;
   const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -970,13 +970,16 @@ hipError_t rows_launch(const Q4Args& a, int waves, dim3 grid, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Products that run on tiles: those of more than 64 rows, and of more than 48
-// where the few-row kernel would read x for too many columns (64 rows, k 4096:
-// 4,096 columns 20 us against 18 on tiles, 16,384 28 against 23, 2 x 16,384 55
-// against 34; k 1024, 2 x 4,096 9.3 against 10).
+// Products that run on tiles.  Up to 128 rows small ones do not (128 rows, 1,024
+// columns from 1,024 k: 9.0 us on tiles, 6.5 by the kernel for few rows; 2,048
+// columns 9.9 and 6.8, 4,096 10.4 and 11.7; 1,024 columns from 16,384 k 22 and
+// 33), up to 64 those whose x the kernel for few rows does not read for too many
+// columns (64 rows, k 4,096: 4,096 columns 17 us on tiles and 13, 16,384 26 and
+// 30, 2 x 16,384 45 and 81; 8,192 from 8,192 26.4 and 25), up to 48 none.
 bool on_tiles(int64_t M, int N, int K, int group, int sides) {
   if ((int64_t)((K + group - 1) / group) * N < 4) return false;  // a tile's loads of scales are four wide
-  return M > 64 || (M > 48 && (int64_t)N * sides > 8192);
+  const int64_t n = (int64_t)N * sides;
+  return M > 128 || (M > 64 && (n > 2048 || K > 2048)) || (M > 48 && n > 8192);
 }
 
 template <class T>
@@ -1005,7 +1008,7 @@ hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
   int nt = n >= 64 * num_cus ? 4 : n >= 32 * num_cus ? 2 : 1;
   if ((int64_t)((a.K + a.group - 1) / a.group) * a.N < 4) nt = 1;
   const int cw = nt > a.sides ? nt / a.sides : 1;
-  int waves = rows_waves(mt);
+  int waves = rows_waves(cw * a.sides, mt);
   while (waves > 2 && waves / 2 >= chunks) waves /= 2;
   const dim3 grid((unsigned)((a.N + 16 * cw - 1) / (16 * cw)), (unsigned)((a.M + 16 * mt - 1) / (16 * mt)));
 #define GP_CASE(c, m, four, nb)                                                                                \
