@@ -176,7 +176,8 @@ struct Cols {
 // ---------------------------------------------------------------------------
 // Waves of a workgroup at most: sixteen where a wave's tiles leave registers for
 // them and k is worth it (20 rows, 4,096 columns from 16,384 k: 18.9 us, with
-// eight 21.1; from 4,096 k 7.4 and 7.5; 48 rows of 4,093 k 14.4 and 14.1).
+// eight 21.1; from 4,096 k 7.4 and 7.5; three tiles a wave, 37 rows, 4,093 columns from
+// 4,072 k: 14.4 and 14.1).
 constexpr int rows_waves(int tiles, int mt) { return mt == 1 || tiles * mt <= 2 ? 16 : 8; }
 
 template <int CW, int S, int MT, int SG>
@@ -622,8 +623,8 @@ hipError_t token_launch(const Q4Args& a, int waves, int ct, int kw, const TokenL
 // Bound by instruction issue: two waves a SIMD run about 430 instructions a
 // chunk for 64 MFMAs (64 and-ors and 48 shifts that make operands, 64 fused
 // multiply-adds of the groups' ends), the matrix cores busy 38% of the time and
-// the vector units 57%.  4,096 rows, 4,096 columns from 4,096 k: 147 us, 0.93
-// PFLOP/s (this card's library product of 16-bit operands of that size: 127).
+// the vector units 57%.  4,096 rows, 4,096 columns from 4,096 k: 142 to 147 us, 0.93
+// to 0.97 PFLOP/s (this card's library product of 16-bit operands of that size: 127).
 // Tried and no faster: operands one to four steps ahead, words copied to LDS
 // two chunks ahead, MFMAs and operand instructions interleaved by the scheduler's
 // groups (163), wave priorities, offsets in scalar registers.
