@@ -187,13 +187,12 @@ struct Half {
   Cols<CW> s[S][SG], z[S][SG];
 };
 
-template <class T, int CW, int S, int MT, int G, bool FOUR, int NB>
+template <class T, int CW, int S, int MT, int G, bool FOUR>
 __global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4Args p) {
   constexpr int SG = G < kHalf ? kHalf / G : 1;  // groups a half (G 128: one every other half)
   constexpr int E = FOUR ? 1 : 4;                // accumulator elements that hold rows (FOUR: at most four rows)
   constexpr int COLS = 16 * CW, NT = S * CW;
   constexpr int TOK = FOUR ? 4 : 16;
-  static_assert(NB % 2 == 0, "a buffer holds first halves or second halves");
   constexpr int PART = rows_waves(NT, MT) * TOK * COLS * S * 4, XS = FOUR ? 0 : rows_waves(NT, MT) * MT * 2048;
   __shared__ __attribute__((aligned(1024))) char lds[PART > XS ? PART : XS];
   const int lane = threadIdx.x & 63, j = lane & 15, lg = lane >> 4;
@@ -338,18 +337,20 @@ __global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4
     }
   };
 
-  // NB halves in flight.  Loads are issued without a condition, so that the
-  // compiler counts them: those past the wave's last chunk read nothing.
+  // Two halves in flight, a chunk (four are slower: 16 rows, 1,024 columns from
+  // 1,024 k 3.3 us and 4.2, 4,096 from 16,384 13.4 and 14.0).  Loads are issued
+  // without a condition, so that the compiler counts them: those past the wave's
+  // last chunk read nothing.
   const int halves = wave < chunks ? 2 * ((chunks - 1 - wave) / waves + 1) : 0;
-  Half<CW, S, MT, SG> q[NB];
+  Half<CW, S, MT, SG> q[2];
   if (halves) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) load(i, q[i], i & 1);
-    for (int t = 0; t < halves; t += NB) {
+    for (int i = 0; i < 2; ++i) load(i, q[i], i & 1);
+    for (int t = 0; t < halves; t += 2) {
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
+      for (int i = 0; i < 2; ++i) {
         mul(t + i, q[i], i & 1);
-        load(t + NB + i, q[i], i & 1);
+        load(t + 2 + i, q[i], i & 1);
       }
     }
   }
@@ -959,13 +960,13 @@ hipError_t tile_launch(const Q4Args& a, int parts, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <class T, int CW, int S, int MT, bool FOUR, int NB>
+template <class T, int CW, int S, int MT, bool FOUR>
 hipError_t rows_launch(const Q4Args& a, int waves, dim3 grid, hipStream_t s) {
   const dim3 block(waves * kWave);
   switch (a.group) {
-    case 32: hipLaunchKernelGGL((q4_rows_kernel<T, CW, S, MT, 32, FOUR, NB>), grid, block, 0, s, a); break;
-    case 64: hipLaunchKernelGGL((q4_rows_kernel<T, CW, S, MT, 64, FOUR, NB>), grid, block, 0, s, a); break;
-    case 128: hipLaunchKernelGGL((q4_rows_kernel<T, CW, S, MT, 128, FOUR, NB>), grid, block, 0, s, a); break;
+    case 32: hipLaunchKernelGGL((q4_rows_kernel<T, CW, S, MT, 32, FOUR>), grid, block, 0, s, a); break;
+    case 64: hipLaunchKernelGGL((q4_rows_kernel<T, CW, S, MT, 64, FOUR>), grid, block, 0, s, a); break;
+    case 128: hipLaunchKernelGGL((q4_rows_kernel<T, CW, S, MT, 128, FOUR>), grid, block, 0, s, a); break;
     default: return hipErrorInvalidValue;
   }
   return hipGetLastError();
@@ -1012,17 +1013,17 @@ hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
   int waves = rows_waves(cw * a.sides, mt);
   while (waves > 2 && waves / 2 >= chunks) waves /= 2;
   const dim3 grid((unsigned)((a.N + 16 * cw - 1) / (16 * cw)), (unsigned)((a.M + 16 * mt - 1) / (16 * mt)));
-#define GP_CASE(c, m, four, nb)                                                                                \
-  if (cw == c && a.sides == 1 && mt == m && (a.M <= 4) == four)                                               \
-    return rows_launch<T, c, 1, m, four, nb>(a, waves, grid, s);                                              \
-  if constexpr (c <= 2)                                                                                       \
-    if (cw == c && a.sides == 2 && mt == m && (a.M <= 4) == four)                                             \
-      return rows_launch<T, c, 2, m, four, 2>(a, waves, grid, s);
-  GP_CASE(1, 1, true, 4) GP_CASE(2, 1, true, 4) GP_CASE(4, 1, true, 2)
-  GP_CASE(1, 1, false, 4) GP_CASE(2, 1, false, 2) GP_CASE(4, 1, false, 2)
-  GP_CASE(1, 2, false, 2) GP_CASE(2, 2, false, 2) GP_CASE(4, 2, false, 2)
-  GP_CASE(1, 3, false, 2) GP_CASE(2, 3, false, 2) GP_CASE(4, 3, false, 2)
-  GP_CASE(1, 4, false, 2) GP_CASE(2, 4, false, 2) GP_CASE(4, 4, false, 2)
+#define GP_CASE(c, m, four)                                       \
+  if (cw == c && a.sides == 1 && mt == m && (a.M <= 4) == four)   \
+    return rows_launch<T, c, 1, m, four>(a, waves, grid, s);      \
+  if constexpr (c <= 2)                                           \
+    if (cw == c && a.sides == 2 && mt == m && (a.M <= 4) == four) \
+      return rows_launch<T, c, 2, m, four>(a, waves, grid, s);
+  GP_CASE(1, 1, true) GP_CASE(2, 1, true) GP_CASE(4, 1, true)
+  GP_CASE(1, 1, false) GP_CASE(2, 1, false) GP_CASE(4, 1, false)
+  GP_CASE(1, 2, false) GP_CASE(2, 2, false) GP_CASE(4, 2, false)
+  GP_CASE(1, 3, false) GP_CASE(2, 3, false) GP_CASE(4, 3, false)
+  GP_CASE(1, 4, false) GP_CASE(2, 4, false) GP_CASE(4, 4, false)
 #undef GP_CASE
   return hipErrorInvalidValue;
 }
