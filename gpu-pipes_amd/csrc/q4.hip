@@ -7,17 +7,20 @@
 // bits: eight k of one column are what one lane of an MFMA holds, so a word is
 // a lane's operand, and the weights need no other layout than [K / 8, N].
 //
-// From a word to an operand.  A 4-bit q in mantissa bits 4 .. 7 of fp16's 64.0
-// is 64 + q, exactly, and in bits 0 .. 3 of bf16's 128.0 it is 128 + q; a shift
-// (three of four need one) and an and-or make two of them, of k and k + 4, so
-// the operand holds the eight k in the order 0 4 1 5 2 6 3 7, and x is put in
-// the same order.  Per group of G rows the matrix cores sum x (B + q), B the 64
-// or 128, and, against a column of ones, x; then
-//   sum x (q - z) = sum x (B + q) - (B + z) sum x
-// in fp32, and times s into the running sum.  The weights are never rounded:
-// what is lost is a few bits of fp32 where the two sums cancel, 2^-24 of sums
-// B / 4 times as large (2^-20 and 2^-19 of theirs; a result's half step is
-// 2^-12 and 2^-9).
+// From a word to an operand.  A byte 0 .. 15 read as e4m3 is q 2^-9, denormal
+// or not; a word masked, and a word >> 4 masked, are four such bytes each, and
+// one conversion by 2^9 makes two of them q in 16 bits, exactly.  The operand
+// holds the eight k in the order 0 2 4 6 1 3 5 7, and x is put in the same
+// order.  Per group of G rows the matrix cores sum x q and, against a column of
+// ones, x; then
+//   sum x (q - z) = sum x q - z sum x
+// in fp32, and times s into the running sum.  The weights are never rounded.
+// s x (q - z) is so the difference of two that are up to 15 and |z| times s x,
+// and an x leaves 2^-24 of those behind where its weight is small or zero.
+// (64 + q and 128 + q, q put into a mantissa, are as many instructions, but
+// leave 2^-24 of 64 to 150 times s x: an x 5,000 times as large as the others,
+// its weights zero, then moves an fp16 result by more than its rounding does,
+// and ten times as many results of 8,192 k differ from an fp32 product's.)
 #include <hip/hip_runtime.h>
 #include <type_traits>
 
@@ -32,9 +35,11 @@ template <class T>
 struct Q4;
 template <>
 struct Q4<F16> : F16 {
-  static constexpr int kShift = 4;  // left, of the lowest q
-  static constexpr unsigned kMask = 0x00F000F0u, kBase = 0x54005400u;
-  static constexpr float kBias = 64.f;
+  // bytes 2 HI and 2 HI + 1 of u, each 0 .. 15
+  template <bool HI>
+  __device__ static unsigned bytes2(unsigned u) {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u, 512.f, HI));
+  }
   __device__ static f4 mma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
   // s + both halves of u
   __device__ static float add2(unsigned u, float s) {
@@ -43,9 +48,10 @@ struct Q4<F16> : F16 {
 };
 template <>
 struct Q4<BF16> : BF16 {
-  static constexpr int kShift = 0;
-  static constexpr unsigned kMask = 0x000F000Fu, kBase = 0x43004300u;
-  static constexpr float kBias = 128.f;
+  template <bool HI>
+  __device__ static unsigned bytes2(unsigned u) {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(u, 512.f, HI));
+  }
   __device__ static f4 mma16(h8 a, h8 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
   }
@@ -54,35 +60,21 @@ struct Q4<BF16> : BF16 {
   }
 };
 
-// The mask and the base of an operand, in registers whose values the compiler
-// does not know: v_and_or_b32 takes no literals, and it would use two
-// instructions with them.
+// The operand q of a word, k order 0 2 4 6 1 3 5 7.
 template <class T>
-struct Q4Bits {
-  unsigned mask = Q4<T>::kMask, base = Q4<T>::kBase;
-  __device__ __forceinline__ Q4Bits() {
-    asm("" : "+s"(mask));
-    asm("" : "+v"(base));
-  }
-  // The operand B + q of a word, k order 0 4 1 5 2 6 3 7.
-  __device__ __forceinline__ h8 operand(unsigned w) const {
-    constexpr int s = Q4<T>::kShift;
-    u32x4 o;
-    o[0] = ((w << s) & mask) | base;
-    o[1] = ((w >> (4 - s)) & mask) | base;
-    o[2] = ((w >> (8 - s)) & mask) | base;
-    o[3] = ((w >> (12 - s)) & mask) | base;
-    return __builtin_bit_cast(h8, o);
-  }
-};
+__device__ __forceinline__ h8 q_operand(unsigned w) {
+  const unsigned e = w & 0x0F0F0F0Fu, d = (w >> 4) & 0x0F0F0F0Fu;
+  return __builtin_bit_cast(h8, u32x4{Q4<T>::template bytes2<false>(e), Q4<T>::template bytes2<true>(e),
+                                      Q4<T>::template bytes2<false>(d), Q4<T>::template bytes2<true>(d)});
+}
 
 // Eight values of x in that order.
 __device__ __forceinline__ h8 x_operand(u32x4 v) {
   u32x4 o;
-  o[0] = __builtin_amdgcn_perm(v[2], v[0], 0x05040100u);
-  o[1] = __builtin_amdgcn_perm(v[2], v[0], 0x07060302u);
-  o[2] = __builtin_amdgcn_perm(v[3], v[1], 0x05040100u);
-  o[3] = __builtin_amdgcn_perm(v[3], v[1], 0x07060302u);
+  o[0] = __builtin_amdgcn_perm(v[1], v[0], 0x05040100u);
+  o[1] = __builtin_amdgcn_perm(v[3], v[2], 0x05040100u);
+  o[2] = __builtin_amdgcn_perm(v[1], v[0], 0x07060302u);
+  o[3] = __builtin_amdgcn_perm(v[3], v[2], 0x07060302u);
   return __builtin_bit_cast(h8, o);
 }
 
@@ -267,7 +259,6 @@ __global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4
     }
   };
 
-  const Q4Bits<T> bits;
   float tot[NT][MT][E] = {};
   f4 acc[NT][MT], sum[MT];
   const h8 ones = __builtin_bit_cast(h8, u32x4{T::kOne * 0x10001u, T::kOne * 0x10001u, T::kOne * 0x10001u,
@@ -293,7 +284,7 @@ __global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4
       }
       h8 b[NT];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) b[t] = bits.operand(q.w[st][t]);
+      for (int t = 0; t < NT; ++t) b[t] = q_operand<T>(q.w[st][t]);
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         h8 a;
@@ -320,7 +311,7 @@ __global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4
 #pragma unroll
           for (int t = 0; t < CW; ++t) {
             const float s = qs.template val<T>(t);
-            const float z = Q4<T>::kBias + (p.side[sd].z ? qz.template val<T>(t) : 8.f);
+            const float z = p.side[sd].z ? qz.template val<T>(t) : 8.f;
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -380,7 +371,7 @@ __global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4
 
 // ---------------------------------------------------------------------------
 // A token, or up to four.  Words come faster than 16-bit operands can be made
-// of them (eight operations a word), so here the operands are 8 bits: a byte
+// of them (seven operations a word), so here the operands are 8 bits: a byte
 // 0 .. 15 read as e4m3 is q 2^-9, denormal or not, and a word is two dwords of
 // such bytes, w and w >> 4 masked -- k in the order 0 2 4 6, 1 3 5 7.  x, in
 // chunks of 128 k, is written with four signed digits to the base 32, each a
@@ -622,7 +613,7 @@ hipError_t token_launch(const Q4Args& a, int waves, int ct, int kw, const TokenL
 // second kernel adds them in order.
 //
 // Bound by instruction issue: two waves a SIMD run about 430 instructions a
-// chunk for 64 MFMAs (64 and-ors and 48 shifts that make operands, 64 fused
+// chunk for 64 MFMAs (64 conversions, 48 masks and shifts for them, 64 fused
 // multiply-adds of the groups' ends), the matrix cores busy 38% of the time and
 // the vector units 57%.  4,096 rows, 4,096 columns from 4,096 k: 142 to 147 us, 0.93
 // to 0.97 PFLOP/s (this card's library product of 16-bit operands of that size: 127).
@@ -703,7 +694,7 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, i
       s = add_dpp<0x4E>(s);                           // quad_perm [2,3,0,1]
       if constexpr (G >= 64) s = add_dpp<0x141>(s);   // row_half_mirror
       if constexpr (G >= 128) s = add_dpp<0x140>(s);  // row_mirror
-      ss[buf][(tid & 15) / (G / 8)][row] = Z ? -s : -(Q4<T>::kBias + 8.f) * s;  // the same from each lane of the group
+      ss[buf][(tid & 15) / (G / 8)][row] = Z ? -s : -8.f * s;  // the same from each lane of the group
     }
   };
   unsigned w[4][CW];
@@ -729,7 +720,6 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, i
     if constexpr (Z) qz[g].load(zp, group_at(c, g), last);
   };
 
-  const Q4Bits<T> bits;
   float tot[CW][MT][4] = {};
   // One chunk.  Registers hold one chunk's words and scales, and each is asked
   // for again, a chunk ahead, when it has been used; the next chunk's x, which
@@ -744,7 +734,7 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, i
     }
     h8 b[CW];
 #pragma unroll
-    for (int t = 0; t < CW; ++t) b[t] = bits.operand(w[0][t]);
+    for (int t = 0; t < CW; ++t) b[t] = q_operand<T>(w[0][t]);
     load_w(c + 1, 0);
     f4 acc[CW][MT];
 #pragma unroll
@@ -755,11 +745,11 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, i
       for (int mt = 0; mt < MT; ++mt) {
         const h8 x = *(const h8*)(xs[buf] + (mt * 16 + j) * (kChunk * 2) + (((st * 4 + lg) ^ j) << 4));
         if (st % SPG == 0) {
-          // a group's sum begins at -(B + z) times that of x
+          // a group's sum begins at -z times that of x
           const f4 m = *(const f4*)&ss[buf][g][mt * 16 + 4 * lg];
 #pragma unroll
           for (int t = 0; t < CW; ++t) {
-            const float z = Q4<T>::kBias + (sd.z ? qz[g].template val<T>(t) : 8.f);
+            const float z = sd.z ? qz[g].template val<T>(t) : 8.f;
             acc[t][mt] = Q4<T>::mma16(x, b[t], Z ? f4{z * m[0], z * m[1], z * m[2], z * m[3]} : m);
           }
         } else {
@@ -768,7 +758,7 @@ __global__ __launch_bounds__(256, 2) void q4_tile_kernel(Q4Args p, int mtiles, i
         }
         if (st < 3) {
 #pragma unroll
-          for (int t = mt * CW / MT; t < (mt + 1) * CW / MT; ++t) bn[t] = bits.operand(w[st < 3 ? st + 1 : 3][t]);
+          for (int t = mt * CW / MT; t < (mt + 1) * CW / MT; ++t) bn[t] = q_operand<T>(w[st < 3 ? st + 1 : 3][t]);
         }
         if ((st + 1) % SPG == 0) {
 #pragma unroll

@@ -581,12 +581,15 @@ int64_t gp_q4_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int we
  * 65536 (the last group may be short), N any up to 2^20, a weight below 2 GiB,
  * M up to 2097152.  b [N], r [M,N] or NULL; act any GP_ACT_*.  Every tensor
  * but wq `dtype`, every pointer 16-byte aligned.
- * Weights are not rounded: products are exact, sums fp32, out rounded once.
+ * Weights are not rounded, sums are fp32, out is rounded once.  A group's sum
+ * is that of x q less z times that of x: it keeps 2^-24 of the larger of the
+ * two, so an x under a small weight leaves an error as under one of 15 or |z|.
  * (With up to four rows a value of x may be taken to 2^-19 of the largest of
  * its 128 neighbours k, about what an fp32 sum of them keeps.  In bf16 values
  * of x below 2^-122 may count as zero.)
- * x has to be finite and, in bf16, 150 times a group's sum of |x| below fp32's
- * largest number: a row of x that is not gives NaN in that row of out alone.
+ * x has to be finite and, in bf16, 15 times (|z| times, where that is more) a
+ * group's sum of |x| below fp32's largest number: a row of x that is not gives
+ * NaN in that row of out alone.  Scales and zeros have to be finite.
  * workspace: scratch of the call's own, workspace_bytes long (16-byte aligned,
  * contents of no matter), as gp_q4_workspace_bytes gives it: with more than 48
  * rows and few columns parts of K are multiplied apart and added in a second

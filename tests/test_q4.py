@@ -555,3 +555,49 @@ def test_more_values_than_32_bits_count(cuda, K, N, two):
             v, d = sides[0][0], r[rows].double().cpu()
             want, bound = v + d, sides[0][1] + 2 * U * (v.abs() + d.abs())
         check(out[rows], want, bound, F16)
+
+
+# ---------------------------------------------------------------------------
+# What an fp32 sum keeps
+# ---------------------------------------------------------------------------
+
+def outlying(M, K, N, group, zeros, dt, seed):
+    """x with a few channels thousands of times as large as the others, and a weight that is exactly zero there."""
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(M, K, generator=gen)
+    at = [3, K // 2 + 7, K - 30]
+    x[:, at] = 5000 * (1 + torch.rand(M, len(at), generator=gen)) * torch.tensor([1.0, -1.0, 1.0])
+    q, s, _ = weight(K, N, group, False, dt, gen)
+    z = torch.randint(0, 16, s.shape, generator=gen).to(dt) if zeros else None
+    for c in at:
+        q[c] = 8 if z is None else z[c // group].long()
+    return x.to(dt), q, s, z
+
+
+def near(x, q, s, z, group):
+    """x W, and a bound for sums in fp32: a group's sum of x q and z times that of x, up to 128 terms of both, take
+    sixteen roundings each at most (eight products a step), of what they have come to."""
+    x, q, s = x.double(), q.double(), s.double()
+    K = q.shape[0]
+    zz = z.double() if z is not None else torch.full_like(s, 8)
+    sr, zr = (t.repeat_interleave(group, 0)[:K] for t in (s, zz))
+    run = torch.zeros(x.shape[0], q.shape[1], dtype=torch.float64)
+    for k in range(0, K, group):
+        run += (x[:, k:k + group] @ (sr * (q - zr))[k:k + group]).abs()
+    return x @ (sr * (q - zr)), 16 * U * (x.abs() @ (sr * (q + zr.abs()))) + 100 * U * run
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(3, 1024, 257), (5, 1024, 256), (16, 1024, 512), (16, 2048, 8192), (40, 1024, 320),
+                                   (64, 1024, 256), (100, 4096, 520), (200, 1024, 256), (600, 1024, 1024)])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_large_values_under_zero_weights(cuda, M, K, N, zeros, dt):
+    """They leave behind what an fp32 sum does: 2^-24 of 15 x 10,000 in a rounding, 0.009, three groups with some ten of
+    them at random, 0.05 at most of results that are about 4.6 sqrt(1024) = 147 (all in units of a scale), 3.4e-4 of
+    them against a half step of 4.9e-4 in fp16, uniform, 2.8e-4.  Typically a quarter of that: a few hundredths more
+    than rounding's own, whose limit is 1.1 in check()."""
+    x, q, s, z = outlying(M, K, N, 64, zeros, dt, M + N)
+    want, bound = near(x, q, s, z, 64)
+    got = gpipes.q4_gemm_out(x.to(cuda), dev(q4.pack(q), cuda), s.to(cuda), dev(z, cuda), group=64)
+    check(got, want, bound, dt)
