@@ -370,40 +370,43 @@ __global__ __launch_bounds__(64 * rows_waves(CW * S, MT)) void q4_rows_kernel(Q4
 }
 
 // ---------------------------------------------------------------------------
-// A token, or up to four.  Words come faster than 16-bit operands can be made
+// One token.  Words come faster than 16-bit operands can be made
 // of them (seven operations a word), so here the operands are 8 bits: a byte
 // 0 .. 15 read as e4m3 is q 2^-9, denormal or not, and a word is two dwords of
 // such bytes, w and w >> 4 masked -- k in the order 0 2 4 6, 1 3 5 7.  x, in
-// chunks of 128 k, is written with four signed digits to the base 32, each a
-// whole number up to 16 that e4m3 holds: x = 2^e (d0 + d1 / 32 + d2 / 32^2 +
-// d3 / 32^3), 2^e such that the chunk's largest value has d0 in [8, 16].  That
-// is x to 2^-19 of the chunk's largest, the last bits of an fp32 sum.
+// chunks of 128 k, is written with six signed digits to the base 32, each a
+// whole number up to 16 that e4m3 holds: x = 2^e (d0 + d1 / 32 + ... + d5 /
+// 32^5), 2^e such that the chunk's largest value has d0 in [8, 16].  That is x
+// to 2^-29 of the chunk's largest, a 32nd of what an fp32 sum keeps of it: a
+// value 10,000 times as large as its neighbours, its weights zero, leaves
+// nothing behind that a result shows.  (With four digits, 2^-19, such a value
+// made twenty times an fp16 result's rounding, with five a tenth of it more.)
 //
 // Whole numbers, because the 8-bit MFMAs add their products with fewer bits
 // than fp32: of products far apart in size they lose what is 2^-14 of the
 // largest (measured).  Those of a digit with q are whole and at most 240, so
-// nothing is lost, and the four digits' sums are added in fp32.
+// nothing is lost, and the six digits' sums are added in fp32.
 //
-// Digit p of token m is row 4 m + p of the MFMA (16 x 16 x 128, whose scale
-// operand brings 2^e / 32^p), so a token's and column's digits are one lane's
-// accumulators.  A group shorter than 128 has an MFMA of its own, where the
-// other blocks of the weight go under 2^-127.
+// Digit p is row p of the MFMA (16 x 16 x 128, whose scale operand brings 2^e /
+// 32^p).  Each row has its own running sum, and the six are added at the end.
+// A group shorter than 128 has an MFMA of its own, where the other blocks of
+// the weight go under 2^-127.
 //
 // Such a call is over in the time of a few memory latencies, and code that no
 // wave has run yet is fetched from memory too.  So all that the workgroup will
 // read is asked for first: x, the scales and kRing chunks of every wave's
 // words, the latter by copies into LDS that hold no registers; and the code
-// is short (rolled loops, no copy of it for a size of group).  One row, 2 x
-// 16,384 columns from 4,096 k: 12.7 us, 5.5 TB/s; 4,096 columns from 16,384 k:
-// 10.2 us, 3.4 TB/s, of which 5 are the words and 2 to 3 the digits of x, that
-// every workgroup makes for itself; 1,024 from 1,024: 3.6 us, the latencies of
-// a launch, two loads and the join.  Rings of four to eight chunks were slower
-// (more LDS to hand out, later first words).
+// is short (rolled loops, no copy of it for a size of group).  2 x 16,384 columns
+// from 4,096 k: 13.5 us, 5.2 TB/s; 4,096 columns from 16,384 k: 10.1 us, 3.5
+// TB/s, of which 5 are the words and 3 the digits of x, that every workgroup
+// makes for itself; 1,024 from 1,024: 3.2 us, the latencies of a launch, two
+// loads and the join.  Rings of four to eight chunks were slower (more LDS to
+// hand out, later first words).
 // ---------------------------------------------------------------------------
 constexpr int kTokenCols = 16;
-constexpr int kDigits = 4;
+constexpr int kDigits = 6;
 constexpr int kRing = 2;  // chunks of 1 KiB that a wave has in flight
-constexpr int kTokenLds = 155 * 1024;  // of dynamic LDS at most: a CU's 160 KiB less 4 for the waves' sums
+constexpr int kTokenLds = 158 * 1024;  // of dynamic LDS at most: a CU's 160 KiB less 2 for the waves' sums
 
 // LDS, in this order: x's digits, rows of K bytes 16 bytes apart in banks; the
 // powers, a byte a chunk; every wave's ring; every wave's scales and zeros, 32
@@ -411,12 +414,12 @@ constexpr int kTokenLds = 155 * 1024;  // of dynamic LDS at most: a CU's 160 KiB
 struct TokenLds {
   int xstride, powers, ring, scales, wave_scales, bytes;
 };
-inline TokenLds token_lds(int M, int K, int group, int waves, int kw, bool z) {
+inline TokenLds token_lds(int K, int group, int waves, int kw, bool z) {
   TokenLds l;
   const int chunks = (K + kChunk - 1) / kChunk, cpw = (chunks + kw - 1) / kw;
   l.xstride = (chunks * kChunk + 255) / 256 * 256 + 16;
-  l.powers = M * kDigits * l.xstride;
-  l.ring = (l.powers + M * chunks + 1023) / 1024 * 1024;
+  l.powers = kDigits * l.xstride;
+  l.ring = (l.powers + chunks + 1023) / 1024 * 1024;
   l.scales = l.ring + waves * kRing * 1024;
   l.wave_scales = (cpw * (kChunk / group) + 7) / 8 * 256;
   l.bytes = l.scales + waves * l.wave_scales * (z ? 2 : 1);
@@ -426,7 +429,7 @@ inline TokenLds token_lds(int M, int K, int group, int waves, int kw, bool z) {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 // Eight values of x, a sixteenth of a chunk (the others are in the lanes of
-// this row of sixteen): their digits to LDS rows 0 .. 3, the chunk's power.
+// this row of sixteen): their digits to LDS rows 0 .. 5, the chunk's power.
 template <class T>
 __device__ __forceinline__ void put_digits(u32x4 v, GP_LDS char* at, int xstride, GP_LDS char* power, bool first) {
   float x[8];
@@ -446,7 +449,7 @@ __device__ __forceinline__ void put_digits(u32x4 v, GP_LDS char* at, int xstride
 #undef GP_DPP_F
   // e, biased; not so small that the last digit's power would pass zero
   int e = (__builtin_bit_cast(int, top) >> 23) - 3;
-  e = e < 20 ? 20 : e;
+  e = e < 25 ? 25 : e;
   const float up = __builtin_bit_cast(float, (254 - e) << 23);
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] *= up;
@@ -474,13 +477,13 @@ __device__ __forceinline__ void put_digits(u32x4 v, GP_LDS char* at, int xstride
 // of weight `side`.
 template <class T>
 __global__ __launch_bounds__(1024) void q4_token_kernel(Q4Args p, int ctshift, int kwshift, int gshift, TokenLds l) {
-  __shared__ float part[16 * kTokenCols * 4];
+  __shared__ float part[16][2][kTokenCols];  // of a wave: the first four digits' sums, the last two's
   GP_LDS char* lds = dyn_lds();
   const int CT = 1 << ctshift, KW = 1 << kwshift;
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, lg = lane >> 4;
   const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kw = wave & (KW - 1), tile = wave >> kwshift, ct = tile & (CT - 1), side = tile >> ctshift;
-  const int N = p.N, K = p.K, M = (int)p.M;
+  const int N = p.N, K = p.K;
   const int n0 = xcd_order(blockIdx.x, gridDim.x) * (kTokenCols * CT);
   const int chunks = (K + kChunk - 1) / kChunk, cpw = (chunks + KW - 1) >> kwshift;
   const int c0 = kw * cpw, nc = chunks - c0 < cpw ? chunks - c0 : cpw;  // may be 0 or less: nothing
@@ -502,7 +505,8 @@ __global__ __launch_bounds__(1024) void q4_token_kernel(Q4Args p, int ctshift, i
   }
   // x: a thread has eight k, and the conversion waits for them
   const int kend = chunks * kChunk;
-  u32x4 xv = __builtin_amdgcn_raw_buffer_load_b128(make_rsrc(p.x, K * 2), tid * 16, 0, 0);
+  const auto xr = make_rsrc(p.x, K * 2);
+  u32x4 xv = __builtin_amdgcn_raw_buffer_load_b128(xr, tid * 16, 0, 0);
   // A chunk's copy: 16 word rows of 16 columns, 16 bytes a lane.  A lane of the
   // MFMA's group lg holds k 16 lg .. + 15 of the chunk and of its second half,
   // so its words are rows 2 lg, 2 lg + 1, 8 + 2 lg, 9 + 2 lg; word i of group lg
@@ -515,30 +519,25 @@ __global__ __launch_bounds__(1024) void q4_token_kernel(Q4Args p, int ctshift, i
 #pragma unroll
   for (int i = 0; i < kRing; ++i, woff += wstep) dma16_buf(wr, (int)(i < nc ? woff : 0xFFFFFFE0u), ring + i * 1024);
   wait_vmcnt<kRing>();  // this wave's scales, and its first part of x
-  auto put = [&](int m, int k) {
+  auto put = [&](int k) {
     if (k < kend)  // rows of sixteen threads, a chunk each
-      put_digits<T>(xv, lds + m * kDigits * l.xstride + k, l.xstride, lds + l.powers + m * chunks + k / kChunk,
-                    !(tid & 15));
+      put_digits<T>(xv, lds + k, l.xstride, lds + l.powers + k / kChunk, !(tid & 15));
   };
-  put(0, tid * 8);
+  put(tid * 8);
 #pragma unroll 1
-  for (int m = 0, k0 = blockDim.x * 8; m < M; ++m, k0 = 0) {
-    const auto xr = make_rsrc((const half_t*)p.x + m * K, K * 2);
-#pragma unroll 1
-    for (; k0 < kend; k0 += blockDim.x * 8) {
-      xv = __builtin_amdgcn_raw_buffer_load_b128(xr, (k0 + tid * 8) * 2, 0, 0);
-      put(m, k0 + tid * 8);
-    }
+  for (int k = (blockDim.x + tid) * 8; k - tid * 8 < kend; k += blockDim.x * 8) {
+    xv = __builtin_amdgcn_raw_buffer_load_b128(xr, k * 2, 0, 0);
+    put(k);
   }
   lds_barrier();
 
-  // Row j of the A operand: token j / 4's digit j % 4 (past the last token another one's, whose sums go unread).
-  const int m = j >> 2 < M ? j >> 2 : M - 1;
-  GP_LDS const char* xl = lds + (m * kDigits + (j & 3)) * l.xstride + c0 * kChunk + lg * 16;
-  GP_LDS const char* pl = lds + l.powers + m * chunks + c0;
+  // Row j of the A operand: digit j (behind the last the last one's again, whose sums go unread).
+  const int digit = j < kDigits ? j : kDigits - 1;
+  GP_LDS const char* xl = lds + digit * l.xstride + c0 * kChunk + lg * 16;
+  GP_LDS const char* pl = lds + l.powers + c0;
   const i32x8 one = {0x01010101, 0x01010101, 0x01010101, 0x01010101, 0x01010101, 0x01010101, 0x01010101, 0x01010101};
   const int ng = kChunk >> gshift, gb = (lg * 32) >> gshift;  // groups a chunk; the one of block lg, whose power this lane gives
-  float tot = 0.f;
+  f4 tot = {0.f, 0.f, 0.f, 0.f};
   int at = 0;
 #pragma unroll 1
   for (int t = 0; t < nc; ++t) {
@@ -549,7 +548,7 @@ __global__ __launch_bounds__(1024) void q4_token_kernel(Q4Args p, int ctshift, i
 #pragma unroll
     for (int i = 0; i < 4; ++i) w[i] = *(GP_LDS const unsigned*)(slot + i * 256 + lg * 64 + j * 4);
     const u32x4 a0 = *(GP_LDS const u32x4*)(xl + t * kChunk), a1 = *(GP_LDS const u32x4*)(xl + t * kChunk + 64);
-    const int pw = (int)*(GP_LDS const unsigned char*)(pl + t) - 5 * (j & 3);
+    const int pw = (int)*(GP_LDS const unsigned char*)(pl + t) - 5 * digit;
     // what was read is in registers before the slot takes the chunk kRing further on
     compiler_fence();
     __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
@@ -570,22 +569,22 @@ __global__ __launch_bounds__(1024) void q4_token_kernel(Q4Args p, int ctshift, i
       const int sat = (t * ng + g) * 32 + j * 2;
       const float s = T::val(*(GP_LDS const half_t*)(sl + sat));
       const float zv = T::val(*(GP_LDS const half_t*)(zl + sat)), z = sd.z ? zv : 8.f;
-      const float v = (d[0] + d[1]) + (d[2] + d[3]), x = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tot = __builtin_fmaf(s, __builtin_fmaf(-z, x, v), tot);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) tot[e] = __builtin_fmaf(s, __builtin_fmaf(-z, sum[e], d[e]), tot[e]);
     }
   }
 
   // the waves of a column tile in their order
-  part[(wave * 4 + lg) * kTokenCols + j] = tot;
+  if (lg < 2) part[wave][lg][j] = lg ? tot[0] + tot[1] : (tot[0] + tot[1]) + (tot[2] + tot[3]);
   __syncthreads();
-  const int n = tid & (kTokenCols - 1), row = (tid / kTokenCols) & 3, tl = tid / (kTokenCols * 4);
-  if (tl < CT && row < M && n0 + tl * kTokenCols + n < N) {
+  const int n = tid & (kTokenCols - 1), tl = tid / kTokenCols;
+  if (tl < CT && n0 + tl * kTokenCols + n < N) {
     float v = 0.f, u = 0.f;
-    const float* pv = part + (tl * KW * 4 + row) * kTokenCols + n;
-    for (int w = 0; w < KW; ++w) v += pv[w * 4 * kTokenCols];
+    auto sum = [&](int w) { return part[w][0][n] + part[w][1][n]; };
+    for (int w = 0; w < KW; ++w) v += sum(tl * KW + w);
     if (p.sides == 2)
-      for (int w = 0; w < KW; ++w) u += pv[(CT * KW + w) * 4 * kTokenCols];
-    q4_store<T>(p, row, n0 + tl * kTokenCols + n, v, u);
+      for (int w = 0; w < KW; ++w) u += sum((CT + tl) * KW + w);
+    q4_store<T>(p, 0, n0 + tl * kTokenCols + n, v, u);
   }
 }
 
@@ -977,13 +976,18 @@ bool on_tiles(int64_t M, int N, int K, int group, int sides) {
 template <class T>
 hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
   const int chunks = (a.K + kChunk - 1) / kChunk;
-  if (a.M <= 4 && a.N % 2 == 0) {
+  // One row, and one only: with this kernel and the one for few rows 4,096
+  // columns from 4,096 k take 4.4 and 4.8 us, 8,192 from 8,192 7.9 and 8.4, 2 x
+  // 16,384 from 4,096 13.5 and 15.2 (the other way round 1,024 from 1,024 3.2 and
+  // 3.0, 8,192 from 16,384 17.8 and 14.5); two rows, with digits enough for an
+  // fp32 sum, 5.6 and 4.9, 9.2 and 8.2, 14.5 and 15.2, three 6.3 and 4.8.
+  if (a.M == 1 && a.N % 2 == 0) {
     int ct = a.N >= 64 * num_cus ? 4 : a.N >= 32 * num_cus ? 2 : 1;
     int kw = 16 / (ct * a.sides);
     while (kw > 1 && kw / 2 >= chunks) kw /= 2;
     const int waves = kw * ct * a.sides;
     const bool z = a.side[0].z || a.side[1].z;
-    const TokenLds l = token_lds((int)a.M, a.K, a.group, waves, kw, z);
+    const TokenLds l = token_lds(a.K, a.group, waves, kw, z);
     if (l.bytes <= kTokenLds) return token_launch<T>(a, waves, ct, kw, l, s);
   }
   if (on_tiles(a.M, a.N, a.K, a.group, a.sides)) {

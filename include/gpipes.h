@@ -584,9 +584,9 @@ int64_t gp_q4_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int we
  * Weights are not rounded, sums are fp32, out is rounded once.  A group's sum
  * is that of x q less z times that of x: it keeps 2^-24 of the larger of the
  * two, so an x under a small weight leaves an error as under one of 15 or |z|.
- * (With up to four rows a value of x may be taken to 2^-19 of the largest of
- * its 128 neighbours k, about what an fp32 sum of them keeps.  In bf16 values
- * of x below 2^-122 may count as zero.)
+ * (With one row a value of x may be taken to 2^-29 of the largest of its 128
+ * neighbours k, a 32nd of what an fp32 sum of them keeps, and in bf16 to 2^-128
+ * at the finest.)
  * x has to be finite and, in bf16, 15 times (|z| times, where that is more) a
  * group's sum of |x| below fp32's largest number: a row of x that is not gives
  * NaN in that row of out alone.  Scales and zeros have to be finite.

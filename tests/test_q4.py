@@ -601,3 +601,39 @@ def test_large_values_under_zero_weights(cuda, M, K, N, zeros, dt):
     want, bound = near(x, q, s, z, 64)
     got = gpipes.q4_gemm_out(x.to(cuda), dev(q4.pack(q), cuda), s.to(cuda), dev(z, cuda), group=64)
     check(got, want, bound, dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 2, 3, 4])
+@pytest.mark.parametrize("K,N,group", [(1024, 256, 64), (4096, 512, 128), (1000, 8208, 32), (2048, 16448, 64)])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_large_values_of_few_tokens_under_zero_weights(cuda, M, K, N, group, zeros, dt):
+    """A single row's x may be taken to 2^-29 of the largest of its 128: 2^-29 of that largest times |W| a product, 2e-5
+    at most, which add up at random to 2e-5 x 6.5 sqrt(3 x 128) / sqrt(3) = 0.0015 in units of a scale, where a result
+    is about 6.5 sqrt(1000) = 200 and its rounding in fp16 0.04 (uniform)."""
+    x, q, s, z = outlying(M, K, N, group, zeros, dt, M + N)
+    want, bound = near(x, q, s, z, group)
+    zr = (z if z is not None else torch.full_like(s, 8)).double().repeat_interleave(group, 0)[:K]
+    w = (s.double().repeat_interleave(group, 0)[:K] * (q - zr)).abs()
+    for k in range(0, K if M == 1 else 0, 128):
+        bound += 2.0 ** -29 * x[:, k:k + 128].abs().amax(1, keepdim=True).double() * w[k:k + 128].sum(0)
+    got = gpipes.q4_gemm_out(x.to(cuda), dev(q4.pack(q), cuda), s.to(cuda), dev(z, cuda), group=group)
+    check(got, want, bound, dt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 2, 3, 4])
+def test_values_of_one_token_do_not_reach_another(cuda, M):
+    """Tokens share a matrix instruction: what the others hold, large, infinite or NaN, leaves a token's bits alone."""
+    gen = torch.Generator().manual_seed(M)
+    for dt, N in ((F16, 128), (BF16, 8208)):
+        x = torch.randn(M, 640, generator=gen).to(dt).to(cuda)
+        q, s, z = weight(640, N, 32, True, dt, gen)
+        args = [dev(t, cuda) for t in (q4.pack(q), s, z)]
+        want = gpipes.q4_gemm_out(x, *args, group=32)
+        for m in range(M):
+            for v in (0.0, 30000.0, float("inf"), float("nan")):
+                other = torch.full_like(x, v)
+                other[m] = x[m]
+                assert torch.equal(gpipes.q4_gemm_out(other, *args, group=32)[m], want[m])
