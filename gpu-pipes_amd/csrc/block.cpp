@@ -87,6 +87,16 @@ int q4_run(const Q4Args& a, int64_t N, int64_t K, hipStream_t stream) {
   if (meet(a.ws, a.ws_bytes / 2, a.x, a.M * K) || meet(a.ws, a.ws_bytes / 2, a.out, a.M * N) ||
       meet(a.ws, a.ws_bytes / 2, a.r, a.M * N))
     return fail(GP_ERR_INVALID_ARG, "the workspace must not overlap x, r or out");
+  const int64_t scales = (K + a.group - 1) / a.group * N;
+  for (int i = 0; i < a.sides; ++i) {
+    const Q4Side& d = a.side[i];
+    auto meets = [&](const void* p, int64_t n) {
+      return meet(p, n, d.wq, K / 4 * N) || meet(p, n, d.s, scales) || meet(p, n, d.z, scales) || meet(p, n, d.b, N);
+    };
+    if (meets(a.out, a.M * N)) return fail(GP_ERR_INVALID_ARG, "out must not overlap a weight, its scales, zeros or b");
+    if (meets(a.ws, a.ws_bytes / 2))
+      return fail(GP_ERR_INVALID_ARG, "the workspace must not overlap a weight, its scales, zeros or b");
+  }
   int dev = 0, ncu = 0;
   if ((rc = current_device_info(&dev, &ncu))) return rc;
   Q4Args b = a;

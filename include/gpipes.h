@@ -596,8 +596,9 @@ int64_t gp_q4_workspace_bytes(int64_t M, int64_t N, int64_t K, int group, int we
  * launch, always in one order.  With less (0 and NULL) the product is computed
  * in one launch, more slowly, and may differ in a sum's last bits.  Calls that
  * may run at the same time, in graphs too, need workspaces of their own.
- * Can be captured into a graph.  out may be r; that it overlaps x, or r
- * otherwise, or that the workspace overlaps one of them, is refused.
+ * Can be captured into a graph.  out may be r; that it overlaps r otherwise, x,
+ * wq, scales, zeros or b, or that the workspace overlaps one of these or out,
+ * is refused.
  * No counterpart in the reference (16-bit weights only).
  */
 int gp_q4_gemm_out(int64_t M, int64_t N, int64_t K, int group, const void* x, const void* wq, const void* scales,

@@ -67,6 +67,20 @@ def test_a_residual_that_overlaps_is_refused():
     assert _call(x=1 << 20, out=1 << 21, r=1 << 22, ws=(1 << 22) + 2032, wsb=16) == -1
 
 
+@pytest.mark.parametrize("what,size,two", [
+    (what, size, two) for what, size in (("wq", 512 * 256 // 2), ("s", 4 * 256 * 2), ("z", 4 * 256 * 2), ("b", 256 * 2),
+                                         ("u", 512 * 256 // 2)) for two in (False, True) if two or what != "u"])
+def test_overlaps_with_the_weight_are_refused(what, size, two):
+    """out and the workspace over the first or the last 16 bytes of a weight's tensors."""
+    at = 1 << 24
+    far = dict(x=1 << 20, out=1 << 21, wq=1 << 22, s=1 << 23, z=5 << 21, b=11 << 20, u=13 << 20)
+    for lo, n in ((at - 2048 + 16, 2048), (at + size - 16, 2048)):  # out's 4 x 256 values
+        assert _call(**{**far, what: at, "out": lo}, two=two) == -1
+        assert "out must not overlap" in gpipes.lib.gp_last_error().decode()
+        assert _call(**{**far, what: at}, ws=lo, wsb=n, two=two) == -1
+        assert "workspace must not overlap" in gpipes.lib.gp_last_error().decode()
+
+
 def test_empty_batch_is_a_noop():
     assert _call(M=0, x=0, out=0) == 0
     assert _call(M=0, x=0, out=0, two=True) == 0
