@@ -20,6 +20,8 @@ import os
 
 import torch
 
+from . import q4
+
 __all__ = [
     "lib", "mgn_fullmlp", "mgn_fullmlp_out", "mgn_linears", "mgn_linears_out",
     "mgn_mlp", "mgn_mlp_out", "IMPL_FUSED", "IMPL_PIPELINED", "IMPL_PIPELINED_SPLIT_LN", "GpipesError",
@@ -29,7 +31,7 @@ __all__ = [
     "dlrm_topmlp_out", "nerf_full", "nerf_full_out", "nerf_full_out_noalloc", "bert_addln_ffn",
     "bert_addln_ffn_out", "nerf_a", "nerf_a_out", "pipe_handoff", "handoff_checksums", "phase_timers",
     "probe_mfma", "fill_normal", "residual_norm_out", "residual_norm", "NORMS", "q4_gemm_out",
-    "q4_gated_out",
+    "q4_gated_out", "q4",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))

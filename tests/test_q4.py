@@ -5,6 +5,9 @@ bound from the arithmetic (product(), below), and as a whole: the error's norm m
 larger than that of the exact result rounded to the element type.
 """
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -100,6 +103,13 @@ def test_python_refuses():
         gpipes.q4_gemm_out(x, wq, s)
     with pytest.raises(RuntimeError, match="CUDA"):
         gpipes.q4_gated_out(x, wq, s, None, wq, s, None)
+
+
+def test_the_package_has_the_weights_module():
+    """As it is named in the documents: gpipes.q4 after `import gpipes` alone."""
+    code = "import gpipes; assert gpipes.q4.pack and 'q4' in gpipes.__all__"
+    path = os.path.dirname(os.path.dirname(gpipes.__file__))
+    subprocess.run([sys.executable, "-c", code], check=True, cwd=path, timeout=120)
 
 
 def test_pack_and_unpack():
