@@ -9,9 +9,10 @@ def pack(q):
     """q [K, N], whole numbers 0 .. 15, K a multiple of 8 -> int32 words [K / 8, N], the lowest k in the lowest bits."""
     if q.dim() != 2 or q.shape[0] % 8:
         raise RuntimeError("q must be [K, N] with K a multiple of 8")
-    if q.numel() and (int(q.min()) < 0 or int(q.max()) > 15):
-        raise RuntimeError("q must be in 0 .. 15")
-    v = q.to(torch.int64).view(-1, 8, q.shape[1])
+    v = q.to(torch.int64)
+    if not bool(((v >= 0) & (v <= 15) & (v == q)).all()):  # a fraction, a NaN or an infinity is no longer what it was
+        raise RuntimeError("q must be whole numbers in 0 .. 15")
+    v = v.view(-1, 8, q.shape[1])
     w = v[:, 0].clone()
     for i in range(1, 8):
         w |= v[:, i] << (4 * i)

@@ -141,6 +141,15 @@ def test_quantize(group, zeros, dt):
     assert (got[:, 3] == 0).all()
 
 
+@pytest.mark.parametrize("v", [3.7, -0.5, 15.5, 1e-3, float("nan"), float("inf")])
+def test_pack_refuses_what_is_no_whole_number(v):
+    q = torch.full((8, 3), 7.0)
+    assert torch.equal(q4.unpack(q4.pack(q)).float(), q)  # whole numbers of any type
+    q[5, 1] = v
+    with pytest.raises(RuntimeError, match="whole numbers"):
+        q4.pack(q)
+
+
 def test_quantize_refuses():
     w = torch.ones(16, 4, dtype=F16)
     for bad, kw in ((w[:9], {}), (w.float(), {}), (w, dict(group=16)), (w * float("inf"), {})):
