@@ -1087,10 +1087,9 @@ def q4_gated_out(x, wq_g, scales_g, zeros_g, wq_u, scales_u, zeros_u, bg=None, b
         N = wq_g.shape[1]
         if out is None:
             out = torch.empty((M, N), dtype=dt, device=x.device)
-        words, groups = (K // 8, N), (-(-K // group), N)
         ok = (group in (32, 64, 128) and K % 8 == 0 and dt in _DTYPES and dev >= 0 and x.is_contiguous()
-              and _q4_weight(wq_g, scales_g, zeros_g, words, groups, dt, dev)
-              and _q4_weight(wq_u, scales_u, zeros_u, words, groups, dt, dev)
+              and _q4_weight(wq_g, scales_g, zeros_g, (K // 8, N), (-(-K // group), N), dt, dev)
+              and _q4_weight(wq_u, scales_u, zeros_u, (K // 8, N), (-(-K // group), N), dt, dev)
               and (bg is None or (bg.dtype is dt and bg.get_device() == dev and bg.shape == (N,) and bg.is_contiguous()))
               and (bu is None or (bu.dtype is dt and bu.get_device() == dev and bu.shape == (N,) and bu.is_contiguous()))
               and out.dtype is dt and out.get_device() == dev and out.shape == (M, N) and out.is_contiguous())

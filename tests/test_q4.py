@@ -105,6 +105,15 @@ def test_python_refuses():
         gpipes.q4_gated_out(x, wq, s, None, wq, s, None)
 
 
+@pytest.mark.parametrize("group", [0, 16, 256, -32, 1.5, None, "128"])
+def test_python_refuses_groups(group):
+    x, wq, s = torch.zeros(1, 64, dtype=F16), torch.zeros(8, 32, dtype=torch.int32), torch.zeros(1, 32, dtype=F16)
+    with pytest.raises(RuntimeError):
+        gpipes.q4_gemm_out(x, wq, s, group=group)
+    with pytest.raises(RuntimeError):
+        gpipes.q4_gated_out(x, wq, s, None, wq, s, None, group=group)
+
+
 def test_the_package_has_the_weights_module():
     """As it is named in the documents: gpipes.q4 after `import gpipes` alone."""
     code = "import gpipes; assert gpipes.q4.pack and 'q4' in gpipes.__all__"
