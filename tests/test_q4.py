@@ -150,6 +150,13 @@ def test_quantize(group, zeros, dt):
     assert (got[:, 3] == 0).all()
 
 
+@pytest.mark.parametrize("dt", [torch.uint8, torch.int64, torch.float32])
+def test_pack_takes_any_strides(dt):
+    q = torch.randint(0, 16, (13, 40), generator=torch.Generator().manual_seed(0)).to(dt).t()
+    wq = q4.pack(q)
+    assert wq.is_contiguous() and torch.equal(wq, q4.pack(q.contiguous())) and torch.equal(q4.unpack(wq).to(dt), q)
+
+
 @pytest.mark.parametrize("v", [3.7, -0.5, 15.5, 1e-3, float("nan"), float("inf")])
 def test_pack_refuses_what_is_no_whole_number(v):
     q = torch.full((8, 3), 7.0)
