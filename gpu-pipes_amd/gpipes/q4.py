@@ -12,7 +12,7 @@ def pack(q):
     v = q.to(torch.int64)
     if not bool(((v >= 0) & (v <= 15) & (v == q)).all()):  # a fraction, a NaN or an infinity is no longer what it was
         raise RuntimeError("q must be whole numbers in 0 .. 15")
-    v = v.reshape(q.shape[0] // 8, 8, q.shape[1])
+    v = v.contiguous().view(-1, 8, q.shape[1])
     w = v[:, 0].clone()
     for i in range(1, 8):
         w |= v[:, i] << (4 * i)
