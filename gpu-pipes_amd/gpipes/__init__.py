@@ -938,11 +938,14 @@ def _misfit(x, named):
 
 def _run_on(dev, fn, args):
     """fn(*args, current stream of device dev) with that device current."""
-    if _raw_stream is not None and _current_device() == dev:
-        rc = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    try:
+        if _raw_stream is not None and _current_device() == dev:
+            rc = fn(*args, _raw_stream(dev))
+        else:
+            with torch.cuda.device(dev):
+                rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    except ctypes.ArgumentError as e:  # an unknown name of a norm or activation, a scale or eps that is no number
+        raise RuntimeError(f"invalid argument: {e}") from None
     if rc:
         _check(rc)
 

@@ -686,3 +686,14 @@ def test_values_of_one_token_do_not_reach_another(cuda, M):
                 other = torch.full_like(x, v)
                 other[m] = x[m]
                 assert torch.equal(gpipes.q4_gemm_out(other, *args, group=32)[m], want[m])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["foo", 9, 1.5, None])
+def test_unknown_activations_raise_runtime_errors(cuda, act):
+    q, s, _ = weight(64, 32, 32, False, F16, torch.Generator().manual_seed(0))
+    x, wq, s = torch.zeros(2, 64, dtype=F16, device=cuda), q4.pack(q).to(cuda), s.to(cuda)
+    with pytest.raises(RuntimeError):
+        gpipes.q4_gemm_out(x, wq, s, act=act, group=32)
+    with pytest.raises(RuntimeError):
+        gpipes.q4_gated_out(x, wq, s, None, wq, s, None, act=act, group=32)

@@ -332,3 +332,12 @@ def test_more_values_than_32_bits_count(cuda):
         (h64, dh), (o64, do) = ref({**a, "x": x[rows], "y": y[rows]})
         check(h[rows], h64, dh, BF16)
         check(out[rows], o64, do, BF16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(norm="foo"), dict(post="foo"), dict(gate_act="foo"), dict(scale="1"), dict(eps=None),
+                                dict(post_eps="x"), dict(norm=7), dict(gate_act=-1)])
+def test_unknown_names_and_no_numbers_raise_runtime_errors(cuda, kw):
+    x = torch.zeros(2, 64, dtype=F16, device=cuda)
+    with pytest.raises(RuntimeError):
+        gpipes.residual_norm_out(x, x, gate=x, **kw)
