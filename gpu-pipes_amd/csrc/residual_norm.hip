@@ -259,11 +259,12 @@ hipError_t residual_norm_launch(const ResidualNormArgs& a, int num_cus, hipStrea
   const int64_t teams = block / kWave / W;
   // Up to four rows a team, so that what belongs to the channels is loaded once
   // for them, but not so many that workgroups get fewer than four a CU
-  // (16,384 x 4,096: four rows 103 us, two 112, sixteen 125).
+  // (16,384 x 4,096: four rows 103 us, two 112, sixteen 125).  More where a
+  // launch would pass the 2^32 - 1 threads that it may have.
   const int64_t groups = (a.M + teams - 1) / teams, most = (groups + 4 * num_cus - 1) / (4 * num_cus);
-  const int64_t rows = most < 4 ? most : 4;
+  const int64_t limit = ((int64_t(1) << 32) - 1) / block, least = (groups + limit - 1) / limit;
+  const int64_t four = most < 4 ? most : 4, rows = four > least ? four : least;
   const int64_t grid = (a.M + teams * rows - 1) / (teams * rows);
-  if (grid > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
   const Args p{a, W, rows, a.gate ? a.M / a.gate_rows : 1};
   return a.dtype == GP_DTYPE_BF16 ? by_tail<BF16>(p, C, block, (unsigned)grid, s)
                                   : by_tail<F16>(p, C, block, (unsigned)grid, s);

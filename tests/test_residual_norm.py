@@ -341,3 +341,19 @@ def test_unknown_names_and_no_numbers_raise_runtime_errors(cuda, kw):
     x = torch.zeros(2, 64, dtype=F16, device=cuda)
     with pytest.raises(RuntimeError):
         gpipes.residual_norm_out(x, x, gate=x, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,gated", [((1 << 28) + 5, False), ((1 << 28) + 6, True), ((1 << 31) + 9, False)])
+def test_more_rows_than_a_launch_has_threads(cuda, M, gated):
+    """2^28 rows of one value and more, sixteen a workgroup of 256, are 2^32 threads: every row all the same."""
+    x = torch.randn(1 << 20, dtype=F16, device=cuda).repeat((M >> 20) + 1)[:M].view(M, 1)
+    gate = torch.tensor([[0.5], [2.0]], dtype=F16, device=cuda) if gated else None
+    h = torch.full((M + 64,), 7.0, dtype=F16, device=cuda)
+    gpipes.residual_norm_out(x, x, gate=gate, scale=0.5, norm="none", h=h[:M].view(M, 1))
+    # h = 1.5 x, or with the gate 1.25 x in the first half and 2 x in the second: fp32 holds all, so one rounding
+    for at in range(0, M, 1 << 28):
+        v, n = x[at:at + (1 << 28), 0], min(1 << 28, M - at)
+        k = 1.5 if not gated else torch.where(torch.arange(at, at + n, device=cuda) < M // 2, 1.25, 2.0)
+        assert torch.equal(h[at:at + n], (v.float() * k).half())
+    assert (h[M:] == 7).all()
