@@ -630,7 +630,7 @@ def near(x, q, s, z, group):
     K = q.shape[0]
     zz = z.double() if z is not None else torch.full_like(s, 8)
     sr, zr = (t.repeat_interleave(group, 0)[:K] for t in (s, zz))
-    run = torch.zeros(x.shape[0], q.shape[1], dtype=torch.float64)
+    run = torch.zeros(x.shape[0], q.shape[1], dtype=torch.float64, device=x.device)
     for k in range(0, K, group):
         run += (x[:, k:k + group] @ (sr * (q - zr))[k:k + group]).abs()
     return x @ (sr * (q - zr)), 16 * U * (x.abs() @ (sr * (q + zr.abs()))) + 100 * U * run
@@ -697,3 +697,144 @@ def test_unknown_activations_raise_runtime_errors(cuda, act):
         gpipes.q4_gemm_out(x, wq, s, act=act, group=32)
     with pytest.raises(RuntimeError):
         gpipes.q4_gated_out(x, wq, s, None, wq, s, None, act=act, group=32)
+
+
+# ---------------------------------------------------------------------------
+# Every kernel that a call can select, at sizes that no tile divides
+# ---------------------------------------------------------------------------
+
+def run_case(M, K, N, group, zeros, dt, d, two, seed):
+    """A product with bias (and a residual), or a gated pair with biases, against the formulas; in 64 bits on the GPU."""
+    gen = torch.Generator().manual_seed(seed)
+    n = lambda *sh: torch.randn(*sh, generator=gen).to(dt).to(d)  # noqa: E731
+    x, sides, args = n(M, K), [], []
+    for _ in range(2 if two else 1):
+        q, s, z = weight(K, N, group, zeros, dt, gen)
+        q, s, z, b = q.to(d), s.to(d), dev(z, d), n(N)
+        v, dv = near(x, q, s, z, group)
+        sides.append((v + b.double(), dv + 2 * U * (v.abs() + b.double().abs())))
+        args.append((q4.pack(q), s, z, b))
+    buf = torch.full((M * N + 512,), 7.0, dtype=dt, device=d)
+    out = buf[:M * N].view(M, N)
+    if two:
+        (g, dg), (u, du) = moved(*sides[0], "silu"), sides[1]
+        want, bound = g * u, dg * (u.abs() + du) + g.abs() * du + 2 * U * (g * u).abs()
+        gpipes.q4_gated_out(x, *args[0][:3], *args[1][:3], bg=args[0][3], bu=args[1][3], group=group, out=out)
+    else:
+        r = n(M, N)
+        v, dv = sides[0]
+        want, bound = v + r.double(), dv + 2 * U * (v.abs() + r.double().abs())
+        gpipes.q4_gemm_out(x, *args[0], r=r, group=group, out=out)
+    check(out, want.cpu(), bound.cpu(), dt)
+    assert (buf[M * N:] == 7).all()
+
+
+# (rows, k, columns), of the pair each weight's: tiles of 64, 128 and 256 columns, k whole and in parts (256 CUs)
+TILES = [(130, 136, 61, False), (130, 520, 61, False), (1030, 136, 5001, False), (700, 4104, 1030, False),
+         (257, 136, 11003, False), (65, 2056, 6001, False), (130, 136, 61, True), (130, 520, 61, True),
+         (257, 136, 8195, True), (700, 4104, 515, True), (130, 136, 8195, True), (65, 2056, 3001, True)]
+# one to four tiles of 16 rows, and up to four rows, by one, two and four columns a lane
+FEW = [(M, K, N, two) for M in (1, 3, 4, 9, 25, 45) for K, N, two in ((1160, 67, False), (392, 8195, False),
+                                                                     (136, 16387, False), (1160, 35, True),
+                                                                     (392, 4099, True), (136, 8195, True))]
+FEW += [(60, 1160, 67, False), (64, 136, 8192, False), (100, 1160, 67, False), (60, 1160, 35, True), (52, 392, 4096, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,two", TILES + FEW)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_every_kernel(cuda, M, K, N, two, group, zeros):
+    for dt in (F16, BF16):
+        print(M, K, N, two, group, zeros, dt, flush=True)
+        run_case(M, K, N, group, zeros, dt, cuda, two, M + N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,two", [(1, 1160, 66, False), (1, 392, 8194, False), (1, 136, 16386, False),
+                                       (1, 520, 130, True), (1, 392, 8198, True), (1, 136, 16390, True)])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_every_width_of_the_one_token_kernel(cuda, M, K, N, two, group, zeros):
+    for dt in (F16, BF16):
+        run_case(M, K, N, group, zeros, dt, cuda, two, N)
+
+
+# ---------------------------------------------------------------------------
+# Rows and calls that must not see each other
+# ---------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(2, 640, 200), (4, 640, 200), (16, 1024, 328), (40, 1024, 328), (64, 1024, 328),
+                                   (100, 4096, 1032), (200, 1024, 328), (700, 512, 2056)])
+@pytest.mark.parametrize("two", [False, True])
+def test_a_row_keeps_its_bits_among_other_rows(cuda, M, K, N, two):
+    """Other values in every other row, large and not finite ones among them, leave a row's bits as they were."""
+    gen = torch.Generator().manual_seed(M + N)
+    sides = []
+    for _ in range(2):
+        q, s, z = weight(K, N, 64, True, BF16, gen)
+        sides += [dev(t, cuda) for t in (q4.pack(q), s, z)]
+
+    def call(x):
+        return gpipes.q4_gated_out(x, *sides, group=64) if two else gpipes.q4_gemm_out(x, *sides[:3], group=64)
+
+    x = torch.randn(M, K, generator=gen).to(BF16).to(cuda)
+    want = call(x)
+    for m in sorted({0, 1, M // 2, M - 1}):
+        for k in (1.0, 1e4, float("nan")):
+            other = (torch.randn(M, K, generator=gen) * k).to(BF16).to(cuda)
+            other[m] = x[m]
+            assert torch.equal(call(other)[m], want[m])
+
+
+@pytest.mark.gpu
+def test_two_streams_and_two_graphs_with_workspaces(cuda):
+    """Calls with parts of k in a workspace, on two streams at once, eager and replayed together."""
+    gen = torch.Generator().manual_seed(9)
+    sets = []
+    for M, K, N in ((100, 4096, 1032), (65, 4096, 520)):
+        assert gpipes.lib.gp_q4_workspace_bytes(M, N, K, 128, 1) > 0
+        q, s, z = weight(K, N, 128, True, F16, gen)
+        x = torch.randn(M, K, generator=gen).to(F16).to(cuda)
+        args = [dev(t, cuda) for t in (q4.pack(q), s, z)]
+        outs = [torch.empty(M, N, dtype=F16, device=cuda) for _ in range(2)]
+        want = gpipes.q4_gemm_out(x, *args)
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            for _ in range(20):
+                gpipes.q4_gemm_out(x, *args, out=outs[0])
+        sets.append((x, args, outs, want, g, torch.cuda.Stream(cuda), torch.cuda.Stream(cuda)))
+    for _ in range(3):
+        for _, _, outs, *_ in sets:
+            outs[0].zero_(), outs[1].zero_()
+        torch.cuda.synchronize()
+        for x, args, outs, want, g, a, b in sets:
+            with torch.cuda.stream(a):
+                g.replay()
+            with torch.cuda.stream(b):
+                for _ in range(20):
+                    gpipes.q4_gemm_out(x, *args, out=outs[1])
+        torch.cuda.synchronize()
+        for x, args, outs, want, *_ in sets:
+            assert torch.equal(outs[0], want) and torch.equal(outs[1], want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 3, 20, 64, 150, 300])
+def test_the_largest_values_of_fp16(cuda, M):
+    """Rows of +-65,504, of fp16's smallest values, and both together, with scales that keep the results in range."""
+    gen = torch.Generator().manual_seed(M)
+    K, N, G = 640, 144, 64
+    x = torch.where(torch.rand(M, K, generator=gen) < 0.5, -65504.0, 65504.0)
+    x[1::3] = torch.randint(-9, 10, x[1::3].shape, generator=gen) * 2.0 ** -24
+    x[2::3, ::2] = torch.randint(-9, 10, x[2::3, ::2].shape, generator=gen) * 2.0 ** -24
+    x = x.to(F16)
+    q, s, z = weight(K, N, G, True, F16, gen)
+    s = (s.double() / 64).to(F16)
+    want, bound = near(x, q, s, z, G)
+    got = gpipes.q4_gemm_out(x.to(cuda), *(dev(t, cuda) for t in (q4.pack(q), s, z)), group=G)
+    if M == 1:
+        bound += 2.0 ** -29 * 65504 * (s.double().repeat_interleave(G, 0) * (q - z.double().repeat_interleave(G, 0))).abs().sum(0)
+    check(got, want, bound, F16)
