@@ -999,9 +999,10 @@ hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
   }
   const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : a.M <= 48 ? 3 : 4;
   // Tiles of 16 columns a wave, both weights' together: as many as leave every
-  // CU a workgroup, so that x is read for more columns at once.
+  // CU a workgroup, so that x is read for more columns at once.  (Four with more
+  // than 48 rows: a whole chip's products of so many columns run on tiles.)
   const int64_t n = (int64_t)a.N * a.sides;
-  int nt = n >= 64 * num_cus ? 4 : n >= 32 * num_cus ? 2 : 1;
+  int nt = n >= 64 * num_cus && mt < 4 ? 4 : n >= 32 * num_cus ? 2 : 1;
   if ((int64_t)((a.K + a.group - 1) / a.group) * a.N < 4) nt = 1;
   const int cw = nt > a.sides ? nt / a.sides : 1;
   int waves = rows_waves(cw * a.sides, mt);
@@ -1010,14 +1011,14 @@ hipError_t launch(const Q4Args& a, int num_cus, hipStream_t s) {
 #define GP_CASE(c, m, four)                                       \
   if (cw == c && a.sides == 1 && mt == m && (a.M <= 4) == four)   \
     return rows_launch<T, c, 1, m, four>(a, waves, grid, s);      \
-  if constexpr (c <= 2)                                           \
+  if constexpr (c <= 2 && c * m < 8)                              \
     if (cw == c && a.sides == 2 && mt == m && (a.M <= 4) == four) \
       return rows_launch<T, c, 2, m, four>(a, waves, grid, s);
   GP_CASE(1, 1, true) GP_CASE(2, 1, true) GP_CASE(4, 1, true)
   GP_CASE(1, 1, false) GP_CASE(2, 1, false) GP_CASE(4, 1, false)
   GP_CASE(1, 2, false) GP_CASE(2, 2, false) GP_CASE(4, 2, false)
   GP_CASE(1, 3, false) GP_CASE(2, 3, false) GP_CASE(4, 3, false)
-  GP_CASE(1, 4, false) GP_CASE(2, 4, false) GP_CASE(4, 4, false)
+  GP_CASE(1, 4, false) GP_CASE(2, 4, false)
 #undef GP_CASE
   return hipErrorInvalidValue;
 }

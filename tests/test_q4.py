@@ -838,3 +838,21 @@ def test_the_largest_values_of_fp16(cuda, M):
     if M == 1:
         bound += 2.0 ** -29 * 65504 * (s.double().repeat_interleave(G, 0) * (q - z.double().repeat_interleave(G, 0))).abs().sum(0)
     check(got, want, bound, F16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [2, 4, 6, 14, 18])
+def test_one_token_of_few_columns(cuda, N):
+    for K, group, two in ((8, 32, False), (64, 32, True), (264, 64, False), (1400, 128, True)):
+        for dt in (F16, BF16):
+            run_case(1, K, N, group, K != 264, dt, cuda, two, N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,group,zeros,two", [(19968, 128, False, False), (19976, 128, False, False),
+                                               (15872, 32, True, False), (15872, 64, True, True), (15880, 64, True, True),
+                                               (15872, 32, False, True), (65536, 128, True, True)])
+def test_one_token_of_the_deepest_k_that_lds_holds(cuda, K, group, zeros, two):
+    """All of a CU's 160 KiB, and the next k, which another kernel takes."""
+    for dt in (F16, BF16):
+        run_case(1, K, 66, group, zeros, dt, cuda, two, K)
