@@ -613,9 +613,9 @@ hipError_t token_launch(const Q4Args& a, int waves, int ct, int kw, const TokenL
 //
 // Bound by instruction issue: two waves a SIMD run about 430 instructions a
 // chunk for 64 MFMAs (64 conversions, 48 masks and shifts for them, 64 fused
-// multiply-adds of the groups' ends), the matrix cores busy 38% of the time and
-// the vector units 57%.  4,096 rows, 4,096 columns from 4,096 k: 142 to 147 us, 0.93
-// to 0.97 PFLOP/s (this card's library product of 16-bit operands of that size: 127).
+// multiply-adds of the groups' ends), the matrix cores busy 43% of the time and
+// the vector units 61%.  4,096 rows, 4,096 columns from 4,096 k: 138 to 144 us, 0.95
+// to 0.99 PFLOP/s (this card's library product of 16-bit operands of that size: 127).
 // Tried and no faster: operands one to four steps ahead, words copied to LDS
 // two chunks ahead, MFMAs and operand instructions interleaved by the scheduler's
 // groups (163), wave priorities, offsets in scalar registers.
@@ -901,7 +901,9 @@ struct TilePlan {
 // columns 50, 37 and 30 us with CW 4, 2 and 1; 1,024 rows, which are one, two and
 // four workgroups a CU, 52, 53 and 63); the second kernel takes 3 us and the
 // workspace's way to memory and back.  128 rows of 4,096 columns from 4,096 k:
-// 64 columns a tile and three parts 20 us, 256 columns in one part 50.
+// 64 columns a tile and three parts 19 us, 256 columns in one part 50.  Not in it:
+// a tile's prologue and epilogue, a third of the time at 1,024 k, and the group
+// and zeros (all of the above: groups of 128 without zeros).
 TilePlan tile_plan(int64_t M, int N, int K, int sides, int num_cus) {
   const int64_t mtiles = (M + kTileRows - 1) / kTileRows;
   const int chunks = (K + kChunk - 1) / kChunk;
@@ -961,12 +963,18 @@ hipError_t rows_launch(const Q4Args& a, int waves, dim3 grid, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Products that run on tiles.  Up to 128 rows small ones do not (128 rows, 1,024
-// columns from 1,024 k: 9.0 us on tiles, 6.5 by the kernel for few rows; 2,048
-// columns 9.9 and 6.8, 4,096 10.4 and 11.7; 1,024 columns from 16,384 k 22 and
-// 33), up to 64 those whose x the kernel for few rows does not read for too many
-// columns (64 rows, k 4,096: 4,096 columns 17 us on tiles and 13, 16,384 26 and
-// 30, 2 x 16,384 45 and 81; 8,192 from 8,192 26.4 and 25), up to 48 none.
+// Products that run on tiles.  Up to 128 rows small ones do not, up to 64 those
+// whose x the kernel for few rows does not read for too many columns, up to 48
+// none.  In us, on tiles / by the kernel for few rows:
+//    65 and 128 rows: 1,024 columns from 1,024 k   9.6 / 6.6,   9.1 / 6.6
+//                     2,048         from 2,048 k  12.1 / 8.4,  11.4 / 8.7
+//                     2,048         from 4,096 k  13.8 / 11.6, 15.7 / 11.8  (the rule errs)
+//                     1,024         from 16,384 k 20.6 / 30,   20.3 / 32
+//                     4,096         from 1,024 k  10.1 / 10.3, 10.3 / 11.4
+//                     4,096         from 4,096 k  16.4 / 20.3, 19.3 / 21.5
+//   64 rows of 4,096 k: 4,096 columns 16.0 / 12.3, 8,192 19.5 / 14.2, 16,384
+//   24.1 / 26.9, 2 x 16,384 35.8 / 53.5; 8,192 from 8,192 24.3 / 23.1
+//   48 rows of 4,096 k: 16,384 columns 23.3 / 15.4, 2 x 16,384 35.5 / 29.3
 bool on_tiles(int64_t M, int N, int K, int group, int sides) {
   if ((int64_t)((K + group - 1) / group) * N < 4) return false;  // a tile's loads of scales are four wide
   const int64_t n = (int64_t)N * sides;
