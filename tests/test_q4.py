@@ -856,3 +856,33 @@ def test_one_token_of_the_deepest_k_that_lds_holds(cuda, K, group, zeros, two):
     """All of a CU's 160 KiB, and the next k, which another kernel takes."""
     for dt in (F16, BF16):
         run_case(1, K, 66, group, zeros, dt, cuda, two, K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N", [(1, 144), (1, 145), (3, 144), (20, 144), (64, 145), (150, 144), (300, 145)])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_large_values_of_bf16(cuda, M, N, zeros):
+    """x up to some 1e35: 15 times a group's sum of |x| stays below fp32's largest number, 3.4e38, and so do results."""
+    gen = torch.Generator().manual_seed(M)
+    K, G = 640, 128
+    x = (torch.randn(M, K, generator=gen) * 2e34).to(BF16)
+    q, s, z = weight(K, N, G, zeros, BF16, gen)
+    assert 16 * 128 * x.double().abs().max() < 3.4e38
+    want, bound = near(x, q, s, z, G)
+    got = gpipes.q4_gemm_out(x.to(cuda), *(dev(t, cuda) for t in (q4.pack(q), s, z)), group=G)
+    check(got / 2.0 ** 110, want / 2.0 ** 110, bound / 2.0 ** 110, BF16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,N", [(1, 520), (1, 521), (2, 520), (16, 521), (48, 520), (64, 521), (130, 520), (700, 1031)])
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_zeros_of_any_value(cuda, M, N, dt):
+    """Negative, fractional and larger than any q."""
+    gen = torch.Generator().manual_seed(M + N)
+    K, G = 1000, 64
+    x = torch.randn(M, K, generator=gen).to(dt)
+    q, s, z = weight(K, N, G, True, dt, gen)
+    z = (torch.randn(z.shape, generator=gen) * 30).to(dt)
+    want, bound = near(x, q, s, z, G)
+    got = gpipes.q4_gemm_out(x.to(cuda), *(dev(t, cuda) for t in (q4.pack(q), s, z)), group=G)
+    check(got, want, bound, dt)
