@@ -1,7 +1,8 @@
 // C ABI of the operators around a language model's feed-forward half: the norms
-// with the residual (gp_residual_norm_out) and the products with 4-bit weights
-// (gp_q4_gemm_out, gp_q4_gated_out).  Argument checks and dispatch; the kernels
-// are in residual_norm.hip and q4.hip.
+// with the residual (gp_residual_norm_out), the products with 4-bit weights
+// (gp_q4_gemm_out, gp_q4_gated_out) and those in 8-bit integers (gp_i8_gemm_out,
+// gp_i8_gated_out).  Argument checks and dispatch; the kernels are in
+// residual_norm.hip, q4.hip and i8.hip.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -106,6 +107,78 @@ int q4_run(const Q4Args& a, int64_t N, int64_t K, hipStream_t stream) {
   return e == hipSuccess ? GP_OK : fail_hip(e, "q4 launch");
 }
 
+// Whether `n` bytes at a and `m` at b have memory in common (NULL has none).
+bool meet_bytes(const void* a, int64_t n, const void* b, int64_t m) {
+  return a && b && (uintptr_t)a < (uintptr_t)b + (uintptr_t)m && (uintptr_t)b < (uintptr_t)a + (uintptr_t)n;
+}
+
+int64_t i8_packed(int64_t N, int64_t K) { return (N + 15) / 16 * ((K + 63) / 64) * 1024; }
+
+int i8_check_weight(int64_t N, int64_t K, const char* n, const char* k) {
+  if (K < 16 || K % 16 || K > kI8MaxK)
+    return fail(GP_ERR_SHAPE, "%s must be a multiple of 16 in [16, %lld] (got %lld)", k, (long long)kI8MaxK, (long long)K);
+  if (N < 1 || N > kQ4MaxDim) return fail(GP_ERR_SHAPE, "%s must be in [1, %lld] (got %lld)", n, (long long)kQ4MaxDim, (long long)N);
+  if (i8_packed(N, K) >= (int64_t(1) << 31)) return fail(GP_ERR_SHAPE, "a packed weight must be smaller than 2 GiB");
+  return GP_OK;
+}
+
+// Scales: 32-bit values of their own alignment.
+int check4(const void* p, const char* name, bool needed) {
+  if (!p) return needed ? fail(GP_ERR_INVALID_ARG, "%s is NULL", name) : GP_OK;
+  if ((uintptr_t)p % 4) return fail(GP_ERR_ALIGN, "%s must be 4-byte aligned", name);
+  return GP_OK;
+}
+
+int i8_check_shape(int64_t M, int64_t N, int64_t K) {
+  int rc = check_rows(M);
+  if (rc || (rc = i8_check_weight(N, K, "N", "K"))) return rc;
+  if (M > (int64_t(1) << 21)) return fail(GP_ERR_SHAPE, "M must be at most 2097152 (got %lld)", (long long)M);
+  return GP_OK;
+}
+
+// a.x is x, 16-bit or (a.xs given) bytes.
+int i8_run(I8Args a, int64_t N, int64_t K, int64_t ws_bytes, hipStream_t stream) {
+  clear_error();
+  int rc;
+  if ((rc = check_dtype(a.dtype)) || (rc = check_act_ext(a.act)) || (rc = i8_check_shape(a.M, N, K))) return rc;
+  if (ws_bytes < 0) return fail(GP_ERR_INVALID_ARG, "workspace_bytes must be >= 0");
+  if (ws_bytes && (rc = check16(a.ws, "workspace", true))) return rc;
+  if (a.r && a.act != GP_ACT_NONE) return fail(GP_ERR_INVALID_ARG, "a residual is added without an activation only");
+  for (int i = 0; i < a.sides; ++i) {
+    const I8Side& d = a.side[i];
+    if ((rc = check16(d.wq, "wq", true)) || (rc = check4(d.s, "w_scales", true)) || (rc = check16(d.b, "b", false)))
+      return rc;
+  }
+  if ((rc = check4(a.xs, "x_scales", false)) || (rc = check16(a.r, "r", false))) return rc;
+  if (a.M == 0) return GP_OK;
+  if ((rc = check16(a.x, "x", true)) || (rc = check16(a.out, "out", true))) return rc;
+  const int64_t out_bytes = a.M * N * 2, x_bytes = a.M * K * (a.xs ? 1 : 2);
+  if (a.r != a.out && meet_bytes(a.out, out_bytes, a.r, out_bytes))
+    return fail(GP_ERR_INVALID_ARG, "out may be r, but not overlap it otherwise");
+  if (meet_bytes(a.ws, ws_bytes, a.out, out_bytes) || meet_bytes(a.ws, ws_bytes, a.r, out_bytes))
+    return fail(GP_ERR_INVALID_ARG, "the workspace must not overlap r or out");
+  auto meets = [&](const void* p, int64_t n) {
+    if (meet_bytes(p, n, a.x, x_bytes) || meet_bytes(p, n, a.xs, a.M * 4)) return true;
+    for (int i = 0; i < a.sides; ++i) {
+      const I8Side& d = a.side[i];
+      if (meet_bytes(p, n, d.wq, i8_packed(N, K)) || meet_bytes(p, n, d.s, N * 4) || meet_bytes(p, n, d.b, N * 2)) return true;
+    }
+    return false;
+  };
+  if (meets(a.out, out_bytes)) return fail(GP_ERR_INVALID_ARG, "out must not overlap x, a weight, scales or b");
+  if (meets(a.ws, ws_bytes)) return fail(GP_ERR_INVALID_ARG, "the workspace must not overlap x, a weight, scales or b");
+  int dev = 0, ncu = 0;
+  if ((rc = current_device_info(&dev, &ncu))) return rc;
+  a.N = (int)N;
+  a.K = (int)K;
+  const int64_t need = i8_workspace(a.M, a.N, a.K, !a.xs, a.sides, ncu);
+  if (ws_bytes < need)
+    return fail(GP_ERR_INVALID_ARG, "workspace_bytes must be at least %lld (got %lld)", (long long)need, (long long)ws_bytes);
+  if (a.xs) a.xq = a.x;
+  const hipError_t e = i8_launch(a, ncu, stream);
+  return e == hipSuccess ? GP_OK : fail_hip(e, "i8 launch");
+}
+
 }  // namespace
 }  // namespace gp
 
@@ -186,6 +259,35 @@ int gp_q4_gated_out(int64_t M, int64_t N, int64_t K, int group, const void* x, c
   const Q4Args a{M,   0,  0,       group, 2, x, {{wq_g, scales_g, zeros_g, b_g}, {wq_u, scales_u, zeros_u, b_u}},
                  nullptr, act, out, dtype, workspace, workspace_bytes};
   return q4_run(a, N, K, (hipStream_t)stream);
+}
+
+int64_t gp_i8_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_int8, int weights) {
+  clear_error();
+  int rc = i8_check_shape(M, N, K);
+  if (rc) return rc;
+  if (x_int8 != 0 && x_int8 != 1) return fail(GP_ERR_INVALID_ARG, "x_int8 must be 0 or 1 (got %d)", x_int8);
+  if (weights != 1 && weights != 2) return fail(GP_ERR_INVALID_ARG, "weights must be 1 or 2 (got %d)", weights);
+  if (M == 0) return 0;
+  int dev = 0, ncu = 0;
+  if ((rc = current_device_info(&dev, &ncu))) return rc;
+  return i8_workspace(M, (int)N, (int)K, !x_int8, weights, ncu);
+}
+
+int gp_i8_gemm_out(int64_t M, int64_t N, int64_t K, const void* x, const void* x_scales, const void* wq,
+                   const void* w_scales, const void* b, const void* r, int act, void* out, void* workspace,
+                   int64_t workspace_bytes, int dtype, void* stream) {
+  const I8Args a{M, 0, 0, 1, x, nullptr, (const float*)x_scales, {{wq, (const float*)w_scales, b}, {}}, r, act, out,
+                 dtype, workspace, nullptr};
+  return i8_run(a, N, K, workspace_bytes, (hipStream_t)stream);
+}
+
+int gp_i8_gated_out(int64_t M, int64_t N, int64_t K, const void* x, const void* x_scales, const void* wq_g,
+                    const void* w_scales_g, const void* b_g, const void* wq_u, const void* w_scales_u, const void* b_u,
+                    int act, void* out, void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+  const I8Args a{M, 0, 0, 2, x, nullptr, (const float*)x_scales,
+                 {{wq_g, (const float*)w_scales_g, b_g}, {wq_u, (const float*)w_scales_u, b_u}}, nullptr, act, out,
+                 dtype, workspace, nullptr};
+  return i8_run(a, N, K, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

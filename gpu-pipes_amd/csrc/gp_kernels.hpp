@@ -328,4 +328,30 @@ struct Q4Args {
 int64_t q4_workspace(int64_t M, int N, int K, int group, int sides, int num_cus);
 hipError_t q4_launch(const Q4Args& a, int num_cus, hipStream_t stream);
 
+// Products in 8-bit integers (gp_i8_gemm_out: one side; gp_i8_gated_out: two,
+// the gate's first).  K a multiple of 16 up to kI8MaxK, packed weights below
+// 2^31 bytes, every pointer 16-byte aligned.
+constexpr int64_t kI8MaxK = 131056;  // 128 * 128 * K < 2^31
+struct I8Side {
+  const void* wq;  // [ceil(N / 16), ceil(K / 64), 1024] bytes
+  const float* s;  // [N]
+  const void* b;   // [N] or null
+};
+struct I8Args {
+  int64_t M;
+  int N, K, sides;
+  const void* x;    // [M, K] 16-bit, where xs is null
+  const void* xq;   // [M, K] bytes, where it is not
+  const float* xs;  // [M]
+  I8Side side[2];
+  const void* r;  // [M, N] or null
+  int act;
+  void* out;  // [M, N]
+  int dtype;
+  void* ws;  // i8_workspace's bytes
+  void* part;  // of them: the sums of parts of k (the launch sets it)
+};
+int64_t i8_workspace(int64_t M, int N, int K, bool x16, int sides, int num_cus);
+hipError_t i8_launch(const I8Args& a, int num_cus, hipStream_t stream);
+
 }  // namespace gp

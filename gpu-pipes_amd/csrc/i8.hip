@@ -1,0 +1,725 @@
+// Products in 8-bit integers with a scale for each row of x and each column of
+// the weight: out = act(x W + b) [or x W + b + r], and the gated pair
+// act(x Wg + bg) * (x Wu + bu).  No counterpart in the reference, whose GEMM
+// stages take 16-bit operands (common/bulksync_gemm.cuh:13-110).
+//
+//   q[m][k] = rint(127 x[m][k] / a[m]), a[m] = max |x[m][.]|, xs[m] = a[m] / 127
+//   (x W)[m][n] = xs[m] ws[n] sum_k q[m][k] wq[k][n]
+//
+// The sums are exact: whole numbers in 32 bits, K at most 131,056.  So neither
+// the order of k nor the number of parts it is cut into changes a result, and
+// a row's bits are the same from every kernel here.
+//
+// Weights.  Blocks of 16 columns by 64 k, 1 KiB: byte 256 g + 16 j + i of block
+// [n / 16][k / 64] is wq[64 (k / 64) + 16 g + i][16 (n / 16) + j], the operand
+// of a 16 x 16 x 64 MFMA as its lanes hold it (lane 16 g + j).  Blocks of a
+// column tile follow each other along k, so a wave streams whole lines and an
+// operand's read from LDS is 1 KiB in a row.  Behind K and N the blocks hold
+// zeros, and a zero times whatever integer lies behind a row of x is zero: rows
+// of x need no padding.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "../../include/gpipes.h"
+#include "gp_kernels.hpp"
+#include "row_ops.hpp"
+
+namespace gp {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef int i4u __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kChunk = 128;  // k that a wave or a workgroup takes at a time: a line of a row of x
+constexpr unsigned kNowhere = 0xFFFFFFE0u;  // a buffer offset past every end: reads bring zeros
+
+__device__ __forceinline__ i32x4 mma8(u32x4 a, u32x4 b, i32x4 c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
+
+// Workgroup b of n, renumbered so that neighbours in the result run on one XCD (b % 8).
+__device__ __forceinline__ int xcd_order(int b, int n) {
+  const int x = b & 7, i = b >> 3, q = n >> 3, rem = n & 7;
+  return x * q + (x < rem ? x : rem) + i;
+}
+
+// ---------------------------------------------------------------------------
+// A row's whole numbers.  With x and a scaled by one power of two, 127 x is
+// exact in fp32 (18 bits) and so is the remainder 127 x - q a; the quotient,
+// corrected once by its remainder, is the correctly rounded one.  A quotient
+// of 11-bit numbers that is not itself halfway between two whole numbers is
+// further from every half than 32 times what it can be off by, so its rounding
+// (ties to even) is that of the exact quotient.
+// ---------------------------------------------------------------------------
+struct RowScale {
+  float up;     // the power of two
+  float top;    // a * up
+  float inv;    // 1 / top, or 0 for a row of zeros and one that is not finite
+  float scale;  // xs
+};
+
+// bits: the largest |x| of the row as the element type's bits (an infinity or NaN is larger than any number).
+template <class T>
+__device__ __forceinline__ RowScale row_scale(unsigned bits) {
+  const float a = T::val(__builtin_bit_cast(half_t, (unsigned short)bits));
+  int e = 254 - (int)(__builtin_bit_cast(unsigned, a) >> 23);
+  e = e < 1 ? 1 : e > 247 ? 247 : e;  // 127 * up stays finite
+  RowScale s;
+  s.up = __builtin_bit_cast(float, (unsigned)e << 23);
+  s.top = a * s.up;
+  const bool finite = a < __builtin_inff();
+  s.inv = finite && a > 0.f ? 1.f / s.top : 0.f;
+  s.scale = finite ? a / 127.f : __builtin_nanf("");
+  return s;
+}
+
+// Four values as bytes.  Adding 1.5 * 2^23 rounds to a whole number, which then stands in the low bits.
+__device__ __forceinline__ unsigned round4(const float* x, const RowScale& s) {
+  unsigned u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = x[i] * (127.f * s.up);
+    float q = t * s.inv;
+    q = __builtin_fmaf(__builtin_fmaf(-q, s.top, t), s.inv, q);
+    u[i] = __builtin_bit_cast(unsigned, q + 12582912.f);
+  }
+  const unsigned lo = __builtin_amdgcn_perm(u[1], u[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(u[3], u[2], 0x04000C0Cu);
+  return s.inv == 0.f ? 0u : lo | hi;  // an infinity times 0 has no whole number
+}
+template <class T>
+__device__ __forceinline__ u32x2 round8(u32x4 v, const RowScale& s) {
+  float f[8];
+  widen8<T>(v, f);
+  return u32x2{round4(f, s), round4(f + 4, s)};
+}
+
+// Larger of the 15-bit magnitudes in both halves.
+__device__ __forceinline__ unsigned top2(unsigned a, unsigned v) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  const u16x2 m = __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, v & 0x7FFF7FFFu));
+  return __builtin_bit_cast(unsigned, m);
+}
+__device__ __forceinline__ unsigned umax(unsigned a, unsigned b) { return a > b ? a : b; }
+// The largest half over the wave, in every lane.
+__device__ __forceinline__ unsigned wave_top(unsigned a) {
+  unsigned m = umax(a & 0xFFFF, a >> 16);
+#define GP_DPP(v, ctrl) (unsigned)__builtin_amdgcn_mov_dpp((int)(v), ctrl, 0xF, 0xF, false)
+  m = umax(m, GP_DPP(m, 0x128));  // row_ror:8
+  m = umax(m, GP_DPP(m, 0x124));
+  m = umax(m, GP_DPP(m, 0x4E));
+  m = umax(m, GP_DPP(m, 0xB1));
+#undef GP_DPP
+  auto p = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  m = umax(p[0], p[1]);
+  p = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  return umax(p[0], p[1]);
+}
+
+// Rows of x to bytes: WPR waves a row, P pieces of eight values a lane held in
+// registers, so that memory is read once; rows longer than that are read again
+// (from L2).  One wave a row up to 2,048 values, four rows a workgroup.
+template <class T, int P, int WPR>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void i8_rows_to_bytes_kernel(const half_t* x, int64_t M, int K,
+                                                                                    char* q, float* xs) {
+  constexpr int STEP = 64 * WPR * 8;
+  __shared__ unsigned part[WPR];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t m = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
+  if (m >= M) return;  // whole waves of one-wave rows only
+  const auto xr = make_rsrc(x + m * K, K * 2);
+  const int at = (WPR == 1 ? lane : (int)threadIdx.x) * 8;
+  u32x4 v[P];
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < P; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, (at + i * STEP) * 2, 0, 0);
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = top2(top, v[i][e]);
+  for (int k = at + P * STEP; k < K; k += STEP) {
+    const u32x4 w = __builtin_amdgcn_raw_buffer_load_b128(xr, k * 2, 0, 0);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = top2(top, w[e]);
+  }
+  top = wave_top(top);
+  if constexpr (WPR > 1) {
+    if (lane == 0) part[wave] = top;
+    __syncthreads();
+    top = wave_top(part[lane & (WPR - 1)]);
+  }
+  const RowScale s = row_scale<T>(top);
+  char* const row = q + m * K;
+#pragma unroll
+  for (int i = 0; i < P; ++i)
+    if (at + i * STEP < K) *(u32x2*)(row + at + i * STEP) = round8<T>(v[i], s);
+  for (int k = at + P * STEP; k < K; k += STEP)
+    *(u32x2*)(row + k) = round8<T>(__builtin_amdgcn_raw_buffer_load_b128(xr, k * 2, 0, 0), s);
+  if (at == 0) xs[m] = s.scale;
+}
+
+template <class T>
+hipError_t rows_to_bytes(const void* x, int64_t M, int K, char* q, float* xs, hipStream_t s) {
+  const half_t* h = (const half_t*)x;
+#define GP_ROWS(p, w) \
+  hipLaunchKernelGGL((i8_rows_to_bytes_kernel<T, p, w>), dim3((unsigned)(w == 1 ? (M + 3) / 4 : M)), dim3(w == 1 ? 256 : 64 * w), 0, s, h, M, K, q, xs)
+  if (K <= 512) GP_ROWS(1, 1);
+  else if (K <= 2048) GP_ROWS(4, 1);
+  else if (K <= 8192) GP_ROWS(4, 4);
+  else GP_ROWS(4, 16);
+#undef GP_ROWS
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Epilogue
+// ---------------------------------------------------------------------------
+// The stages' activations and SiLU; a NaN stays one under every one of them.
+__device__ __forceinline__ float act8(float v, int act) { return act == GP_ACT_RELU ? (v < 0.f ? 0.f : v) : apply_act_ext(v, act); }
+
+// n of eight neighbouring outputs of a row from column n: the sums a (and u of
+// the second weight), already times both scales.
+template <class T, int S>
+__device__ __forceinline__ void finish8(const I8Args& p, int64_t m, int n, int cnt, float (&v)[8], float (&u)[8]) {
+  float t[8];
+  if (p.side[0].b) {
+    load8<T>((const half_t*)p.side[0].b + n, cnt, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += t[e];
+  }
+  if (p.act == GP_ACT_RELU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
+  } else {
+    apply_act8(v, p.act);
+  }
+  if constexpr (S == 2) {
+    if (p.side[1].b) {
+      load8<T>((const half_t*)p.side[1].b + n, cnt, t);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] += t[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= u[e];
+  }
+  if (p.r) {
+    load8<T>((const half_t*)p.r + m * p.N + n, cnt, t);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += t[e];
+  }
+  store8<T>((half_t*)p.out + m * p.N + n, cnt, v);
+}
+
+// One output.
+template <class T, int S>
+__device__ __forceinline__ void finish1(const I8Args& p, int64_t m, int n, float v, float u) {
+  if (p.side[0].b) v += T::val(((const half_t*)p.side[0].b)[n]);
+  v = act8(v, p.act);
+  if constexpr (S == 2) v *= p.side[1].b ? u + T::val(((const half_t*)p.side[1].b)[n]) : u;
+  if (p.r) v += T::val(((const half_t*)p.r)[m * p.N + n]);
+  ((half_t*)p.out)[m * p.N + n] = T::cvt1(v);
+}
+
+// ---------------------------------------------------------------------------
+// Few rows.  A wave multiplies its share of k with NT tiles of 16 columns (of
+// two weights NT / 2 of each); words and x go through a ring of R chunks in
+// LDS that is the wave's own, so that many loads are in flight and no barrier
+// lies between them, and the waves' sums are joined through LDS.
+// XL: at most four rows of 16-bit x, which the workgroup makes bytes of itself.
+// ---------------------------------------------------------------------------
+constexpr int rows_ring(int nt, int mt, bool xl) { return xl ? (nt == 1 ? 4 : 2) : nt + mt <= 3 ? 3 : 2; }
+constexpr int slot_bytes(int nt, int mt, bool xl) { return (nt + (xl ? 0 : mt)) * 2048; }
+constexpr int kRowsLds = 156 * 1024;  // of dynamic LDS at most
+// Waves of a workgroup at most, a power of two: sixteen, or as many as have room for their rings.
+constexpr int rows_waves(int nt, int mt, bool xl) {
+  const int fit = (kRowsLds - (xl ? 20 * 1024 : 0)) / (rows_ring(nt, mt, xl) * slot_bytes(nt, mt, xl));
+  return fit >= 16 ? 16 : fit >= 8 ? 8 : 4;
+}
+
+struct RowsPlan {
+  int nt, mt, kw, cg;  // column tiles a wave, row tiles, waves along k, waves along the columns
+  bool xl;
+  int xstride, bytes;  // XL: of a row's bytes; LDS
+};
+
+template <class T, int S, int NT, int MT, bool XL>
+__global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8Args p, int kwshift, int mshift, int xstride) {
+  constexpr int R = rows_ring(NT, MT, XL), SLOT = slot_bytes(NT, MT, XL), NI = SLOT / 1024, CW = NT / S;
+  __shared__ unsigned tops[16];
+  GP_LDS char* lds = dyn_lds();
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, lg = lane >> 4;
+  const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int KW = 1 << kwshift, kw = wave & (KW - 1), cg = wave >> kwshift, CG = waves >> kwshift;
+  const int N = p.N, K = p.K, N16 = (N + 15) / 16, K64 = (K + 63) / 64, chunks = (K + kChunk - 1) / kChunk;
+  const int t0 = xcd_order(blockIdx.x, gridDim.x) * (CW * CG);  // the workgroup's first tile of columns
+  const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
+  const int rows = p.M - m0 < 16 * MT ? (int)(p.M - m0) : 16 * MT;
+
+  // 16-bit x first: what follows is not waited for with it
+  constexpr int XP = 4;
+  u32x4 xv[XL ? XP : 1];
+  const int tpr = blockDim.x >> mshift, xrow = XL ? tid / tpr : 0, xat = XL ? (tid - xrow * tpr) * 8 : 0;
+  if constexpr (XL) {
+    const auto xr = make_rsrc(p.x, (int)p.M * K * 2);
+#pragma unroll
+    for (int i = 0; i < XP; ++i) {
+      const int k = xat + i * tpr * 8;
+      xv[i] = __builtin_amdgcn_raw_buffer_load_b128(xr, k < K ? (xrow * K + k) * 2 : (int)kNowhere, 0, 0);
+    }
+  }
+
+  GP_LDS char* const ring = lds + wave * (R * SLOT);
+  const int wbytes = N16 * K64 * 1024;
+  const auto wr0 = make_rsrc(p.side[0].wq, wbytes);
+  const auto wr1 = make_rsrc(p.side[S - 1].wq, wbytes);
+  const auto xr8 = make_rsrc((const char*)p.xq + m0 * K, rows * K);
+  unsigned wo[CW];
+#pragma unroll
+  for (int t = 0; t < CW; ++t) {
+    const int n16 = t0 + cg * CW + t;
+    wo[t] = n16 < N16 ? (unsigned)(n16 * K64) * 1024u + (unsigned)lane * 16u : 0xC0000000u;
+  }
+  // 16-byte piece c of row r lies at c ^ (r / 2) % 8: sixteen rows' reads of one piece fall into different banks
+  const int dr = lane >> 3;
+  unsigned xo[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) xo[h] = (unsigned)((8 * h + dr) * K + (((lane & 7) ^ (((8 * h + dr) >> 1) & 7)) << 4));
+
+  auto issue = [&](int c, int slot) {
+    GP_LDS char* at = ring + slot * SLOT;
+    const bool in = c < chunks;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int t = 0; t < CW; ++t)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          dma16_buf(s ? wr1 : wr0, (int)(in && 2 * c + b < K64 ? wo[t] + (unsigned)(2 * c + b) * 1024u : kNowhere),
+                    at + (s * CW + t) * 2048 + b * 1024);
+    if constexpr (!XL) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          dma16_buf(xr8, (int)(in ? xo[h] + (unsigned)(mt * 16 * K + c * kChunk) : kNowhere),
+                    at + NT * 2048 + mt * 2048 + h * 1024);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < R; ++i) issue(kw + i * KW, i);
+
+  GP_LDS char* const xl = lds + waves * (R * SLOT);
+  float* const xsl = (float*)tops;
+  float lscale = 0.f;
+  if constexpr (XL) {
+    unsigned top = 0;
+#pragma unroll
+    for (int i = 0; i < XP; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = top2(top, xv[i][e]);
+    top = wave_top(top);
+    if (lane == 0) tops[wave] = top;
+    lds_barrier();
+    const int wpr = waves >> mshift;
+    top = wave_top(tops[xrow * wpr + (lane & (wpr - 1))]);
+    const RowScale s = row_scale<T>(top);
+#pragma unroll
+    for (int i = 0; i < XP; ++i) {
+      const int k = xat + i * tpr * 8;
+      if (k < K) *(GP_LDS u32x2*)(xl + xrow * xstride + k) = round8<T>(xv[i], s);
+    }
+    lscale = s.scale;
+    lds_barrier();
+    if (tid - xrow * tpr == 0) xsl[xrow] = lscale;  // read behind the next barrier
+  }
+
+  i32x4 acc[NT][MT] = {};
+  const int nc = kw < chunks ? (chunks - 1 - kw) / KW + 1 : 0;
+  const int sw = (j >> 1) & 7;
+  int at = 0;
+  for (int t = 0; t < nc; ++t) {
+    const int c = kw + t * KW;
+    wait_vmcnt<(R - 1) * NI>();
+    compiler_fence();
+    GP_LDS char* slot = ring + at * SLOT;
+    u32x4 b[2][NT], a[2][MT];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) b[h][n] = *(GP_LDS const u32x4*)(slot + n * 2048 + h * 1024 + lane * 16);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        if constexpr (XL)
+          a[h][mt] = *(GP_LDS const u32x4*)(xl + (j & ((1 << mshift) - 1)) * xstride + c * kChunk + h * 64 + lg * 16);
+        else
+          a[h][mt] = *(GP_LDS const u32x4*)(slot + NT * 2048 + mt * 2048 + j * 128 + (((4 * h + lg) ^ sw) << 4));
+      }
+    }
+    // what was read is in registers before the slot takes the chunk R further on
+    compiler_fence();
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    issue(c + R * KW, at);
+    at = at + 1 == R ? 0 : at + 1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[n][mt] = mma8(a[h][mt], b[h][n], acc[n][mt]);
+  }
+
+  // The waves' sums: wave (cg, kw) leaves rows of 16 NT in its own part of the ring.
+  wait_vmcnt<0>();
+  compiler_fence();
+  constexpr int LD = 16 * NT;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) *(GP_LDS int*)(ring + ((mt * 16 + 4 * lg + e) * LD + n * 16 + j) * 4) = acc[n][mt][e];
+  __syncthreads();
+  const int cols = 16 * CW * CG;
+  for (int i = tid; i < rows * cols; i += blockDim.x) {
+    const int m = i / cols, c = i - m * cols, g = c / (16 * CW), n = t0 * 16 + c;
+    if (n >= N) continue;
+    GP_LDS const char* from = lds + (g << kwshift) * (R * SLOT) + (m * LD + (c - g * 16 * CW)) * 4;
+    int v = 0, u = 0;
+    for (int w = 0; w < KW; ++w) {
+      v += *(GP_LDS const int*)(from + w * (R * SLOT));
+      if (S == 2) u += *(GP_LDS const int*)(from + w * (R * SLOT) + 16 * CW * 4);
+    }
+    const float xsc = XL ? xsl[m] : p.xs[m0 + m];
+    finish1<T, S>(p, m0 + m, n, (float)v * p.side[0].s[n] * xsc, S == 2 ? (float)u * p.side[S - 1].s[n] * xsc : 0.f);
+  }
+}
+
+template <class T, int S, int NT, int MT, bool XL>
+hipError_t rows_launch_one(const I8Args& a, const RowsPlan& l, int mshift, hipStream_t s) {
+  const auto kern = &i8_rows_kernel<T, S, NT, MT, XL>;
+  if (l.bytes > 60 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kRowsLds);
+    if (e != hipSuccess) return e;
+  }
+  const int tiles = (a.N + 15) / 16, per = NT / S * l.cg;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((tiles + per - 1) / per), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
+                     dim3(l.kw * l.cg * kWave), l.bytes, s, a, __builtin_ctz(l.kw), mshift, l.xstride);
+  return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: tiles of BM rows by BN columns (of two weights BN / 2 of each),
+// chunks of 128 k through a ring of R in LDS.  The weight is the MFMA's first
+// operand, so that a lane's four sums are of one row; which columns a tile's 16
+// operand rows are is chosen so that a lane's sums of its NT tiles are 4 NT
+// neighbouring columns: results leave as whole 16-byte pieces, without a way
+// through LDS.  Where tiles are few, several workgroups share one, each with a
+// part of k, leave their sums in a workspace, and a second kernel adds them.
+// ---------------------------------------------------------------------------
+template <class T, int S, int BM, int BN, int WM, int WN, int R, int EU>
+__global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, int mtiles, int ntiles) {
+  constexpr int NW = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, NS = NT / S;
+  constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW, NI = XI + WI;  // copies of 1 KiB a wave and chunk
+  constexpr int XB = BM * kChunk, SLOT = XB + BN * kChunk;
+  constexpr int SB = BN / 16 / S;  // blocks of a weight in a chunk's half
+  static_assert(NW % 2 == 0 && XI * 8 * NW == BM && WI * 8 * NW == BN && WI % 2 == 0, "copies");
+  __shared__ __attribute__((aligned(1024))) char ringmem[R * SLOT];
+  GP_LDS char* const lds = (GP_LDS char*)ringmem;
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, lg = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
+  const int N = p.N, K = p.K, K64 = (K + 63) / 64, N16 = (N + 15) / 16, chunks = (K + kChunk - 1) / kChunk;
+  // Neighbours of one XCD take eight row tiles of a column tile, then of the next.
+  const int id = xcd_order(blockIdx.x, gridDim.x);
+  const int gm0 = id / (8 * ntiles) * 8, rest = id % (8 * ntiles);
+  const int gm = mtiles - gm0 < 8 ? mtiles - gm0 : 8;
+  const int64_t m0 = (int64_t)(gm0 + rest % gm) * BM;
+  const int nb0 = rest / gm * SB;  // first block of columns
+  const int rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
+  const auto xr = make_rsrc((const char*)p.xq + m0 * K, rows * K);
+  const auto wr0 = make_rsrc(p.side[0].wq, N16 * K64 * 1024);
+  const auto wr1 = make_rsrc(p.side[S - 1].wq, N16 * K64 * 1024);
+
+  // Copies.  x: eight rows each, piece c of row r at c ^ (r / 2) % 8.  Weight:
+  // one block each, piece q of local block l at q ^ 4 (l % 4), which keeps the
+  // sixteen columns that an operand takes from several blocks in different banks.
+  unsigned xo[XI], wo[WI];
+#pragma unroll
+  for (int q = 0; q < XI; ++q) {
+    const int row = 8 * (q * NW + wave) + (lane >> 3);
+    xo[q] = (unsigned)(row * K + (((lane & 7) ^ ((row >> 1) & 7)) << 4));
+  }
+  const int kb = wave & 1;  // of the chunk's two blocks along k
+#pragma unroll
+  for (int q = 0; q < WI; ++q) {
+    const int l = (q * NW + wave) >> 1, n16 = nb0 + l % SB;
+    wo[q] = n16 < N16 ? (unsigned)(n16 * K64 + kb) * 1024u + (unsigned)((lane ^ (4 * (l & 3))) << 4) : 0xC0000000u;
+  }
+  auto issue = [&](int c, int c1, int slot) {
+    GP_LDS char* at = lds + slot * SLOT;
+    const bool in = c < c1;
+#pragma unroll
+    for (int q = 0; q < XI; ++q)
+      dma16_buf(xr, (int)(in ? xo[q] + (unsigned)c * kChunk : kNowhere), at + (q * NW + wave) * 1024);
+    const bool win = in && 2 * c + kb < K64;
+#pragma unroll
+    for (int q = 0; q < WI; ++q)
+      dma16_buf(S == 2 && q >= WI / 2 ? wr1 : wr0, (int)(win ? wo[q] + (unsigned)c * 2048u : kNowhere),
+                at + XB + (q * NW + wave) * 1024);
+  };
+  // Operands.
+  int xa[2], wa[S][NS];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) xa[h] = (wm * MT * 16 + j) * 128 + (((4 * h + lg) ^ ((j >> 1) & 7)) << 4);
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+#pragma unroll
+    for (int t = 0; t < NS; ++t) {
+      const int n = 4 * NS * (j >> 2) + 4 * t + (j & 3), l = s * SB + wn * NS + (n >> 4);
+      wa[s][t] = XB + l * 2048 + (((lg * 16 + (n & 15)) ^ (4 * (l & 3))) << 4);
+    }
+
+  const int per = (chunks + gridDim.y - 1) / gridDim.y, c0 = blockIdx.y * per, c1 = c0 + per < chunks ? c0 + per : chunks;
+  i32x4 acc[S][NS][MT] = {};
+#pragma unroll
+  for (int i = 0; i < R - 1; ++i) issue(c0 + i, c1, i);
+  int at = 0;
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    wait_vmcnt<(R - 2) * NI>();
+    lds_barrier();
+    const int next = at == 0 ? R - 1 : at - 1;
+    issue(c + R - 1, c1, next);
+    GP_LDS const char* slot = lds + at * SLOT;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u32x4 w[S][NS], x[MT];
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int t = 0; t < NS; ++t) w[s][t] = *(GP_LDS const u32x4*)(slot + wa[s][t] + h * 1024);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) x[m] = *(GP_LDS const u32x4*)(slot + xa[h] + m * 2048);
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+          for (int t = 0; t < NS; ++t) acc[s][t][m] = mma8(w[s][t], x[m], acc[s][t][m]);
+    }
+    at = at + 1 == R ? 0 : at + 1;
+  }
+
+  // A lane's columns: 4 NS from n0 of each weight, of row j of each row tile.
+  const int n0 = nb0 * 16 + wn * (16 * NS) + 4 * NS * lg;
+  if (gridDim.y > 1) {
+    int* const part = (int*)p.part + (int64_t)blockIdx.y * S * p.M * N;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = wm * MT * 16 + m * 16 + j;
+      if (row >= rows) continue;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        int* to = part + ((int64_t)s * p.M + m0 + row) * N + n0;
+#pragma unroll
+        for (int t = 0; t < NS; ++t) {
+          if (n0 + 4 * t + 4 <= N)
+            *(i4u*)(to + 4 * t) = acc[s][t][m];
+          else
+#pragma unroll
+            for (int e = 0; e < 3; ++e)
+              if (n0 + 4 * t + e < N) to[4 * t + e] = acc[s][t][m][e];
+        }
+      }
+    }
+    return;
+  }
+  constexpr int W8 = NS >= 2 ? 2 : 1;  // sums of up to eight columns at a time
+#pragma unroll
+  for (int g = 0; g < NS / W8; ++g) {
+    const int n = n0 + 4 * W8 * g, cnt = N - n < 4 * W8 ? N - n : 4 * W8;
+    if (cnt <= 0) continue;
+    float sc[S][8] = {};
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int e = 0; e < 4 * W8; ++e)
+        if (e < cnt) sc[s][e] = p.side[s].s[n + e];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = wm * MT * 16 + m * 16 + j;
+      if (row >= rows) continue;
+      const float xsc = p.xs[m0 + row];
+      float v[8] = {}, u[8] = {};
+#pragma unroll
+      for (int t = 0; t < W8; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[4 * t + e] = (float)acc[0][W8 * g + t][m][e] * sc[0][4 * t + e] * xsc;
+          if (S == 2) u[4 * t + e] = (float)acc[S - 1][W8 * g + t][m][e] * sc[S - 1][4 * t + e] * xsc;
+        }
+      finish8<T, S>(p, m0 + row, n, cnt, v, u);
+    }
+  }
+}
+
+// The parts of k added, and the epilogue: eight columns of a row a thread.
+template <class T, int S>
+__global__ __launch_bounds__(256) void i8_join_kernel(I8Args p, int parts) {
+  const int pieces = (p.N + 7) / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.M * pieces) return;
+  const int64_t m = i / pieces;
+  const int n = (int)(i - m * pieces) * 8, cnt = p.N - n < 8 ? p.N - n : 8;
+  int a[S][8] = {};
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k)
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const int* at = (const int*)p.part + (((int64_t)k * S + s) * p.M + m) * p.N + n;
+      if (cnt >= 8) {
+        const i4u lo = *(const i4u*)at, hi = *(const i4u*)(at + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[s][e] += lo[e], a[s][4 + e] += hi[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (e < cnt) a[s][e] += at[e];
+      }
+    }
+  const float xsc = p.xs[m];
+  float v[8], u[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    v[e] = e < cnt ? (float)a[0][e] * p.side[0].s[n + e] * xsc : 0.f;
+    u[e] = S == 2 && e < cnt ? (float)a[S - 1][e] * p.side[S - 1].s[n + e] * xsc : 0.f;
+  }
+  finish8<T, S>(p, m, n, cnt, v, u);
+}
+
+// ---------------------------------------------------------------------------
+// Which kernel
+// ---------------------------------------------------------------------------
+struct TilePlan {
+  int size, parts;  // 64, 128 or 256; parts of k
+};
+
+TilePlan tile_plan(int64_t M, int N, int K, int sides, int num_cus) {
+  const int chunks = (K + kChunk - 1) / kChunk;
+  TilePlan best{256, 1};
+  float least = 0.f;
+  for (int size : {256, 128, 64}) {
+    const int64_t cols = size / sides, tiles = (M + size - 1) / size * ((N + cols - 1) / cols);
+    const int fit = size == 256 ? 1 : 2;  // workgroups a CU
+    const float step = size == 256 ? 1.6f : size == 128 ? 0.5f : 0.25f;
+    for (int parts = 1; parts <= 8 && parts <= chunks; ++parts) {
+      const int64_t turns = (tiles * parts + (int64_t)fit * num_cus - 1) / ((int64_t)fit * num_cus);
+      float t = (float)((chunks + parts - 1) / parts + 3) * step * (float)turns;
+      if (parts > 1) t += 3.f + (float)parts * (float)M * (float)N * (float)sides * 8.f / 4e6f;
+      if (least == 0.f || t < least) best = TilePlan{size, parts}, least = t;
+    }
+  }
+  return best;
+}
+
+bool on_tiles(int64_t M) { return M > 64; }
+
+bool own_bytes(int64_t M, int K) { return M <= 4 && K * (M <= 1 ? 1 : M <= 2 ? 2 : 4) <= 16384; }
+
+template <class T, int S>
+hipError_t rows_launch(const I8Args& a, bool x16, int num_cus, hipStream_t s) {
+  RowsPlan l{};
+  l.xl = x16;
+  const int tiles = (a.N + 15) / 16 * S, chunks = (a.K + kChunk - 1) / kChunk;
+  l.mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+  int per = tiles >= 4 * num_cus ? 4 : tiles >= 2 * num_cus ? 2 : 1;  // tiles a workgroup
+  if (per < S) per = S;
+  l.nt = per > 2 && l.mt == 1 ? 2 : per;
+  const int ring = rows_ring(l.nt, l.mt, l.xl) * slot_bytes(l.nt, l.mt, l.xl);
+  l.cg = per / l.nt;
+  const int mshift = a.M <= 1 ? 0 : a.M <= 2 ? 1 : 2;
+  l.xstride = (chunks * kChunk + 255) / 256 * 256 + 64;
+  const int xbytes = l.xl ? l.xstride << mshift : 0;
+  const int waves = rows_waves(l.nt, l.mt, l.xl);
+  // no more waves than chunks, but for 16-bit x its threads
+  int need = 1;
+  if (l.xl)
+    while (need * kWave * 32 < (a.K << mshift) || need < (1 << mshift)) need *= 2;
+  l.kw = waves / l.cg;
+  while (l.kw > 1 && l.kw / 2 >= chunks && l.kw / 2 * l.cg >= need) l.kw /= 2;
+  l.bytes = l.kw * l.cg * ring + xbytes;
+#define GP_CASE(n, m)                                                              \
+  if constexpr (n >= S)                                                            \
+    if (l.nt == n && l.mt == m) {                                                  \
+      if constexpr (m == 1)                                                        \
+        if (l.xl) return rows_launch_one<T, S, n, m, true>(a, l, mshift, s);       \
+      return rows_launch_one<T, S, n, m, false>(a, l, mshift, s);                  \
+    }
+  GP_CASE(1, 1) GP_CASE(2, 1) GP_CASE(1, 2) GP_CASE(2, 2) GP_CASE(4, 2) GP_CASE(1, 4) GP_CASE(2, 4) GP_CASE(4, 4)
+#undef GP_CASE
+  return hipErrorInvalidValue;
+}
+
+template <class T, int S>
+hipError_t tile_launch(const I8Args& a, const TilePlan& plan, hipStream_t s) {
+  const int64_t cols = plan.size / S, mtiles = (a.M + plan.size - 1) / plan.size, ntiles = (a.N + cols - 1) / cols;
+  if (mtiles * ntiles > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)(mtiles * ntiles), (unsigned)plan.parts);
+  if (plan.size == 256)
+    hipLaunchKernelGGL((i8_tile_kernel<T, S, 256, 256, 2, 4, 2, 2>), grid, dim3(512), 0, s, a, (int)mtiles, (int)ntiles);
+  else if (plan.size == 128)
+    hipLaunchKernelGGL((i8_tile_kernel<T, S, 128, 128, 2, 2, 2, 2>), grid, dim3(256), 0, s, a, (int)mtiles, (int)ntiles);
+  else
+    hipLaunchKernelGGL((i8_tile_kernel<T, S, 64, 64, 2, 2, 4, 2>), grid, dim3(256), 0, s, a, (int)mtiles, (int)ntiles);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || plan.parts == 1) return e;
+  const int64_t pieces = a.M * ((a.N + 7) / 8);
+  hipLaunchKernelGGL((i8_join_kernel<T, S>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, a, plan.parts);
+  return hipGetLastError();
+}
+
+// The workspace: bytes and scales of 16-bit rows, then the parts' sums.
+struct Layout {
+  int64_t xs, part, bytes;
+};
+Layout layout(int64_t M, int N, int K, bool x16, int sides, int num_cus) {
+  Layout l{};
+  if (x16 && !own_bytes(M, K)) {
+    l.xs = (M * K + 255) / 256 * 256;
+    l.part = (l.xs + M * 4 + 255) / 256 * 256;
+  }
+  l.bytes = l.part;
+  if (on_tiles(M)) {
+    const TilePlan p = tile_plan(M, N, K, sides, num_cus);
+    if (p.parts > 1) l.bytes += (int64_t)p.parts * sides * M * N * 4;
+  }
+  return l;
+}
+
+template <class T, int S>
+hipError_t launch(I8Args a, int num_cus, hipStream_t s) {
+  const bool x16 = !a.xs, xl = x16 && own_bytes(a.M, a.K);
+  const Layout l = layout(a.M, a.N, a.K, x16, S, num_cus);
+  if (x16 && !xl) {
+    a.xq = (char*)a.ws;
+    a.xs = (float*)((char*)a.ws + l.xs);
+    const hipError_t e = rows_to_bytes<T>(a.x, a.M, a.K, (char*)a.ws, (float*)a.xs, s);
+    if (e != hipSuccess) return e;
+  }
+  if (!on_tiles(a.M)) return rows_launch<T, S>(a, xl, num_cus, s);
+  a.part = (char*)a.ws + l.part;
+  return tile_launch<T, S>(a, tile_plan(a.M, a.N, a.K, S, num_cus), s);
+}
+
+}  // namespace
+
+int64_t i8_workspace(int64_t M, int N, int K, bool x16, int sides, int num_cus) {
+  return layout(M, N, K, x16, sides, num_cus).bytes;
+}
+
+hipError_t i8_launch(const I8Args& a, int num_cus, hipStream_t s) {
+  if (a.dtype == GP_DTYPE_BF16) return a.sides == 2 ? launch<BF16, 2>(a, num_cus, s) : launch<BF16, 1>(a, num_cus, s);
+  return a.sides == 2 ? launch<F16, 2>(a, num_cus, s) : launch<F16, 1>(a, num_cus, s);
+}
+
+}  // namespace gp

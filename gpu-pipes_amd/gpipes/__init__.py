@@ -20,7 +20,7 @@ import os
 
 import torch
 
-from . import q4
+from . import i8, q4
 
 __all__ = [
     "lib", "mgn_fullmlp", "mgn_fullmlp_out", "mgn_linears", "mgn_linears_out",
@@ -31,7 +31,7 @@ __all__ = [
     "dlrm_topmlp_out", "nerf_full", "nerf_full_out", "nerf_full_out_noalloc", "bert_addln_ffn",
     "bert_addln_ffn_out", "nerf_a", "nerf_a_out", "pipe_handoff", "handoff_checksums", "phase_timers",
     "probe_mfma", "fill_normal", "residual_norm_out", "residual_norm", "NORMS", "q4_gemm_out",
-    "q4_gated_out", "q4",
+    "q4_gated_out", "q4", "i8_gemm_out", "i8_gated_out", "i8",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -45,7 +45,7 @@ IMPL_FUSED = 0
 IMPL_PIPELINED = 1
 IMPL_PIPELINED_SPLIT_LN = 2
 _IMPLS = {"fused": IMPL_FUSED, "pipelined": IMPL_PIPELINED, "pipelined_split_ln": IMPL_PIPELINED_SPLIT_LN}
-# "silu" (GP_ACT_SILU) is the residual norm's gate's and the 4-bit products' only
+# "silu" (GP_ACT_SILU) is the residual norm's gate's and the 4-bit and 8-bit products' only
 ACTS = {"none": 0, "relu": 1, "gelu_tanh": 2, "sigmoid": 3, "silu": 4}
 NORMS = {"none": 0, "layer": 1, "rms": 2}
 ROUTES = {"ident": 0, "broadcast": 1, "split": 2, "drain": 3, "handoff": 4, "reload": 5}
@@ -126,6 +126,12 @@ def _load():
     L.gp_q4_workspace_bytes.argtypes = [i64, i64, i64, i32, i32]
     L.gp_q4_workspace_bytes.restype = i64
     L.gp_q4_gated_out.restype = i32
+    L.gp_i8_workspace_bytes.argtypes = [i64, i64, i64, i32, i32]
+    L.gp_i8_workspace_bytes.restype = i64
+    L.gp_i8_gemm_out.argtypes = [i64, i64, i64] + [vp] * 6 + [i32, vp, vp, i64, i32, vp]
+    L.gp_i8_gemm_out.restype = i32
+    L.gp_i8_gated_out.argtypes = [i64, i64, i64] + [vp] * 8 + [i32, vp, vp, i64, i32, vp]
+    L.gp_i8_gated_out.restype = i32
     for name in ("gp_mlp_out", "gp_dlrm_botmlp_out", "gp_dlrm_topmlp_out", "gp_nerf_full_out", "gp_gemm_out",
                  "gp_gemm_dtype_out", "gp_bert_ffn_out", "gp_bert_ffn_dtype_out", "gp_linear_out", "gp_linear_layer_norm_out", "gp_layer_norm_out", "gp_add_out",
                  "gp_concat_out", "gp_pipe_ident", "gp_pipeline_check"):
@@ -1107,5 +1113,122 @@ def q4_gated_out(x, wq_g, scales_g, zeros_g, wq_u, scales_u, zeros_u, bg=None, b
             (M, N, K, group, x.data_ptr(), wq_g.data_ptr(), scales_g.data_ptr(),
              None if zeros_g is None else zeros_g.data_ptr(), None if bg is None else bg.data_ptr(), wq_u.data_ptr(),
              scales_u.data_ptr(), None if zeros_u is None else zeros_u.data_ptr(),
+             None if bu is None else bu.data_ptr(), ACTS.get(act, act), out.data_ptr(), at, n, _DTYPES[dt]))
+    return out
+
+
+def _i8_weight(wq, scales, blocks, N, dev):
+    """Whether an 8-bit weight's tensors fit: packed blocks and a scale for each of N columns."""
+    return (wq.dtype is torch.int8 and wq.get_device() == dev and wq.shape == blocks and wq.is_contiguous()
+            and scales.dtype is torch.float32 and scales.get_device() == dev and scales.shape == (N,)
+            and scales.is_contiguous())
+
+
+def _i8_workspace(M, N, K, int8, weights, x):
+    """(tensor, address, bytes) of an 8-bit product's workspace: the call's own, from torch's allocator, which hands it
+    on in the stream's order and keeps it for a graph that is being captured."""
+    with _on(x):
+        n = lib.gp_i8_workspace_bytes(M, N, K, int8, weights)
+    if n < 0:
+        _check(n)
+    if n == 0:
+        return None, None, 0
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    return ws, ws.data_ptr(), n
+
+
+def _i8_refuse(x, xs, out, named):
+    """Raises for what is wrong with an 8-bit product's x, xs, out or tensors: (name, tensor, kind)."""
+    if xs is None:
+        _check_rows(x)
+        dt = x.dtype
+    else:
+        _check_input("x", x, dtype=torch.int8)
+        if x.dim() != 2:
+            raise RuntimeError("x must be 2-D")
+        if out is None:
+            raise RuntimeError("out must be given with an int8 x")
+        _check_input("out", out, dtype=_dtype_of(out))
+        dt = out.dtype
+    M, K = x.shape
+    scales = named[1][1]
+    _check_input(named[1][0], scales, dtype=torch.float32)
+    if scales.dim() != 1 or scales.shape[0] < 1:
+        raise RuntimeError(f"{named[1][0]} must be [N]")
+    if K < 1 or K % 16:
+        raise RuntimeError(f"K must be a multiple of 16 (got {K})")
+    N = scales.shape[0]
+    shapes = {"blocks": i8.packed_shape(K, N), "scales": (N,), "bias": (N,), "rows": (M, N), "xs": (M,)}
+    types = {"blocks": torch.int8, "scales": torch.float32, "xs": torch.float32}
+    _misfit(x, [(name, t, shapes[kind], types.get(kind, dt)) for name, t, kind in named + [("xs", xs, "xs")]])
+
+
+def i8_gemm_out(x, wq, scales, xs=None, b=None, r=None, act="none", out=None):
+    """out[M,N] = act(x @ W + b), or x @ W + b + r, in 8-bit integers (gp_i8_gemm_out): wq int8, packed blocks of
+    q [K, N] (gpipes.i8.pack), scales float32 [N], W[k, n] = scales[n] * q[k, n].  x float16 or bfloat16 [M, K], each
+    row rounded here to whole numbers times max|x| / 127; or int8, with a scale for each row, xs float32 [M], and out
+    given.  K a multiple of 16, any N; M from one token to whole prompts.  b, r and out have x's type (b, r that of
+    out where x is int8).  act: a name of ACTS."""
+    try:
+        dev = x.get_device()
+        M, K = x.shape
+        N = scales.shape[0]
+        if xs is None:
+            dt = x.dtype
+            if out is None:
+                out = torch.empty((M, N), dtype=dt, device=x.device)
+        else:
+            dt = out.dtype
+        ok = (K % 16 == 0 and K > 0 and dt in _DTYPES and dev >= 0 and x.is_contiguous()
+              and (xs is None or (x.dtype is torch.int8 and xs.dtype is torch.float32 and xs.get_device() == dev
+                                  and xs.shape == (M,) and xs.is_contiguous()))
+              and _i8_weight(wq, scales, (-(-N // 16), -(-K // 64), 1024), N, dev)
+              and (b is None or (b.dtype is dt and b.get_device() == dev and b.shape == (N,) and b.is_contiguous()))
+              and (r is None or (r.dtype is dt and r.get_device() == dev and r.shape == (M, N) and r.is_contiguous()))
+              and out.dtype is dt and out.get_device() == dev and out.shape == (M, N) and out.is_contiguous())
+    except (AttributeError, ValueError, IndexError, TypeError):  # no tensors, or of another rank
+        ok = False
+    if not ok:
+        _i8_refuse(x, xs, out, [("wq", wq, "blocks"), ("scales", scales, "scales"), ("b", b, "bias"), ("r", r, "rows"),
+                                ("out", out, "rows")])
+    ws, at, n = (None, None, 0) if M == 1 and K <= 16384 else _i8_workspace(M, N, K, xs is not None, 1, x)
+    _run_on(dev, lib.gp_i8_gemm_out,
+            (M, N, K, x.data_ptr(), None if xs is None else xs.data_ptr(), wq.data_ptr(), scales.data_ptr(),
+             None if b is None else b.data_ptr(), None if r is None else r.data_ptr(), ACTS.get(act, act),
+             out.data_ptr(), at, n, _DTYPES[dt]))
+    return out
+
+
+def i8_gated_out(x, wq_g, scales_g, wq_u, scales_u, xs=None, bg=None, bu=None, act="silu", out=None):
+    """out[M,N] = act(x @ Wg + bg) * (x @ Wu + bu), the first half of a gated feed-forward block, x and both
+    weights as i8_gemm_out's, the weights of one shape (gp_i8_gated_out)."""
+    try:
+        dev = x.get_device()
+        M, K = x.shape
+        N = scales_g.shape[0]
+        if xs is None:
+            dt = x.dtype
+            if out is None:
+                out = torch.empty((M, N), dtype=dt, device=x.device)
+        else:
+            dt = out.dtype
+        blocks = (-(-N // 16), -(-K // 64), 1024)
+        ok = (K % 16 == 0 and K > 0 and dt in _DTYPES and dev >= 0 and x.is_contiguous()
+              and (xs is None or (x.dtype is torch.int8 and xs.dtype is torch.float32 and xs.get_device() == dev
+                                  and xs.shape == (M,) and xs.is_contiguous()))
+              and _i8_weight(wq_g, scales_g, blocks, N, dev) and _i8_weight(wq_u, scales_u, blocks, N, dev)
+              and (bg is None or (bg.dtype is dt and bg.get_device() == dev and bg.shape == (N,) and bg.is_contiguous()))
+              and (bu is None or (bu.dtype is dt and bu.get_device() == dev and bu.shape == (N,) and bu.is_contiguous()))
+              and out.dtype is dt and out.get_device() == dev and out.shape == (M, N) and out.is_contiguous())
+    except (AttributeError, ValueError, IndexError, TypeError):
+        ok = False
+    if not ok:
+        _i8_refuse(x, xs, out, [("wq_g", wq_g, "blocks"), ("scales_g", scales_g, "scales"), ("wq_u", wq_u, "blocks"),
+                                ("scales_u", scales_u, "scales"), ("bg", bg, "bias"), ("bu", bu, "bias"),
+                                ("out", out, "rows")])
+    ws, at, n = (None, None, 0) if M == 1 and K <= 16384 else _i8_workspace(M, N, K, xs is not None, 2, x)
+    _run_on(dev, lib.gp_i8_gated_out,
+            (M, N, K, x.data_ptr(), None if xs is None else xs.data_ptr(), wq_g.data_ptr(), scales_g.data_ptr(),
+             None if bg is None else bg.data_ptr(), wq_u.data_ptr(), scales_u.data_ptr(),
              None if bu is None else bu.data_ptr(), ACTS.get(act, act), out.data_ptr(), at, n, _DTYPES[dt]))
     return out

@@ -57,7 +57,7 @@ extern "C" {
 #define GP_ACT_RELU 1
 #define GP_ACT_GELU_TANH 2
 #define GP_ACT_SIGMOID 3
-/* v / (1 + e^-v): gp_residual_norm_out's gate and the 4-bit products only. */
+/* v / (1 + e^-v): gp_residual_norm_out's gate, the 4-bit and the 8-bit products only. */
 #define GP_ACT_SILU 4
 
 /* Norms of gp_residual_norm_out over a row of D values, variance biased:  */
@@ -615,6 +615,53 @@ int gp_q4_gated_out(int64_t M, int64_t N, int64_t K, int group, const void* x, c
                     const void* zeros_g, const void* b_g, const void* wq_u, const void* scales_u, const void* zeros_u,
                     const void* b_u, int act, void* out, void* workspace, int64_t workspace_bytes, int dtype,
                     void* stream);
+
+/*
+ * Bytes of workspace that gp_i8_gemm_out (weights 1) or gp_i8_gated_out
+ * (weights 2) needs at these sizes on the current device, with x in 8 bits
+ * (x_int8 1) or 16 (0); negative: GP_ERR_*.
+ */
+int64_t gp_i8_workspace_bytes(int64_t M, int64_t N, int64_t K, int x_int8, int weights);
+
+/*
+ * Products in 8-bit integers, one token to whole prompts:
+ *   out[M,N] = act(x W + b), or x W + b + r (act GP_ACT_NONE),
+ *   (x W)[m][n] = x_scales[m] * w_scales[n] * sum over k of xq[m][k] * wq[k][n].
+ * x_scales given: x is int8 [M, K], the xq themselves, and x_scales float [M].
+ * x_scales NULL: x is 16-bit [M, K], and a row is rounded here to
+ *   xq[m][k] = 127 x[m][k] / a to the nearest whole number, ties to even,
+ *   x_scales[m] = a / 127, with a = max over k of |x[m][k]|,
+ * exactly so.  A row of zeros has scale 0; a row that is not finite has scale NaN.
+ * wq: int8 blocks [ceil(N / 16)][ceil(K / 64)][1024]; byte 256 g + 16 j + i of
+ * block [a][b] is wq[64 b + 16 g + i][16 a + j], zeros behind K and N.
+ * w_scales: float [N].  K a multiple of 16 up to 131056, N any up to 2^20, a
+ * packed weight below 2 GiB, M up to 2097152.  b [N], r [M,N] or NULL, of the
+ * element type `dtype` as out and a 16-bit x; act any GP_ACT_*.  Scales 4-byte
+ * aligned, every other pointer 16.  Integers may take all of -128 .. 127.
+ * Sums over k are exact; they are scaled in fp32, by w_scales[n] first, and out
+ * is rounded once.  A row's result does not depend on the other rows.  A row
+ * with a scale of NaN gives NaN in that row of out alone.
+ * workspace: scratch of the call's own, of at least gp_i8_workspace_bytes
+ * (16-byte aligned, contents of no matter; NULL and 0 where that is 0).  Calls
+ * that may run at the same time, in graphs too, need workspaces of their own.
+ * Can be captured into a graph.  out may be r; that it overlaps r otherwise, x,
+ * wq, scales or b, or that the workspace overlaps one of these or out, is
+ * refused.
+ * No counterpart in the reference (16-bit operands only).
+ */
+int gp_i8_gemm_out(int64_t M, int64_t N, int64_t K, const void* x, const void* x_scales, const void* wq,
+                   const void* w_scales, const void* b, const void* r, int act, void* out, void* workspace,
+                   int64_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * The first half of a gated feed-forward block:
+ *   out[M,N] = act(x Wg + b_g) * (x Wu + b_u),
+ * x and both weights as in gp_i8_gemm_out, the weights of one shape.  The two
+ * products stay in fp32 until out.
+ */
+int gp_i8_gated_out(int64_t M, int64_t N, int64_t K, const void* x, const void* x_scales, const void* wq_g,
+                    const void* w_scales_g, const void* b_g, const void* wq_u, const void* w_scales_u, const void* b_u,
+                    int act, void* out, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
 
 #ifdef __cplusplus
 }
