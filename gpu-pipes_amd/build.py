@@ -38,7 +38,7 @@ HIP_FLAGS = [
 VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 
 SOURCES = ["mgn_fused.hip", "mgn_pipelined.hip", "stages.hip", "gemm.hip", "gemm_tile.hip", "ffn_fused.hip", "nerf_fused.hip", "dlrm_fused.hip", "status.hip",
-           "bert_addln_pipelined.hip", "bert_ffn_pipelined.hip", "nerf_a_pipelined.hip", "probe.hip", "synth.hip", "residual_norm.hip", "q4.hip", "i8.hip", "capi.cpp", "ffn.cpp", "mlp.cpp", "block.cpp", "arena.cpp"]
+           "bert_addln_pipelined.hip", "bert_ffn_pipelined.hip", "nerf_a_pipelined.hip", "probe.hip", "synth.hip", "residual_norm.hip", "q4.hip", "i8.hip", "route.hip", "capi.cpp", "ffn.cpp", "mlp.cpp", "block.cpp", "arena.cpp"]
 SOURCE_FLAGS = {"gemm.hip": [], "ffn_fused.hip": [], "nerf_fused.hip": [], "dlrm_fused.hip": []}
 
 

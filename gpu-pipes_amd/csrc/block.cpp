@@ -1,8 +1,8 @@
 // C ABI of the operators around a language model's feed-forward half: the norms
 // with the residual (gp_residual_norm_out), the products with 4-bit weights
-// (gp_q4_gemm_out, gp_q4_gated_out) and those in 8-bit integers (gp_i8_gemm_out,
-// gp_i8_gated_out).  Argument checks and dispatch; the kernels are in
-// residual_norm.hip, q4.hip and i8.hip.
+// (gp_q4_gemm_out, gp_q4_gated_out), those in 8-bit integers (gp_i8_gemm_out,
+// gp_i8_gated_out) and the routing to experts (gp_route_out).  Argument checks
+// and dispatch; the kernels are in residual_norm.hip, q4.hip, i8.hip and route.hip.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -288,6 +288,44 @@ int gp_i8_gated_out(int64_t M, int64_t N, int64_t K, const void* x, const void* 
                  {{wq_g, (const float*)w_scales_g, b_g}, {wq_u, (const float*)w_scales_u, b_u}}, nullptr, act, out,
                  dtype, workspace, nullptr};
   return i8_run(a, N, K, workspace_bytes, (hipStream_t)stream);
+}
+
+int gp_route_out(int64_t T, int64_t E, int k, const void* logits, const void* bias, int score, int groups,
+                 int top_groups, int group_score, int renorm, float scale, void* weights, void* ids, int dtype,
+                 void* stream) {
+  clear_error();
+  int rc;
+  if (dtype != GP_DTYPE_F32 && (rc = check_dtype(dtype))) return rc;
+  if (T < 0) return fail(GP_ERR_INVALID_ARG, "T must be >= 0 (got %lld)", (long long)T);
+  if (T > (int64_t(1) << 30)) return fail(GP_ERR_SHAPE, "T too large (%lld)", (long long)T);
+  if (E < 1 || E > kRouteMaxE) return fail(GP_ERR_SHAPE, "E must be in [1, %d] (got %lld)", kRouteMaxE, (long long)E);
+  if (score != GP_SCORE_SOFTMAX && score != GP_SCORE_SIGMOID) return fail(GP_ERR_INVALID_ARG, "unknown score %d", score);
+  if (group_score != GP_GROUP_MAX && group_score != GP_GROUP_TOP2)
+    return fail(GP_ERR_INVALID_ARG, "unknown group score %d", group_score);
+  if (groups < 1 || groups > kRouteMaxGroups || E % groups)
+    return fail(GP_ERR_SHAPE, "groups must divide E and be at most %d (got %d)", kRouteMaxGroups, groups);
+  if (top_groups < 1 || top_groups > groups)
+    return fail(GP_ERR_SHAPE, "top_groups must be in [1, groups] (got %d)", top_groups);
+  if (k < 1 || k > kRouteMaxK || k > E / groups * top_groups)
+    return fail(GP_ERR_SHAPE, "k must be in [1, %d] and at most the experts of top_groups groups (got %d)", kRouteMaxK, k);
+  if (renorm != 0 && renorm != 1) return fail(GP_ERR_INVALID_ARG, "renorm must be 0 or 1 (got %d)", renorm);
+  if (!std::isfinite(scale)) return fail(GP_ERR_INVALID_ARG, "scale must be finite");
+  if ((rc = check4(bias, "bias", false))) return rc;
+  if (T == 0) return GP_OK;
+  if (!logits) return fail(GP_ERR_INVALID_ARG, "logits is NULL");
+  const int64_t size = dtype == GP_DTYPE_F32 ? 4 : 2;
+  if ((uintptr_t)logits % size) return fail(GP_ERR_ALIGN, "logits must be aligned to its elements");
+  if ((rc = check4(weights, "weights", true)) || (rc = check4(ids, "ids", true))) return rc;
+  if (meet_bytes(weights, T * k * 4, ids, T * k * 4)) return fail(GP_ERR_INVALID_ARG, "weights and ids must not overlap");
+  for (const void* o : {(const void*)weights, (const void*)ids})
+    if (meet_bytes(o, T * k * 4, logits, T * E * size) || meet_bytes(o, T * k * 4, bias, E * 4))
+      return fail(GP_ERR_INVALID_ARG, "weights and ids must not overlap the logits or the bias");
+  int dev = 0, ncu = 0;
+  if ((rc = current_device_info(&dev, &ncu))) return rc;
+  const RouteExpertsArgs a{T,     (int)E, k, logits, (const float*)bias, score, groups, top_groups, group_score, renorm,
+                    scale, (float*)weights, (int*)ids, dtype};
+  const hipError_t e = route_experts_launch(a, (hipStream_t)stream);
+  return e == hipSuccess ? GP_OK : fail_hip(e, "route launch");
 }
 
 }  // extern "C"

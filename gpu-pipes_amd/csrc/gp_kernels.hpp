@@ -354,4 +354,20 @@ struct I8Args {
 int64_t i8_workspace(int64_t M, int N, int K, bool x16, int sides, int num_cus);
 hipError_t i8_launch(const I8Args& a, int num_cus, hipStream_t stream);
 
+// Tokens' experts and weights (gp_route_out); E up to kRouteMaxE, k up to kRouteMaxK,
+// groups up to kRouteMaxGroups.
+constexpr int kRouteMaxE = 1024, kRouteMaxK = 32, kRouteMaxGroups = 64;
+struct RouteExpertsArgs {
+  int64_t T;
+  int E, k;
+  const void* logits;  // [T, E]
+  const float* bias;   // [E] or null
+  int score, groups, top_groups, group_score, renorm;
+  float scale;
+  float* weights;  // [T, k]
+  int* ids;        // [T, k]
+  int dtype;       // of the logits
+};
+hipError_t route_experts_launch(const RouteExpertsArgs& a, hipStream_t stream);
+
 }  // namespace gp

@@ -32,6 +32,7 @@ __all__ = [
     "bert_addln_ffn_out", "nerf_a", "nerf_a_out", "pipe_handoff", "handoff_checksums", "phase_timers",
     "probe_mfma", "fill_normal", "residual_norm_out", "residual_norm", "NORMS", "q4_gemm_out",
     "q4_gated_out", "q4", "i8_gemm_out", "i8_gated_out", "i8",
+    "route_out", "SCORES", "GROUP_SCORES",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -48,6 +49,8 @@ _IMPLS = {"fused": IMPL_FUSED, "pipelined": IMPL_PIPELINED, "pipelined_split_ln"
 # "silu" (GP_ACT_SILU) is the residual norm's gate's and the 4-bit and 8-bit products' only
 ACTS = {"none": 0, "relu": 1, "gelu_tanh": 2, "sigmoid": 3, "silu": 4}
 NORMS = {"none": 0, "layer": 1, "rms": 2}
+SCORES = {"softmax": 0, "sigmoid": 1}
+GROUP_SCORES = {"max": 0, "top2": 1}
 ROUTES = {"ident": 0, "broadcast": 1, "split": 2, "drain": 3, "handoff": 4, "reload": 5}
 
 
@@ -132,6 +135,8 @@ def _load():
     L.gp_i8_gemm_out.restype = i32
     L.gp_i8_gated_out.argtypes = [i64, i64, i64] + [vp] * 8 + [i32, vp, vp, i64, i32, vp]
     L.gp_i8_gated_out.restype = i32
+    L.gp_route_out.argtypes = [i64, i64, i32, vp, vp, i32, i32, i32, i32, i32, f32, vp, vp, i32, vp]
+    L.gp_route_out.restype = i32
     for name in ("gp_mlp_out", "gp_dlrm_botmlp_out", "gp_dlrm_topmlp_out", "gp_nerf_full_out", "gp_gemm_out",
                  "gp_gemm_dtype_out", "gp_bert_ffn_out", "gp_bert_ffn_dtype_out", "gp_linear_out", "gp_linear_layer_norm_out", "gp_layer_norm_out", "gp_add_out",
                  "gp_concat_out", "gp_pipe_ident", "gp_pipeline_check"):
@@ -1232,3 +1237,48 @@ def i8_gated_out(x, wq_g, scales_g, wq_u, scales_u, xs=None, bg=None, bu=None, a
              None if bg is None else bg.data_ptr(), wq_u.data_ptr(), scales_u.data_ptr(),
              None if bu is None else bu.data_ptr(), ACTS.get(act, act), out.data_ptr(), at, n, _DTYPES[dt]))
     return out
+
+
+_LOGITS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # GP_DTYPE_*
+
+
+def route_out(logits, k, bias=None, score="softmax", groups=1, top_groups=1, group_score="max", renorm=True, scale=1.0,
+              weights=None, ids=None):
+    """The k best of E experts for each token, and their weights (gp_route_out): logits [T, E] float16, bfloat16 or
+    float32, bias float32 [E], which counts for the choice alone.  score: a name of SCORES; groups of neighbouring
+    experts, of which the top_groups best by group_score (a name of GROUP_SCORES) are chosen from first.  Returns
+    (weights float32 [T, k], ids int32 [T, k]), the best first: the chosen scores, divided by their sum (renorm), times
+    scale.  Experts with a logit of -inf are never chosen; an id of -1 with weight 0 says that none was left."""
+    try:
+        dev = logits.get_device()
+        T, E = logits.shape
+        if weights is None:
+            weights = torch.empty((T, k), dtype=torch.float32, device=logits.device)
+        if ids is None:
+            ids = torch.empty((T, k), dtype=torch.int32, device=logits.device)
+        ok = (logits.dtype in _LOGITS and dev >= 0 and logits.is_contiguous()
+              and (bias is None or (bias.dtype is torch.float32 and bias.get_device() == dev and bias.shape == (E,)
+                                    and bias.is_contiguous()))
+              and weights.dtype is torch.float32 and weights.get_device() == dev and weights.shape == (T, k)
+              and weights.is_contiguous() and ids.dtype is torch.int32 and ids.get_device() == dev
+              and ids.shape == (T, k) and ids.is_contiguous())
+    except (AttributeError, ValueError, IndexError, TypeError):
+        ok = False
+    except RuntimeError as e:  # torch.empty of a negative k
+        raise RuntimeError(f"k must be a whole number of experts (got {k}): {e}") from None
+    if not ok:
+        if not isinstance(logits, torch.Tensor) or logits.dtype not in _LOGITS:
+            raise RuntimeError("logits must be a float16, bfloat16 or float32 torch.Tensor")
+        _check_input("logits", logits, dtype=logits.dtype)
+        if logits.dim() != 2:
+            raise RuntimeError("logits must be 2-D")
+        if not isinstance(k, int):
+            raise RuntimeError(f"k must be a whole number (got {k})")
+        T, E = logits.shape
+        _misfit(logits, [("bias", bias, (E,), torch.float32), ("weights", weights, (T, k), torch.float32),
+                         ("ids", ids, (T, k), torch.int32)])
+    _run_on(dev, lib.gp_route_out,
+            (T, E, k, logits.data_ptr(), None if bias is None else bias.data_ptr(), SCORES.get(score, score), groups,
+             top_groups, GROUP_SCORES.get(group_score, group_score), renorm, scale, weights.data_ptr(), ids.data_ptr(),
+             _LOGITS[logits.dtype]))
+    return weights, ids

@@ -44,6 +44,7 @@ extern "C" {
 /* Element types of the *_dtype_out entry points (16-bit storage, fp32 accumulation). */
 #define GP_DTYPE_F16 0  /* IEEE binary16 */
 #define GP_DTYPE_BF16 1 /* bfloat16      */
+#define GP_DTYPE_F32 2  /* binary32: the logits of gp_route_out only */
 /* Or-ed into the dtype of gp_mgn_mlp_dtype_out (GP_IMPL_FUSED),               */
 /* gp_bert_ffn_dtype_out and gp_bert_addln_ffn_dtype_out (GP_IMPL_FUSED): out  */
 /* is memory that nothing has been written to.  What a launch that fails on    */
@@ -64,6 +65,12 @@ extern "C" {
 #define GP_NORM_NONE 0  /* the row as it is                                 */
 #define GP_NORM_LAYER 1 /* (v - mean) / sqrt(var + eps) * gamma + beta      */
 #define GP_NORM_RMS 2   /* v / sqrt(mean(v^2) + eps) * gamma + beta         */
+
+/* Scores of gp_route_out, and by what a group of experts is ranked. */
+#define GP_SCORE_SOFTMAX 0
+#define GP_SCORE_SIGMOID 1
+#define GP_GROUP_MAX 0  /* its largest                     */
+#define GP_GROUP_TOP2 1 /* the sum of its two largest      */
 
 /* Library version as 0xMMmmpp. */
 int gp_version(void);
@@ -662,6 +669,33 @@ int gp_i8_gemm_out(int64_t M, int64_t N, int64_t K, const void* x, const void* x
 int gp_i8_gated_out(int64_t M, int64_t N, int64_t K, const void* x, const void* x_scales, const void* wq_g,
                     const void* w_scales_g, const void* b_g, const void* wq_u, const void* w_scales_u, const void* b_u,
                     int act, void* out, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * Routing of tokens to experts: for each of T tokens the k best of E experts
+ * and their weights.
+ *   s = softmax or sigmoid of logits[t]            (score)
+ *   c = s + bias, or, bias NULL, the order of the logits themselves
+ *   the top_groups best of `groups` groups of E / groups neighbouring experts,
+ *     by group_score: the group's largest c, or the sum of its two largest
+ *     (bias NULL: of its two largest s); groups == top_groups: all of them
+ *   ids[t][0 .. k - 1] = the k largest c in those groups, the largest first
+ *   weights[t][j] = s of ids[t][j], divided by the k chosen ones' sum where
+ *     renorm is 1, times scale.
+ * Of equal ones the lowest expert, or group, comes first.  Scores are compared
+ * in 64 bits, and weights are rounded once.
+ * An expert whose logit is -inf, or whose bias is, is never chosen: where fewer than
+ * k others are left, what remains of ids is -1 with weights 0 (a sum of 0 gives
+ * weights 0 too).  A group none of whose experts can be chosen comes last.  A row with a
+ * NaN (in c too), or with softmax a logit of +inf, gets NaN weights and the ids 0 .. k - 1.
+ * logits [T, E] of `dtype` (GP_DTYPE_F32 too); bias float [E] or NULL; weights
+ * float [T, k], ids int32 [T, k].  E up to 1024, groups up to 64 and a divisor
+ * of E, k up to 32 and to the experts of top_groups groups.  Pointers aligned
+ * to their elements.  One launch, no workspace: can be captured into a graph.
+ * No counterpart in the reference.
+ */
+int gp_route_out(int64_t T, int64_t E, int k, const void* logits, const void* bias, int score, int groups,
+                 int top_groups, int group_score, int renorm, float scale, void* weights, void* ids, int dtype,
+                 void* stream);
 
 #ifdef __cplusplus
 }
