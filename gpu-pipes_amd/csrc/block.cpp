@@ -1,7 +1,8 @@
 // C ABI of the operators around a language model's feed-forward half: the norms
 // with the residual (gp_residual_norm_out), the products with 4-bit weights
 // (gp_q4_gemm_out, gp_q4_gated_out), those in 8-bit integers (gp_i8_gemm_out,
-// gp_i8_gated_out) and the routing to experts (gp_route_out).  Argument checks
+// gp_i8_gated_out), the routing to experts (gp_route_out) and their feed-forward
+// block (gp_i8_experts_out).  Argument checks
 // and dispatch; the kernels are in residual_norm.hip, q4.hip, i8.hip and route.hip.
 #include <hip/hip_runtime.h>
 
@@ -179,6 +180,53 @@ int i8_run(I8Args a, int64_t N, int64_t K, int64_t ws_bytes, hipStream_t stream)
   return e == hipSuccess ? GP_OK : fail_hip(e, "i8 launch");
 }
 
+int experts_check_shape(int64_t T, int64_t H, int64_t F, int64_t E, int topk) {
+  if (T < 0) return fail(GP_ERR_INVALID_ARG, "T must be >= 0 (got %lld)", (long long)T);
+  int rc;
+  if ((rc = i8_check_weight(F, H, "F", "H")) || (rc = i8_check_weight(H, F, "H", "F"))) return rc;
+  if (E < 1 || E > kExpertsMaxE) return fail(GP_ERR_SHAPE, "E must be in [1, %d] (got %lld)", kExpertsMaxE, (long long)E);
+  if (topk < 1 || topk > kExpertsMaxK) return fail(GP_ERR_SHAPE, "topk must be in [1, %d] (got %d)", kExpertsMaxK, topk);
+  if (T > (int64_t(1) << 21) || T * H >= (int64_t(1) << 31))
+    return fail(GP_ERR_SHAPE, "T must be at most 2097152, and T * H below 2^31 (got %lld, %lld)", (long long)T, (long long)H);
+  return GP_OK;
+}
+
+int experts_run(const ExpertsArgs& a, int64_t ws_bytes, hipStream_t stream) {
+  int rc;
+  if ((rc = check_dtype(a.dtype)) || (rc = check_act_ext(a.act))) return rc;
+  if (ws_bytes < 0) return fail(GP_ERR_INVALID_ARG, "workspace_bytes must be >= 0");
+  if (ws_bytes && (rc = check16(a.ws, "workspace", true))) return rc;
+  if ((rc = check16(a.wg, "wq_g", true)) || (rc = check4(a.sg, "w_scales_g", true)) || (rc = check16(a.wu, "wq_u", true)) ||
+      (rc = check4(a.su, "w_scales_u", true)) || (rc = check16(a.wd, "wq_d", true)) ||
+      (rc = check4(a.sd, "w_scales_d", true)) || (rc = check16(a.r, "r", false)))
+    return rc;
+  if (a.T == 0) return GP_OK;
+  if ((rc = check16(a.x, "x", true)) || (rc = check4(a.ids, "ids", true)) || (rc = check4(a.weights, "weights", true)) ||
+      (rc = check16(a.out, "out", true)))
+    return rc;
+  const int64_t bytes = a.T * a.H * 2, P = a.T * a.topk;
+  if (a.r != a.out && meet_bytes(a.out, bytes, a.r, bytes))
+    return fail(GP_ERR_INVALID_ARG, "out may be r, but not overlap it otherwise");
+  if (meet_bytes(a.ws, ws_bytes, a.out, bytes) || meet_bytes(a.ws, ws_bytes, a.r, bytes))
+    return fail(GP_ERR_INVALID_ARG, "the workspace must not overlap r or out");
+  auto meets = [&](const void* p, int64_t n) {
+    const int64_t E = a.E, up = E * i8_packed(a.F, a.H), down = E * i8_packed(a.H, a.F);
+    return meet_bytes(p, n, a.x, bytes) || meet_bytes(p, n, a.ids, P * 4) || meet_bytes(p, n, a.weights, P * 4) ||
+           meet_bytes(p, n, a.wg, up) || meet_bytes(p, n, a.sg, E * a.F * 4) || meet_bytes(p, n, a.wu, up) ||
+           meet_bytes(p, n, a.su, E * a.F * 4) || meet_bytes(p, n, a.wd, down) || meet_bytes(p, n, a.sd, E * a.H * 4);
+  };
+  if (meets(a.out, bytes)) return fail(GP_ERR_INVALID_ARG, "out must not overlap x, ids, weights, an expert's weight or scales");
+  if (meets(a.ws, ws_bytes))
+    return fail(GP_ERR_INVALID_ARG, "the workspace must not overlap x, ids, weights, an expert's weight or scales");
+  int dev = 0, ncu = 0;
+  if ((rc = current_device_info(&dev, &ncu))) return rc;
+  const int64_t need = i8_experts_workspace(a.T, a.H, a.F, a.E, a.topk);
+  if (ws_bytes < need)
+    return fail(GP_ERR_INVALID_ARG, "workspace_bytes must be at least %lld (got %lld)", (long long)need, (long long)ws_bytes);
+  const hipError_t e = i8_experts_launch(a, ncu, stream);
+  return e == hipSuccess ? GP_OK : fail_hip(e, "i8 experts launch");
+}
+
 }  // namespace
 }  // namespace gp
 
@@ -326,6 +374,26 @@ int gp_route_out(int64_t T, int64_t E, int k, const void* logits, const void* bi
                     scale, (float*)weights, (int*)ids, dtype};
   const hipError_t e = route_experts_launch(a, (hipStream_t)stream);
   return e == hipSuccess ? GP_OK : fail_hip(e, "route launch");
+}
+
+int64_t gp_i8_experts_workspace_bytes(int64_t T, int64_t H, int64_t F, int64_t E, int topk) {
+  clear_error();
+  const int rc = experts_check_shape(T, H, F, E, topk);
+  if (rc) return rc;
+  return T == 0 ? 0 : i8_experts_workspace(T, (int)H, (int)F, (int)E, topk);
+}
+
+int gp_i8_experts_out(int64_t T, int64_t H, int64_t F, int64_t E, int topk, const void* x, const void* ids,
+                      const void* weights, const void* wq_g, const void* w_scales_g, const void* wq_u,
+                      const void* w_scales_u, const void* wq_d, const void* w_scales_d, int act, const void* r, void* out,
+                      void* workspace, int64_t workspace_bytes, int dtype, void* stream) {
+  clear_error();
+  const int rc = experts_check_shape(T, H, F, E, topk);
+  if (rc) return rc;
+  const ExpertsArgs a{T, (int)H, (int)F, (int)E, topk, x, (const int*)ids, (const float*)weights, wq_g, wq_u, wq_d,
+                      (const float*)w_scales_g, (const float*)w_scales_u, (const float*)w_scales_d, act, r, out, dtype,
+                      workspace};
+  return experts_run(a, workspace_bytes, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -354,6 +354,26 @@ struct I8Args {
 int64_t i8_workspace(int64_t M, int N, int K, bool x16, int sides, int num_cus);
 hipError_t i8_launch(const I8Args& a, int num_cus, hipStream_t stream);
 
+// A feed-forward block of experts (gp_i8_experts_out): H and F multiples of 16
+// up to kI8MaxK, T * H below 2^31 and T * topk below 2^28.
+constexpr int kExpertsMaxE = 1024, kExpertsMaxK = 32;
+struct ExpertsArgs {
+  int64_t T;
+  int H, F, E, topk;
+  const void* x;         // [T, H]
+  const int* ids;        // [T, topk]
+  const float* weights;  // [T, topk]
+  const void *wg, *wu, *wd;  // [E] packed weights
+  const float *sg, *su, *sd;  // [E, F], [E, F], [E, H]
+  int act;
+  const void* r;  // [T, H] or null
+  void* out;      // [T, H]
+  int dtype;
+  void* ws;
+};
+int64_t i8_experts_workspace(int64_t T, int H, int F, int E, int topk);
+hipError_t i8_experts_launch(const ExpertsArgs& a, int num_cus, hipStream_t stream);
+
 // Tokens' experts and weights (gp_route_out); E up to kRouteMaxE, k up to kRouteMaxK,
 // groups up to kRouteMaxGroups.
 constexpr int kRouteMaxE = 1024, kRouteMaxK = 32, kRouteMaxGroups = 64;

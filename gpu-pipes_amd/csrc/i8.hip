@@ -119,15 +119,16 @@ __device__ __forceinline__ unsigned wave_top(unsigned a) {
 
 // Rows of x to bytes: WPR waves a row, P pieces of eight values a lane held in
 // registers, so that memory is read once; rows longer than that are read again
-// (from L2).  One wave a row up to 2,048 values, four rows a workgroup.
+// (from L2).  One wave a row up to 2,048 values, four rows a workgroup.  count:
+// where it is given, the rows that there are.
 template <class T, int P, int WPR>
 __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void i8_rows_to_bytes_kernel(const half_t* x, int64_t M, int K,
-                                                                                    char* q, float* xs) {
+                                                                                    char* q, float* xs, const int* count) {
   constexpr int STEP = 64 * WPR * 8;
   __shared__ unsigned part[WPR];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t m = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-  if (m >= M) return;  // whole waves of one-wave rows only
+  if (m >= M || (count && m >= *count)) return;  // whole waves of one-wave rows only
   const auto xr = make_rsrc(x + m * K, K * 2);
   const int at = (WPR == 1 ? lane : (int)threadIdx.x) * 8;
   u32x4 v[P];
@@ -160,10 +161,10 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void i8_rows_to_bytes_ke
 }
 
 template <class T>
-hipError_t rows_to_bytes(const void* x, int64_t M, int K, char* q, float* xs, hipStream_t s) {
+hipError_t rows_to_bytes(const void* x, int64_t M, int K, char* q, float* xs, hipStream_t s, const int* count = nullptr) {
   const half_t* h = (const half_t*)x;
 #define GP_ROWS(p, w) \
-  hipLaunchKernelGGL((i8_rows_to_bytes_kernel<T, p, w>), dim3((unsigned)(w == 1 ? (M + 3) / 4 : M)), dim3(w == 1 ? 256 : 64 * w), 0, s, h, M, K, q, xs)
+  hipLaunchKernelGGL((i8_rows_to_bytes_kernel<T, p, w>), dim3((unsigned)(w == 1 ? (M + 3) / 4 : M)), dim3(w == 1 ? 256 : 64 * w), 0, s, h, M, K, q, xs, count)
   if (K <= 512) GP_ROWS(1, 1);
   else if (K <= 2048) GP_ROWS(4, 1);
   else if (K <= 8192) GP_ROWS(4, 4);
@@ -222,6 +223,24 @@ __device__ __forceinline__ void finish1(const I8Args& p, int64_t m, int n, float
 }
 
 // ---------------------------------------------------------------------------
+// Experts: a product's rows lie in runs, one an expert, each cut into tiles.
+// UP: tile rows are tokens of x, gathered, the results one after the other;
+// DOWN: the rows one after the other, the results in fp32 at their (token,
+// choice) pairs.
+// ---------------------------------------------------------------------------
+enum { DENSE, UP, DOWN };
+struct TileRec {
+  int expert, row0, rows, pad;
+};
+struct I8Group {
+  const TileRec* tiles;
+  const int* info;  // tiles and rows that there are
+  const int* tok;   // of a row: its token
+  const int* pair;  // and its pair, token * topk + choice
+  int64_t wbytes;   // of an expert's packed weight
+};
+
+// ---------------------------------------------------------------------------
 // Few rows.  A wave multiplies its share of k with NT tiles of 16 columns (of
 // two weights NT / 2 of each); words and x go through a ring of R chunks in
 // LDS that is the wave's own, so that many loads are in flight and no barrier
@@ -243,8 +262,9 @@ struct RowsPlan {
   int xstride, bytes;  // XL: of a row's bytes; LDS
 };
 
-template <class T, int S, int NT, int MT, bool XL>
-__global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8Args p, int kwshift, int mshift, int xstride) {
+template <class T, int S, int NT, int MT, bool XL, int MODE>
+__global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8Args p, I8Group grp, int kwshift,
+                                                                             int mshift, int xstride) {
   constexpr int R = rows_ring(NT, MT, XL), SLOT = slot_bytes(NT, MT, XL), NI = SLOT / 1024, CW = NT / S;
   __shared__ unsigned tops[16];
   GP_LDS char* lds = dyn_lds();
@@ -253,8 +273,16 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
   const int KW = 1 << kwshift, kw = wave & (KW - 1), cg = wave >> kwshift, CG = waves >> kwshift;
   const int N = p.N, K = p.K, N16 = (N + 15) / 16, K64 = (K + 63) / 64, chunks = (K + kChunk - 1) / kChunk;
   const int t0 = xcd_order(blockIdx.x, gridDim.x) * (CW * CG);  // the workgroup's first tile of columns
-  const int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
-  const int rows = p.M - m0 < 16 * MT ? (int)(p.M - m0) : 16 * MT;
+  int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
+  int rows = p.M - m0 < 16 * MT ? (int)(p.M - m0) : 16 * MT;
+  if constexpr (MODE != DENSE) {
+    if ((int)blockIdx.y >= grp.info[0]) return;
+    const TileRec rec = grp.tiles[blockIdx.y];
+    m0 = rec.row0, rows = rec.rows;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      p.side[s].wq = (const char*)p.side[s].wq + rec.expert * grp.wbytes, p.side[s].s += (int64_t)rec.expert * N;
+  }
 
   // 16-bit x first: what follows is not waited for with it
   constexpr int XP = 4;
@@ -273,7 +301,7 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
   const int wbytes = N16 * K64 * 1024;
   const auto wr0 = make_rsrc(p.side[0].wq, wbytes);
   const auto wr1 = make_rsrc(p.side[S - 1].wq, wbytes);
-  const auto xr8 = make_rsrc((const char*)p.xq + m0 * K, rows * K);
+  const auto xr8 = MODE == UP ? make_rsrc(p.xq, (int)(p.M * K)) : make_rsrc((const char*)p.xq + m0 * K, rows * K);
   unsigned wo[CW];
 #pragma unroll
   for (int t = 0; t < CW; ++t) {
@@ -282,9 +310,16 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
   }
   // 16-byte piece c of row r lies at c ^ (r / 2) % 8: sixteen rows' reads of one piece fall into different banks
   const int dr = lane >> 3;
-  unsigned xo[2];
+  unsigned xo[MT][2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) xo[h] = (unsigned)((8 * h + dr) * K + (((lane & 7) ^ (((8 * h + dr) >> 1) & 7)) << 4));
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int row = mt * 16 + 8 * h + dr;
+      const unsigned piece = (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) << 4);
+      if constexpr (MODE == UP) row = row < rows ? grp.tok[m0 + row] : -1;
+      xo[mt][h] = MODE == UP && row < 0 ? 0x80000000u : (unsigned)row * (unsigned)K + piece;
+    }
 
   auto issue = [&](int c, int slot) {
     GP_LDS char* at = ring + slot * SLOT;
@@ -302,7 +337,7 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          dma16_buf(xr8, (int)(in ? xo[h] + (unsigned)(mt * 16 * K + c * kChunk) : kNowhere),
+          dma16_buf(xr8, (int)(in ? xo[mt][h] + (unsigned)(c * kChunk) : kNowhere),
                     at + NT * 2048 + mt * 2048 + h * 1024);
     }
   };
@@ -390,21 +425,24 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
       v += *(GP_LDS const int*)(from + w * (R * SLOT));
       if (S == 2) u += *(GP_LDS const int*)(from + w * (R * SLOT) + 16 * CW * 4);
     }
-    const float xsc = XL ? xsl[m] : p.xs[m0 + m];
-    finish1<T, S>(p, m0 + m, n, (float)v * p.side[0].s[n] * xsc, S == 2 ? (float)u * p.side[S - 1].s[n] * xsc : 0.f);
+    const float xsc = XL ? xsl[m] : p.xs[MODE == UP ? grp.tok[m0 + m] : m0 + m];
+    if constexpr (MODE == DOWN)
+      ((float*)p.out)[(int64_t)grp.pair[m0 + m] * N + n] = (float)v * p.side[0].s[n] * xsc;
+    else
+      finish1<T, S>(p, m0 + m, n, (float)v * p.side[0].s[n] * xsc, S == 2 ? (float)u * p.side[S - 1].s[n] * xsc : 0.f);
   }
 }
 
-template <class T, int S, int NT, int MT, bool XL>
-hipError_t rows_launch_one(const I8Args& a, const RowsPlan& l, int mshift, hipStream_t s) {
-  const auto kern = &i8_rows_kernel<T, S, NT, MT, XL>;
+template <class T, int S, int NT, int MT, bool XL, int MODE>
+hipError_t rows_launch_one(const I8Args& a, const I8Group& g, int64_t mtiles, const RowsPlan& l, int mshift, hipStream_t s) {
+  const auto kern = &i8_rows_kernel<T, S, NT, MT, XL, MODE>;
   if (l.bytes > 60 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kRowsLds);
     if (e != hipSuccess) return e;
   }
   const int tiles = (a.N + 15) / 16, per = NT / S * l.cg;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((tiles + per - 1) / per), (unsigned)((a.M + 16 * MT - 1) / (16 * MT))),
-                     dim3(l.kw * l.cg * kWave), l.bytes, s, a, __builtin_ctz(l.kw), mshift, l.xstride);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((tiles + per - 1) / per), (unsigned)mtiles), dim3(l.kw * l.cg * kWave),
+                     l.bytes, s, a, g, __builtin_ctz(l.kw), mshift, l.xstride);
   return hipGetLastError();
 }
 
@@ -417,8 +455,8 @@ hipError_t rows_launch_one(const I8Args& a, const RowsPlan& l, int mshift, hipSt
 // through LDS.  Where tiles are few, several workgroups share one, each with a
 // part of k, leave their sums in a workspace, and a second kernel adds them.
 // ---------------------------------------------------------------------------
-template <class T, int S, int BM, int BN, int WM, int WN, int R, int EU>
-__global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, int mtiles, int ntiles) {
+template <class T, int S, int BM, int BN, int WM, int WN, int R, int EU, int MODE>
+__global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8Group g, int mtiles, int ntiles) {
   constexpr int NW = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, NS = NT / S;
   constexpr int XI = BM / 8 / NW, WI = BN / 8 / NW, NI = XI + WI;  // copies of 1 KiB a wave and chunk
   constexpr int XB = BM * kChunk, SLOT = XB + BN * kChunk;
@@ -433,10 +471,19 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, int
   const int id = xcd_order(blockIdx.x, gridDim.x);
   const int gm0 = id / (8 * ntiles) * 8, rest = id % (8 * ntiles);
   const int gm = mtiles - gm0 < 8 ? mtiles - gm0 : 8;
-  const int64_t m0 = (int64_t)(gm0 + rest % gm) * BM;
+  int64_t m0 = (int64_t)(gm0 + rest % gm) * BM;
   const int nb0 = rest / gm * SB;  // first block of columns
-  const int rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
-  const auto xr = make_rsrc((const char*)p.xq + m0 * K, rows * K);
+  int rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
+  if constexpr (MODE != DENSE) {
+    const int ti = gm0 + rest % gm;
+    if (ti >= g.info[0]) return;
+    const TileRec rec = g.tiles[ti];
+    m0 = rec.row0, rows = rec.rows;
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      p.side[s].wq = (const char*)p.side[s].wq + rec.expert * g.wbytes, p.side[s].s += (int64_t)rec.expert * N;
+  }
+  const auto xr = MODE == UP ? make_rsrc(p.xq, (int)(p.M * K)) : make_rsrc((const char*)p.xq + m0 * K, rows * K);
   const auto wr0 = make_rsrc(p.side[0].wq, N16 * K64 * 1024);
   const auto wr1 = make_rsrc(p.side[S - 1].wq, N16 * K64 * 1024);
 
@@ -446,8 +493,10 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, int
   unsigned xo[XI], wo[WI];
 #pragma unroll
   for (int q = 0; q < XI; ++q) {
-    const int row = 8 * (q * NW + wave) + (lane >> 3);
-    xo[q] = (unsigned)(row * K + (((lane & 7) ^ ((row >> 1) & 7)) << 4));
+    int row = 8 * (q * NW + wave) + (lane >> 3);
+    const unsigned piece = (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) << 4);
+    if constexpr (MODE == UP) row = row < rows ? g.tok[m0 + row] : -1;
+    xo[q] = MODE == UP && row < 0 ? 0x80000000u : (unsigned)row * (unsigned)K + piece;
   }
   const int kb = wave & 1;  // of the chunk's two blocks along k
 #pragma unroll
@@ -512,7 +561,7 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, int
 
   // A lane's columns: 4 NS from n0 of each weight, of row j of each row tile.
   const int n0 = nb0 * 16 + wn * (16 * NS) + 4 * NS * lg;
-  if (gridDim.y > 1) {
+  if (MODE == DENSE && gridDim.y > 1) {
     int* const part = (int*)p.part + (int64_t)blockIdx.y * S * p.M * N;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -536,8 +585,8 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, int
   }
   constexpr int W8 = NS >= 2 ? 2 : 1;  // sums of up to eight columns at a time
 #pragma unroll
-  for (int g = 0; g < NS / W8; ++g) {
-    const int n = n0 + 4 * W8 * g, cnt = N - n < 4 * W8 ? N - n : 4 * W8;
+  for (int c = 0; c < NS / W8; ++c) {
+    const int n = n0 + 4 * W8 * c, cnt = N - n < 4 * W8 ? N - n : 4 * W8;
     if (cnt <= 0) continue;
     float sc[S][8] = {};
 #pragma unroll
@@ -549,16 +598,22 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, int
     for (int m = 0; m < MT; ++m) {
       const int row = wm * MT * 16 + m * 16 + j;
       if (row >= rows) continue;
-      const float xsc = p.xs[m0 + row];
+      const float xsc = p.xs[MODE == UP ? g.tok[m0 + row] : m0 + row];
       float v[8] = {}, u[8] = {};
 #pragma unroll
       for (int t = 0; t < W8; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          v[4 * t + e] = (float)acc[0][W8 * g + t][m][e] * sc[0][4 * t + e] * xsc;
-          if (S == 2) u[4 * t + e] = (float)acc[S - 1][W8 * g + t][m][e] * sc[S - 1][4 * t + e] * xsc;
+          v[4 * t + e] = (float)acc[0][W8 * c + t][m][e] * sc[0][4 * t + e] * xsc;
+          if (S == 2) u[4 * t + e] = (float)acc[S - 1][W8 * c + t][m][e] * sc[S - 1][4 * t + e] * xsc;
         }
-      finish8<T, S>(p, m0 + row, n, cnt, v, u);
+      if constexpr (MODE == DOWN) {  // N a multiple of 16 here
+        float* const to = (float*)p.out + (int64_t)g.pair[m0 + row] * N + n;
+#pragma unroll
+        for (int t = 0; t < W8; ++t) *(f4*)(to + 4 * t) = f4{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]};
+      } else {
+        finish8<T, S>(p, m0 + row, n, cnt, v, u);
+      }
     }
   }
 }
@@ -626,12 +681,13 @@ bool on_tiles(int64_t M) { return M > 64; }
 
 bool own_bytes(int64_t M, int K) { return M <= 4 && K * (M <= 1 ? 1 : M <= 2 ? 2 : 4) <= 16384; }
 
-template <class T, int S>
-hipError_t rows_launch(const I8Args& a, bool x16, int num_cus, hipStream_t s) {
+// mtiles: of 16 mt rows.  A product of experts (MODE) has them from its plan.
+template <class T, int S, int MODE>
+hipError_t rows_launch(const I8Args& a, const I8Group& g, int mt, int64_t mtiles, bool x16, int num_cus, hipStream_t s) {
   RowsPlan l{};
   l.xl = x16;
+  l.mt = mt;
   const int tiles = (a.N + 15) / 16 * S, chunks = (a.K + kChunk - 1) / kChunk;
-  l.mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
   int per = tiles >= 4 * num_cus ? 4 : tiles >= 2 * num_cus ? 2 : 1;  // tiles a workgroup
   if (per < S) per = S;
   l.nt = per > 2 && l.mt == 1 ? 2 : per;
@@ -648,34 +704,38 @@ hipError_t rows_launch(const I8Args& a, bool x16, int num_cus, hipStream_t s) {
   l.kw = waves / l.cg;
   while (l.kw > 1 && l.kw / 2 >= chunks && l.kw / 2 * l.cg >= need) l.kw /= 2;
   l.bytes = l.kw * l.cg * ring + xbytes;
-#define GP_CASE(n, m)                                                              \
-  if constexpr (n >= S)                                                            \
-    if (l.nt == n && l.mt == m) {                                                  \
-      if constexpr (m == 1)                                                        \
-        if (l.xl) return rows_launch_one<T, S, n, m, true>(a, l, mshift, s);       \
-      return rows_launch_one<T, S, n, m, false>(a, l, mshift, s);                  \
+#define GP_CASE(n, m)                                                                          \
+  if constexpr (n >= S)                                                                        \
+    if (l.nt == n && l.mt == m) {                                                              \
+      if constexpr (m == 1 && MODE == DENSE)                                                   \
+        if (l.xl) return rows_launch_one<T, S, n, m, true, MODE>(a, g, mtiles, l, mshift, s);  \
+      return rows_launch_one<T, S, n, m, false, MODE>(a, g, mtiles, l, mshift, s);             \
     }
   GP_CASE(1, 1) GP_CASE(2, 1) GP_CASE(1, 2) GP_CASE(2, 2) GP_CASE(4, 2) GP_CASE(1, 4) GP_CASE(2, 4) GP_CASE(4, 4)
 #undef GP_CASE
   return hipErrorInvalidValue;
 }
 
-template <class T, int S>
-hipError_t tile_launch(const I8Args& a, const TilePlan& plan, hipStream_t s) {
-  const int64_t cols = plan.size / S, mtiles = (a.M + plan.size - 1) / plan.size, ntiles = (a.N + cols - 1) / cols;
+template <class T, int S, int MODE>
+hipError_t tile_launch(const I8Args& a, const I8Group& g, int64_t mtiles, const TilePlan& plan, hipStream_t s) {
+  const int64_t cols = plan.size / S, ntiles = (a.N + cols - 1) / cols;
   if (mtiles * ntiles > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
   const dim3 grid((unsigned)(mtiles * ntiles), (unsigned)plan.parts);
-  if (plan.size == 256)
-    hipLaunchKernelGGL((i8_tile_kernel<T, S, 256, 256, 2, 4, 2, 2>), grid, dim3(512), 0, s, a, (int)mtiles, (int)ntiles);
-  else if (plan.size == 128)
-    hipLaunchKernelGGL((i8_tile_kernel<T, S, 128, 128, 2, 2, 2, 2>), grid, dim3(256), 0, s, a, (int)mtiles, (int)ntiles);
-  else
-    hipLaunchKernelGGL((i8_tile_kernel<T, S, 64, 64, 2, 2, 4, 2>), grid, dim3(256), 0, s, a, (int)mtiles, (int)ntiles);
+#define GP_TILE(size, wm, wn, r)                                                                                  \
+  hipLaunchKernelGGL((i8_tile_kernel<T, S, size, size, wm, wn, r, 2, MODE>), grid, dim3(64 * wm * wn), 0, s, a, g, \
+                     (int)mtiles, (int)ntiles)
+  if (plan.size == 256) GP_TILE(256, 2, 4, 2);
+  else if (plan.size == 128) GP_TILE(128, 2, 2, 2);
+  else GP_TILE(64, 2, 2, 4);
+#undef GP_TILE
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || plan.parts == 1) return e;
-  const int64_t pieces = a.M * ((a.N + 7) / 8);
-  hipLaunchKernelGGL((i8_join_kernel<T, S>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, a, plan.parts);
-  return hipGetLastError();
+  if constexpr (MODE == DENSE) {
+    if (e != hipSuccess || plan.parts == 1) return e;
+    const int64_t pieces = a.M * ((a.N + 7) / 8);
+    hipLaunchKernelGGL((i8_join_kernel<T, S>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, a, plan.parts);
+    return hipGetLastError();
+  }
+  return e;
 }
 
 // The workspace: bytes and scales of 16-bit rows, then the parts' sums.
@@ -706,15 +766,179 @@ hipError_t launch(I8Args a, int num_cus, hipStream_t s) {
     const hipError_t e = rows_to_bytes<T>(a.x, a.M, a.K, (char*)a.ws, (float*)a.xs, s);
     if (e != hipSuccess) return e;
   }
-  if (!on_tiles(a.M)) return rows_launch<T, S>(a, xl, num_cus, s);
+  if (!on_tiles(a.M)) {
+    const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
+    return rows_launch<T, S, DENSE>(a, I8Group{}, mt, (a.M + 16 * mt - 1) / (16 * mt), xl, num_cus, s);
+  }
   a.part = (char*)a.ws + l.part;
-  return tile_launch<T, S>(a, tile_plan(a.M, a.N, a.K, S, num_cus), s);
+  const TilePlan plan = tile_plan(a.M, a.N, a.K, S, num_cus);
+  return tile_launch<T, S, DENSE>(a, I8Group{}, (a.M + plan.size - 1) / plan.size, plan, s);
+}
+
+// ---------------------------------------------------------------------------
+// A feed-forward block of experts.  out[t] = r[t] + sum over j of w[t][j] *
+// Down(act(x Wg) * (x Wu)) of expert ids[t][j].
+//
+// The pairs (token, choice) are put in order of their experts, so that an
+// expert's rows are one product; its rows are tokens of x, which the first
+// product gathers while it copies them.  The pairs' results go back to their
+// places in fp32 and are added in the order of the choices: nothing depends on
+// the order in which workgroups end.
+// ---------------------------------------------------------------------------
+
+// One workgroup an expert: counts of all experts (whole numbers, in LDS), where
+// the expert's rows and tiles begin, and its pairs in their order.
+__global__ __launch_bounds__(1024) void i8_plan_kernel(const int* ids, int64_t P, int E, int topk, int tile, TileRec* tiles,
+                                                      int* info, int* tok, int* pair) {
+  __shared__ int count[kExpertsMaxE];
+  __shared__ int own[16], sums[16][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e = blockIdx.x;
+  if (tid < E) count[tid] = 0;
+  __syncthreads();
+  const int64_t seg = ((P + 15) / 16 + 63) / 64 * 64, lo = wave * seg, hi = lo + seg < P ? lo + seg : P;
+  int mine = 0;
+  for (int64_t i = lo; i < hi; i += 64) {
+    const int id = i + lane < hi ? ids[i + lane] : -1;
+    if ((unsigned)id < (unsigned)E) atomicAdd(&count[id], 1);
+    mine += __popcll(__ballot(id == e));
+  }
+  if (lane == 0) own[wave] = mine;
+  __syncthreads();
+  // rows and tiles of the experts before this one, and of all
+  const int c = tid < E ? count[tid] : 0, n = (c + tile - 1) / tile;
+  int v[4] = {tid < e ? c : 0, tid < e ? n : 0, c, n};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v[k] += __shfl_xor(v[k], d);
+    if (lane == 0) sums[wave][k] = v[k];
+  }
+  __syncthreads();
+  int row0 = 0, tile0 = 0, allrows = 0, alltiles = 0, before = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    row0 += sums[w][0], tile0 += sums[w][1], allrows += sums[w][2], alltiles += sums[w][3];
+    before += w < wave ? own[w] : 0;
+  }
+  if (e == 0 && tid == 0) info[0] = alltiles, info[1] = allrows;
+  const int rows = count[e];
+  for (int i = tid; i * tile < rows; i += 1024)
+    tiles[tile0 + i] = TileRec{e, row0 + i * tile, rows - i * tile < tile ? rows - i * tile : tile, 0};
+  if (mine == 0) return;
+  int at = row0 + before;
+  for (int64_t i = lo; i < hi; i += 64) {
+    const bool hit = i + lane < hi && ids[i + lane] == e;
+    const unsigned long long b = __ballot(hit);
+    if (hit) {
+      const int to = at + __popcll(b & ((1ull << lane) - 1));
+      tok[to] = (int)((i + lane) / topk);
+      pair[to] = (int)(i + lane);
+    }
+    at += __popcll(b);
+  }
+}
+
+// The pairs' results times their weights, in the order of the choices, and r:
+// eight columns of a token a thread.
+template <class T>
+__global__ __launch_bounds__(256) void i8_combine_kernel(ExpertsArgs p, const float* y) {
+  const int pieces = p.H / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.T * pieces) return;
+  const int64_t t = i / pieces;
+  const int n = (int)(i - t * pieces) * 8;
+  float v[8] = {}, f[8];
+#pragma unroll 4
+  for (int j = 0; j < p.topk; ++j) {
+    const int64_t at = t * p.topk + j;
+    if ((unsigned)p.ids[at] >= (unsigned)p.E) continue;
+    const float w = p.weights[at];
+    const f4 lo = *(const f4*)(y + at * p.H + n), hi = *(const f4*)(y + at * p.H + n + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(w, lo[e], v[e]), v[4 + e] = __builtin_fmaf(w, hi[e], v[4 + e]);
+  }
+  if (p.r) {
+    load8<T>((const half_t*)p.r + t * p.H + n, 8, f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += f[e];
+  }
+  store8<T>((half_t*)p.out + t * p.H + n, 8, v);
+}
+
+// Rows of a tile, by the rows that an expert has on average.
+int experts_tile(int64_t P, int E) {
+  const int64_t n = P / E;
+  return n >= 192 ? 256 : n >= 64 ? 128 : n >= 24 ? 64 : 16;
+}
+
+struct ExpertsLayout {
+  int tile;
+  int64_t max_tiles, xq, xs, tiles, info, tok, pair, h, hq, hs, y, bytes;
+};
+ExpertsLayout experts_layout(int64_t T, int H, int F, int E, int topk) {
+  ExpertsLayout l{};
+  const int64_t P = T * topk;
+  l.tile = experts_tile(P, E);
+  l.max_tiles = P / l.tile + (P < E ? P : E);
+  auto take = [&](int64_t n) {
+    const int64_t at = l.bytes;
+    l.bytes += (n + 255) / 256 * 256;
+    return at;
+  };
+  l.xq = take(T * H);
+  l.xs = take(T * 4);
+  l.tiles = take(l.max_tiles * (int64_t)sizeof(TileRec));
+  l.info = take(8);
+  l.tok = take(P * 4);
+  l.pair = take(P * 4);
+  l.h = take(P * F * 2);
+  l.hq = take(P * F);
+  l.hs = take(P * 4);
+  l.y = take(P * H * 4);
+  return l;
+}
+
+template <class T, int S, int MODE>
+hipError_t experts_product(const I8Args& a, const I8Group& g, const ExpertsLayout& l, int num_cus, hipStream_t s) {
+  if (l.tile == 16) return rows_launch<T, S, MODE>(a, g, 1, l.max_tiles, false, num_cus, s);
+  return tile_launch<T, S, MODE>(a, g, l.max_tiles, TilePlan{l.tile, 1}, s);
+}
+
+template <class T>
+hipError_t experts_run(const ExpertsArgs& p, int num_cus, hipStream_t s) {
+  const int64_t P = p.T * p.topk;
+  const ExpertsLayout l = experts_layout(p.T, p.H, p.F, p.E, p.topk);
+  char* const ws = (char*)p.ws;
+  I8Group g{(const TileRec*)(ws + l.tiles), (const int*)(ws + l.info), (const int*)(ws + l.tok), (const int*)(ws + l.pair), 0};
+  hipLaunchKernelGGL(i8_plan_kernel, dim3(p.E), dim3(1024), 0, s, p.ids, P, p.E, p.topk, l.tile, (TileRec*)(ws + l.tiles),
+                     (int*)(ws + l.info), (int*)(ws + l.tok), (int*)(ws + l.pair));
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  if ((e = rows_to_bytes<T>(p.x, p.T, p.H, ws + l.xq, (float*)(ws + l.xs), s)) != hipSuccess) return e;
+  I8Args up{p.T, p.F, p.H, 2, nullptr, ws + l.xq, (const float*)(ws + l.xs), {{p.wg, p.sg, nullptr}, {p.wu, p.su, nullptr}},
+            nullptr, p.act, ws + l.h, p.dtype, nullptr, nullptr};
+  g.wbytes = (int64_t)((p.F + 15) / 16) * ((p.H + 63) / 64) * 1024;
+  if ((e = experts_product<T, 2, UP>(up, g, l, num_cus, s)) != hipSuccess) return e;
+  if ((e = rows_to_bytes<T>(ws + l.h, P, p.F, ws + l.hq, (float*)(ws + l.hs), s, g.info + 1)) != hipSuccess) return e;
+  I8Args down{P, p.H, p.F, 1, nullptr, ws + l.hq, (const float*)(ws + l.hs), {{p.wd, p.sd, nullptr}, {}},
+              nullptr, GP_ACT_NONE, ws + l.y, p.dtype, nullptr, nullptr};
+  g.wbytes = (int64_t)((p.H + 15) / 16) * ((p.F + 63) / 64) * 1024;
+  if ((e = experts_product<F16, 1, DOWN>(down, g, l, num_cus, s)) != hipSuccess) return e;
+  const int64_t pieces = p.T * (p.H / 8);
+  hipLaunchKernelGGL((i8_combine_kernel<T>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, p, (const float*)(ws + l.y));
+  return hipGetLastError();
 }
 
 }  // namespace
 
 int64_t i8_workspace(int64_t M, int N, int K, bool x16, int sides, int num_cus) {
   return layout(M, N, K, x16, sides, num_cus).bytes;
+}
+
+int64_t i8_experts_workspace(int64_t T, int H, int F, int E, int topk) { return experts_layout(T, H, F, E, topk).bytes; }
+
+hipError_t i8_experts_launch(const ExpertsArgs& a, int num_cus, hipStream_t s) {
+  return a.dtype == GP_DTYPE_BF16 ? experts_run<BF16>(a, num_cus, s) : experts_run<F16>(a, num_cus, s);
 }
 
 hipError_t i8_launch(const I8Args& a, int num_cus, hipStream_t s) {

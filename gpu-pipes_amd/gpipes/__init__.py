@@ -32,7 +32,7 @@ __all__ = [
     "bert_addln_ffn_out", "nerf_a", "nerf_a_out", "pipe_handoff", "handoff_checksums", "phase_timers",
     "probe_mfma", "fill_normal", "residual_norm_out", "residual_norm", "NORMS", "q4_gemm_out",
     "q4_gated_out", "q4", "i8_gemm_out", "i8_gated_out", "i8",
-    "route_out", "SCORES", "GROUP_SCORES",
+    "i8_experts_out", "route_out", "SCORES", "GROUP_SCORES",
 ]
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -135,6 +135,10 @@ def _load():
     L.gp_i8_gemm_out.restype = i32
     L.gp_i8_gated_out.argtypes = [i64, i64, i64] + [vp] * 8 + [i32, vp, vp, i64, i32, vp]
     L.gp_i8_gated_out.restype = i32
+    L.gp_i8_experts_workspace_bytes.argtypes = [i64] * 4 + [i32]
+    L.gp_i8_experts_workspace_bytes.restype = i64
+    L.gp_i8_experts_out.argtypes = [i64] * 4 + [i32] + [vp] * 9 + [i32, vp, vp, vp, i64, i32, vp]
+    L.gp_i8_experts_out.restype = i32
     L.gp_route_out.argtypes = [i64, i64, i32, vp, vp, i32, i32, i32, i32, i32, f32, vp, vp, i32, vp]
     L.gp_route_out.restype = i32
     for name in ("gp_mlp_out", "gp_dlrm_botmlp_out", "gp_dlrm_topmlp_out", "gp_nerf_full_out", "gp_gemm_out",
@@ -1282,3 +1286,67 @@ def route_out(logits, k, bias=None, score="softmax", groups=1, top_groups=1, gro
              top_groups, GROUP_SCORES.get(group_score, group_score), renorm, scale, weights.data_ptr(), ids.data_ptr(),
              _LOGITS[logits.dtype]))
     return weights, ids
+
+
+def i8_experts_out(x, ids, weights, wq_g, scales_g, wq_u, scales_u, wq_d, scales_d, act="silu", r=None, out=None):
+    """The feed-forward block of experts in 8-bit integers (gp_i8_experts_out):
+
+        out[t] = r[t] + sum over j of weights[t, j] * (act(x[t] @ Wg) * (x[t] @ Wu)) @ Wd of expert ids[t, j]
+
+    x, r (None: nothing), out [T, H] float16 or bfloat16; ids int32 and weights float32 [T, k], as route_out gives
+    them; an id outside 0 .. E - 1 adds nothing.  wq_g, wq_u: E packed weights [H, F], wq_d: [F, H] (gpipes.i8.pack
+    of [E, K, N]), scales_g, scales_u float32 [E, F], scales_d [E, H].  Each product is i8_gemm_out's of 16-bit rows,
+    the first half's result rounded to x's type between them.  H and F multiples of 16; T from one token to prompts."""
+    try:
+        dt, dev = x.dtype, x.get_device()
+        T, H = x.shape
+        E, F = scales_g.shape
+        k = ids.shape[1]
+        if out is None:
+            out = torch.empty((T, H), dtype=dt, device=x.device)
+        up, down = (E, -(-F // 16), -(-H // 64), 1024), (E, -(-H // 16), -(-F // 64), 1024)
+        ok = (dt in _DTYPES and dev >= 0 and x.is_contiguous() and H % 16 == 0 and F % 16 == 0
+              and ids.dtype is torch.int32 and ids.get_device() == dev and ids.shape == (T, k) and ids.is_contiguous()
+              and weights.dtype is torch.float32 and weights.get_device() == dev and weights.shape == (T, k)
+              and weights.is_contiguous()
+              and _i8_experts(wq_g, scales_g, up, (E, F), dev) and _i8_experts(wq_u, scales_u, up, (E, F), dev)
+              and _i8_experts(wq_d, scales_d, down, (E, H), dev)
+              and (r is None or (r.dtype is dt and r.get_device() == dev and r.shape == (T, H) and r.is_contiguous()))
+              and out.dtype is dt and out.get_device() == dev and out.shape == (T, H) and out.is_contiguous())
+    except (AttributeError, ValueError, IndexError, TypeError):
+        ok = False
+    if not ok:
+        _check_rows(x)
+        T, H = x.shape
+        _check_input("scales_g", scales_g, dtype=torch.float32)
+        if scales_g.dim() != 2:
+            raise RuntimeError("scales_g must be [E, F]")
+        E, F = scales_g.shape
+        if H < 1 or F < 1 or H % 16 or F % 16:
+            raise RuntimeError(f"H and F must be multiples of 16 (got {H}, {F})")
+        _check_input("ids", ids, dtype=torch.int32)
+        if ids.dim() != 2:
+            raise RuntimeError("ids must be [T, k]")
+        k = ids.shape[1]
+        up, down = (E, *i8.packed_shape(H, F)), (E, *i8.packed_shape(F, H))
+        f32, i8t = torch.float32, torch.int8
+        _misfit(x, [("ids", ids, (T, k), torch.int32), ("weights", weights, (T, k), f32), ("wq_g", wq_g, up, i8t),
+                    ("scales_g", scales_g, (E, F), f32), ("wq_u", wq_u, up, i8t), ("scales_u", scales_u, (E, F), f32),
+                    ("wq_d", wq_d, down, i8t), ("scales_d", scales_d, (E, H), f32), ("r", r, (T, H), x.dtype),
+                    ("out", out, (T, H), x.dtype)])
+    n = lib.gp_i8_experts_workspace_bytes(T, H, F, E, k)
+    if n < 0:
+        _check(n)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    _run_on(dev, lib.gp_i8_experts_out,
+            (T, H, F, E, k, x.data_ptr(), ids.data_ptr(), weights.data_ptr(), wq_g.data_ptr(), scales_g.data_ptr(),
+             wq_u.data_ptr(), scales_u.data_ptr(), wq_d.data_ptr(), scales_d.data_ptr(), ACTS.get(act, act),
+             None if r is None else r.data_ptr(), out.data_ptr(), ws.data_ptr() if n else None, n, _DTYPES[dt]))
+    return out
+
+
+def _i8_experts(wq, scales, blocks, shape, dev):
+    """Whether the tensors of E packed weights fit."""
+    return (wq.dtype is torch.int8 and wq.get_device() == dev and wq.shape == blocks and wq.is_contiguous()
+            and scales.dtype is torch.float32 and scales.get_device() == dev and scales.shape == shape
+            and scales.is_contiguous())

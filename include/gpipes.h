@@ -697,6 +697,40 @@ int gp_route_out(int64_t T, int64_t E, int k, const void* logits, const void* bi
                  int top_groups, int group_score, int renorm, float scale, void* weights, void* ids, int dtype,
                  void* stream);
 
+/* Bytes of workspace that gp_i8_experts_out needs at these sizes; negative: GP_ERR_*. */
+int64_t gp_i8_experts_workspace_bytes(int64_t T, int64_t H, int64_t F, int64_t E, int topk);
+
+/*
+ * The feed-forward block of experts in 8-bit integers, one token to whole prompts:
+ *   out[t] = r[t] + sum over j < topk of weights[t][j] * y(t, ids[t][j]),
+ *   y(t, e) = (act(x[t] Wg_e) * (x[t] Wu_e)) Wd_e,
+ * every product as in gp_i8_gemm_out, with a row of 16 bits: the rows of x, and
+ * what lies between an expert's two halves, rounded to `dtype` first, as
+ * gp_i8_gated_out would store it.  y stays in fp32; it is multiplied and added
+ * in the order of j, then r, and out is rounded once.
+ * x, r (or NULL), out [T, H] of `dtype`; ids int32 and weights float [T, topk],
+ * as gp_route_out gives them.  An id outside 0 .. E - 1 adds nothing, whatever
+ * its weight; an id may occur in a token more than once.
+ * wq_g, wq_u: E weights [H, F], wq_d: E weights [F, H], each packed as in
+ * gp_i8_gemm_out, one after the other; w_scales_g, w_scales_u float [E, F],
+ * w_scales_d float [E, H].  H and F multiples of 16 up to 131056, an expert's
+ * packed weight below 2 GiB, E up to 1024, topk up to 32, T up to 2097152 with
+ * T * H below 2^31.  x, weights of experts, r, out and workspace 16-byte
+ * aligned, everything else 4.
+ * A token that is not finite, or that is not behind an expert's first half, gives NaN in its row of out alone.
+ * workspace: scratch of the call's own, of at least
+ * gp_i8_experts_workspace_bytes.  Calls that may run at the same time, in graphs
+ * too, need workspaces of their own.  Nothing comes back to the host, and the
+ * launches depend on sizes alone: can be captured into a graph, and replayed
+ * with other ids.  out may be r; that it overlaps r otherwise or any other
+ * operand, or that the workspace overlaps one of them, is refused.
+ * No counterpart in the reference.
+ */
+int gp_i8_experts_out(int64_t T, int64_t H, int64_t F, int64_t E, int topk, const void* x, const void* ids,
+                      const void* weights, const void* wq_g, const void* w_scales_g, const void* wq_u,
+                      const void* w_scales_u, const void* wq_d, const void* w_scales_d, int act, const void* r, void* out,
+                      void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
