@@ -220,7 +220,7 @@ int experts_run(const ExpertsArgs& a, int64_t ws_bytes, hipStream_t stream) {
     return fail(GP_ERR_INVALID_ARG, "the workspace must not overlap x, ids, weights, an expert's weight or scales");
   int dev = 0, ncu = 0;
   if ((rc = current_device_info(&dev, &ncu))) return rc;
-  const int64_t need = i8_experts_workspace(a.T, a.H, a.F, a.E, a.topk);
+  const int64_t need = i8_experts_workspace(a.T, a.H, a.F, a.E, a.topk, ncu);
   if (ws_bytes < need)
     return fail(GP_ERR_INVALID_ARG, "workspace_bytes must be at least %lld (got %lld)", (long long)need, (long long)ws_bytes);
   const hipError_t e = i8_experts_launch(a, ncu, stream);
@@ -378,9 +378,12 @@ int gp_route_out(int64_t T, int64_t E, int k, const void* logits, const void* bi
 
 int64_t gp_i8_experts_workspace_bytes(int64_t T, int64_t H, int64_t F, int64_t E, int topk) {
   clear_error();
-  const int rc = experts_check_shape(T, H, F, E, topk);
+  int rc = experts_check_shape(T, H, F, E, topk);
   if (rc) return rc;
-  return T == 0 ? 0 : i8_experts_workspace(T, (int)H, (int)F, (int)E, topk);
+  if (T == 0) return 0;
+  int dev = 0, ncu = 0;
+  if ((rc = current_device_info(&dev, &ncu))) return rc;
+  return i8_experts_workspace(T, (int)H, (int)F, (int)E, topk, ncu);
 }
 
 int gp_i8_experts_out(int64_t T, int64_t H, int64_t F, int64_t E, int topk, const void* x, const void* ids,

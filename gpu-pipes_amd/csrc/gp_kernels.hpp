@@ -371,7 +371,7 @@ struct ExpertsArgs {
   int dtype;
   void* ws;
 };
-int64_t i8_experts_workspace(int64_t T, int H, int F, int E, int topk);
+int64_t i8_experts_workspace(int64_t T, int H, int F, int E, int topk, int num_cus);
 hipError_t i8_experts_launch(const ExpertsArgs& a, int num_cus, hipStream_t stream);
 
 // Tokens' experts and weights (gp_route_out); E up to kRouteMaxE, k up to kRouteMaxK,

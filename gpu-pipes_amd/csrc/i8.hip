@@ -238,6 +238,9 @@ struct I8Group {
   const int* tok;   // of a row: its token
   const int* pair;  // and its pair, token * topk + choice
   int64_t wbytes;   // of an expert's packed weight
+  // Few tokens: every pair a tile by itself, without a plan.
+  const int* ids;
+  int topk, experts;
 };
 
 // ---------------------------------------------------------------------------
@@ -276,8 +279,16 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
   int64_t m0 = (int64_t)blockIdx.y * (16 * MT);
   int rows = p.M - m0 < 16 * MT ? (int)(p.M - m0) : 16 * MT;
   if constexpr (MODE != DENSE) {
-    if ((int)blockIdx.y >= grp.info[0]) return;
-    const TileRec rec = grp.tiles[blockIdx.y];
+    TileRec rec{0, (int)blockIdx.y, 1, 0};
+    if constexpr (XL) {  // a pair; its token's row is the first of p.x
+      rec.expert = grp.ids[blockIdx.y];
+      if ((unsigned)rec.expert >= (unsigned)grp.experts) return;
+      p.x = (const half_t*)p.x + (int64_t)(blockIdx.y / grp.topk) * K;
+      p.M = 1;
+    } else {
+      if ((int)blockIdx.y >= grp.info[0]) return;
+      rec = grp.tiles[blockIdx.y];
+    }
     m0 = rec.row0, rows = rec.rows;
 #pragma unroll
     for (int s = 0; s < S; ++s)
@@ -679,35 +690,47 @@ TilePlan tile_plan(int64_t M, int N, int K, int sides, int num_cus) {
 
 bool on_tiles(int64_t M) { return M > 64; }
 
+// Up to here each token's experts run by themselves.
+constexpr int64_t kTokenRows = 2;
+
 bool own_bytes(int64_t M, int K) { return M <= 4 && K * (M <= 1 ? 1 : M <= 2 ? 2 : 4) <= 16384; }
 
-// mtiles: of 16 mt rows.  A product of experts (MODE) has them from its plan.
+// mtiles: of 16 mt rows.  A product of experts (MODE) has them from its plan; busy: those that are worth counting.
 template <class T, int S, int MODE>
-hipError_t rows_launch(const I8Args& a, const I8Group& g, int mt, int64_t mtiles, bool x16, int num_cus, hipStream_t s) {
+hipError_t rows_launch(const I8Args& a, const I8Group& g, int mt, int64_t mtiles, int64_t busy, bool x16, int num_cus,
+                       hipStream_t s) {
   RowsPlan l{};
   l.xl = x16;
   l.mt = mt;
-  const int tiles = (a.N + 15) / 16 * S, chunks = (a.K + kChunk - 1) / kChunk;
+  const int chunks = (a.K + kChunk - 1) / kChunk, rows = MODE == DENSE ? (int)a.M : 1;
+  const int64_t tiles = (int64_t)((a.N + 15) / 16) * S * busy;
   int per = tiles >= 4 * num_cus ? 4 : tiles >= 2 * num_cus ? 2 : 1;  // tiles a workgroup
   if (per < S) per = S;
   l.nt = per > 2 && l.mt == 1 ? 2 : per;
-  const int ring = rows_ring(l.nt, l.mt, l.xl) * slot_bytes(l.nt, l.mt, l.xl);
-  l.cg = per / l.nt;
-  const int mshift = a.M <= 1 ? 0 : a.M <= 2 ? 1 : 2;
-  l.xstride = (chunks * kChunk + 255) / 256 * 256 + 64;
-  const int xbytes = l.xl ? l.xstride << mshift : 0;
   const int waves = rows_waves(l.nt, l.mt, l.xl);
-  // no more waves than chunks, but for 16-bit x its threads
-  int need = 1;
-  if (l.xl)
+  const int ring = rows_ring(l.nt, l.mt, l.xl) * slot_bytes(l.nt, l.mt, l.xl);
+  const int mshift = rows <= 1 ? 0 : rows <= 2 ? 1 : 2;
+  l.xstride = (chunks * kChunk + 255) / 256 * 256 + 64;
+  int xbytes = 0;
+  if (l.xl) {
+    // the workgroup's threads make the bytes: as many waves as there can be, but no more than chunks and x need
+    int need = 1;
     while (need * kWave * 32 < (a.K << mshift) || need < (1 << mshift)) need *= 2;
-  l.kw = waves / l.cg;
-  while (l.kw > 1 && l.kw / 2 >= chunks && l.kw / 2 * l.cg >= need) l.kw /= 2;
+    xbytes = l.xstride << mshift;
+    l.cg = per / l.nt;
+    l.kw = waves / l.cg;
+    while (l.kw > 1 && l.kw / 2 >= chunks && l.kw / 2 * l.cg >= need) l.kw /= 2;
+  } else {
+    // k over as many waves as fill the chip with eight a CU; workgroups of four waves and more
+    l.kw = waves;
+    while (l.kw > 1 && (l.kw / 2 >= chunks || tiles / l.nt * (l.kw / 2) >= 8 * num_cus)) l.kw /= 2;
+    l.cg = l.kw < 4 ? 4 / l.kw : 1;
+  }
   l.bytes = l.kw * l.cg * ring + xbytes;
 #define GP_CASE(n, m)                                                                          \
   if constexpr (n >= S)                                                                        \
     if (l.nt == n && l.mt == m) {                                                              \
-      if constexpr (m == 1 && MODE == DENSE)                                                   \
+      if constexpr (m == 1 && MODE != DOWN)                                                    \
         if (l.xl) return rows_launch_one<T, S, n, m, true, MODE>(a, g, mtiles, l, mshift, s);  \
       return rows_launch_one<T, S, n, m, false, MODE>(a, g, mtiles, l, mshift, s);             \
     }
@@ -768,7 +791,8 @@ hipError_t launch(I8Args a, int num_cus, hipStream_t s) {
   }
   if (!on_tiles(a.M)) {
     const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
-    return rows_launch<T, S, DENSE>(a, I8Group{}, mt, (a.M + 16 * mt - 1) / (16 * mt), xl, num_cus, s);
+    const int64_t mtiles = (a.M + 16 * mt - 1) / (16 * mt);
+    return rows_launch<T, S, DENSE>(a, I8Group{}, mt, mtiles, mtiles, xl, num_cus, s);
   }
   a.part = (char*)a.ws + l.part;
   const TilePlan plan = tile_plan(a.M, a.N, a.K, S, num_cus);
@@ -865,6 +889,124 @@ __global__ __launch_bounds__(256) void i8_combine_kernel(ExpertsArgs p, const fl
   store8<T>((half_t*)p.out + t * p.H + n, 8, v);
 }
 
+// A few tokens' second half and their sums in one launch: wave (choice, kw) of a
+// token's workgroup multiplies its share of k of its choice's expert with the
+// workgroup's COLS columns, and the choices are added in their order.  With
+// eight columns a workgroup takes half of each block, whole lines still, so that
+// twice as many CUs have work.
+constexpr int kTokenRing = 2;
+constexpr int kTokenSlot = 2048;  // bytes of a wave's ring: 128 k of sixteen columns or 256 of eight
+constexpr int kTokenPieces = 8;   // of eight values a thread makes bytes of
+
+template <class T, int COLS>
+__global__ __launch_bounds__(1024) void i8_token_down_kernel(ExpertsArgs p, const half_t* h, int64_t wbytes, int kwshift,
+                                                            int xstride) {
+  constexpr int KB = 32 / COLS, XP = kTokenPieces;  // blocks of 64 k a slot
+  __shared__ unsigned tops[16];
+  __shared__ float hs[16];
+  __shared__ int part[16][COLS];
+  GP_LDS char* lds = dyn_lds();
+  const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, lg = lane >> 4;
+  const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int KW = 1 << kwshift, kw = wave & (KW - 1), slot = wave >> kwshift;
+  const int F = p.F, K64 = (F + 63) / 64, steps = (K64 + KB - 1) / KB;
+  const int64_t t = blockIdx.y, pair = t * p.topk + slot;
+  const int n0 = xcd_order(blockIdx.x, gridDim.x) * COLS, n16 = n0 >> 4;
+  const int e = p.ids[pair];
+  const bool valid = (unsigned)e < (unsigned)p.E;
+
+  const int tpr = KW * 64, at = (tid - slot * tpr) * 8;
+  u32x4 v[XP];
+  const auto hr = make_rsrc(h + pair * F, valid ? F * 2 : 0);  // what lies there for an id of no expert is not read
+#pragma unroll
+  for (int i = 0; i < XP; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(hr, (at + i * tpr * 8) * 2, 0, 0);
+  const auto wr = make_rsrc((const char*)p.wd + (valid ? e : 0) * wbytes, valid ? (int)wbytes : 0);
+  GP_LDS char* const ring = lds + wave * (kTokenRing * kTokenSlot);
+  // a copy: lane l fetches column l % COLS of block l / (4 COLS)
+  const int lb = lane / (4 * COLS), lp = lane % (4 * COLS);
+  const unsigned wo = (unsigned)(n16 * K64 + lb) * 1024u + (unsigned)((lp / COLS * 16 + (n0 & 15) + lp % COLS) * 16);
+  auto issue = [&](int c, int at) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int b = c * KB + i * (KB / 2);
+      dma16_buf(wr, (int)(b + lb < K64 ? wo + (unsigned)b * 1024u : kNowhere), ring + at * kTokenSlot + i * 1024);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kTokenRing; ++i) issue(kw + i * KW, i);
+
+  unsigned top = 0;
+#pragma unroll
+  for (int i = 0; i < XP; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) top = top2(top, v[i][k]);
+  top = wave_top(top);
+  if (lane == 0) tops[wave] = top;
+  lds_barrier();
+  top = wave_top(tops[(slot << kwshift) + (lane & (KW - 1))]);
+  const RowScale sc = row_scale<T>(top);
+  GP_LDS char* const xl = lds + waves * (kTokenRing * kTokenSlot) + slot * xstride;
+#pragma unroll
+  for (int i = 0; i < XP; ++i) {
+    const int k = at + i * tpr * 8;
+    if (k < F) *(GP_LDS u32x2*)(xl + k) = round8<T>(v[i], sc);
+  }
+  if (at == 0) hs[slot] = sc.scale;
+  lds_barrier();
+
+  i32x4 acc = {};
+  int s = 0;
+  for (int c = kw; c < steps; c += KW) {
+    wait_vmcnt<(kTokenRing - 1) * 2>();
+    compiler_fence();
+    u32x4 a[KB], b[KB];
+#pragma unroll
+    for (int i = 0; i < KB; ++i) {
+      a[i] = *(GP_LDS const u32x4*)(xl + (c * KB + i) * 64 + lg * 16);
+      b[i] = *(GP_LDS const u32x4*)(ring + s * kTokenSlot + (i * 4 * COLS + lg * COLS + (j & (COLS - 1))) * 16);
+    }
+    compiler_fence();
+    __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+    issue(c + kTokenRing * KW, s);
+    s = s + 1 == kTokenRing ? 0 : s + 1;
+#pragma unroll
+    for (int i = 0; i < KB; ++i) acc = mma8(a[i], b[i], acc);
+  }
+  wait_vmcnt<0>();
+  if (lane < COLS) part[wave][lane] = acc[0];  // every row of the operand was the same
+  __syncthreads();
+  const int n = n0 + tid;
+  if (tid < COLS && n < p.H) {
+    float out = 0.f;
+    for (int k = 0; k < p.topk; ++k) {
+      const int id = p.ids[t * p.topk + k];
+      if ((unsigned)id >= (unsigned)p.E) continue;
+      int sum = 0;
+      for (int w = 0; w < KW; ++w) sum += part[(k << kwshift) + w][tid];
+      const float y = (float)sum * p.sd[(int64_t)id * p.H + n] * hs[k];
+      out = __builtin_fmaf(p.weights[t * p.topk + k], y, out);
+    }
+    if (p.r) out += T::val(((const half_t*)p.r)[t * p.H + n]);
+    ((half_t*)p.out)[t * p.H + n] = T::cvt1(out);
+  }
+}
+
+// How a few tokens' second half is laid out; kw 0: it has no room.
+struct TokenPlan {
+  int kw, cols, xstride, bytes;
+};
+TokenPlan token_plan(int64_t T, int H, int F, int topk, int num_cus) {
+  TokenPlan l{};
+  if (T > kTokenRows || topk > 16 || !own_bytes(1, H)) return l;
+  int kw = 1;
+  while (2 * kw * topk <= 16) kw *= 2;
+  l.cols = (int64_t)H / 16 * T >= num_cus ? 16 : 8;
+  l.xstride = (F + 255) / 256 * 256 + 64;
+  l.bytes = topk * (kw * kTokenRing * kTokenSlot + l.xstride);
+  if (F <= kw * 64 * 8 * kTokenPieces && l.bytes <= kRowsLds) l.kw = kw;
+  return l;
+}
+
 // Rows of a tile, by the rows that an expert has on average.
 int experts_tile(int64_t P, int E) {
   const int64_t n = P / E;
@@ -875,7 +1017,7 @@ struct ExpertsLayout {
   int tile;
   int64_t max_tiles, xq, xs, tiles, info, tok, pair, h, hq, hs, y, bytes;
 };
-ExpertsLayout experts_layout(int64_t T, int H, int F, int E, int topk) {
+ExpertsLayout experts_layout(int64_t T, int H, int F, int E, int topk, int num_cus) {
   ExpertsLayout l{};
   const int64_t P = T * topk;
   l.tile = experts_tile(P, E);
@@ -885,6 +1027,10 @@ ExpertsLayout experts_layout(int64_t T, int H, int F, int E, int topk) {
     l.bytes += (n + 255) / 256 * 256;
     return at;
   };
+  if (token_plan(T, H, F, topk, num_cus).kw) {
+    l.h = take(P * F * 2);
+    return l;
+  }
   l.xq = take(T * H);
   l.xs = take(T * 4);
   l.tiles = take(l.max_tiles * (int64_t)sizeof(TileRec));
@@ -899,17 +1045,40 @@ ExpertsLayout experts_layout(int64_t T, int H, int F, int E, int topk) {
 }
 
 template <class T, int S, int MODE>
-hipError_t experts_product(const I8Args& a, const I8Group& g, const ExpertsLayout& l, int num_cus, hipStream_t s) {
-  if (l.tile == 16) return rows_launch<T, S, MODE>(a, g, 1, l.max_tiles, false, num_cus, s);
+hipError_t experts_product(const I8Args& a, const I8Group& g, const ExpertsLayout& l, int64_t pairs, int num_cus,
+                           hipStream_t s) {
+  if (l.tile == 16) {
+    const int64_t busy = pairs < g.experts ? pairs : g.experts;
+    return rows_launch<T, S, MODE>(a, g, 1, l.max_tiles, busy, false, num_cus, s);
+  }
   return tile_launch<T, S, MODE>(a, g, l.max_tiles, TilePlan{l.tile, 1}, s);
 }
 
 template <class T>
 hipError_t experts_run(const ExpertsArgs& p, int num_cus, hipStream_t s) {
   const int64_t P = p.T * p.topk;
-  const ExpertsLayout l = experts_layout(p.T, p.H, p.F, p.E, p.topk);
+  const int64_t up_bytes = (int64_t)((p.F + 15) / 16) * ((p.H + 63) / 64) * 1024;
+  const int64_t down_bytes = (int64_t)((p.H + 15) / 16) * ((p.F + 63) / 64) * 1024;
+  const ExpertsLayout l = experts_layout(p.T, p.H, p.F, p.E, p.topk, num_cus);
   char* const ws = (char*)p.ws;
-  I8Group g{(const TileRec*)(ws + l.tiles), (const int*)(ws + l.info), (const int*)(ws + l.tok), (const int*)(ws + l.pair), 0};
+  const TokenPlan tp = token_plan(p.T, p.H, p.F, p.topk, num_cus);
+  if (tp.kw) {
+    const I8Group g{nullptr, nullptr, nullptr, nullptr, up_bytes, p.ids, p.topk, p.E};
+    const I8Args up{p.T, p.F, p.H, 2, p.x, nullptr, nullptr, {{p.wg, p.sg, nullptr}, {p.wu, p.su, nullptr}},
+                    nullptr, p.act, ws + l.h, p.dtype, nullptr, nullptr};
+    const hipError_t e = rows_launch<T, 2, UP>(up, g, 1, P, P, true, num_cus, s);
+    if (e != hipSuccess) return e;
+    const auto kern = tp.cols == 8 ? &i8_token_down_kernel<T, 8> : &i8_token_down_kernel<T, 16>;
+    if (tp.bytes > 60 * 1024) {
+      const hipError_t e2 = hipFuncSetAttribute((const void*)kern, hipFuncAttributeMaxDynamicSharedMemorySize, kRowsLds);
+      if (e2 != hipSuccess) return e2;
+    }
+    hipLaunchKernelGGL(kern, dim3(p.H / tp.cols, (unsigned)p.T), dim3(p.topk * tp.kw * kWave), tp.bytes, s, p,
+                       (const half_t*)(ws + l.h), down_bytes, __builtin_ctz(tp.kw), tp.xstride);
+    return hipGetLastError();
+  }
+  I8Group g{(const TileRec*)(ws + l.tiles), (const int*)(ws + l.info), (const int*)(ws + l.tok), (const int*)(ws + l.pair), 0,
+            p.ids, p.topk, p.E};
   hipLaunchKernelGGL(i8_plan_kernel, dim3(p.E), dim3(1024), 0, s, p.ids, P, p.E, p.topk, l.tile, (TileRec*)(ws + l.tiles),
                      (int*)(ws + l.info), (int*)(ws + l.tok), (int*)(ws + l.pair));
   hipError_t e = hipGetLastError();
@@ -917,13 +1086,13 @@ hipError_t experts_run(const ExpertsArgs& p, int num_cus, hipStream_t s) {
   if ((e = rows_to_bytes<T>(p.x, p.T, p.H, ws + l.xq, (float*)(ws + l.xs), s)) != hipSuccess) return e;
   I8Args up{p.T, p.F, p.H, 2, nullptr, ws + l.xq, (const float*)(ws + l.xs), {{p.wg, p.sg, nullptr}, {p.wu, p.su, nullptr}},
             nullptr, p.act, ws + l.h, p.dtype, nullptr, nullptr};
-  g.wbytes = (int64_t)((p.F + 15) / 16) * ((p.H + 63) / 64) * 1024;
-  if ((e = experts_product<T, 2, UP>(up, g, l, num_cus, s)) != hipSuccess) return e;
+  g.wbytes = up_bytes;
+  if ((e = experts_product<T, 2, UP>(up, g, l, P, num_cus, s)) != hipSuccess) return e;
   if ((e = rows_to_bytes<T>(ws + l.h, P, p.F, ws + l.hq, (float*)(ws + l.hs), s, g.info + 1)) != hipSuccess) return e;
   I8Args down{P, p.H, p.F, 1, nullptr, ws + l.hq, (const float*)(ws + l.hs), {{p.wd, p.sd, nullptr}, {}},
               nullptr, GP_ACT_NONE, ws + l.y, p.dtype, nullptr, nullptr};
-  g.wbytes = (int64_t)((p.H + 15) / 16) * ((p.F + 63) / 64) * 1024;
-  if ((e = experts_product<F16, 1, DOWN>(down, g, l, num_cus, s)) != hipSuccess) return e;
+  g.wbytes = down_bytes;
+  if ((e = experts_product<F16, 1, DOWN>(down, g, l, P, num_cus, s)) != hipSuccess) return e;
   const int64_t pieces = p.T * (p.H / 8);
   hipLaunchKernelGGL((i8_combine_kernel<T>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, p, (const float*)(ws + l.y));
   return hipGetLastError();
@@ -935,7 +1104,9 @@ int64_t i8_workspace(int64_t M, int N, int K, bool x16, int sides, int num_cus) 
   return layout(M, N, K, x16, sides, num_cus).bytes;
 }
 
-int64_t i8_experts_workspace(int64_t T, int H, int F, int E, int topk) { return experts_layout(T, H, F, E, topk).bytes; }
+int64_t i8_experts_workspace(int64_t T, int H, int F, int E, int topk, int num_cus) {
+  return experts_layout(T, H, F, E, topk, num_cus).bytes;
+}
 
 hipError_t i8_experts_launch(const ExpertsArgs& a, int num_cus, hipStream_t s) {
   return a.dtype == GP_DTYPE_BF16 ? experts_run<BF16>(a, num_cus, s) : experts_run<F16>(a, num_cus, s);

@@ -1334,7 +1334,8 @@ def i8_experts_out(x, ids, weights, wq_g, scales_g, wq_u, scales_u, wq_d, scales
                     ("scales_g", scales_g, (E, F), f32), ("wq_u", wq_u, up, i8t), ("scales_u", scales_u, (E, F), f32),
                     ("wq_d", wq_d, down, i8t), ("scales_d", scales_d, (E, H), f32), ("r", r, (T, H), x.dtype),
                     ("out", out, (T, H), x.dtype)])
-    n = lib.gp_i8_experts_workspace_bytes(T, H, F, E, k)
+    with _on(x):
+        n = lib.gp_i8_experts_workspace_bytes(T, H, F, E, k)
     if n < 0:
         _check(n)
     ws = torch.empty(n, dtype=torch.uint8, device=x.device)

@@ -697,7 +697,7 @@ int gp_route_out(int64_t T, int64_t E, int k, const void* logits, const void* bi
                  int top_groups, int group_score, int renorm, float scale, void* weights, void* ids, int dtype,
                  void* stream);
 
-/* Bytes of workspace that gp_i8_experts_out needs at these sizes; negative: GP_ERR_*. */
+/* Bytes of workspace that gp_i8_experts_out needs at these sizes on the current device; negative: GP_ERR_*. */
 int64_t gp_i8_experts_workspace_bytes(int64_t T, int64_t H, int64_t F, int64_t E, int topk);
 
 /*
