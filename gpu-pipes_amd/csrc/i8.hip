@@ -25,6 +25,9 @@
 #include "gp_kernels.hpp"
 #include "row_ops.hpp"
 
+// No sum is fused with a product that the source does not fuse: what one kernel rounds, every kernel rounds.
+#pragma clang fp contract(off)
+
 namespace gp {
 namespace {
 
@@ -179,16 +182,33 @@ hipError_t rows_to_bytes(const void* x, int64_t M, int K, char* q, float* xs, hi
 // The stages' activations and SiLU; a NaN stays one under every one of them.
 __device__ __forceinline__ float act8(float v, int act) { return act == GP_ACT_RELU ? (v < 0.f ? 0.f : v) : apply_act_ext(v, act); }
 
-// n of eight neighbouring outputs of a row from column n: the sums a (and u of
-// the second weight), already times both scales.
-template <class T, int S>
-__device__ __forceinline__ void finish8(const I8Args& p, int64_t m, int n, int cnt, float (&v)[8], float (&u)[8]) {
-  float t[8];
-  if (p.side[0].b) {
-    load8<T>((const half_t*)p.side[0].b + n, cnt, t);
+// The first cnt of eight values from column n of a row of N, zeros behind them.
+// Loads under a condition each are waited for one by one, so a row's end is read
+// with what lies before it (and a scale with zeros behind N, by the buffer's range).
+template <class T>
+__device__ __forceinline__ void load_row8(const half_t* row, int n, int cnt, int N, float (&f)[8]) {
+  if (N >= 8)
+    load8<T, true>(row + n, cnt, f);
+  else
+    load8<T>(row + n, cnt, f);
+}
+__device__ __forceinline__ void load_scales8(const float* s, int n, int N, float (&f)[8]) {
+  const auto r = make_rsrc(s, N * 4);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += t[e];
+  for (int h = 0; h < 2; ++h) {
+    const f4 v = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, (n + 4 * h) * 4, 0, 0));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[4 * h + e] = v[e];
   }
+}
+
+// cnt of eight neighbouring outputs of a row from column n: v (and u of the second
+// weight) the sums times both scales, b the biases, zeros where there are none.
+template <class T, int S>
+__device__ __forceinline__ void finish8(const I8Args& p, int64_t m, int n, int cnt, float (&v)[8], float (&u)[8],
+                                        const float (&b)[S][8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += b[0][e];
   if (p.act == GP_ACT_RELU) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
@@ -196,16 +216,12 @@ __device__ __forceinline__ void finish8(const I8Args& p, int64_t m, int n, int c
     apply_act8(v, p.act);
   }
   if constexpr (S == 2) {
-    if (p.side[1].b) {
-      load8<T>((const half_t*)p.side[1].b + n, cnt, t);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) u[e] += t[e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= u[e];
+    for (int e = 0; e < 8; ++e) v[e] *= u[e] + b[1][e];
   }
   if (p.r) {
-    load8<T>((const half_t*)p.r + m * p.N + n, cnt, t);
+    float t[8];
+    load_row8<T>((const half_t*)p.r + m * p.N, n, cnt, p.N, t);
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] += t[e];
   }
@@ -215,9 +231,9 @@ __device__ __forceinline__ void finish8(const I8Args& p, int64_t m, int n, int c
 // One output.
 template <class T, int S>
 __device__ __forceinline__ void finish1(const I8Args& p, int64_t m, int n, float v, float u) {
-  if (p.side[0].b) v += T::val(((const half_t*)p.side[0].b)[n]);
+  v += p.side[0].b ? T::val(((const half_t*)p.side[0].b)[n]) : 0.f;
   v = act8(v, p.act);
-  if constexpr (S == 2) v *= p.side[1].b ? u + T::val(((const half_t*)p.side[1].b)[n]) : u;
+  if constexpr (S == 2) v *= u + (p.side[1].b ? T::val(((const half_t*)p.side[1].b)[n]) : 0.f);
   if (p.r) v += T::val(((const half_t*)p.r)[m * p.N + n]);
   ((half_t*)p.out)[m * p.N + n] = T::cvt1(v);
 }
@@ -473,8 +489,12 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
   constexpr int XB = BM * kChunk, SLOT = XB + BN * kChunk;
   constexpr int SB = BN / 16 / S;  // blocks of a weight in a chunk's half
   static_assert(NW % 2 == 0 && XI * 8 * NW == BM && WI * 8 * NW == BN && WI % 2 == 0, "copies");
-  __shared__ __attribute__((aligned(1024))) char ringmem[R * SLOT];
-  GP_LDS char* const lds = (GP_LDS char*)ringmem;
+  // One array for all: with several the compiler waits for every copy in flight before it reads the ring
+  // (64 x 64: 0.6 us a chunk instead of 0.29).
+  __shared__ __attribute__((aligned(1024))) char mem[R * SLOT + BM * (MODE == DOWN ? 8 : 4)];
+  GP_LDS char* const lds = (GP_LDS char*)mem;
+  GP_LDS float* const rowscale = (GP_LDS float*)(lds + R * SLOT);
+  GP_LDS int* const rowpair = (GP_LDS int*)(lds + R * SLOT + BM * 4);
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
   const int N = p.N, K = p.K, K64 = (K + 63) / 64, N16 = (N + 15) / 16, chunks = (K + kChunk - 1) / kChunk;
@@ -540,39 +560,72 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
     }
 
   const int per = (chunks + gridDim.y - 1) / gridDim.y, c0 = blockIdx.y * per, c1 = c0 + per < chunks ? c0 + per : chunks;
+  // A chunk is multiplied in steps: half of its k, and with eight row tiles half
+  // of them.  A step's operands are read from LDS while the step before it is
+  // multiplied, a chunk's first ones too: at its last step every operand of the
+  // chunk is in registers, so that behind one barrier its slot takes the chunk R
+  // further on and the next slot is read.
+  constexpr int G = MT > 4 ? 2 : 1, MG = MT / G, STEPS = 2 * G;
   i32x4 acc[S][NS][MT] = {};
-#pragma unroll
-  for (int i = 0; i < R - 1; ++i) issue(c0 + i, c1, i);
-  int at = 0;
-#pragma unroll 1
-  for (int c = c0; c < c1; ++c) {
-    wait_vmcnt<(R - 2) * NI>();
-    lds_barrier();
-    const int next = at == 0 ? R - 1 : at - 1;
-    issue(c + R - 1, c1, next);
-    GP_LDS const char* slot = lds + at * SLOT;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      u32x4 w[S][NS], x[MT];
+  u32x4 w[2][S][NS], x[2][MG];
+  auto read = [&](int q, GP_LDS const char* slot) {  // step q of the chunk in slot
+    const int h = q / G;
+    if (q % G == 0) {
 #pragma unroll
       for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int t = 0; t < NS; ++t) w[s][t] = *(GP_LDS const u32x4*)(slot + wa[s][t] + h * 1024);
+        for (int t = 0; t < NS; ++t) w[h][s][t] = *(GP_LDS const u32x4*)(slot + wa[s][t] + h * 1024);
+    }
 #pragma unroll
-      for (int m = 0; m < MT; ++m) x[m] = *(GP_LDS const u32x4*)(slot + xa[h] + m * 2048);
+    for (int m = 0; m < MG; ++m) x[q & 1][m] = *(GP_LDS const u32x4*)(slot + xa[h] + (q % G * MG + m) * 2048);
+  };
+  // the rows' scales and pairs first: what follows is not waited for with them
+  float rs = 0.f;
+  int rp = 0;
+  if (tid < rows) {
+    rs = p.xs[MODE == UP ? g.tok[m0 + tid] : m0 + tid];
+    if (MODE == DOWN) rp = g.pair[m0 + tid];
+  }
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+  for (int i = 0; i < R; ++i) issue(c0 + i, c1, i);
+  if (tid < BM) {
+    rowscale[tid] = rs;
+    if (MODE == DOWN) rowpair[tid] = rp;
+  }
+  wait_vmcnt<(R - 1) * NI>();
+  lds_barrier();
+  read(0, lds);
+  int at = 0;
+#pragma unroll 1
+  for (int c = c0; c < c1; ++c) {
+    GP_LDS const char* slot = lds + at * SLOT;
+#pragma unroll
+    for (int q = 0; q < STEPS; ++q) {
+      if (q + 1 < STEPS) {
+        read(q + 1, slot);
+      } else {
+        wait_vmcnt<(R - 2) * NI>();
+        lds_barrier();
+        issue(c + R, c1, at);
+        at = at + 1 == R ? 0 : at + 1;
+        read(0, lds + at * SLOT);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int m = 0; m < MG; ++m)
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
-          for (int t = 0; t < NS; ++t) acc[s][t][m] = mma8(w[s][t], x[m], acc[s][t][m]);
+          for (int t = 0; t < NS; ++t)
+            acc[s][t][q % G * MG + m] = mma8(w[q / G][s][t], x[q & 1][m], acc[s][t][q % G * MG + m]);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    at = at + 1 == R ? 0 : at + 1;
   }
+  wait_vmcnt<0>();
 
-  // A lane's columns: 4 NS from n0 of each weight, of row j of each row tile.
-  const int n0 = nb0 * 16 + wn * (16 * NS) + 4 * NS * lg;
   if (MODE == DENSE && gridDim.y > 1) {
+    // a lane's columns: 4 NS from n0 of each weight, of row j of each row tile
+    const int n0 = nb0 * 16 + wn * (16 * NS) + 4 * NS * lg;
     int* const part = (int*)p.part + (int64_t)blockIdx.y * S * p.M * N;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
@@ -594,36 +647,64 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
     }
     return;
   }
-  constexpr int W8 = NS >= 2 ? 2 : 1;  // sums of up to eight columns at a time
+  // Out through LDS, a wave's sums through its own part of it: eight neighbouring
+  // columns of a row a lane then, whole lines a wave, and a short rolled loop with
+  // the epilogue once (code is fetched from memory: with the epilogue unrolled over
+  // a lane's sums, a tile of 256 x 256 took 18 us besides its chunks).  Piece c of
+  // four sums of row r lies at c ^ r.
+  constexpr int OC = 16 * NS, NP = 4 * NS * S;                       // a wave's columns of out; pieces a row
+  constexpr int HM = NW * MT * 16 * NP * 16 > R * SLOT ? MT / 2 : MT;  // row tiles at a time
+  static_assert(NW * HM * 16 * NP * 16 <= R * SLOT, "the sums fit the ring");
+  constexpr int LPR = OC / 8, RPI = 64 / LPR;  // lanes a row, rows a turn
+  GP_LDS char* const mine = lds + wave * (HM * 16 * NP * 16);
+  const int oc = lane % LPR, orow = lane / LPR;
+  const int n = nb0 * 16 + wn * OC + oc * 8, cnt = N - n < 8 ? N - n : 8;
+  float sc[S][8], b[S][8];
 #pragma unroll
-  for (int c = 0; c < NS / W8; ++c) {
-    const int n = n0 + 4 * W8 * c, cnt = N - n < 4 * W8 ? N - n : 4 * W8;
-    if (cnt <= 0) continue;
-    float sc[S][8] = {};
+  for (int s = 0; s < S; ++s) {
+    load_scales8(p.side[s].s, n, N, sc[s]);
+    if (MODE == DENSE && p.side[s].b) {
+      load_row8<T>((const half_t*)p.side[s].b, n, cnt, N, b[s]);
+    } else {
 #pragma unroll
-    for (int s = 0; s < S; ++s)
+      for (int e = 0; e < 8; ++e) b[s][e] = 0.f;
+    }
+  }
+  lds_barrier();  // every wave is done with the ring
 #pragma unroll
-      for (int e = 0; e < 4 * W8; ++e)
-        if (e < cnt) sc[s][e] = p.side[s].s[n + e];
+  for (int half = 0; half < MT / HM; ++half) {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int row = wm * MT * 16 + m * 16 + j;
-      if (row >= rows) continue;
-      const float xsc = p.xs[MODE == UP ? g.tok[m0 + row] : m0 + row];
-      float v[8] = {}, u[8] = {};
+    for (int m = 0; m < HM; ++m)
 #pragma unroll
-      for (int t = 0; t < W8; ++t)
+      for (int s = 0; s < S; ++s)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[4 * t + e] = (float)acc[0][W8 * c + t][m][e] * sc[0][4 * t + e] * xsc;
-          if (S == 2) u[4 * t + e] = (float)acc[S - 1][W8 * c + t][m][e] * sc[S - 1][4 * t + e] * xsc;
+        for (int t = 0; t < NS; ++t)
+          *(GP_LDS i32x4*)(mine + (m * 16 + j) * (NP * 16) + (((s * 4 * NS + NS * lg + t) ^ (j & (NP - 1))) << 4)) =
+              acc[s][t][half * HM + m];
+    const int row0 = wm * MT * 16 + half * HM * 16;
+#pragma unroll 1
+    for (int it = 0; it < HM * 16; it += RPI) {
+      const int lrow = it + orow, row = row0 + lrow;
+      if (row >= rows || cnt <= 0) continue;
+      const float xsc = rowscale[row];
+      float v[8], u[8];
+      auto take = [&](int s, float (&to)[8]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const i32x4 a = *(GP_LDS const i32x4*)(mine + lrow * (NP * 16) +
+                                                 (((s * 4 * NS + 2 * oc + h) ^ (lrow & (NP - 1))) << 4));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) to[4 * h + e] = (float)a[e] * sc[s][4 * h + e] * xsc;
         }
+      };
+      take(0, v);
       if constexpr (MODE == DOWN) {  // N a multiple of 16 here
-        float* const to = (float*)p.out + (int64_t)g.pair[m0 + row] * N + n;
-#pragma unroll
-        for (int t = 0; t < W8; ++t) *(f4*)(to + 4 * t) = f4{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]};
+        float* const to = (float*)p.out + (int64_t)rowpair[row] * N + n;
+        *(f4*)to = f4{v[0], v[1], v[2], v[3]};
+        *(f4*)(to + 4) = f4{v[4], v[5], v[6], v[7]};
       } else {
-        finish8<T, S>(p, m0 + row, n, cnt, v, u);
+        if constexpr (S == 2) take(1, u);
+        finish8<T, S>(p, m0 + row, n, cnt, v, u, b);
       }
     }
   }
@@ -654,13 +735,18 @@ __global__ __launch_bounds__(256) void i8_join_kernel(I8Args p, int parts) {
       }
     }
   const float xsc = p.xs[m];
-  float v[8], u[8];
+  float v[8], u[8], sc[S][8], b[S][8] = {};
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    load_scales8(p.side[s].s, n, p.N, sc[s]);
+    if (p.side[s].b) load_row8<T>((const half_t*)p.side[s].b, n, cnt, p.N, b[s]);
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    v[e] = e < cnt ? (float)a[0][e] * p.side[0].s[n + e] * xsc : 0.f;
-    u[e] = S == 2 && e < cnt ? (float)a[S - 1][e] * p.side[S - 1].s[n + e] * xsc : 0.f;
+    v[e] = (float)a[0][e] * sc[0][e] * xsc;
+    u[e] = (float)a[S - 1][e] * sc[S - 1][e] * xsc;
   }
-  finish8<T, S>(p, m, n, cnt, v, u);
+  finish8<T, S>(p, m, n, cnt, v, u, b);
 }
 
 // ---------------------------------------------------------------------------
