@@ -498,17 +498,20 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
   const int N = p.N, K = p.K, K64 = (K + 63) / 64, N16 = (N + 15) / 16, chunks = (K + kChunk - 1) / kChunk;
-  // Neighbours of one XCD take eight row tiles of a column tile, then of the next.
-  const int id = xcd_order(blockIdx.x, gridDim.x);
+  // Neighbours of one XCD take eight row tiles of a column tile, then of the
+  // next.  Experts' tiles are counted by the plan, and the launch has workgroups for the most that there can be.
+  if constexpr (MODE != DENSE) {
+    mtiles = g.info[0];
+    if ((int)blockIdx.x >= mtiles * ntiles) return;
+  }
+  const int id = xcd_order(blockIdx.x, MODE == DENSE ? (int)gridDim.x : mtiles * ntiles);
   const int gm0 = id / (8 * ntiles) * 8, rest = id % (8 * ntiles);
   const int gm = mtiles - gm0 < 8 ? mtiles - gm0 : 8;
   int64_t m0 = (int64_t)(gm0 + rest % gm) * BM;
   const int nb0 = rest / gm * SB;  // first block of columns
   int rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
   if constexpr (MODE != DENSE) {
-    const int ti = gm0 + rest % gm;
-    if (ti >= g.info[0]) return;
-    const TileRec rec = g.tiles[ti];
+    const TileRec rec = g.tiles[gm0 + rest % gm];
     m0 = rec.row0, rows = rec.rows;
 #pragma unroll
     for (int s = 0; s < S; ++s)
@@ -559,7 +562,9 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
       wa[s][t] = XB + l * 2048 + (((lg * 16 + (n & 15)) ^ (4 * (l & 3))) << 4);
     }
 
-  const int per = (chunks + gridDim.y - 1) / gridDim.y, c0 = blockIdx.y * per, c1 = c0 + per < chunks ? c0 + per : chunks;
+  const int per = (chunks + gridDim.y - 1) / gridDim.y;
+  int c0 = blockIdx.y * per;
+  const int c1 = c0 + per < chunks ? c0 + per : chunks;
   // A chunk is multiplied in steps: half of its k, and with eight row tiles half
   // of them.  A step's operands are read from LDS while the step before it is
   // multiplied, a chunk's first ones too: at its last step every operand of the
@@ -596,6 +601,16 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
   lds_barrier();
   read(0, lds);
   int at = 0;
+  if (wm * MT * 16 >= rows) {  // a wave behind the last row only copies
+#pragma unroll 1
+    for (int c = c0; c < c1; ++c) {
+      wait_vmcnt<(R - 2) * NI>();
+      lds_barrier();
+      issue(c + R, c1, at);
+      at = at + 1 == R ? 0 : at + 1;
+    }
+    c0 = c1;
+  }
 #pragma unroll 1
   for (int c = c0; c < c1; ++c) {
     GP_LDS const char* slot = lds + at * SLOT;
@@ -756,17 +771,28 @@ struct TilePlan {
   int size, parts;  // 64, 128 or 256; parts of k
 };
 
+// The time of a product of `tiles` tiles on tiles, in us: a chunk takes one
+// workgroup of a CU `alone`, and the two that share a CU `pair` (256 x 256: has
+// a CU by itself, and takes longer where it fills the chip, whose power is then the limit),
+// and what is not chunks takes `fixed` a turn.  Measured, K 4,096 (M x N: 64,
+// 128, 256):  512 x 4,096 16.4, 24.5, 52;  1,024 x 4,096 29.8, 27.1, 52.7;
+// 4,096 x 4,096 108, 75, 64;  the estimate: 16.5, 25.5, 49.6;  29.6, 25.5, 49.6;  107, 75, 64.
+float tile_time(int size, int64_t tiles, int chunks, int num_cus) {
+  const int64_t n = (tiles + num_cus - 1) / num_cus;  // workgroups of the fullest CU
+  if (size == 256) return (float)n * (8.f + (float)chunks * (tiles * 2 > num_cus ? 1.74f : 1.3f));
+  const float alone = size == 128 ? 0.64f : 0.2f, pair = size == 128 ? 1.05f : 0.4f;
+  return 4.f + (float)(n / 2 + n % 2) + (float)chunks * ((float)(n / 2) * pair + (float)(n % 2) * alone);
+}
+
 TilePlan tile_plan(int64_t M, int N, int K, int sides, int num_cus) {
   const int chunks = (K + kChunk - 1) / kChunk;
   TilePlan best{256, 1};
   float least = 0.f;
   for (int size : {256, 128, 64}) {
     const int64_t cols = size / sides, tiles = (M + size - 1) / size * ((N + cols - 1) / cols);
-    const int fit = size == 256 ? 1 : 2;  // workgroups a CU
-    const float step = size == 256 ? 1.6f : size == 128 ? 0.5f : 0.25f;
-    for (int parts = 1; parts <= 8 && parts <= chunks; ++parts) {
-      const int64_t turns = (tiles * parts + (int64_t)fit * num_cus - 1) / ((int64_t)fit * num_cus);
-      float t = (float)((chunks + parts - 1) / parts + 3) * step * (float)turns;
+    for (int parts = 1; parts <= 16 && parts <= chunks; ++parts) {
+      float t = tile_time(size, tiles * parts, (chunks + parts - 1) / parts, num_cus);
+      // the second kernel, and the sums' way to memory and back
       if (parts > 1) t += 3.f + (float)parts * (float)M * (float)N * (float)sides * 8.f / 4e6f;
       if (least == 0.f || t < least) best = TilePlan{size, parts}, least = t;
     }
@@ -774,7 +800,17 @@ TilePlan tile_plan(int64_t M, int N, int K, int sides, int num_cus) {
   return best;
 }
 
-bool on_tiles(int64_t M) { return M > 64; }
+// Products that run on tiles: up to 64 rows those whose x the kernel for few rows
+// would read for too many columns.  In us, on tiles / by the kernel for few rows:
+//   32 rows: 4,096 columns from 4,096 k 10.8 / 6.5, from 16,384 17.1 / 13.4, 16,384 from 4,096 13.0 / 16.3,
+//            2 x 16,384 28.7 / 36.7
+//   48 and 64 rows: 4,096 from 4,096 9.7 / 9.2, 8,192 from 8,192 16.9 / 18.4, 16,384 from 4,096 13.2 / 19.3,
+//            2 x 8,192 from 2,048 12.4 / 15.6, 2 x 16,384 from 4,096 29.6 / 43.0
+//   16 rows: 8,192 from 8,192 18.5 / 15.2, 16,384 from 4,096 12.7 / 12.9
+bool on_tiles(int64_t M, int N, int sides) {
+  const int64_t n = (int64_t)N * sides;
+  return M > 64 || (M > 32 && n > 4096) || (M > 16 && n > 8192);
+}
 
 // Up to here each token's experts run by themselves.
 constexpr int64_t kTokenRows = 2;
@@ -858,7 +894,7 @@ Layout layout(int64_t M, int N, int K, bool x16, int sides, int num_cus) {
     l.part = (l.xs + M * 4 + 255) / 256 * 256;
   }
   l.bytes = l.part;
-  if (on_tiles(M)) {
+  if (on_tiles(M, N, sides)) {
     const TilePlan p = tile_plan(M, N, K, sides, num_cus);
     if (p.parts > 1) l.bytes += (int64_t)p.parts * sides * M * N * 4;
   }
@@ -875,7 +911,7 @@ hipError_t launch(I8Args a, int num_cus, hipStream_t s) {
     const hipError_t e = rows_to_bytes<T>(a.x, a.M, a.K, (char*)a.ws, (float*)a.xs, s);
     if (e != hipSuccess) return e;
   }
-  if (!on_tiles(a.M)) {
+  if (!on_tiles(a.M, a.N, S)) {
     const int mt = a.M <= 16 ? 1 : a.M <= 32 ? 2 : 4;
     const int64_t mtiles = (a.M + 16 * mt - 1) / (16 * mt);
     return rows_launch<T, S, DENSE>(a, I8Group{}, mt, mtiles, mtiles, xl, num_cus, s);
@@ -897,54 +933,74 @@ hipError_t launch(I8Args a, int num_cus, hipStream_t s) {
 // ---------------------------------------------------------------------------
 
 // One workgroup an expert: counts of all experts (whole numbers, in LDS), where
-// the expert's rows and tiles begin, and its pairs in their order.
+// the expert's rows and tiles begin, and its pairs in their order.  Whole tiles
+// come first and the experts' last, shorter ones behind all of them.  Loads of
+// ids are in batches, and up to 8,192 pairs stay in registers for the second
+// pass: one after the other they were 12 us for 8,192 pairs of 8 experts.
 __global__ __launch_bounds__(1024) void i8_plan_kernel(const int* ids, int64_t P, int E, int topk, int tile, TileRec* tiles,
                                                       int* info, int* tok, int* pair) {
+  constexpr int B = 8, SUMS = 6;
   __shared__ int count[kExpertsMaxE];
-  __shared__ int own[16], sums[16][4];
+  __shared__ int own[16], sums[16][SUMS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e = blockIdx.x;
   if (tid < E) count[tid] = 0;
   __syncthreads();
   const int64_t seg = ((P + 15) / 16 + 63) / 64 * 64, lo = wave * seg, hi = lo + seg < P ? lo + seg : P;
+  const auto r = make_rsrc(ids, (int)(P * 4));
+  int id[B];
+  auto load = [&](int64_t base) {
+#pragma unroll
+    for (int q = 0; q < B; ++q) id[q] = (int)__builtin_amdgcn_raw_buffer_load_b32(r, (int)((base + q * 64 + lane) * 4), 0, 0);
+#pragma unroll
+    for (int q = 0; q < B; ++q) id[q] = base + q * 64 + lane < hi ? id[q] : -1;
+  };
   int mine = 0;
-  for (int64_t i = lo; i < hi; i += 64) {
-    const int id = i + lane < hi ? ids[i + lane] : -1;
-    if ((unsigned)id < (unsigned)E) atomicAdd(&count[id], 1);
-    mine += __popcll(__ballot(id == e));
+  for (int64_t base = lo; base < hi; base += B * 64) {
+    load(base);
+#pragma unroll
+    for (int q = 0; q < B; ++q) {
+      if ((unsigned)id[q] < (unsigned)E) atomicAdd(&count[id[q]], 1);
+      mine += __popcll(__ballot(id[q] == e));
+    }
   }
   if (lane == 0) own[wave] = mine;
   __syncthreads();
-  // rows and tiles of the experts before this one, and of all
-  const int c = tid < E ? count[tid] : 0, n = (c + tile - 1) / tile;
-  int v[4] = {tid < e ? c : 0, tid < e ? n : 0, c, n};
+  // of the experts before this one, and of all: rows, whole tiles, shorter ones
+  const int c = tid < E ? count[tid] : 0, n = c / tile, m = c % tile ? 1 : 0;
+  const bool before = tid < e;
+  int v[SUMS] = {before ? c : 0, before ? n : 0, before ? m : 0, c, n, m};
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
+  for (int k = 0; k < SUMS; ++k) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) v[k] += __shfl_xor(v[k], d);
     if (lane == 0) sums[wave][k] = v[k];
   }
   __syncthreads();
-  int row0 = 0, tile0 = 0, allrows = 0, alltiles = 0, before = 0;
+  int t[SUMS] = {}, at = 0;
 #pragma unroll
   for (int w = 0; w < 16; ++w) {
-    row0 += sums[w][0], tile0 += sums[w][1], allrows += sums[w][2], alltiles += sums[w][3];
-    before += w < wave ? own[w] : 0;
+#pragma unroll
+    for (int k = 0; k < SUMS; ++k) t[k] += sums[w][k];
+    at += w < wave ? own[w] : 0;
   }
-  if (e == 0 && tid == 0) info[0] = alltiles, info[1] = allrows;
-  const int rows = count[e];
-  for (int i = tid; i * tile < rows; i += 1024)
-    tiles[tile0 + i] = TileRec{e, row0 + i * tile, rows - i * tile < tile ? rows - i * tile : tile, 0};
+  const int row0 = t[0], rows = count[e], whole = rows / tile;
+  if (e == 0 && tid == 0) info[0] = t[4] + t[5], info[1] = t[3];
+  for (int i = tid; i < whole; i += 1024) tiles[t[1] + i] = TileRec{e, row0 + i * tile, tile, 0};
+  if (tid == 0 && rows % tile) tiles[t[4] + t[2]] = TileRec{e, row0 + whole * tile, rows % tile, 0};
   if (mine == 0) return;
-  int at = row0 + before;
-  for (int64_t i = lo; i < hi; i += 64) {
-    const bool hit = i + lane < hi && ids[i + lane] == e;
-    const unsigned long long b = __ballot(hit);
-    if (hit) {
-      const int to = at + __popcll(b & ((1ull << lane) - 1));
-      tok[to] = (int)((i + lane) / topk);
-      pair[to] = (int)(i + lane);
+  at += row0;
+  for (int64_t base = lo; base < hi; base += B * 64) {
+    if (seg > B * 64) load(base);
+#pragma unroll
+    for (int q = 0; q < B; ++q) {
+      const unsigned long long b = __ballot(id[q] == e);
+      if (id[q] == e) {
+        const int to = at + __popcll(b & ((1ull << lane) - 1)), p = (int)(base + q * 64 + lane);
+        tok[to] = p / topk;
+        pair[to] = p;
+      }
+      at += __popcll(b);
     }
-    at += __popcll(b);
   }
 }
 
