@@ -254,6 +254,7 @@ struct I8Group {
   const int* tok;   // of a row: its token
   const int* pair;  // and its pair, token * topk + choice
   int64_t wbytes;   // of an expert's packed weight
+  int shift;        // a tile of the plan is 2^shift of the product's
   // Few tokens: every pair a tile by itself, without a plan.
   const int* ids;
   int topk, experts;
@@ -489,55 +490,100 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
   constexpr int XB = BM * kChunk, SLOT = XB + BN * kChunk;
   constexpr int SB = BN / 16 / S;  // blocks of a weight in a chunk's half
   static_assert(NW % 2 == 0 && XI * 8 * NW == BM && WI * 8 * NW == BN && WI % 2 == 0, "copies");
+  static_assert(BM <= 64 * NW && BN <= 64 * NW, "a thread for each row and column");
   // One array for all: with several the compiler waits for every copy in flight before it reads the ring
   // (64 x 64: 0.6 us a chunk instead of 0.29).
-  __shared__ __attribute__((aligned(1024))) char mem[R * SLOT + BM * (MODE == DOWN ? 8 : 4)];
+  __shared__ __attribute__((aligned(1024))) char mem[R * SLOT + BN * 8 + BM * (MODE == DOWN ? 8 : 4)];
   GP_LDS char* const lds = (GP_LDS char*)mem;
-  GP_LDS float* const rowscale = (GP_LDS float*)(lds + R * SLOT);
-  GP_LDS int* const rowpair = (GP_LDS int*)(lds + R * SLOT + BM * 4);
+  GP_LDS float* const colscale = (GP_LDS float*)(lds + R * SLOT);  // of the tile's columns, a weight's after the other's
+  GP_LDS float* const colbias = colscale + BN;
+  GP_LDS float* const rowscale = colbias + BN;
+  GP_LDS int* const rowpair = (GP_LDS int*)(rowscale + BM);
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, lg = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wave % WN, wm = wave / WN;
   const int N = p.N, K = p.K, K64 = (K + 63) / 64, N16 = (N + 15) / 16, chunks = (K + kChunk - 1) / kChunk;
-  // Neighbours of one XCD take eight row tiles of a column tile, then of the
-  // next.  Experts' tiles are counted by the plan, and the launch has workgroups for the most that there can be.
-  if constexpr (MODE != DENSE) {
-    mtiles = g.info[0];
-    if ((int)blockIdx.x >= mtiles * ntiles) return;
-  }
-  const int id = xcd_order(blockIdx.x, MODE == DENSE ? (int)gridDim.x : mtiles * ntiles);
-  const int gm0 = id / (8 * ntiles) * 8, rest = id % (8 * ntiles);
-  const int gm = mtiles - gm0 < 8 ? mtiles - gm0 : 8;
-  int64_t m0 = (int64_t)(gm0 + rest % gm) * BM;
-  const int nb0 = rest / gm * SB;  // first block of columns
-  int rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
-  if constexpr (MODE != DENSE) {
-    const TileRec rec = g.tiles[gm0 + rest % gm];
-    m0 = rec.row0, rows = rec.rows;
-#pragma unroll
-    for (int s = 0; s < S; ++s)
-      p.side[s].wq = (const char*)p.side[s].wq + rec.expert * g.wbytes, p.side[s].s += (int64_t)rec.expert * N;
-  }
-  const auto xr = MODE == UP ? make_rsrc(p.xq, (int)(p.M * K)) : make_rsrc((const char*)p.xq + m0 * K, rows * K);
-  const auto wr0 = make_rsrc(p.side[0].wq, N16 * K64 * 1024);
-  const auto wr1 = make_rsrc(p.side[S - 1].wq, N16 * K64 * 1024);
+  const int kb = wave & 1;  // of a chunk's two blocks along k
+  // Experts' tiles are counted by the plan, whose tiles this one may be a part of.
+  if constexpr (MODE != DENSE) mtiles = g.info[0] << g.shift;
+  const int total = mtiles * ntiles;
+  if ((int)blockIdx.x >= total) return;
 
-  // Copies.  x: eight rows each, piece c of row r at c ^ (r / 2) % 8.  Weight:
-  // one block each, piece q of local block l at q ^ 4 (l % 4), which keeps the
-  // sixteen columns that an operand takes from several blocks in different banks.
+  // A workgroup of 256 x 256 has its CU for itself, and takes one tile after the
+  // other, every gridDim.x-th; where two share a CU, one's beginnings and ends
+  // lie under the other's chunks, and a workgroup for every tile is better
+  // (8,192^3 with tiles of 64: 839 us, one after the other 907).
+  constexpr bool LOOP = BM == 256;
+  int64_t m0;
+  int rows, nb0;  // rows there are; first block of columns
+  __amdgpu_buffer_rsrc_t xr, wr0, wr1;
   unsigned xo[XI], wo[WI];
+  // of row and column tid
+  float rs, cs, cb;
+  int rp;
+  auto setup = [&](int b) {
+    const int lane = opaque(threadIdx.x & 63), tid = opaque(threadIdx.x);  // offsets are made anew: there are no registers to keep them
+    // Neighbours of one XCD take eight row tiles of a column tile, then of the next.
+    const int id = xcd_order(b, total);
+    const int gm0 = id / (8 * ntiles) * 8, rest = id % (8 * ntiles);
+    const int gm = mtiles - gm0 < 8 ? mtiles - gm0 : 8, mt = gm0 + rest % gm;
+    nb0 = rest / gm * SB;
+    int64_t expert = 0;
+    if constexpr (MODE == DENSE) {
+      m0 = (int64_t)mt * BM;
+      rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
+    } else {
+      const TileRec rec = g.tiles[mt >> g.shift];
+      const int part = (mt & ((1 << g.shift) - 1)) * BM;
+      m0 = rec.row0 + part;
+      rows = rec.rows - part < BM ? rec.rows - part : BM;  // 0 and less: a part behind the rows
+      rows = rows < 0 ? 0 : rows;
+      expert = rec.expert;
+    }
+    xr = MODE == UP ? make_rsrc(p.xq, (int)(p.M * K)) : make_rsrc((const char*)p.xq + m0 * K, rows * K);
+    wr0 = make_rsrc((const char*)p.side[0].wq + expert * g.wbytes, N16 * K64 * 1024);
+    wr1 = make_rsrc((const char*)p.side[S - 1].wq + expert * g.wbytes, N16 * K64 * 1024);
+    // Copies.  x: eight rows each, piece c of row r at c ^ (r / 2) % 8.  Weight:
+    // one block each, piece q of local block l at q ^ 4 (l % 4), which keeps the
+    // sixteen columns that an operand takes from several blocks in different banks.
+    int tok[XI];
+    if constexpr (MODE == UP) {  // loads under a condition each would be waited for one by one
+      const auto tr = make_rsrc(g.tok + m0, rows * 4);
 #pragma unroll
-  for (int q = 0; q < XI; ++q) {
-    int row = 8 * (q * NW + wave) + (lane >> 3);
-    const unsigned piece = (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) << 4);
-    if constexpr (MODE == UP) row = row < rows ? g.tok[m0 + row] : -1;
-    xo[q] = MODE == UP && row < 0 ? 0x80000000u : (unsigned)row * (unsigned)K + piece;
-  }
-  const int kb = wave & 1;  // of the chunk's two blocks along k
+      for (int q = 0; q < XI; ++q)
+        tok[q] = (int)__builtin_amdgcn_raw_buffer_load_b32(tr, (8 * (q * NW + wave) + (lane >> 3)) * 4, 0, 0);
+    }
 #pragma unroll
-  for (int q = 0; q < WI; ++q) {
-    const int l = (q * NW + wave) >> 1, n16 = nb0 + l % SB;
-    wo[q] = n16 < N16 ? (unsigned)(n16 * K64 + kb) * 1024u + (unsigned)((lane ^ (4 * (l & 3))) << 4) : 0xC0000000u;
-  }
+    for (int q = 0; q < XI; ++q) {
+      const int row = 8 * (q * NW + wave) + (lane >> 3);
+      const unsigned piece = (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) << 4);
+      xo[q] = (unsigned)(MODE == UP ? tok[q] : row) * (unsigned)K + piece;
+      if (MODE == UP && row >= rows) xo[q] = 0x80000000u;
+    }
+#pragma unroll
+    for (int q = 0; q < WI; ++q) {
+      const int l = (q * NW + wave) >> 1, n16 = nb0 + l % SB;
+      wo[q] = n16 < N16 ? (unsigned)(n16 * K64 + kb) * 1024u + (unsigned)((lane ^ (4 * (l & 3))) << 4) : 0xC0000000u;
+    }
+    // What the epilogue needs of each row and column, a thread each; it goes to LDS when the last tile's is done with.
+    rs = cs = cb = 0.f, rp = 0;
+    if (tid < rows) {
+      rs = p.xs[MODE == UP ? g.tok[m0 + tid] : m0 + tid];
+      if (MODE == DOWN) rp = g.pair[m0 + tid];
+    }
+    const int s = tid / (BN / S), n = nb0 * 16 + tid % (BN / S);
+    if (tid < BN && n < N) {
+      const I8Side d = s ? p.side[S - 1] : p.side[0];
+      cs = d.s[expert * N + n];
+      if (MODE == DENSE && d.b) cb = T::val(((const half_t*)d.b)[n]);
+    }
+  };
+  auto publish = [&] {
+    if (tid < BM) {
+      rowscale[tid] = rs;
+      if (MODE == DOWN) rowpair[tid] = rp;
+    }
+    if (tid < BN) colscale[tid] = cs, colbias[tid] = cb;
+  };
   auto issue = [&](int c, int c1, int slot) {
     GP_LDS char* at = lds + slot * SLOT;
     const bool in = c < c1;
@@ -562,8 +608,7 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
       wa[s][t] = XB + l * 2048 + (((lg * 16 + (n & 15)) ^ (4 * (l & 3))) << 4);
     }
 
-  const int per = (chunks + gridDim.y - 1) / gridDim.y;
-  int c0 = blockIdx.y * per;
+  const int per = (chunks + gridDim.y - 1) / gridDim.y, c0 = blockIdx.y * per;
   const int c1 = c0 + per < chunks ? c0 + per : chunks;
   // A chunk is multiplied in steps: half of its k, and with eight row tiles half
   // of them.  A step's operands are read from LDS while the step before it is
@@ -571,157 +616,160 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
   // chunk is in registers, so that behind one barrier its slot takes the chunk R
   // further on and the next slot is read.
   constexpr int G = MT > 4 ? 2 : 1, MG = MT / G, STEPS = 2 * G;
-  i32x4 acc[S][NS][MT] = {};
-  u32x4 w[2][S][NS], x[2][MG];
-  auto read = [&](int q, GP_LDS const char* slot) {  // step q of the chunk in slot
-    const int h = q / G;
-    if (q % G == 0) {
-#pragma unroll
-      for (int s = 0; s < S; ++s)
-#pragma unroll
-        for (int t = 0; t < NS; ++t) w[h][s][t] = *(GP_LDS const u32x4*)(slot + wa[s][t] + h * 1024);
-    }
-#pragma unroll
-    for (int m = 0; m < MG; ++m) x[q & 1][m] = *(GP_LDS const u32x4*)(slot + xa[h] + (q % G * MG + m) * 2048);
-  };
-  // the rows' scales and pairs first: what follows is not waited for with them
-  float rs = 0.f;
-  int rp = 0;
-  if (tid < rows) {
-    rs = p.xs[MODE == UP ? g.tok[m0 + tid] : m0 + tid];
-    if (MODE == DOWN) rp = g.pair[m0 + tid];
-  }
+
+  int b = blockIdx.x;
+  setup(b);
 #pragma unroll
   for (int i = 0; i < R; ++i) issue(c0 + i, c1, i);
-  if (tid < BM) {
-    rowscale[tid] = rs;
-    if (MODE == DOWN) rowpair[tid] = rp;
-  }
-  wait_vmcnt<(R - 1) * NI>();
-  lds_barrier();
-  read(0, lds);
-  int at = 0;
-  if (wm * MT * 16 >= rows) {  // a wave behind the last row only copies
+  publish();
 #pragma unroll 1
-    for (int c = c0; c < c1; ++c) {
-      wait_vmcnt<(R - 2) * NI>();
-      lds_barrier();
-      issue(c + R, c1, at);
-      at = at + 1 == R ? 0 : at + 1;
-    }
-    c0 = c1;
-  }
-#pragma unroll 1
-  for (int c = c0; c < c1; ++c) {
-    GP_LDS const char* slot = lds + at * SLOT;
+  for (;;) {
+    i32x4 acc[S][NS][MT] = {};
+    u32x4 w[2][S][NS], x[2][MG];
+    auto read = [&](int q, GP_LDS const char* slot) {  // step q of the chunk in slot
+      const int h = q / G;
+      if (q % G == 0) {
 #pragma unroll
-    for (int q = 0; q < STEPS; ++q) {
-      if (q + 1 < STEPS) {
-        read(q + 1, slot);
-      } else {
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+          for (int t = 0; t < NS; ++t) w[h][s][t] = *(GP_LDS const u32x4*)(slot + wa[s][t] + h * 1024);
+      }
+#pragma unroll
+      for (int m = 0; m < MG; ++m) x[q & 1][m] = *(GP_LDS const u32x4*)(slot + xa[h] + (q % G * MG + m) * 2048);
+    };
+    wait_vmcnt<(R - 1) * NI>();
+    lds_barrier();
+    read(0, lds);
+    int at = 0, c = c0;
+    // A wave behind the last row only copies.  (In the smaller kernels this branch makes the compiler wait for a step's
+    // reads at once: 128 rows of 4,096 from 4,096 11.0 us instead of 10.3.)
+    if (LOOP && wm * MT * 16 >= rows) {
+#pragma unroll 1
+      for (; c < c1; ++c) {
         wait_vmcnt<(R - 2) * NI>();
         lds_barrier();
         issue(c + R, c1, at);
         at = at + 1 == R ? 0 : at + 1;
-        read(0, lds + at * SLOT);
       }
-      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll 1
+    for (; c < c1; ++c) {
+      GP_LDS const char* slot = lds + at * SLOT;
 #pragma unroll
-      for (int m = 0; m < MG; ++m)
+      for (int q = 0; q < STEPS; ++q) {
+        if (q + 1 < STEPS) {
+          read(q + 1, slot);
+        } else {
+          wait_vmcnt<(R - 2) * NI>();
+          lds_barrier();
+          issue(c + R, c1, at);
+          at = at + 1 == R ? 0 : at + 1;
+          read(0, lds + at * SLOT);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int m = 0; m < MG; ++m)
+#pragma unroll
+          for (int s = 0; s < S; ++s)
+#pragma unroll
+            for (int t = 0; t < NS; ++t)
+              acc[s][t][q % G * MG + m] = mma8(w[q / G][s][t], x[q & 1][m], acc[s][t][q % G * MG + m]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    wait_vmcnt<0>();
+    lds_barrier();  // every wave is done with the ring
+
+    if (MODE == DENSE && gridDim.y > 1) {
+      // a lane's columns: 4 NS from n0 of each weight, of row j of each row tile
+      const int n0 = nb0 * 16 + wn * (16 * NS) + 4 * NS * lg;
+      int* const part = (int*)p.part + (int64_t)blockIdx.y * S * p.M * N;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int row = wm * MT * 16 + m * 16 + j;
+        if (row >= rows) continue;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          int* to = part + ((int64_t)s * p.M + m0 + row) * N + n0;
+#pragma unroll
+          for (int t = 0; t < NS; ++t) {
+            if (n0 + 4 * t + 4 <= N)
+              *(i4u*)(to + 4 * t) = acc[s][t][m];
+            else
+#pragma unroll
+              for (int e = 0; e < 3; ++e)
+                if (n0 + 4 * t + e < N) to[4 * t + e] = acc[s][t][m][e];
+          }
+        }
+      }
+      return;  // such a launch has a workgroup for every tile
+    }
+
+    // The next tile's first chunk, where there is one, is copied while this one leaves through the
+    // other slots: a wave's sums through its own part of them, eight neighbouring
+    // columns of a row a lane then, whole lines a wave, and a short rolled loop with
+    // the epilogue once (code is fetched from memory: with the epilogue unrolled over
+    // a lane's sums, and loads under conditions, a tile of 256 x 256 took 18 us
+    // besides its chunks).  Piece c of four sums of row r lies at c ^ r.
+    constexpr int OC = 16 * NS, NP = 4 * NS * S;  // a wave's columns of out; pieces a row
+    constexpr int ROOM = (R - 1) * SLOT / (NW * 16 * NP * 16), HM = ROOM >= MT ? MT : ROOM >= 4 ? 4 : ROOM >= 2 ? 2 : 1;
+    static_assert(ROOM >= 1, "a row tile's sums fit the other slots");
+    constexpr int LPR = OC / 8, RPI = 64 / LPR;  // lanes a row, rows a turn
+    const int lane = opaque(threadIdx.x & 63), j = lane & 15, lg = lane >> 4;
+    const int64_t out0 = m0;
+    const int last = rows, oc = lane % LPR, orow = lane / LPR, col = wn * OC + oc * 8;
+    const int n = nb0 * 16 + col, cnt = N - n < 8 ? N - n : 8;
+    b += gridDim.x;
+    const bool more = LOOP && b < total;
+    if (more) {
+      setup(b);
+      issue(c0, c1, 0);
+    }
+    GP_LDS char* const mine = lds + SLOT + wave * (HM * 16 * NP * 16);
+#pragma unroll
+    for (int part = 0; part < MT / HM; ++part) {
+#pragma unroll
+      for (int m = 0; m < HM; ++m)
 #pragma unroll
         for (int s = 0; s < S; ++s)
 #pragma unroll
           for (int t = 0; t < NS; ++t)
-            acc[s][t][q % G * MG + m] = mma8(w[q / G][s][t], x[q & 1][m], acc[s][t][q % G * MG + m]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  }
-  wait_vmcnt<0>();
-
-  if (MODE == DENSE && gridDim.y > 1) {
-    // a lane's columns: 4 NS from n0 of each weight, of row j of each row tile
-    const int n0 = nb0 * 16 + wn * (16 * NS) + 4 * NS * lg;
-    int* const part = (int*)p.part + (int64_t)blockIdx.y * S * p.M * N;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int row = wm * MT * 16 + m * 16 + j;
-      if (row >= rows) continue;
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        int* to = part + ((int64_t)s * p.M + m0 + row) * N + n0;
-#pragma unroll
-        for (int t = 0; t < NS; ++t) {
-          if (n0 + 4 * t + 4 <= N)
-            *(i4u*)(to + 4 * t) = acc[s][t][m];
-          else
-#pragma unroll
-            for (int e = 0; e < 3; ++e)
-              if (n0 + 4 * t + e < N) to[4 * t + e] = acc[s][t][m][e];
-        }
-      }
-    }
-    return;
-  }
-  // Out through LDS, a wave's sums through its own part of it: eight neighbouring
-  // columns of a row a lane then, whole lines a wave, and a short rolled loop with
-  // the epilogue once (code is fetched from memory: with the epilogue unrolled over
-  // a lane's sums, a tile of 256 x 256 took 18 us besides its chunks).  Piece c of
-  // four sums of row r lies at c ^ r.
-  constexpr int OC = 16 * NS, NP = 4 * NS * S;                       // a wave's columns of out; pieces a row
-  constexpr int HM = NW * MT * 16 * NP * 16 > R * SLOT ? MT / 2 : MT;  // row tiles at a time
-  static_assert(NW * HM * 16 * NP * 16 <= R * SLOT, "the sums fit the ring");
-  constexpr int LPR = OC / 8, RPI = 64 / LPR;  // lanes a row, rows a turn
-  GP_LDS char* const mine = lds + wave * (HM * 16 * NP * 16);
-  const int oc = lane % LPR, orow = lane / LPR;
-  const int n = nb0 * 16 + wn * OC + oc * 8, cnt = N - n < 8 ? N - n : 8;
-  float sc[S][8], b[S][8];
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    load_scales8(p.side[s].s, n, N, sc[s]);
-    if (MODE == DENSE && p.side[s].b) {
-      load_row8<T>((const half_t*)p.side[s].b, n, cnt, N, b[s]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) b[s][e] = 0.f;
-    }
-  }
-  lds_barrier();  // every wave is done with the ring
-#pragma unroll
-  for (int half = 0; half < MT / HM; ++half) {
-#pragma unroll
-    for (int m = 0; m < HM; ++m)
-#pragma unroll
-      for (int s = 0; s < S; ++s)
-#pragma unroll
-        for (int t = 0; t < NS; ++t)
-          *(GP_LDS i32x4*)(mine + (m * 16 + j) * (NP * 16) + (((s * 4 * NS + NS * lg + t) ^ (j & (NP - 1))) << 4)) =
-              acc[s][t][half * HM + m];
-    const int row0 = wm * MT * 16 + half * HM * 16;
+            *(GP_LDS i32x4*)(mine + (m * 16 + j) * (NP * 16) + (((s * 4 * NS + NS * lg + t) ^ (j & (NP - 1))) << 4)) =
+                acc[s][t][part * HM + m];
+      const int row0 = wm * MT * 16 + part * HM * 16;
 #pragma unroll 1
-    for (int it = 0; it < HM * 16; it += RPI) {
-      const int lrow = it + orow, row = row0 + lrow;
-      if (row >= rows || cnt <= 0) continue;
-      const float xsc = rowscale[row];
-      float v[8], u[8];
-      auto take = [&](int s, float (&to)[8]) {
+      for (int it = 0; it < HM * 16; it += RPI) {
+        const int lrow = it + orow, row = row0 + lrow;
+        if (row >= last || cnt <= 0) continue;
+        const float xsc = rowscale[row];
+        float v[8], u[8], bias[S][8];
+        auto take = [&](int s, float (&to)[8]) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const i32x4 a = *(GP_LDS const i32x4*)(mine + lrow * (NP * 16) +
-                                                 (((s * 4 * NS + 2 * oc + h) ^ (lrow & (NP - 1))) << 4));
+          for (int h = 0; h < 2; ++h) {
+            const i32x4 a = *(GP_LDS const i32x4*)(mine + lrow * (NP * 16) +
+                                                   (((s * 4 * NS + 2 * oc + h) ^ (lrow & (NP - 1))) << 4));
+            const f4 sc = *(GP_LDS const f4*)(colscale + s * (BN / S) + col + 4 * h);
+            const f4 bi = *(GP_LDS const f4*)(colbias + s * (BN / S) + col + 4 * h);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) to[4 * h + e] = (float)a[e] * sc[s][4 * h + e] * xsc;
+            for (int e = 0; e < 4; ++e) to[4 * h + e] = (float)a[e] * sc[e] * xsc, bias[s][4 * h + e] = bi[e];
+          }
+        };
+        take(0, v);
+        if constexpr (MODE == DOWN) {  // N a multiple of 16 here
+          float* const to = (float*)p.out + (int64_t)rowpair[row] * N + n;
+          *(f4*)to = f4{v[0], v[1], v[2], v[3]};
+          *(f4*)(to + 4) = f4{v[4], v[5], v[6], v[7]};
+        } else {
+          if constexpr (S == 2) take(1, u);
+          finish8<T, S>(p, out0 + row, n, cnt, v, u, bias);
         }
-      };
-      take(0, v);
-      if constexpr (MODE == DOWN) {  // N a multiple of 16 here
-        float* const to = (float*)p.out + (int64_t)rowpair[row] * N + n;
-        *(f4*)to = f4{v[0], v[1], v[2], v[3]};
-        *(f4*)(to + 4) = f4{v[4], v[5], v[6], v[7]};
-      } else {
-        if constexpr (S == 2) take(1, u);
-        finish8<T, S>(p, m0 + row, n, cnt, v, u, b);
       }
     }
+    if (!more) return;
+    lds_barrier();  // the other slots, and the rows' and columns' values, are done with
+#pragma unroll
+    for (int i = 1; i < R; ++i) issue(c0 + i, c1, i);
+    publish();
   }
 }
 
@@ -862,10 +910,12 @@ hipError_t rows_launch(const I8Args& a, const I8Group& g, int mt, int64_t mtiles
 }
 
 template <class T, int S, int MODE>
-hipError_t tile_launch(const I8Args& a, const I8Group& g, int64_t mtiles, const TilePlan& plan, hipStream_t s) {
-  const int64_t cols = plan.size / S, ntiles = (a.N + cols - 1) / cols;
+hipError_t tile_launch(const I8Args& a, const I8Group& g, int64_t mtiles, const TilePlan& plan, int num_cus, hipStream_t s) {
+  const int64_t cols = plan.size / S, ntiles = (a.N + cols - 1) / cols, fit = plan.size == 256 ? num_cus : int64_t(1) << 31;
   if (mtiles * ntiles > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)(mtiles * ntiles), (unsigned)plan.parts);
+  // of 256 x 256 as many workgroups as the chip holds; one for every tile else, and where k is in parts
+  const int64_t wgs = plan.parts > 1 || mtiles * ntiles < fit ? mtiles * ntiles : fit;
+  const dim3 grid((unsigned)wgs, (unsigned)plan.parts);
 #define GP_TILE(size, wm, wn, r)                                                                                  \
   hipLaunchKernelGGL((i8_tile_kernel<T, S, size, size, wm, wn, r, 2, MODE>), grid, dim3(64 * wm * wn), 0, s, a, g, \
                      (int)mtiles, (int)ntiles)
@@ -918,7 +968,7 @@ hipError_t launch(I8Args a, int num_cus, hipStream_t s) {
   }
   a.part = (char*)a.ws + l.part;
   const TilePlan plan = tile_plan(a.M, a.N, a.K, S, num_cus);
-  return tile_launch<T, S, DENSE>(a, I8Group{}, (a.M + plan.size - 1) / plan.size, plan, s);
+  return tile_launch<T, S, DENSE>(a, I8Group{}, (a.M + plan.size - 1) / plan.size, plan, num_cus, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -1149,20 +1199,40 @@ TokenPlan token_plan(int64_t T, int H, int F, int topk, int num_cus) {
   return l;
 }
 
-// Rows of a tile, by the rows that an expert has on average.
-int experts_tile(int64_t P, int E) {
-  const int64_t n = P / E;
-  return n >= 192 ? 256 : n >= 64 ? 128 : n >= 24 ? 64 : 16;
+// Rows of the tiles of both halves: 16 (the kernel for few rows) where an expert
+// has fewer than 24 on average, else what takes least by the estimate, with half
+// a tile more an expert for the last ones.  In us, both halves on 256 / on 128 /
+// 256 and 128: 4,096 tokens, 2 of 8 experts of 2,048 x 8,192 584 / 612 / 568; 8 of
+// 64 of 2,048 x 1,024 425 / 458 / 449; 512, 4 of 16 of 2,048 x 1,024 74 / 65 / 69.
+struct ExpertsTiles {
+  int up, down;
+};
+ExpertsTiles experts_tiles(int64_t P, int H, int F, int E, int num_cus) {
+  if (P / E < 24) return {16, 16};
+  auto best = [&](int N, int K, int sides) {
+    int size = 0;
+    float least = 0.f;
+    for (int s : {256, 128, 64}) {
+      const int64_t cols = s / sides, tiles = (P / s + E / 2 + 1) * ((N + cols - 1) / cols);
+      float t = tile_time(s, tiles, (K + kChunk - 1) / kChunk, num_cus);
+      if (s < 256) t += 4.f * (float)((tiles + num_cus - 1) / num_cus);  // the gather's way to a tile's first chunk
+      if (size == 0 || t < least) size = s, least = t;
+    }
+    return size;
+  };
+  return {best(F, H, 2), best(H, F, 1)};
 }
 
 struct ExpertsLayout {
-  int tile;
+  ExpertsTiles size;
+  int tile;  // of the plan: the larger one
   int64_t max_tiles, xq, xs, tiles, info, tok, pair, h, hq, hs, y, bytes;
 };
 ExpertsLayout experts_layout(int64_t T, int H, int F, int E, int topk, int num_cus) {
   ExpertsLayout l{};
   const int64_t P = T * topk;
-  l.tile = experts_tile(P, E);
+  l.size = experts_tiles(P, H, F, E, num_cus);
+  l.tile = l.size.up > l.size.down ? l.size.up : l.size.down;
   l.max_tiles = P / l.tile + (P < E ? P : E);
   auto take = [&](int64_t n) {
     const int64_t at = l.bytes;
@@ -1187,13 +1257,14 @@ ExpertsLayout experts_layout(int64_t T, int H, int F, int E, int topk, int num_c
 }
 
 template <class T, int S, int MODE>
-hipError_t experts_product(const I8Args& a, const I8Group& g, const ExpertsLayout& l, int64_t pairs, int num_cus,
+hipError_t experts_product(const I8Args& a, I8Group g, const ExpertsLayout& l, int size, int64_t pairs, int num_cus,
                            hipStream_t s) {
-  if (l.tile == 16) {
+  if (size == 16) {
     const int64_t busy = pairs < g.experts ? pairs : g.experts;
     return rows_launch<T, S, MODE>(a, g, 1, l.max_tiles, busy, false, num_cus, s);
   }
-  return tile_launch<T, S, MODE>(a, g, l.max_tiles, TilePlan{l.tile, 1}, s);
+  g.shift = __builtin_ctz(l.tile / size);
+  return tile_launch<T, S, MODE>(a, g, l.max_tiles << g.shift, TilePlan{size, 1}, num_cus, s);
 }
 
 template <class T>
@@ -1205,7 +1276,7 @@ hipError_t experts_run(const ExpertsArgs& p, int num_cus, hipStream_t s) {
   char* const ws = (char*)p.ws;
   const TokenPlan tp = token_plan(p.T, p.H, p.F, p.topk, num_cus);
   if (tp.kw) {
-    const I8Group g{nullptr, nullptr, nullptr, nullptr, up_bytes, p.ids, p.topk, p.E};
+    const I8Group g{nullptr, nullptr, nullptr, nullptr, up_bytes, 0, p.ids, p.topk, p.E};
     const I8Args up{p.T, p.F, p.H, 2, p.x, nullptr, nullptr, {{p.wg, p.sg, nullptr}, {p.wu, p.su, nullptr}},
                     nullptr, p.act, ws + l.h, p.dtype, nullptr, nullptr};
     const hipError_t e = rows_launch<T, 2, UP>(up, g, 1, P, P, true, num_cus, s);
@@ -1220,7 +1291,7 @@ hipError_t experts_run(const ExpertsArgs& p, int num_cus, hipStream_t s) {
     return hipGetLastError();
   }
   I8Group g{(const TileRec*)(ws + l.tiles), (const int*)(ws + l.info), (const int*)(ws + l.tok), (const int*)(ws + l.pair), 0,
-            p.ids, p.topk, p.E};
+            0, p.ids, p.topk, p.E};
   hipLaunchKernelGGL(i8_plan_kernel, dim3(p.E), dim3(1024), 0, s, p.ids, P, p.E, p.topk, l.tile, (TileRec*)(ws + l.tiles),
                      (int*)(ws + l.info), (int*)(ws + l.tok), (int*)(ws + l.pair));
   hipError_t e = hipGetLastError();
@@ -1229,12 +1300,12 @@ hipError_t experts_run(const ExpertsArgs& p, int num_cus, hipStream_t s) {
   I8Args up{p.T, p.F, p.H, 2, nullptr, ws + l.xq, (const float*)(ws + l.xs), {{p.wg, p.sg, nullptr}, {p.wu, p.su, nullptr}},
             nullptr, p.act, ws + l.h, p.dtype, nullptr, nullptr};
   g.wbytes = up_bytes;
-  if ((e = experts_product<T, 2, UP>(up, g, l, P, num_cus, s)) != hipSuccess) return e;
+  if ((e = experts_product<T, 2, UP>(up, g, l, l.size.up, P, num_cus, s)) != hipSuccess) return e;
   if ((e = rows_to_bytes<T>(ws + l.h, P, p.F, ws + l.hq, (float*)(ws + l.hs), s, g.info + 1)) != hipSuccess) return e;
   I8Args down{P, p.H, p.F, 1, nullptr, ws + l.hq, (const float*)(ws + l.hs), {{p.wd, p.sd, nullptr}, {}},
               nullptr, GP_ACT_NONE, ws + l.y, p.dtype, nullptr, nullptr};
   g.wbytes = down_bytes;
-  if ((e = experts_product<F16, 1, DOWN>(down, g, l, P, num_cus, s)) != hipSuccess) return e;
+  if ((e = experts_product<F16, 1, DOWN>(down, g, l, l.size.down, P, num_cus, s)) != hipSuccess) return e;
   const int64_t pieces = p.T * (p.H / 8);
   hipLaunchKernelGGL((i8_combine_kernel<T>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, p, (const float*)(ws + l.y));
   return hipGetLastError();
