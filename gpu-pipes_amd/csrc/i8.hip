@@ -122,18 +122,18 @@ __device__ __forceinline__ unsigned wave_top(unsigned a) {
 
 // Rows of x to bytes: WPR waves a row, P pieces of eight values a lane held in
 // registers, so that memory is read once; rows longer than that are read again
-// (from L2).  One wave a row up to 2,048 values, four rows a workgroup.  count:
-// where it is given, the rows that there are.
-template <class T, int P, int WPR>
-__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void i8_rows_to_bytes_kernel(const half_t* x, int64_t M, int K,
-                                                                                    char* q, float* xs, const int* count) {
+// (from L2).  One wave a row up to 2,048 values.  block: of WAVES / WPR rows.
+// count: where it is given, the rows that there are.  part: one value a wave.
+template <class T, int P, int WPR, int WAVES>
+__device__ __forceinline__ void rows_to_bytes(const half_t* x, int64_t M, int K, char* q, float* xs, const int* count,
+                                              int64_t block, unsigned* part) {
   constexpr int STEP = 64 * WPR * 8;
-  __shared__ unsigned part[WPR];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t m = WPR == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
-  if (m >= M || (count && m >= *count)) return;  // whole waves of one-wave rows only
-  const auto xr = make_rsrc(x + m * K, K * 2);
-  const int at = (WPR == 1 ? lane : (int)threadIdx.x) * 8;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, first = wave / WPR * WPR;
+  int64_t m = block * (WAVES / WPR) + wave / WPR;
+  const bool in = m < M && !(count && m >= *count);
+  m = in ? m : 0;  // such a wave reads nothing, but comes to the barrier
+  const auto xr = make_rsrc(x + m * K, in ? K * 2 : 0);
+  const int at = (lane + (wave - first) * 64) * 8;
   u32x4 v[P];
   unsigned top = 0;
 #pragma unroll
@@ -151,8 +151,9 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void i8_rows_to_bytes_ke
   if constexpr (WPR > 1) {
     if (lane == 0) part[wave] = top;
     __syncthreads();
-    top = wave_top(part[lane & (WPR - 1)]);
+    top = wave_top(part[first + (lane & (WPR - 1))]);
   }
+  if (!in) return;
   const RowScale s = row_scale<T>(top);
   char* const row = q + m * K;
 #pragma unroll
@@ -162,16 +163,23 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void i8_rows_to_bytes_ke
     *(u32x2*)(row + k) = round8<T>(__builtin_amdgcn_raw_buffer_load_b128(xr, k * 2, 0, 0), s);
   if (at == 0) xs[m] = s.scale;
 }
+template <class T, int P, int WPR, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void i8_rows_to_bytes_kernel(const half_t* x, int64_t M, int K, char* q, float* xs,
+                                                                     const int* count) {
+  __shared__ unsigned part[WAVES];
+  rows_to_bytes<T, P, WPR, WAVES>(x, M, K, q, xs, count, blockIdx.x, part);
+}
 
 template <class T>
-hipError_t rows_to_bytes(const void* x, int64_t M, int K, char* q, float* xs, hipStream_t s, const int* count = nullptr) {
+hipError_t rows_to_bytes_launch(const void* x, int64_t M, int K, char* q, float* xs, hipStream_t s, const int* count = nullptr) {
   const half_t* h = (const half_t*)x;
-#define GP_ROWS(p, w) \
-  hipLaunchKernelGGL((i8_rows_to_bytes_kernel<T, p, w>), dim3((unsigned)(w == 1 ? (M + 3) / 4 : M)), dim3(w == 1 ? 256 : 64 * w), 0, s, h, M, K, q, xs, count)
-  if (K <= 512) GP_ROWS(1, 1);
-  else if (K <= 2048) GP_ROWS(4, 1);
-  else if (K <= 8192) GP_ROWS(4, 4);
-  else GP_ROWS(4, 16);
+#define GP_ROWS(p, w, waves)                                                                                           \
+  hipLaunchKernelGGL((i8_rows_to_bytes_kernel<T, p, w, waves>), dim3((unsigned)((M + waves / w - 1) / (waves / w))), \
+                     dim3(64 * waves), 0, s, h, M, K, q, xs, count)
+  if (K <= 512) GP_ROWS(1, 1, 4);
+  else if (K <= 2048) GP_ROWS(4, 1, 4);
+  else if (K <= 8192) GP_ROWS(4, 4, 4);
+  else GP_ROWS(4, 16, 16);
 #undef GP_ROWS
   return hipGetLastError();
 }
@@ -958,7 +966,7 @@ hipError_t launch(I8Args a, int num_cus, hipStream_t s) {
   if (x16 && !xl) {
     a.xq = (char*)a.ws;
     a.xs = (float*)((char*)a.ws + l.xs);
-    const hipError_t e = rows_to_bytes<T>(a.x, a.M, a.K, (char*)a.ws, (float*)a.xs, s);
+    const hipError_t e = rows_to_bytes_launch<T>(a.x, a.M, a.K, (char*)a.ws, (float*)a.xs, s);
     if (e != hipSuccess) return e;
   }
   if (!on_tiles(a.M, a.N, S)) {
@@ -987,9 +995,17 @@ hipError_t launch(I8Args a, int num_cus, hipStream_t s) {
 // come first and the experts' last, shorter ones behind all of them.  Loads of
 // ids are in batches, and up to 8,192 pairs stay in registers for the second
 // pass: one after the other they were 12 us for 8,192 pairs of 8 experts.
+// The workgroups behind the experts' make the tokens' rows bytes meanwhile.
+template <class T, int WPR>
 __global__ __launch_bounds__(1024) void i8_plan_kernel(const int* ids, int64_t P, int E, int topk, int tile, TileRec* tiles,
-                                                      int* info, int* tok, int* pair) {
+                                                      int* info, int* tok, int* pair, const half_t* x, int H, char* q,
+                                                      float* xs) {
   constexpr int B = 8, SUMS = 6;
+  if ((int)blockIdx.x >= E) {
+    __shared__ unsigned part[16];
+    rows_to_bytes<T, 4, WPR, 16>(x, P / topk, H, q, xs, nullptr, blockIdx.x - E, part);
+    return;
+  }
   __shared__ int count[kExpertsMaxE];
   __shared__ int own[16], sums[16][SUMS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e = blockIdx.x;
@@ -1292,16 +1308,18 @@ hipError_t experts_run(const ExpertsArgs& p, int num_cus, hipStream_t s) {
   }
   I8Group g{(const TileRec*)(ws + l.tiles), (const int*)(ws + l.info), (const int*)(ws + l.tok), (const int*)(ws + l.pair), 0,
             0, p.ids, p.topk, p.E};
-  hipLaunchKernelGGL(i8_plan_kernel, dim3(p.E), dim3(1024), 0, s, p.ids, P, p.E, p.topk, l.tile, (TileRec*)(ws + l.tiles),
-                     (int*)(ws + l.info), (int*)(ws + l.tok), (int*)(ws + l.pair));
+  const int wpr = p.H <= 2048 ? 1 : p.H <= 8192 ? 4 : 16;
+  const auto plan = wpr == 1 ? &i8_plan_kernel<T, 1> : wpr == 4 ? &i8_plan_kernel<T, 4> : &i8_plan_kernel<T, 16>;
+  hipLaunchKernelGGL(plan, dim3((unsigned)(p.E + (p.T + 16 / wpr - 1) / (16 / wpr))), dim3(1024), 0, s, p.ids, P, p.E, p.topk,
+                     l.tile, (TileRec*)(ws + l.tiles), (int*)(ws + l.info), (int*)(ws + l.tok), (int*)(ws + l.pair),
+                     (const half_t*)p.x, p.H, ws + l.xq, (float*)(ws + l.xs));
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  if ((e = rows_to_bytes<T>(p.x, p.T, p.H, ws + l.xq, (float*)(ws + l.xs), s)) != hipSuccess) return e;
   I8Args up{p.T, p.F, p.H, 2, nullptr, ws + l.xq, (const float*)(ws + l.xs), {{p.wg, p.sg, nullptr}, {p.wu, p.su, nullptr}},
             nullptr, p.act, ws + l.h, p.dtype, nullptr, nullptr};
   g.wbytes = up_bytes;
   if ((e = experts_product<T, 2, UP>(up, g, l, l.size.up, P, num_cus, s)) != hipSuccess) return e;
-  if ((e = rows_to_bytes<T>(ws + l.h, P, p.F, ws + l.hq, (float*)(ws + l.hs), s, g.info + 1)) != hipSuccess) return e;
+  if ((e = rows_to_bytes_launch<T>(ws + l.h, P, p.F, ws + l.hq, (float*)(ws + l.hs), s, g.info + 1)) != hipSuccess) return e;
   I8Args down{P, p.H, p.F, 1, nullptr, ws + l.hq, (const float*)(ws + l.hs), {{p.wd, p.sd, nullptr}, {}},
               nullptr, GP_ACT_NONE, ws + l.y, p.dtype, nullptr, nullptr};
   g.wbytes = down_bytes;

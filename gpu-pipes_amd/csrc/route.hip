@@ -6,14 +6,26 @@
 //   the k best c in those groups, ties to the lowest expert;  w = s, divided by their sum (renorm), times scale
 //
 // Which of two experts is better can hang on the last bits of their scores, so
-// scores that are compared are in 64 bits; without a bias, and with groups by
-// their largest, the logits decide and stay in 32.  Weights are made for the
-// chosen experts alone, in 64 bits, and rounded once.
+// the order is that of scores in 64 bits: scores in 32 bits decide where they are
+// further apart than they can be off, and a wave with a token whose choice is
+// closer than that makes its choices again in 64.  Without a bias, and with groups
+// by their largest, the logits decide.  Weights are made for the chosen experts
+// alone, in 64 bits, and rounded once.
+//
+// How far scores in 32 bits can be off, in units u = 2^-24: an exponential by 2 of
+// itself (v_exp_f32) and its argument's roundings, a reciprocal by 2 (v_rcp_f32).
+// Sigmoid, s = 1 / (1 + e): 0.23 (argument; s (1 - s) |l| < 0.23) + 0.5 (exponential;
+// s (1 - s) <= 1/4) + 3 (sum, reciprocal), and c's own rounding |c|: below 2^-21 of |c|
+// or of 1, whichever is more.  Softmax: 1 + 2 + 3 for e and the reciprocal, and
+// its sum, of up to 22 additions and of exponentials whose arguments are 8 on
+// average at most, by 22 + 2 * 8 + 2 of itself: below 2^-18.
 //
 // A token has 16 lanes up to 256 experts (four tokens a wave, and every exchange
 // between lanes a DPP rotation), 64 above.  Bound by instructions: an argument's
 // maximum over a token is V compares a lane and four or six exchanges, k times.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "../../include/gpipes.h"
 #include "gp_device.hpp"
@@ -25,6 +37,10 @@ namespace {
 template <int CTRL>
 __device__ __forceinline__ int dpp(int v) {
   return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, false);
+}
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) {
+  return (unsigned)dpp<CTRL>((int)v);
 }
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
@@ -80,25 +96,6 @@ __device__ __forceinline__ V over_token(V v, F f) {
   }
   return v;
 }
-// The best (key, index) over a token's lanes: the largest key, of equal ones the lowest index.
-template <int LPT, class K>
-__device__ __forceinline__ void best_of_token(K& k, int& i) {
-  auto take = [&](K k2, int i2) {
-    const bool b = k2 > k || (k2 == k && i2 < i);
-    k = b ? k2 : k, i = b ? i2 : i;
-  };
-  take(dpp<0x128>(k), dpp<0x128>(i));
-  take(dpp<0x124>(k), dpp<0x124>(i));
-  take(dpp<0x122>(k), dpp<0x122>(i));
-  take(dpp<0x121>(k), dpp<0x121>(i));
-  if constexpr (LPT == 64) {
-    K ka, kb;
-    int ia, ib;
-    halves<16>(k, ka, kb), halves<16>(i, ia, ib), k = ka, i = ia, take(kb, ib);
-    halves<32>(k, ka, kb), halves<32>(i, ia, ib), k = ka, i = ia, take(kb, ib);
-  }
-}
-
 __device__ __forceinline__ float logit(const void* l, int64_t at, int dtype) {
   if (dtype == GP_DTYPE_F32) return ((const float*)l)[at];
   const half_t h = ((const half_t*)l)[at];
@@ -107,135 +104,349 @@ __device__ __forceinline__ float logit(const void* l, int64_t at, int dtype) {
 __device__ __forceinline__ double sigmoid64(float l) { return 1.0 / (1.0 + exp(-(double)l)); }
 
 constexpr int kWaves = 4;
+constexpr int kRouteLds = 128 + 136;  // bytes a token: sixteen keys of 64 bits, kRouteMaxK + 1 experts (and a gap)
 
-// Lane i of a token holds experts i, i + LPT, ...  K: the keys' type, double where scores are compared.
-template <class K, int LPT, int V>
-__global__ __launch_bounds__(64 * kWaves) void route_experts_kernel(RouteExpertsArgs p) {
-  constexpr int TPW = 64 / LPT, VG = kRouteMaxGroups / LPT, VK = (kRouteMaxK + LPT - 1) / LPT;
-  constexpr bool D = sizeof(K) == 8;
-  extern __shared__ __attribute__((aligned(16))) char mem[];  // of a wave: a token's keys one after the other
-  const K none = -(K)__builtin_inff();
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & (LPT - 1);
-  const int64_t token = ((int64_t)blockIdx.x * kWaves + wave) * TPW + lane / LPT;
-  const int64_t t = token < p.T ? token : p.T - 1;  // every lane takes part in the exchanges
-  const int E = p.E;
-  const float inf = __builtin_inff();
+// What a token's lanes know of it: lane i holds experts i, i + LPT, ...
+template <int V>
+struct Token {
+  float l[V];  // logits, -inf behind the last expert
+  float top;   // the largest
+  int64_t t;   // the token
+  float bias[V];
+};
 
-  float l[V];
-  float top = -inf;
-  bool bad = false;
+// A wave's own LDS: what its lanes have written is there for all of them.
+__device__ __forceinline__ void wave_lds() {
+  compiler_fence();
+  __builtin_amdgcn_s_waitcnt(kWaitLgkm0);
+  compiler_fence();
+}
+
+// The largest of the keys and the lowest expert that has it; it is taken out of them.
+template <int LPT, class K, int V>
+__device__ __forceinline__ int take_best(K (&key)[V], int i, K& best) {
+  K m = key[0];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = v * LPT + i;
-    l[v] = e < E ? logit(p.logits, t * E + e, p.dtype) : -inf;
-    bad |= l[v] != l[v];
-    top = l[v] > top ? l[v] : top;
-  }
-  top = over_token<LPT>(top, [](float a, float b) { return a > b ? a : b; });
+  for (int v = 1; v < V; ++v) m = key[v] > m ? key[v] : m;
+  best = over_token<LPT>(m, [](K a, K b) { return a > b ? a : b; });
+  int at = 1 << 20;
+#pragma unroll
+  for (int v = V - 1; v >= 0; --v) at = key[v] == best ? v * LPT + i : at;
+  at = over_token<LPT>(at, [](int a, int b) { return a < b ? a : b; });
+#pragma unroll
+  for (int v = 0; v < V; ++v) key[v] = at == v * LPT + i ? -(K)__builtin_inff() : key[v];
+  return at;
+}
+
+// a from b, a >= b, where each may be off by `off` of itself or of 1.  Equal
+// infinities are not, nothing (b) is far from everything.
+__device__ __forceinline__ bool apart(float a, float b, float off) {
+  return !(b > -__builtin_inff()) || a - b > off * fmaxf(fmaxf(fabsf(a), fabsf(b)), 1.f);
+}
+
+// Keys of a token's experts: the logits, or (SCORES) c in K's precision, -inf for
+// those that cannot be chosen.
+template <class K, bool SCORES, int LPT, int V>
+__device__ __forceinline__ void make_keys(const RouteExpertsArgs& p, const Token<V>& x, K (&key)[V], K (&rank)[V], bool& bad) {
   const bool softmax = p.score == GP_SCORE_SOFTMAX;
-  bad |= softmax && top == inf;
-
-  // The softmax's denominator, where scores themselves are asked for.
-  double sum = 1.0;
-  if (softmax && (D || !p.renorm)) {
-    sum = 0.0;
+  const float inf = __builtin_inff();
+  K sum = 1;
+  if (SCORES && softmax) {
+    sum = 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum += l[v] == -inf ? 0.0 : exp((double)l[v] - (double)top);
-    sum = over_token<LPT>(sum, [](double a, double b) { return a + b; });
+    for (int v = 0; v < V; ++v) {
+      if constexpr (sizeof(K) == 8)
+        sum += x.l[v] == -inf ? 0.0 : exp((double)x.l[v] - (double)x.top);
+      else
+        sum += x.l[v] == -inf ? 0.f : __builtin_amdgcn_exp2f((x.l[v] - x.top) * 1.4426950408889634f);
+    }
+    sum = over_token<LPT>(sum, [](K a, K b) { return a + b; });
   }
-  auto score = [&](float x) { return softmax ? exp((double)x - (double)top) / sum : sigmoid64(x); };
-
-  K key[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    key[v] = (K)l[v];
-    if constexpr (D) {
-      if (p.bias && l[v] != -inf) {
-        key[v] = score(l[v]) + (double)p.bias[v * LPT + i];
-        bad |= key[v] != key[v];
+    key[v] = rank[v] = (K)x.l[v];
+    if constexpr (SCORES) {
+      K s;
+      if constexpr (sizeof(K) == 8) {
+        s = softmax ? exp((double)x.l[v] - (double)x.top) / sum : sigmoid64(x.l[v]);
+      } else {
+        const float e = __builtin_amdgcn_exp2f((softmax ? x.l[v] - x.top : -x.l[v]) * 1.4426950408889634f);
+        s = softmax ? e * __builtin_amdgcn_rcpf((float)sum) : __builtin_amdgcn_rcpf(1.f + e);
+      }
+      const bool out = x.l[v] == -inf;
+      if (p.bias) {
+        const K c = s + (K)x.bias[v];
+        bad |= c != c && !out;
+        key[v] = rank[v] = out ? key[v] : c;
+      } else {
+        rank[v] = out ? key[v] : s;
       }
     }
   }
+}
 
-  if (p.top_groups < p.groups) {
-    K* const rank = (K*)mem + (wave * TPW + lane / LPT) * E;
-    const int size = E / p.groups;
+// Leaves the keys of the top_groups best groups.  at: the token's place in the
+// wave's LDS.  Whether the last of them is further than `off` from the first of the
+// others comes back.
+template <class K, int LPT, int V>
+__device__ __forceinline__ bool keep_groups(const RouteExpertsArgs& p, K (&key)[V], const K (&rank)[V], int i, K* at, float off) {
+  const K none = -(K)__builtin_inff();
+  const int size = p.E / p.groups;
+  wave_lds();  // what was there is done with
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int e = v * LPT + i;
-      K r = key[v];
-      if constexpr (D)
-        if (!p.bias && l[v] != -inf) r = score(l[v]);
-      if (e < E) rank[e] = r;
-    }
-    lds_barrier();
+  for (int v = 0; v < V; ++v)
+    if (v * LPT + i < p.E) at[v * LPT + i] = rank[v];
+  wave_lds();
+  bool sure = true;
+  unsigned long long kept = 0;
+  auto select = [&](auto vg) {
+    constexpr int VG = decltype(vg)::value;
     K g[VG];
-    unsigned long long kept = 0;
 #pragma unroll
     for (int v = 0; v < VG; ++v) {
-      const int gi = v * LPT + i;
+      const int gi = v * LPT + i < p.groups ? v * LPT + i : p.groups - 1;
       K a = none, b = none;  // the group's two best
-      if (gi < p.groups)
-        for (int e = 0; e < size; ++e) {
-          const K r = rank[gi * size + e];
-          b = r > a ? a : r > b ? r : b;
+      for (int e = 0; e < size; ++e) {
+        const K r = at[gi * size + e];
+        if constexpr (sizeof(K) == 4) {
+          b = __builtin_amdgcn_fmed3f(a, b, r);
+          a = fmaxf(a, r);
+        } else {
+          const K low = r > a ? a : r;
+          b = low > b ? low : b;
           a = r > a ? r : a;
         }
+      }
       g[v] = p.group_score == GP_GROUP_TOP2 && b > none ? a + b : a;
+      g[v] = v * LPT + i < p.groups ? g[v] : none;
     }
-    for (int n = 0; n < p.top_groups; ++n) {
-      K bk = none;
-      int bi = 1 << 20;
-#pragma unroll
-      for (int v = 0; v < VG; ++v)
-        if (g[v] > bk) bk = g[v], bi = v * LPT + i;
-      best_of_token<LPT>(bk, bi);
-      if (bk > none) kept |= 1ull << bi;  // of groups with no expert left none is kept
-#pragma unroll
-      for (int v = 0; v < VG; ++v)
-        if (bi == v * LPT + i) g[v] = none;
+    K last = none;
+    for (int n = 0; n < p.top_groups + (off > 0.f); ++n) {
+      K best;
+      const int of = take_best<LPT>(g, i, best);
+      if (n < p.top_groups) {
+        if (best > none) kept |= 1ull << (of & 63);  // of groups with no expert left none is kept
+      } else {
+        sure = apart((float)last, (float)best, off);
+      }
+      last = best;
     }
-    const float per = 1.f / (float)size;
+  };
+  if (p.groups <= LPT)
+    select(std::integral_constant<int, 1>{});
+  else
+    select(std::integral_constant<int, kRouteMaxGroups / LPT>{});
+  const float per = 1.f / (float)size;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int of = (int)(((float)(v * LPT + i) + 0.5f) * per);  // exact: below 2^10
-      if (!(kept >> (of & 63) & 1)) key[v] = none;
-    }
+  for (int v = 0; v < V; ++v) {
+    const int of = (int)(((float)(v * LPT + i) + 0.5f) * per);  // exact: below 2^10
+    if (!(kept >> (of & 63) & 1)) key[v] = none;
   }
+  return sure;
+}
 
-  // One after the other; lane n % LPT keeps the n-th.
-  int id[VK];
+// A token's experts in the definition's order, lane n % LPT keeping the n-th in
+// id[n / LPT]: scores (K double) in 64 bits, logits (float) as they are.
+template <class K, bool SCORES, int LPT, int V, int VK>
+__device__ __forceinline__ void choose(const RouteExpertsArgs& p, const Token<V>& x, int i, K* at, int (&id)[VK], bool& bad) {
+  K key[V], rank[V];
+  make_keys<K, SCORES, LPT>(p, x, key, rank, bad);
+  if (p.top_groups < p.groups) keep_groups<K, LPT>(p, key, rank, i, at, 0.f);
 #pragma unroll
   for (int s = 0; s < VK; ++s) id[s] = -1;
   for (int n = 0; n < p.k; ++n) {
-    K bk = none;
-    int bi = 1 << 20;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (key[v] > bk) bk = key[v], bi = v * LPT + i;
-    best_of_token<LPT>(bk, bi);
-    if (!(bk > none)) bi = -1;
+    K best;
+    const int e = take_best<LPT>(key, i, best);
 #pragma unroll
     for (int s = 0; s < VK; ++s)
-      if (n == s * LPT + i) id[s] = bi;
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (bi == v * LPT + i) key[v] = none;
+      if (n == s * LPT + i && best > -(K)__builtin_inff()) id[s] = e;
   }
+}
+
+// The same in fewer instructions, with keys of 32 bits of which the best one is a
+// minimum: the distance d from the largest key, less its last bits, and in their
+// place which of its lane's experts it is.  16-bit logits fit as they are, with the
+// expert below them (of equal ones the lowest comes first), and no choice is in
+// doubt.  Else one is where the next d is no further than scores, or what d has
+// lost, may be off: then the k best and those after them that are too close to the
+// last, up to sixteen, are put in order by their keys in 64 bits, one a lane.  What
+// that does not settle (a softmax, whose sum is needed in 64 bits, groups too close
+// to each other, more candidates) comes back as false.  list, cand: a token's places
+// in LDS for its experts and sixteen keys.
+template <bool SCORES, int LPT, int V>
+__device__ __forceinline__ bool choose_fast(const RouteExpertsArgs& p, const Token<V>& x, int i, float* at, int* list, double* cand, bool& bad) {
+  constexpr unsigned mask = V <= 1 ? 0 : V <= 2 ? 1 : V <= 4 ? 3 : V <= 8 ? 7 : 15;
+  constexpr float lost = 2.f * (float)(mask + 1) / (1 << 23);  // of d: its last bits, and two roundings
+  const float inf = __builtin_inff();
+  // of a score; its sum of two is off by twice that and its own rounding
+  const float off = !SCORES ? 0.f : p.score == GP_SCORE_SOFTMAX ? 1.f / (1 << 18) : 1.f / (1 << 21);
+  const bool exact = !SCORES && p.dtype != GP_DTYPE_F32;
+  float key[V], rank[V];
+  make_keys<float, SCORES, LPT>(p, x, key, rank, bad);
+  bool sure = true;
+  if (p.top_groups < p.groups) sure = keep_groups<float, LPT>(p, key, rank, i, at, 5.f * off);
+  float top = -inf;
+#pragma unroll
+  for (int v = 0; v < V; ++v) top = fmaxf(top, key[v]);
+  top = over_token<LPT>(top, [](float a, float b) { return fmaxf(a, b); });
+  sure &= exact || top < inf;
+  unsigned u[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    unsigned k;
+    if (exact) {
+      // a 16-bit logit's bits are the upper ones of bf16's float; fp16 goes back to its own
+      const float l = key[v] + 0.f;  // -0 is 0
+      const unsigned h = p.dtype == GP_DTYPE_BF16 ? __builtin_bit_cast(unsigned, l) >> 16
+                                                  : (unsigned)__builtin_bit_cast(unsigned short, (half_t)l);
+      k = ((h & 0x8000u ? h : ~h & 0x7FFFu) << 16) | (unsigned)(v * LPT + i);  // larger ones first
+    } else {
+      k = (__builtin_bit_cast(unsigned, top - key[v]) & ~mask) | v;
+    }
+    u[v] = key[v] == -inf ? ~0u : k;
+  }
+  float last = 0.f;
+  unsigned m;
+  bool found, close = false;  // too close to the one before
+  // The n-th best: out of the keys, and its expert at list[n].
+  auto next = [&](int n) {
+    unsigned mine = u[0];
+#pragma unroll
+    for (int v = 1; v < V; ++v) mine = u[v] < mine ? u[v] : mine;
+    m = over_token<LPT>(mine, [](unsigned a, unsigned b) { return a < b ? a : b; });
+#pragma unroll
+    for (int v = 0; v < V; ++v) u[v] = u[v] == m ? ~0u : u[v];
+    found = m != ~0u;
+    if (mine == m) list[n] = !found ? -1 : exact ? (int)(m & 0xFFFFu) : (int)(m & mask) * LPT + i;
+    if (!exact) {
+      const float d = __builtin_bit_cast(float, m & ~mask);
+      close = found && !(d - last > 2.f * off * fmaxf(fmaxf(fabsf(top), fabsf(top - d)), 1.f) + lost * d);
+      last = d;
+      // two lanes with one key: both were taken out
+      const unsigned long long won = __ballot(mine == m) >> (threadIdx.x & 63 & ~(LPT - 1));
+      sure &= !found || __popcll(LPT == 64 ? won : won & 0xFFFF) == 1;
+    }
+  };
+  bool doubt = false;
+  for (int n = 0; n < p.k + !exact; ++n) {
+    next(n);
+    doubt |= n > 0 && close;
+  }
+  if (exact || !__any(doubt)) return sure;
+  constexpr int MOST = 16;
+  if ((SCORES && p.score == GP_SCORE_SOFTMAX) || p.k >= MOST) return sure && !doubt;
+  // candidates: k, and while each is too close to the one before, the next ones
+  int q = p.k;
+  bool open = close;
+  for (int n = p.k; __any(open); ++n) {
+    if (n >= MOST) {
+      sure &= !open;
+      break;
+    }
+    if (n > p.k) {
+      next(n);
+      open &= close;
+    }
+    q += open;
+  }
+  wave_lds();
+  const bool one = i < q && i < MOST;
+  int e = one ? list[i] : -1;
+  double c = -(double)inf;
+  if (e >= 0) {
+    const float l = logit(p.logits, x.t * p.E + e, p.dtype);
+    c = SCORES && p.bias ? sigmoid64(l) + (double)p.bias[e] : (double)l;
+  }
+  if (i < MOST) cand[i] = c;
+  wave_lds();
+  int better = 0;
+#pragma unroll 1
+  for (int n = 0; n < MOST; ++n) {
+    const double o = cand[n];
+    const int oe = n < q ? list[n] : -1;
+    better += oe >= 0 && (o > c || (o == c && oe < e));
+  }
+  wave_lds();
+  if (e >= 0 && better < p.k) list[better] = e;
+  return sure;
+}
+
+template <bool SCORES, int LPT, int V>
+__global__ __launch_bounds__(64 * kWaves) void route_experts_kernel(RouteExpertsArgs p) {
+  constexpr int TPW = 64 / LPT, VK = (kRouteMaxK + LPT - 1) / LPT;
+  extern __shared__ __attribute__((aligned(16))) char mem[];  // each token's choice, then (with groups) its keys
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & (LPT - 1);
+  const int64_t token = ((int64_t)blockIdx.x * kWaves + wave) * TPW + lane / LPT;
+  const int64_t t = token < p.T ? token : p.T - 1;  // every lane takes part in the exchanges
+  const float inf = __builtin_inff();
+  const bool softmax = p.score == GP_SCORE_SOFTMAX;
+
+  // loads under a condition each would be waited for one by one: the last expert's again instead
+  Token<V> x;
+  x.t = t;
+  if (p.dtype == GP_DTYPE_F32) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) x.l[v] = ((const float*)p.logits)[t * p.E + (v * LPT + i < p.E ? v * LPT + i : p.E - 1)];
+  } else {
+    half_t h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = ((const half_t*)p.logits)[t * p.E + (v * LPT + i < p.E ? v * LPT + i : p.E - 1)];
+#pragma unroll
+    for (int v = 0; v < V; ++v) x.l[v] = p.dtype == GP_DTYPE_F16 ? F16::val(h[v]) : BF16::val(h[v]);
+  }
+  if (SCORES && p.bias) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) x.bias[v] = p.bias[v * LPT + i < p.E ? v * LPT + i : p.E - 1];
+  }
+  x.top = -inf;
+  bool bad = false;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    x.l[v] = v * LPT + i < p.E ? x.l[v] : -inf;
+    bad |= x.l[v] != x.l[v];
+    x.top = x.l[v] > x.top ? x.l[v] : x.top;
+  }
+  x.top = over_token<LPT>(x.top, [](float a, float b) { return a > b ? a : b; });
+  bad |= softmax && x.top == inf;
+
+  // 32 bits settle nearly every token; where a choice is too close for them, the wave makes its choices again.
+  int id[VK];
+  typedef typename std::conditional<SCORES, double, float>::type K;
+  const int place = wave * TPW + lane / LPT;
+  double* const cand = (double*)mem + place * 16;
+  int* const list = (int*)(mem + kWaves * TPW * 128) + place * (kRouteMaxK + 1);
+  K* const at = (K*)(mem + kRouteLds * kWaves * TPW) + place * p.E;
+  const bool sure = choose_fast<SCORES, LPT, V>(p, x, i, (float*)at, list, cand, bad);
+  wave_lds();
+#pragma unroll
+  for (int s = 0; s < VK; ++s) id[s] = s * LPT + i < p.k ? list[s * LPT + i] : -1;
+  if (__any(!sure && !bad)) choose<K, SCORES, LPT, V>(p, x, i, at, id, bad);
 
   // Weights: of a softmax that is divided by the chosen ones' sum, relative to the largest of them.
   const bool relative = softmax && p.renorm;
-  float x[VK], xtop = -inf;
+  double sum = 1.0;
+  if (softmax && !p.renorm) {
+    sum = 0.0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) sum += x.l[v] == -inf ? 0.0 : exp((double)x.l[v] - (double)x.top);
+    sum = over_token<LPT>(sum, [](double a, double b) { return a + b; });
+  }
+  float l[VK], ltop = -inf;
 #pragma unroll
   for (int s = 0; s < VK; ++s) {
-    x[s] = id[s] < 0 ? -inf : logit(p.logits, t * E + id[s], p.dtype);
-    xtop = x[s] > xtop ? x[s] : xtop;
+    l[s] = -inf;
+    if (s * LPT < p.k && id[s] >= 0) l[s] = logit(p.logits, t * p.E + id[s], p.dtype);
+    ltop = l[s] > ltop ? l[s] : ltop;
   }
-  if (relative) xtop = over_token<LPT>(xtop, [](float a, float b) { return a > b ? a : b; });
+  if (relative) ltop = over_token<LPT>(ltop, [](float a, float b) { return a > b ? a : b; });
   double w[VK], total = 0.0;
 #pragma unroll
   for (int s = 0; s < VK; ++s) {
-    w[s] = id[s] < 0 ? 0.0 : relative ? exp((double)x[s] - (double)xtop) : score(x[s]);
+    w[s] = 0.0;
+    if (s * LPT < p.k && id[s] >= 0) {
+      w[s] = softmax ? exp((double)l[s] - (double)(relative ? ltop : x.top)) : sigmoid64(l[s]);
+      if (!relative) w[s] /= sum;
+    }
     total += w[s];
   }
   if (p.renorm) total = over_token<LPT>(total, [](double a, double b) { return a + b; });
@@ -244,37 +455,37 @@ __global__ __launch_bounds__(64 * kWaves) void route_experts_kernel(RouteExperts
   for (int s = 0; s < VK; ++s) {
     const int n = s * LPT + i;
     if (n >= p.k || token >= p.T) continue;
-    const double v = p.renorm ? (total > 0.0 ? w[s] / total : 0.0) : w[s];
+    const double v = !p.renorm ? w[s] : total > 0.0 ? w[s] / total : 0.0;
     p.weights[t * p.k + n] = any ? __builtin_nanf("") : (float)(v * (double)p.scale);
     p.ids[t * p.k + n] = any ? n : id[s];
   }
 }
 
-template <class K, int LPT, int V>
+template <bool SCORES, int LPT, int V>
 hipError_t launch_one(const RouteExpertsArgs& a, hipStream_t s) {
   const int64_t per = kWaves * (64 / LPT);
-  const int bytes = a.top_groups < a.groups ? (int)(per * a.E * sizeof(K)) : 0;
-  const auto kern = &route_experts_kernel<K, LPT, V>;
+  const int bytes = (int)per * (kRouteLds + (a.top_groups < a.groups ? a.E * (SCORES ? 8 : 4) : 0));
+  const auto kern = &route_experts_kernel<SCORES, LPT, V>;
   hipLaunchKernelGGL(kern, dim3((unsigned)((a.T + per - 1) / per)), dim3(64 * kWaves), bytes, s, a);
   return hipGetLastError();
 }
 
-template <class K>
+template <bool SCORES>
 hipError_t launch(const RouteExpertsArgs& a, hipStream_t s) {
-  if (a.E <= 16) return launch_one<K, 16, 1>(a, s);
-  if (a.E <= 32) return launch_one<K, 16, 2>(a, s);
-  if (a.E <= 64) return launch_one<K, 16, 4>(a, s);
-  if (a.E <= 128) return launch_one<K, 16, 8>(a, s);
-  if (a.E <= 256) return launch_one<K, 16, 16>(a, s);
-  if (a.E <= 512) return launch_one<K, 64, 8>(a, s);
-  return launch_one<K, 64, 16>(a, s);
+  if (a.E <= 16) return launch_one<SCORES, 16, 1>(a, s);
+  if (a.E <= 32) return launch_one<SCORES, 16, 2>(a, s);
+  if (a.E <= 64) return launch_one<SCORES, 16, 4>(a, s);
+  if (a.E <= 128) return launch_one<SCORES, 16, 8>(a, s);
+  if (a.E <= 256) return launch_one<SCORES, 16, 16>(a, s);
+  if (a.E <= 512) return launch_one<SCORES, 64, 8>(a, s);
+  return launch_one<SCORES, 64, 16>(a, s);
 }
 
 }  // namespace
 
 hipError_t route_experts_launch(const RouteExpertsArgs& a, hipStream_t s) {
   const bool scores = a.bias || (a.top_groups < a.groups && a.group_score == GP_GROUP_TOP2);
-  return scores ? launch<double>(a, s) : launch<float>(a, s);
+  return scores ? launch<true>(a, s) : launch<false>(a, s);
 }
 
 }  // namespace gp

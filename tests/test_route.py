@@ -157,6 +157,27 @@ def test_ties_go_to_the_lowest(cuda, score, bias):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+def test_zeros_of_both_signs_and_steps_of_the_type(cuda, dt):
+    """-0 ties with 0; logits one step of their type apart do not; 16-bit ones that nearly all tie."""
+    gen = torch.Generator().manual_seed(4)
+    for E in (8, 64, 128, 200, 512, 1000):
+        logits = torch.zeros(12, E)
+        logits[0, ::2] = -0.0
+        logits[1] = -1.0
+        logits[1, E // 2], logits[1, E // 3] = -0.0, 0.0
+        eps = torch.finfo(dt).eps
+        logits[2:6] = 1 + eps * torch.randint(0, 4, (4, E), generator=gen)
+        logits[6:9] = -1 - eps * torch.randint(0, 4, (3, E), generator=gen)
+        logits[9:] = torch.randn(3, E, generator=gen) * 1e-3 + 100
+        logits = logits.to(dt)
+        check(cuda, logits, 5)
+        check(cuda, logits, 4, groups=2, top_groups=1)
+        check(cuda, logits, 5, score="sigmoid", bias=torch.zeros(E))
+        check(cuda, logits, 4, score="sigmoid", groups=2, top_groups=1, group_score="top2")
+
+
+@pytest.mark.gpu
 def test_scores_that_32_bits_cannot_tell_apart(cuda):
     """Saturated sigmoids, whose logits still differ, and biases that differ by less than a score's 32 bits keep."""
     logits = torch.tensor([[40.0, 41.0, 39.0, 60.0, 30.0, 42.0, 20.0, 50.0]])
