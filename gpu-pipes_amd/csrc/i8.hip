@@ -275,7 +275,7 @@ struct I8Group {
 // lies between them, and the waves' sums are joined through LDS.
 // XL: at most four rows of 16-bit x, which the workgroup makes bytes of itself.
 // ---------------------------------------------------------------------------
-constexpr int rows_ring(int nt, int mt, bool xl) { return xl ? (nt == 1 ? 4 : 2) : nt + mt <= 3 ? 3 : 2; }
+constexpr int rows_ring(int nt, int mt, bool xl) { return xl ? 2 : nt + mt <= 3 ? 3 : 2; }
 constexpr int slot_bytes(int nt, int mt, bool xl) { return (nt + (xl ? 0 : mt)) * 2048; }
 constexpr int kRowsLds = 156 * 1024;  // of dynamic LDS at most
 // Waves of a workgroup at most, a power of two: sixteen, or as many as have room for their rings.
@@ -868,8 +868,12 @@ bool on_tiles(int64_t M, int N, int sides) {
   return M > 64 || (M > 32 && n > 4096) || (M > 16 && n > 8192);
 }
 
-// Up to here each token's experts run by themselves.
-constexpr int64_t kTokenRows = 2;
+// Tokens whose experts run by themselves: two, or up to eight where most of them
+// will have different ones (an expert that two tokens choose is read twice, but the
+// plan, h's bytes and the sums are no launches of their own).  In us, so / with a plan:
+//   8 of 64 experts of 2,048 x 1,024:  2 tokens 28 / -, 4 43.3 / 52.6, 6 60.3 / 65.6, 8 73.8 / 72.2
+//   4 of 16 of 2,048 x 4,096:  3 58.4 / 57.8, 4 69.9 / 68.9, 8 124.7 / 78.7;  2 of 32 of 1,024 x 512:  8 14.0 / 22.2
+bool few_tokens(int64_t T, int E, int topk) { return T <= 2 || (T <= 8 && 4 * T * topk <= 3 * E); }
 
 bool own_bytes(int64_t M, int K) { return M <= 4 && K * (M <= 1 ? 1 : M <= 2 ? 2 : 4) <= 16384; }
 
@@ -882,7 +886,12 @@ hipError_t rows_launch(const I8Args& a, const I8Group& g, int mt, int64_t mtiles
   l.mt = mt;
   const int chunks = (a.K + kChunk - 1) / kChunk, rows = MODE == DENSE ? (int)a.M : 1;
   const int64_t tiles = (int64_t)((a.N + 15) / 16) * S * busy;
-  int per = tiles >= 4 * num_cus ? 4 : tiles >= 2 * num_cus ? 2 : 1;  // tiles a workgroup
+  // Tiles a workgroup: as many as leave every CU a workgroup, so that x is read for
+  // more columns at once; of one row, whose bytes cost little, every CU two, of
+  // eight waves, one's bytes and sums under the other's copies (one row / four rows with two and with one: 16,384
+  // columns from 4,096 k 12.4 / 14.7 and 12.8 / 13.4 us, 8,192 from 8,192 12.2 and 13.0).
+  const int64_t full = (int64_t)num_cus * (l.xl && rows == 1 ? 2 : 1);
+  int per = tiles >= 4 * full ? 4 : tiles >= 2 * full ? 2 : 1;
   if (per < S) per = S;
   l.nt = per > 2 && l.mt == 1 ? 2 : per;
   const int waves = rows_waves(l.nt, l.mt, l.xl);
@@ -897,7 +906,8 @@ hipError_t rows_launch(const I8Args& a, const I8Group& g, int mt, int64_t mtiles
     xbytes = l.xstride << mshift;
     l.cg = per / l.nt;
     l.kw = waves / l.cg;
-    while (l.kw > 1 && l.kw / 2 >= chunks && l.kw / 2 * l.cg >= need) l.kw /= 2;
+    const bool two = tiles / per >= 2 * num_cus;
+    while (l.kw > 1 && (l.kw / 2 >= chunks || (two && l.kw * l.cg > 8)) && l.kw / 2 * l.cg >= need) l.kw /= 2;
   } else {
     // k over as many waves as fill the chip with eight a CU; workgroups of four waves and more
     l.kw = waves;
@@ -1203,9 +1213,9 @@ __global__ __launch_bounds__(1024) void i8_token_down_kernel(ExpertsArgs p, cons
 struct TokenPlan {
   int kw, cols, xstride, bytes;
 };
-TokenPlan token_plan(int64_t T, int H, int F, int topk, int num_cus) {
+TokenPlan token_plan(int64_t T, int H, int F, int E, int topk, int num_cus) {
   TokenPlan l{};
-  if (T > kTokenRows || topk > 16 || !own_bytes(1, H)) return l;
+  if (!few_tokens(T, E, topk) || topk > 16 || !own_bytes(1, H)) return l;
   int kw = 1;
   while (2 * kw * topk <= 16) kw *= 2;
   l.cols = (int64_t)H / 16 * T >= num_cus ? 16 : 8;
@@ -1255,7 +1265,7 @@ ExpertsLayout experts_layout(int64_t T, int H, int F, int E, int topk, int num_c
     l.bytes += (n + 255) / 256 * 256;
     return at;
   };
-  if (token_plan(T, H, F, topk, num_cus).kw) {
+  if (token_plan(T, H, F, E, topk, num_cus).kw) {
     l.h = take(P * F * 2);
     return l;
   }
@@ -1290,7 +1300,7 @@ hipError_t experts_run(const ExpertsArgs& p, int num_cus, hipStream_t s) {
   const int64_t down_bytes = (int64_t)((p.H + 15) / 16) * ((p.F + 63) / 64) * 1024;
   const ExpertsLayout l = experts_layout(p.T, p.H, p.F, p.E, p.topk, num_cus);
   char* const ws = (char*)p.ws;
-  const TokenPlan tp = token_plan(p.T, p.H, p.F, p.topk, num_cus);
+  const TokenPlan tp = token_plan(p.T, p.H, p.F, p.E, p.topk, num_cus);
   if (tp.kw) {
     const I8Group g{nullptr, nullptr, nullptr, nullptr, up_bytes, 0, p.ids, p.topk, p.E};
     const I8Args up{p.T, p.F, p.H, 2, p.x, nullptr, nullptr, {{p.wg, p.sg, nullptr}, {p.wu, p.su, nullptr}},
