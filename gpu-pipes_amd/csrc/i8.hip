@@ -211,12 +211,15 @@ __device__ __forceinline__ void load_scales8(const float* s, int n, int N, float
 }
 
 // cnt of eight neighbouring outputs of a row from column n: v (and u of the second
-// weight) the sums times both scales, b the biases, zeros where there are none.
-template <class T, int S>
+// weight) the sums times both scales, b the biases, zeros where there are none
+// (BIAS false: of a product that has none).
+template <class T, int S, bool BIAS = true>
 __device__ __forceinline__ void finish8(const I8Args& p, int64_t m, int n, int cnt, float (&v)[8], float (&u)[8],
                                         const float (&b)[S][8]) {
+  if constexpr (BIAS) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] += b[0][e];
+    for (int e = 0; e < 8; ++e) v[e] += b[0][e];
+  }
   if (p.act == GP_ACT_RELU) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = v[e] < 0.f ? 0.f : v[e];
@@ -225,7 +228,7 @@ __device__ __forceinline__ void finish8(const I8Args& p, int64_t m, int n, int c
   }
   if constexpr (S == 2) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] *= u[e] + b[1][e];
+    for (int e = 0; e < 8; ++e) v[e] *= BIAS ? u[e] + b[1][e] : u[e];
   }
   if (p.r) {
     float t[8];
@@ -295,6 +298,8 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
                                                                              int mshift, int xstride) {
   constexpr int R = rows_ring(NT, MT, XL), SLOT = slot_bytes(NT, MT, XL), NI = SLOT / 1024, CW = NT / S;
   __shared__ unsigned tops[16];
+  __shared__ float rowscale[16 * MT];
+  __shared__ int rowpair[MODE == DOWN ? 16 * MT : 1];
   GP_LDS char* lds = dyn_lds();
   const int tid = threadIdx.x, lane = tid & 63, j = lane & 15, lg = lane >> 4;
   const int waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -351,11 +356,21 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      int row = mt * 16 + 8 * h + dr;
+      const int row = mt * 16 + 8 * h + dr;
       const unsigned piece = (unsigned)(((lane & 7) ^ ((row >> 1) & 7)) << 4);
-      if constexpr (MODE == UP) row = row < rows ? grp.tok[m0 + row] : -1;
-      xo[mt][h] = MODE == UP && row < 0 ? 0x80000000u : (unsigned)row * (unsigned)K + piece;
+      int from = row;
+      if constexpr (MODE == UP && !XL)
+        from = (int)__builtin_amdgcn_raw_buffer_load_b32(make_rsrc(grp.tok + m0, rows * 4), row * 4, 0, 0);
+      xo[mt][h] = (unsigned)from * (unsigned)K + piece;
+      if (MODE == UP && row >= rows) xo[mt][h] = 0x80000000u;
     }
+  // What the epilogue needs of each row, asked for before the ring so as not to be waited for behind it.
+  float rs = 0.f;
+  int rp = 0;
+  if (!XL && tid < rows) {
+    rs = p.xs[MODE == UP ? grp.tok[m0 + tid] : m0 + tid];
+    if (MODE == DOWN) rp = grp.pair[m0 + tid];
+  }
 
   auto issue = [&](int c, int slot) {
     GP_LDS char* at = ring + slot * SLOT;
@@ -379,10 +394,12 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
   };
 #pragma unroll
   for (int i = 0; i < R; ++i) issue(kw + i * KW, i);
+  if (!XL && tid < rows) {
+    rowscale[tid] = rs;
+    if (MODE == DOWN) rowpair[tid] = rp;
+  }
 
   GP_LDS char* const xl = lds + waves * (R * SLOT);
-  float* const xsl = (float*)tops;
-  float lscale = 0.f;
   if constexpr (XL) {
     unsigned top = 0;
 #pragma unroll
@@ -400,9 +417,8 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
       const int k = xat + i * tpr * 8;
       if (k < K) *(GP_LDS u32x2*)(xl + xrow * xstride + k) = round8<T>(xv[i], s);
     }
-    lscale = s.scale;
+    if (xat == 0) rowscale[xrow] = s.scale;
     lds_barrier();
-    if (tid - xrow * tpr == 0) xsl[xrow] = lscale;  // read behind the next barrier
   }
 
   i32x4 acc[NT][MT] = {};
@@ -461,9 +477,9 @@ __global__ __launch_bounds__(64 * rows_waves(NT, MT, XL)) void i8_rows_kernel(I8
       v += *(GP_LDS const int*)(from + w * (R * SLOT));
       if (S == 2) u += *(GP_LDS const int*)(from + w * (R * SLOT) + 16 * CW * 4);
     }
-    const float xsc = XL ? xsl[m] : p.xs[MODE == UP ? grp.tok[m0 + m] : m0 + m];
+    const float xsc = rowscale[m];
     if constexpr (MODE == DOWN)
-      ((float*)p.out)[(int64_t)grp.pair[m0 + m] * N + n] = (float)v * p.side[0].s[n] * xsc;
+      ((float*)p.out)[(int64_t)rowpair[m] * N + n] = (float)v * p.side[0].s[n] * xsc;
     else
       finish1<T, S>(p, m0 + m, n, (float)v * p.side[0].s[n] * xsc, S == 2 ? (float)u * p.side[S - 1].s[n] * xsc : 0.f);
   }
@@ -627,6 +643,7 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
 
   int b = blockIdx.x;
   setup(b);
+  if (!LOOP && MODE != DENSE && rows <= 0) return;  // a plan's tile may end before its last part
 #pragma unroll
   for (int i = 0; i < R; ++i) issue(c0 + i, c1, i);
   publish();
@@ -734,6 +751,17 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
       issue(c0, c1, 0);
     }
     GP_LDS char* const mine = lds + SLOT + wave * (HM * 16 * NP * 16);
+    float sc[S][8], bias[S][8] = {};
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const f4 v = *(GP_LDS const f4*)(colscale + s * (BN / S) + col + 4 * h);
+        f4 b = {};
+        if constexpr (MODE == DENSE) b = *(GP_LDS const f4*)(colbias + s * (BN / S) + col + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[s][4 * h + e] = v[e], bias[s][4 * h + e] = b[e];
+      }
 #pragma unroll
     for (int part = 0; part < MT / HM; ++part) {
 #pragma unroll
@@ -750,16 +778,14 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
         const int lrow = it + orow, row = row0 + lrow;
         if (row >= last || cnt <= 0) continue;
         const float xsc = rowscale[row];
-        float v[8], u[8], bias[S][8];
+        float v[8], u[8];
         auto take = [&](int s, float (&to)[8]) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const i32x4 a = *(GP_LDS const i32x4*)(mine + lrow * (NP * 16) +
                                                    (((s * 4 * NS + 2 * oc + h) ^ (lrow & (NP - 1))) << 4));
-            const f4 sc = *(GP_LDS const f4*)(colscale + s * (BN / S) + col + 4 * h);
-            const f4 bi = *(GP_LDS const f4*)(colbias + s * (BN / S) + col + 4 * h);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) to[4 * h + e] = (float)a[e] * sc[e] * xsc, bias[s][4 * h + e] = bi[e];
+            for (int e = 0; e < 4; ++e) to[4 * h + e] = (float)a[e] * sc[s][4 * h + e] * xsc;
           }
         };
         take(0, v);
@@ -769,7 +795,7 @@ __global__ __launch_bounds__(64 * WM * WN, EU) void i8_tile_kernel(I8Args p, I8G
           *(f4*)(to + 4) = f4{v[4], v[5], v[6], v[7]};
         } else {
           if constexpr (S == 2) take(1, u);
-          finish8<T, S>(p, out0 + row, n, cnt, v, u, bias);
+          finish8<T, S, MODE == DENSE>(p, out0 + row, n, cnt, v, u, bias);
         }
       }
     }
@@ -891,9 +917,9 @@ hipError_t rows_launch(const I8Args& a, const I8Group& g, int mt, int64_t mtiles
   // eight waves, one's bytes and sums under the other's copies (one row / four rows with two and with one: 16,384
   // columns from 4,096 k 12.4 / 14.7 and 12.8 / 13.4 us, 8,192 from 8,192 12.2 and 13.0).
   const int64_t full = (int64_t)num_cus * (l.xl && rows == 1 ? 2 : 1);
-  int per = tiles >= 4 * full ? 4 : tiles >= 2 * full ? 2 : 1;
+  int per = l.mt == 1 && tiles >= 4 * full ? 4 : tiles >= 2 * full ? 2 : 1;
   if (per < S) per = S;
-  l.nt = per > 2 && l.mt == 1 ? 2 : per;
+  l.nt = per > 2 ? 2 : per;
   const int waves = rows_waves(l.nt, l.mt, l.xl);
   const int ring = rows_ring(l.nt, l.mt, l.xl) * slot_bytes(l.nt, l.mt, l.xl);
   const int mshift = rows <= 1 ? 0 : rows <= 2 ? 1 : 2;
@@ -915,14 +941,14 @@ hipError_t rows_launch(const I8Args& a, const I8Group& g, int mt, int64_t mtiles
     l.cg = l.kw < 4 ? 4 / l.kw : 1;
   }
   l.bytes = l.kw * l.cg * ring + xbytes;
-#define GP_CASE(n, m)                                                                          \
-  if constexpr (n >= S)                                                                        \
-    if (l.nt == n && l.mt == m) {                                                              \
-      if constexpr (m == 1 && MODE != DOWN)                                                    \
-        if (l.xl) return rows_launch_one<T, S, n, m, true, MODE>(a, g, mtiles, l, mshift, s);  \
-      return rows_launch_one<T, S, n, m, false, MODE>(a, g, mtiles, l, mshift, s);             \
+#define GP_CASE(n, m)                                                                         \
+  if constexpr (n >= S && (m == 1 || MODE == DENSE))                                          \
+    if (l.nt == n && l.mt == m) {                                                             \
+      if constexpr (m == 1 && MODE != DOWN)                                                   \
+        if (l.xl) return rows_launch_one<T, S, n, m, true, MODE>(a, g, mtiles, l, mshift, s); \
+      return rows_launch_one<T, S, n, m, false, MODE>(a, g, mtiles, l, mshift, s);            \
     }
-  GP_CASE(1, 1) GP_CASE(2, 1) GP_CASE(1, 2) GP_CASE(2, 2) GP_CASE(4, 2) GP_CASE(1, 4) GP_CASE(2, 4) GP_CASE(4, 4)
+  GP_CASE(1, 1) GP_CASE(2, 1) GP_CASE(1, 2) GP_CASE(2, 2) GP_CASE(1, 4) GP_CASE(2, 4)
 #undef GP_CASE
   return hipErrorInvalidValue;
 }

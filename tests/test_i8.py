@@ -549,3 +549,49 @@ def test_rows_behind_out_stay(cuda):
         assert bool((full[:32] == 7).all()) and bool((full[32 + M:] == 7).all())
         want, d = side(*i8.quantize_rows(x), (wq, s), None)
         check(out, want, d, F16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N,two", [
+    (4090, 4096, 8190, False),  # 512 tiles of 256 x 256: two a workgroup, the last ones short
+    (2040, 4096, 8190, True), (4090, 2064, 8200, False), (1040, 4096, 4100, False), (300, 2064, 4100, True),
+    (70, 16384, 40, False), (90, 8208, 72, True)])  # few tiles: parts of k
+def test_every_size_of_tile(cuda, M, K, N, two):
+    if two:
+        gated(cuda, M, K, N, F16, bias=True)
+        gated(cuda, M, K, N, BF16, int8=True, act="gelu_tanh")
+    else:
+        linear(cuda, M, K, N, F16, bias=True, residual=True)
+        linear(cuda, M, K, N, BF16, int8=True, act="silu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 3, 17, 40, 100, 300])
+def test_scales_of_any_alignment(cuda, M):
+    """Scales that begin 4, 8 and 12 bytes behind a 16-byte border, as a slice's do."""
+    K, N = 528, 101
+    gen = torch.Generator().manual_seed(M)
+    for off in (1, 2, 3):
+        wq, s = weight(K, N, gen, cuda)
+        x, xs = rows(M, K, F16, gen, cuda, True)
+        ss, xx = (torch.full((v.numel() + 8,), float("nan"), device=cuda) for v in (s, xs))
+        ss[off:off + N], xx[off:off + M] = s, xs
+        out = torch.empty(M, N, dtype=F16, device=cuda)
+        gpipes.i8_gemm_out(x, i8.pack(wq), ss[off:off + N], xs=xx[off:off + M], out=out)
+        want, d = side(x, xs, (wq, s), None)
+        check(out, want, d, F16)
+
+
+@pytest.mark.gpu
+def test_one_weight_for_both_sides(cuda):
+    """The same tensors as gate and as the other weight, and calls one after the other with one output."""
+    K, N = 272, 80
+    gen = torch.Generator().manual_seed(1)
+    wq, s = weight(K, N, gen, cuda)
+    for M in (1, 20, 130):
+        x, _ = rows(M, K, F16, gen, cuda)
+        out = torch.empty(M, N, dtype=F16, device=cuda)
+        for _ in range(3):
+            gpipes.i8_gated_out(x, i8.pack(wq), s, i8.pack(wq), s, act="none", out=out)
+        v, d = side(*i8.quantize_rows(x), (wq, s), None)
+        check(out, v * v, 2 * d * v.abs() + d * d + U * v * v, F16)

@@ -189,6 +189,14 @@ def test_wide_deep_and_many(cuda, T, H, F, E, k, how):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T,H,F,E,k", [(4096, 1024, 2048, 4, 2), (4096, 2048, 4096, 8, 2), (700, 1024, 1040, 16, 2), (1000, 272, 2064, 30, 1)])
+@pytest.mark.parametrize("how", ["spread", "some", "one"])
+def test_every_size_of_tile(cuda, T, H, F, E, k, how):
+    """Both halves on tiles of 256, of 256 and 128, of 128 and 64 rows; all tokens with one expert too."""
+    case(cuda, T, H, F, E, k, BF16, how, residual=True)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("T", [1, 3, 50, 400, 1500])
 def test_uneven_experts(cuda, T):
     """All tokens with one expert, all but one, and none with any."""
