@@ -186,6 +186,40 @@ inline void q4_gated_out(int64_t M, int64_t N, int64_t K, int group, const void*
                         workspace, workspace_bytes, dtype, stream));
 }
 
+// Products in 8-bit integers (gp_i8_gemm_out, gp_i8_gated_out); x_scales null: x
+// is 16-bit.  workspace as gp_i8_workspace_bytes says.
+inline void i8_gemm_out(int64_t M, int64_t N, int64_t K, const void* x, const void* x_scales, const void* wq,
+                        const void* w_scales, const void* b, const void* r, int act, void* out, void* workspace,
+                        int64_t workspace_bytes, int dtype = GP_DTYPE_F16, void* stream = nullptr) {
+  check(gp_i8_gemm_out(M, N, K, x, x_scales, wq, w_scales, b, r, act, out, workspace, workspace_bytes, dtype, stream));
+}
+inline void i8_gated_out(int64_t M, int64_t N, int64_t K, const void* x, const void* x_scales, const void* wq_g,
+                         const void* w_scales_g, const void* b_g, const void* wq_u, const void* w_scales_u,
+                         const void* b_u, int act, void* out, void* workspace, int64_t workspace_bytes,
+                         int dtype = GP_DTYPE_F16, void* stream = nullptr) {
+  check(gp_i8_gated_out(M, N, K, x, x_scales, wq_g, w_scales_g, b_g, wq_u, w_scales_u, b_u, act, out, workspace,
+                        workspace_bytes, dtype, stream));
+}
+
+// Tokens' experts and their weights (gp_route_out).
+inline void route_out(int64_t T, int64_t E, int k, const void* logits, const void* bias, int score, int groups,
+                      int top_groups, int group_score, bool renorm, float scale, void* weights, void* ids,
+                      int dtype = GP_DTYPE_F32, void* stream = nullptr) {
+  check(gp_route_out(T, E, k, logits, bias, score, groups, top_groups, group_score, renorm ? 1 : 0, scale, weights, ids,
+                     dtype, stream));
+}
+
+// The feed-forward block of experts (gp_i8_experts_out); workspace as
+// gp_i8_experts_workspace_bytes says.
+inline void i8_experts_out(int64_t T, int64_t H, int64_t F, int64_t E, int topk, const void* x, const void* ids,
+                           const void* weights, const void* wq_g, const void* w_scales_g, const void* wq_u,
+                           const void* w_scales_u, const void* wq_d, const void* w_scales_d, int act, const void* r,
+                           void* out, void* workspace, int64_t workspace_bytes, int dtype = GP_DTYPE_F16,
+                           void* stream = nullptr) {
+  check(gp_i8_experts_out(T, H, F, E, topk, x, ids, weights, wq_g, w_scales_g, wq_u, w_scales_u, wq_d, w_scales_d, act,
+                          r, out, workspace, workspace_bytes, dtype, stream));
+}
+
 }  // namespace gpipes
 
 #endif  // GPIPES_HPP
