@@ -167,15 +167,20 @@ template <class T, int P, int WPR, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void i8_rows_to_bytes_kernel(const half_t* x, int64_t M, int K, char* q, float* xs,
                                                                      const int* count) {
   __shared__ unsigned part[WAVES];
-  rows_to_bytes<T, P, WPR, WAVES>(x, M, K, q, xs, count, blockIdx.x, part);
+  rows_to_bytes<T, P, WPR, WAVES>(x, M, K, q, xs, count, (int64_t)blockIdx.y * gridDim.x + blockIdx.x, part);
 }
 
 template <class T>
 hipError_t rows_to_bytes_launch(const void* x, int64_t M, int K, char* q, float* xs, hipStream_t s, const int* count = nullptr) {
   const half_t* h = (const half_t*)x;
-#define GP_ROWS(p, w, waves)                                                                                           \
-  hipLaunchKernelGGL((i8_rows_to_bytes_kernel<T, p, w, waves>), dim3((unsigned)((M + waves / w - 1) / (waves / w))), \
-                     dim3(64 * waves), 0, s, h, M, K, q, xs, count)
+  // a launch holds fewer than 2^32 threads along an axis, and experts have up to 2^26 rows
+  auto grid = [&](int rows) {
+    const int64_t n = (M + rows - 1) / rows, most = 1 << 20, y = (n + most - 1) / most;
+    return dim3((unsigned)((n + y - 1) / y), (unsigned)y);
+  };
+#define GP_ROWS(p, w, waves)                                                                                        \
+  hipLaunchKernelGGL((i8_rows_to_bytes_kernel<T, p, w, waves>), grid(waves / w), dim3(64 * waves), 0, s, h, M, K, q, \
+                     xs, count)
   if (K <= 512) GP_ROWS(1, 1, 4);
   else if (K <= 2048) GP_ROWS(4, 1, 4);
   else if (K <= 8192) GP_ROWS(4, 4, 4);
@@ -964,9 +969,10 @@ hipError_t rows_launch(const I8Args& a, const I8Group& g, int mt, int64_t mtiles
 template <class T, int S, int MODE>
 hipError_t tile_launch(const I8Args& a, const I8Group& g, int64_t mtiles, const TilePlan& plan, int num_cus, hipStream_t s) {
   const int64_t cols = plan.size / S, ntiles = (a.N + cols - 1) / cols, fit = plan.size == 256 ? num_cus : int64_t(1) << 31;
-  if (mtiles * ntiles > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
+  if (mtiles * ntiles >= int64_t(1) << 31) return hipErrorInvalidValue;
   // of 256 x 256 as many workgroups as the chip holds; one for every tile else, and where k is in parts
   const int64_t wgs = plan.parts > 1 || mtiles * ntiles < fit ? mtiles * ntiles : fit;
+  if (wgs * (plan.size == 256 ? 512 : 256) >= int64_t(1) << 32) return hipErrorInvalidValue;  // more threads than a launch holds
   const dim3 grid((unsigned)wgs, (unsigned)plan.parts);
 #define GP_TILE(size, wm, wn, r)                                                                                  \
   hipLaunchKernelGGL((i8_tile_kernel<T, S, size, size, wm, wn, r, 2, MODE>), grid, dim3(64 * wm * wn), 0, s, a, g, \

@@ -422,3 +422,18 @@ def test_a_short_workspace_is_refused(cuda):
     assert str(need) in gpipes.lib.gp_last_error().decode()
     assert _call(T=40, H=64, F=64, E=4, ws=t["ws"].data_ptr(), wsb=need, **{**at, "r": 0}) == 0
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_more_pairs_than_a_launch_of_one_axis_holds(cuda):
+    """2^26 pairs: their first and last tokens have the bits that they have in calls by themselves."""
+    T, H, F, E, k = 1 << 21, 16, 16, 32, 32
+    p = experts(E, H, F, torch.Generator().manual_seed(5), cuda)
+    gen = torch.Generator(device=cuda).manual_seed(5)
+    x = torch.randn(T, H, generator=gen, device=cuda).to(F16)
+    ids = torch.randint(-1, E, (T, k), generator=gen, device=cuda, dtype=torch.int32)
+    w = torch.rand(T, k, generator=gen, device=cuda)
+    got = run(x, ids, w, p)
+    for lo in (0, T // 2, T - 1000):
+        part = slice(lo, lo + 1000)
+        assert torch.equal(got[part], run(x[part].contiguous(), ids[part].contiguous(), w[part].contiguous(), p))
