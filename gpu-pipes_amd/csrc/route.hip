@@ -379,7 +379,8 @@ __global__ __launch_bounds__(64 * kWaves) void route_experts_kernel(RouteExperts
   constexpr int TPW = 64 / LPT, VK = (kRouteMaxK + LPT - 1) / LPT;
   extern __shared__ __attribute__((aligned(16))) char mem[];  // each token's choice, then (with groups) its keys
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & (LPT - 1);
-  const int64_t token = ((int64_t)blockIdx.x * kWaves + wave) * TPW + lane / LPT;
+  const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  const int64_t token = (block * kWaves + wave) * TPW + lane / LPT;
   const int64_t t = token < p.T ? token : p.T - 1;  // every lane takes part in the exchanges
   const float inf = __builtin_inff();
   const bool softmax = p.score == GP_SCORE_SOFTMAX;
@@ -469,7 +470,9 @@ hipError_t launch_one(const RouteExpertsArgs& a, hipStream_t s) {
   const int64_t per = kWaves * (64 / LPT);
   const int bytes = (int)per * (kRouteLds + (a.top_groups < a.groups ? a.E * (SCORES ? 8 : 4) : 0));
   const auto kern = &route_experts_kernel<SCORES, LPT, V>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)((a.T + per - 1) / per)), dim3(64 * kWaves), bytes, s, a);
+  // a launch holds fewer than 2^32 threads along an axis
+  const int64_t n = (a.T + per - 1) / per, most = 1 << 20, y = (n + most - 1) / most;
+  hipLaunchKernelGGL(kern, dim3((unsigned)((n + y - 1) / y), (unsigned)y), dim3(64 * kWaves), bytes, s, a);
   return hipGetLastError();
 }
 

@@ -317,3 +317,16 @@ def test_graph_and_streams(cuda):
         torch.cuda.synchronize()
         for (x, kw, w, ids, g, st), (ww, wi) in zip(sets, want):
             assert torch.equal(w, ww) and torch.equal(ids, wi)
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_a_launch_of_one_axis_holds(cuda):
+    T = (1 << 28) + 5
+    logits = torch.empty(T, 2, dtype=F16, device=cuda)
+    logits[:, 0] = 0
+    logits[:, 1] = torch.arange(T, device=cuda) % 3 - 1  # -1; 0, where the lower expert is first; 1
+    weights, ids = gpipes.route_out(logits, 1, score="sigmoid", renorm=False)
+    assert torch.equal(ids[:, 0] == 1, logits[:, 1] == 1) and bool((ids >= 0).all())
+    low, high = 0.5, 1 / (1 + 2.718281828459045 ** -1)
+    for n, w in ((0, low), (1, high)):  # a weight is the score in 64 bits, rounded once: 2^-24 of it
+        assert bool(((weights[ids == n].double() - w).abs() <= 2.0 ** -24 * w * (1 + 1e-6)).all())
