@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -21,6 +22,42 @@ def cuda():
     if not torch.cuda.is_available():
         pytest.skip("no GPU visible")
     return torch.device("cuda:0")
+
+
+@pytest.fixture(scope="session", autouse=True)
+def captures_without_collections():
+    """torch waits for the device when a CUDAGraph object ends; while a stream is being captured that is an error,
+    and one in a destructor ends the process.  A test that keeps the error of a refused capture leaves its graph in a
+    cycle (error, traceback, frame), and such a graph ends when the collector runs, which can be inside the next
+    capture: so garbage is collected before a capture begins, and not during it."""
+    import torch
+    graph = torch.cuda.graph
+    enter, leave = graph.__enter__, graph.__exit__
+    was = []  # of the captures that are open: whether the collector was on
+
+    def begin(self):
+        gc.collect()
+        was.append(gc.isenabled())
+        gc.disable()
+        try:
+            return enter(self)
+        except BaseException:
+            end()
+            raise
+
+    def end():
+        if was.pop():
+            gc.enable()
+
+    def finish(self, *args):
+        try:
+            return leave(self, *args)
+        finally:
+            end()
+
+    graph.__enter__, graph.__exit__ = begin, finish
+    yield
+    graph.__enter__, graph.__exit__ = enter, leave
 
 
 def bf16_to_f32(bits):
