@@ -109,7 +109,8 @@ __device__ __forceinline__ double sigmoid64(float l) { return 1.0 / (1.0 + exp(-
 constexpr int kWaves = 4;
 constexpr int kRouteLds = 128 + 136;  // bytes a token: sixteen keys of 64 bits, kRouteMaxK + 1 experts (and a gap)
 
-// What a token's lanes know of it: lane i holds experts i, i + LPT, ...
+// What a token's lanes know of it: lane i holds experts i, i + LPT, ...  No
+// logit is NaN, and none makes its c one: a row that has such has -inf here.
 template <int V>
 struct Token {
   float l[V];  // logits, -inf behind the last expert
@@ -125,7 +126,8 @@ __device__ __forceinline__ void wave_lds() {
   compiler_fence();
 }
 
-// The largest of the keys and the lowest expert that has it; it is taken out of them.
+// The largest of the keys and the lowest expert that has it; it is taken out of
+// them.  No key is NaN: lanes would come to different largest ones, and to no expert.
 template <int LPT, class K, int V>
 __device__ __forceinline__ int take_best(K (&key)[V], int i, K& best) {
   K m = key[0];
@@ -150,7 +152,7 @@ __device__ __forceinline__ bool apart(float a, float b, float off) {
 // Keys of a token's experts: the logits, or (SCORES) c in K's precision, -inf for
 // those that cannot be chosen.
 template <class K, bool SCORES, int LPT, int V>
-__device__ __forceinline__ void make_keys(const RouteExpertsArgs& p, const Token<V>& x, K (&key)[V], K (&rank)[V], bool& bad) {
+__device__ __forceinline__ void make_keys(const RouteExpertsArgs& p, const Token<V>& x, K (&key)[V], K (&rank)[V]) {
   const bool softmax = p.score == GP_SCORE_SOFTMAX;
   const float inf = __builtin_inff();
   K sum = 1;
@@ -178,9 +180,7 @@ __device__ __forceinline__ void make_keys(const RouteExpertsArgs& p, const Token
       }
       const bool out = x.l[v] == -inf;
       if (p.bias) {
-        const K c = s + (K)x.bias[v];
-        bad |= c != c && !out;
-        key[v] = rank[v] = out ? key[v] : c;
+        key[v] = rank[v] = out ? key[v] : s + (K)x.bias[v];
       } else {
         rank[v] = out ? key[v] : s;
       }
@@ -251,9 +251,9 @@ __device__ __forceinline__ bool keep_groups(const RouteExpertsArgs& p, K (&key)[
 // A token's experts in the definition's order, lane n % LPT keeping the n-th in
 // id[n / LPT]: scores (K double) in 64 bits, logits (float) as they are.
 template <class K, bool SCORES, int LPT, int V, int VK>
-__device__ __forceinline__ void choose(const RouteExpertsArgs& p, const Token<V>& x, int i, K* at, int (&id)[VK], bool& bad) {
+__device__ __forceinline__ void choose(const RouteExpertsArgs& p, const Token<V>& x, int i, K* at, int (&id)[VK]) {
   K key[V], rank[V];
-  make_keys<K, SCORES, LPT>(p, x, key, rank, bad);
+  make_keys<K, SCORES, LPT>(p, x, key, rank);
   if (p.top_groups < p.groups) keep_groups<K, LPT>(p, key, rank, i, at, 0.f);
 #pragma unroll
   for (int s = 0; s < VK; ++s) id[s] = -1;
@@ -277,7 +277,7 @@ __device__ __forceinline__ void choose(const RouteExpertsArgs& p, const Token<V>
 // to each other, more candidates) comes back as false.  list, cand: a token's places
 // in LDS for its experts and sixteen keys.
 template <bool SCORES, int LPT, int V>
-__device__ __forceinline__ bool choose_fast(const RouteExpertsArgs& p, const Token<V>& x, int i, float* at, int* list, double* cand, bool& bad) {
+__device__ __forceinline__ bool choose_fast(const RouteExpertsArgs& p, const Token<V>& x, int i, float* at, int* list, double* cand) {
   constexpr unsigned mask = V <= 1 ? 0 : V <= 2 ? 1 : V <= 4 ? 3 : V <= 8 ? 7 : 15;
   constexpr float lost = 2.f * (float)(mask + 1) / (1 << 23);  // of d: its last bits, and two roundings
   const float inf = __builtin_inff();
@@ -285,7 +285,7 @@ __device__ __forceinline__ bool choose_fast(const RouteExpertsArgs& p, const Tok
   const float off = !SCORES ? 0.f : p.score == GP_SCORE_SOFTMAX ? 1.f / (1 << 18) : 1.f / (1 << 21);
   const bool exact = !SCORES && p.dtype != GP_DTYPE_F32;
   float key[V], rank[V];
-  make_keys<float, SCORES, LPT>(p, x, key, rank, bad);
+  make_keys<float, SCORES, LPT>(p, x, key, rank);
   bool sure = true;
   if (p.top_groups < p.groups) sure = keep_groups<float, LPT>(p, key, rank, i, at, 5.f * off);
   float top = -inf;
@@ -356,7 +356,7 @@ __device__ __forceinline__ bool choose_fast(const RouteExpertsArgs& p, const Tok
   const bool one = i < q && i < MOST;
   int e = one ? list[i] : -1;
   double c = -(double)inf;
-  if (e >= 0) {
+  if ((unsigned)e < (unsigned)p.E) {
     const float l = logit(p.logits, x.t * p.E + e, p.dtype);
     c = SCORES && p.bias ? sigmoid64(l) + (double)p.bias[e] : (double)l;
   }
@@ -402,16 +402,23 @@ __global__ __launch_bounds__(64 * kWaves) void route_experts_kernel(RouteExperts
 #pragma unroll
     for (int v = 0; v < V; ++v) x.bias[v] = p.bias[v * LPT + i < p.E ? v * LPT + i : p.E - 1];
   }
+  // A row with a NaN (scores are 0 to 1, so c is one where the logit or the bias is) or, with softmax, a +inf
+  // has no choice to make: to what follows its experts are as those that cannot be chosen.
   x.top = -inf;
-  bool bad = false;
+  bool nan = false;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     x.l[v] = v * LPT + i < p.E ? x.l[v] : -inf;
-    bad |= x.l[v] != x.l[v];
+    nan |= x.l[v] != x.l[v];
+    if (SCORES && p.bias) nan |= x.bias[v] != x.bias[v] && x.l[v] > -inf;
     x.top = x.l[v] > x.top ? x.l[v] : x.top;
   }
   x.top = over_token<LPT>(x.top, [](float a, float b) { return a > b ? a : b; });
-  bad |= softmax && x.top == inf;
+  nan |= softmax && x.top == inf;
+  const bool bad = over_token<LPT>((int)nan, [](int a, int b) { return a | b; });
+  x.top = bad ? -inf : x.top;
+#pragma unroll
+  for (int v = 0; v < V; ++v) x.l[v] = bad ? -inf : x.l[v];
 
   // 32 bits settle nearly every token; where a choice is too close for them, the wave makes its choices again.
   int id[VK];
@@ -420,11 +427,11 @@ __global__ __launch_bounds__(64 * kWaves) void route_experts_kernel(RouteExperts
   double* const cand = (double*)mem + place * 16;
   int* const list = (int*)(mem + kWaves * TPW * 128) + place * (kRouteMaxK + 1);
   K* const at = (K*)(mem + kRouteLds * kWaves * TPW) + place * p.E;
-  const bool sure = choose_fast<SCORES, LPT, V>(p, x, i, (float*)at, list, cand, bad);
+  const bool sure = choose_fast<SCORES, LPT, V>(p, x, i, (float*)at, list, cand);
   wave_lds();
 #pragma unroll
   for (int s = 0; s < VK; ++s) id[s] = s * LPT + i < p.k ? list[s * LPT + i] : -1;
-  if (__any(!sure && !bad)) choose<K, SCORES, LPT, V>(p, x, i, at, id, bad);
+  if (__any(!sure)) choose<K, SCORES, LPT, V>(p, x, i, at, id);
 
   // Weights: of a softmax that is divided by the chosen ones' sum, relative to the largest of them.
   const bool relative = softmax && p.renorm;
@@ -439,7 +446,7 @@ __global__ __launch_bounds__(64 * kWaves) void route_experts_kernel(RouteExperts
 #pragma unroll
   for (int s = 0; s < VK; ++s) {
     l[s] = -inf;
-    if (s * LPT < p.k && id[s] >= 0) l[s] = logit(p.logits, t * p.E + id[s], p.dtype);
+    if (s * LPT < p.k && (unsigned)id[s] < (unsigned)p.E) l[s] = logit(p.logits, t * p.E + id[s], p.dtype);
     ltop = l[s] > ltop ? l[s] : ltop;
   }
   if (relative) ltop = over_token<LPT>(ltop, [](float a, float b) { return a > b ? a : b; });
@@ -454,14 +461,13 @@ __global__ __launch_bounds__(64 * kWaves) void route_experts_kernel(RouteExperts
     total += w[s];
   }
   if (p.renorm) total = over_token<LPT>(total, [](double a, double b) { return a + b; });
-  const int any = over_token<LPT>((int)bad, [](int a, int b) { return a | b; });
 #pragma unroll
   for (int s = 0; s < VK; ++s) {
     const int n = s * LPT + i;
     if (n >= p.k || token >= p.T) continue;
     const double v = !p.renorm ? w[s] : total > 0.0 ? w[s] / total : 0.0;
-    p.weights[t * p.k + n] = any ? __builtin_nanf("") : (float)(v * (double)p.scale);
-    p.ids[t * p.k + n] = any ? n : id[s];
+    p.weights[t * p.k + n] = bad ? __builtin_nanf("") : (float)(v * (double)p.scale);
+    p.ids[t * p.k + n] = bad ? n : id[s];
   }
 }
 
