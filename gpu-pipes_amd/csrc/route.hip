@@ -143,12 +143,6 @@ __device__ __forceinline__ int take_best(K (&key)[V], int i, K& best) {
   return at;
 }
 
-// a from b, a >= b, where each may be off by `off` of itself or of 1.  Equal
-// infinities are not, nothing (b) is far from everything.
-__device__ __forceinline__ bool apart(float a, float b, float off) {
-  return !(b > -__builtin_inff()) || a - b > off * fmaxf(fmaxf(fabsf(a), fabsf(b)), 1.f);
-}
-
 // Keys of a token's experts: the logits, or (SCORES) c in K's precision, -inf for
 // those that cannot be chosen.
 template <class K, bool SCORES, int LPT, int V>
@@ -189,8 +183,12 @@ __device__ __forceinline__ void make_keys(const RouteExpertsArgs& p, const Token
 }
 
 // Leaves the keys of the top_groups best groups.  at: the token's place in the
-// wave's LDS.  Whether the last of them is further than `off` from the first of the
-// others comes back.
+// wave's LDS.  off: how far a c can be from its value, of itself or of 1 (0: not at
+// all).  Whether every group that is kept is certain to be better than every
+// other one comes back.  A group's sum is as far from its value as its terms are,
+// however small it is itself: terms of |c| <= m and the sum's rounding 2.25 off m,
+// the bound's own 0.25 off m, so 3 off m.  A sum of finite terms that is not finite
+// is no value at all; one with an infinite term is exact.
 template <class K, int LPT, int V>
 __device__ __forceinline__ bool keep_groups(const RouteExpertsArgs& p, K (&key)[V], const K (&rank)[V], int i, K* at, float off) {
   const K none = -(K)__builtin_inff();
@@ -205,6 +203,8 @@ __device__ __forceinline__ bool keep_groups(const RouteExpertsArgs& p, K (&key)[
   auto select = [&](auto vg) {
     constexpr int VG = decltype(vg)::value;
     K g[VG];
+    float least[VG], most[VG];  // what the group's value may be
+    bool lost = false;          // a sum past fp32's range
 #pragma unroll
     for (int v = 0; v < VG; ++v) {
       const int gi = v * LPT + i < p.groups ? v * LPT + i : p.groups - 1;
@@ -220,19 +220,35 @@ __device__ __forceinline__ bool keep_groups(const RouteExpertsArgs& p, K (&key)[
           a = r > a ? r : a;
         }
       }
-      g[v] = p.group_score == GP_GROUP_TOP2 && b > none ? a + b : a;
+      const bool two = p.group_score == GP_GROUP_TOP2 && b > none;
+      g[v] = two ? a + b : a;
+      if constexpr (sizeof(K) == 4) {
+        // an infinite m makes NaNs here, which the minimum and the maximum below pass over
+        const float d = 3.f * off * fmaxf(fmaxf(fabsf(a), two ? fabsf(b) : 1.f), 1.f);
+        lost |= two && a < -none && fabsf(g[v]) == -none;
+        least[v] = g[v] - d;
+        most[v] = v * LPT + i < p.groups ? g[v] + d : none;
+      }
       g[v] = v * LPT + i < p.groups ? g[v] : none;
     }
-    K last = none;
-    for (int n = 0; n < p.top_groups + (off > 0.f); ++n) {
+    for (int n = 0; n < p.top_groups; ++n) {
       K best;
       const int of = take_best<LPT>(g, i, best);
-      if (n < p.top_groups) {
-        if (best > none) kept |= 1ull << (of & 63);  // of groups with no expert left none is kept
-      } else {
-        sure = apart((float)last, (float)best, off);
+      if (best > none) kept |= 1ull << (of & 63);  // of groups with no expert left none is kept
+    }
+    if constexpr (sizeof(K) == 4) {
+      if (off > 0.f) {
+        float in = -none, out = lost ? -none : none;
+#pragma unroll
+        for (int v = 0; v < VG; ++v) {
+          const bool is = kept >> (v * LPT + i & 63) & 1;
+          in = fminf(in, is ? least[v] : -none);
+          out = fmaxf(out, is ? none : most[v]);
+        }
+        in = over_token<LPT>(in, [](float a, float b) { return fminf(a, b); });
+        out = over_token<LPT>(out, [](float a, float b) { return fmaxf(a, b); });
+        sure = in > out;
       }
-      last = best;
     }
   };
   if (p.groups <= LPT)
@@ -281,13 +297,12 @@ __device__ __forceinline__ bool choose_fast(const RouteExpertsArgs& p, const Tok
   constexpr unsigned mask = V <= 1 ? 0 : V <= 2 ? 1 : V <= 4 ? 3 : V <= 8 ? 7 : 15;
   constexpr float lost = 2.f * (float)(mask + 1) / (1 << 23);  // of d: its last bits, and two roundings
   const float inf = __builtin_inff();
-  // of a score; its sum of two is off by twice that and its own rounding
   const float off = !SCORES ? 0.f : p.score == GP_SCORE_SOFTMAX ? 1.f / (1 << 18) : 1.f / (1 << 21);
   const bool exact = !SCORES && p.dtype != GP_DTYPE_F32;
   float key[V], rank[V];
   make_keys<float, SCORES, LPT>(p, x, key, rank);
   bool sure = true;
-  if (p.top_groups < p.groups) sure = keep_groups<float, LPT>(p, key, rank, i, at, 5.f * off);
+  if (p.top_groups < p.groups) sure = keep_groups<float, LPT>(p, key, rank, i, at, off);
   float top = -inf;
 #pragma unroll
   for (int v = 0; v < V; ++v) top = fmaxf(top, key[v]);
