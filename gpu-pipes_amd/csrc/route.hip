@@ -187,8 +187,10 @@ __device__ __forceinline__ void make_keys(const RouteExpertsArgs& p, const Token
 // all).  Whether every group that is kept is certain to be better than every
 // other one comes back.  A group's sum is as far from its value as its terms are,
 // however small it is itself: terms of |c| <= m and the sum's rounding 2.25 off m,
-// the bound's own 0.25 off m, so 3 off m.  A sum of finite terms that is not finite
-// is no value at all; one with an infinite term is exact.
+// the bound's own 0.25 off m, so 3 off m.  A sum of finite terms above fp32's range is
+// no value at all; for one below it (a group masked by the type's lowest value)
+// stands the lowest value, with -inf as its least: 16,384 tokens with such a group
+// 12.9 us instead of 20.7 in 64 bits.  A sum with an infinite term is exact.
 template <class K, int LPT, int V>
 __device__ __forceinline__ bool keep_groups(const RouteExpertsArgs& p, K (&key)[V], const K (&rank)[V], int i, K* at, float off) {
   const K none = -(K)__builtin_inff();
@@ -204,7 +206,7 @@ __device__ __forceinline__ bool keep_groups(const RouteExpertsArgs& p, K (&key)[
     constexpr int VG = decltype(vg)::value;
     K g[VG];
     float least[VG], most[VG];  // what the group's value may be
-    bool lost = false;          // a sum past fp32's range
+    bool lost = false;          // a sum above fp32's range
 #pragma unroll
     for (int v = 0; v < VG; ++v) {
       const int gi = v * LPT + i < p.groups ? v * LPT + i : p.groups - 1;
@@ -225,8 +227,9 @@ __device__ __forceinline__ bool keep_groups(const RouteExpertsArgs& p, K (&key)[
       if constexpr (sizeof(K) == 4) {
         // an infinite m makes NaNs here, which the minimum and the maximum below pass over
         const float d = 3.f * off * fmaxf(fmaxf(fabsf(a), two ? fabsf(b) : 1.f), 1.f);
-        lost |= two && a < -none && fabsf(g[v]) == -none;
-        least[v] = g[v] - d;
+        lost |= two && a < -none && g[v] == -none;
+        g[v] = two ? fmaxf(g[v], -3.4028234664e38f) : g[v];
+        least[v] = g[v] - d;  // below the lowest value: -inf, d being more than half its step there
         most[v] = v * LPT + i < p.groups ? g[v] + d : none;
       }
       g[v] = v * LPT + i < p.groups ? g[v] : none;
