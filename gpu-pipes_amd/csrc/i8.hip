@@ -281,7 +281,7 @@ struct I8Group {
 // two weights NT / 2 of each); words and x go through a ring of R chunks in
 // LDS that is the wave's own, so that many loads are in flight and no barrier
 // lies between them, and the waves' sums are joined through LDS.
-// XL: at most four rows of 16-bit x, which the workgroup makes bytes of itself.
+// XL: at most four rows of 16-bit x (own_bytes), which the workgroup makes bytes of itself.
 // Bound by the weights' loads: a token's 2 x 16,384 columns from 4,096 k 27.8 us
 // (134 MB, 4.8 TB/s), 4,096 from 16,384 k 11.7 to 13.3; 16 rows of 8,192 from 8,192 12.1.
 // ---------------------------------------------------------------------------
@@ -914,6 +914,7 @@ bool on_tiles(int64_t M, int N, int sides) {
 //   4 of 16 of 2,048 x 4,096:  3 58.4 / 57.8, 4 69.9 / 68.9, 8 124.7 / 78.7;  2 of 32 of 1,024 x 512:  8 14.0 / 22.2
 bool few_tokens(int64_t T, int E, int topk) { return T <= 2 || (T <= 8 && 4 * T * topk <= 3 * E); }
 
+// Rows of 16-bit x that the kernel for few rows makes bytes of itself: up to four (three as four) of 16,384 values together.
 bool own_bytes(int64_t M, int K) { return M <= 4 && K * (M <= 1 ? 1 : M <= 2 ? 2 : 4) <= 16384; }
 
 // mtiles: of 16 mt rows.  A product of experts (MODE) has them from its plan; busy: those that are worth counting.

@@ -23,8 +23,8 @@
 // A token has 16 lanes up to 256 experts (four tokens a wave, and every exchange
 // between lanes a DPP rotation), 64 above.  Bound by instructions: an argument's
 // maximum over a token is V compares a lane and four or six exchanges, k times.
-// 16,384 tokens to 6 of 128 experts in 8 groups: 10.6 to 12.4 us among other calls by
-// card, 12.8 in a graph, 1,067 vector instructions a wave (793 without groups); with all scores in
+// 16,384 tokens to 6 of 128 experts in 8 groups: 11.8 us among other calls, 11.9 in a
+// graph, 1,119 vector instructions a wave (814 without groups); with all scores in
 // 64 bits 16.6 in a graph.
 #include <hip/hip_runtime.h>
 
